@@ -38,6 +38,7 @@ EXPORTS = (
     "ix_gdn_window_record_size", "ix_gdn_decode_window", "ix_gdn_decode_window_mfma", "ix_gdn_commit_window",
     "ix_bf16_gemv", "ix_bf16_gemv_pair", "ix_bf16_gemv_split", "ix_mmvq_q8_0", "ix_gdn_in_proj_width", "ix_gdn_in_proj",
     "ix_gdn_version", "ix_gdn_decode_noalloc", "ix_q8_1_quantize", "ix_gdn_commit_window_layers",
+    "ix_add_rms_norm", "ix_kv8_append", "ix_kv8_read",
 )
 
 
@@ -71,15 +72,30 @@ class OutGate(ctypes.Structure):
     ]
 
 
+class Kv8(ctypes.Structure):
+    """``ix_kv8`` (include/ix_gdn.h): a paged key/value cache in 8 bits; see :func:`kv8_cache`."""
+
+    _fields_ = [
+        ("n_pages", ctypes.c_int), ("page", ctypes.c_int), ("h_kv", ctypes.c_int), ("d", ctypes.c_int),
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+    ]
+
+
+class Rows(ctypes.Structure):
+    """``ix_rows`` (include/ix_gdn.h): bf16 token rows with a stride. Calls take tensors in its place."""
+
+    _fields_ = [("p", ctypes.c_void_p), ("stride", ctypes.c_longlong)]
+
+
 def make_cfg(h_k=16, h_v=32, d_k=128, d_v=128, d_conv=4, head_map=HEAD_MOD, conv_act=ACT_NONE,
              q_scale=1.0, l2_eps=1e-6) -> Cfg:
     """Layer description; defaults are the reference's semantics at the Qwen3-Next shape."""
     return Cfg(h_k, h_v, d_k, d_v, d_conv, head_map, conv_act, q_scale, l2_eps)
 
 
-# Arguments of every symbol: a layer description (c) or output gate (g) by reference, a tensor's address (p), the
-# stream (s); i, l, z and f are an int, a long long, a size_t and a float.
-_TYPES = {**dict.fromkeys("cgps", ctypes.c_void_p), "i": ctypes.c_int, "l": ctypes.c_longlong, "z": ctypes.c_size_t,
+# Arguments of every symbol: a layer description (c), output gate (g) or cache (k) by reference, token rows (r), a
+# tensor's address (p), the stream (s); i, l, z and f are an int, a long long, a size_t and a float.
+_TYPES = {**dict.fromkeys("cgkrps", ctypes.c_void_p), "i": ctypes.c_int, "l": ctypes.c_longlong, "z": ctypes.c_size_t,
           "f": ctypes.c_float}
 _I, _Z = ctypes.c_int, ctypes.c_size_t
 _SIGNATURES = {
@@ -111,6 +127,9 @@ _SIGNATURES = {
     "ix_gdn_decode_noalloc": ("cipppppppppps", _I),
     "ix_q8_1_quantize": ("ppls", _I),
     "ix_gdn_commit_window_layers": ("ciiippppps", _I),
+    "ix_add_rms_norm": ("iipppppffppps", _I),
+    "ix_kv8_append": ("kiipppirrs", _I),
+    "ix_kv8_read": ("kiipppipps", _I),
 }
 
 _lib = None
@@ -143,6 +162,22 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
+def _rows(t):
+    """``ix_rows`` of a bf16 CUDA tensor whose rows (its first dimension) are dense (None for None)."""
+    if t is None or isinstance(t, ctypes.Structure):
+        return t
+    if not t.is_cuda:
+        raise ValueError("baloon_amd: tensors must be on the GPU")
+    if t.element_size() != 2 or t.dim() < 2:
+        raise ValueError("baloon_amd: token rows are bf16 tensors of two dimensions or more")
+    dense = 1
+    for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if n != 1 and st != dense:
+            raise ValueError("baloon_amd: token rows must be dense")
+        dense *= n
+    return Rows(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), dense))
+
+
 def _stream(s) -> int | None:
     if s is None:
         import torch
@@ -164,7 +199,8 @@ def _through_ctypes(name, args) -> int:
     """A launcher's call with ctypes' conversions: for arguments that the extension leaves to it (anything but
     plain tensors, ints, floats, structures and streams), and for every call where there is no extension."""
     convert = {"c": lambda v: _byref(v, Cfg), "g": lambda v: None if v is None else _byref(v, OutGate),
-               "p": _ptr, "s": _stream}
+               "k": lambda v: None if v is None else _byref(v, Kv8),
+               "r": lambda v: None if v is None else _byref(_rows(v), Rows), "p": _ptr, "s": _stream}
     fn = getattr(lib(), name)
     args = [convert[t](v) if t in convert else v for t, v in zip(_SIGNATURES[name][0], args)]
     try:
@@ -388,6 +424,42 @@ def ix_gdn_in_proj_width(cfg: Cfg) -> int:
 def ix_gdn_in_proj(cfg: Cfg, B, hidden, h, w, x, z, a, b, y=None, s=None) -> int:
     """[x | z | a | b] = h W^T for B rows: h [B][hidden], W [N][hidden] bf16 -> bf16 pieces."""
     return _bind.ix_gdn_in_proj(cfg, B, hidden, h, w, x, z, a, b, y, s)
+
+
+# ---- between the GDN layers -------------------------------------------------------------------
+
+def ix_add_rms_norm(rows, n, x, res, res_out, weight, weight_offset, eps, y=None, y_bf16=None, y_q8_1=None,
+                    s=None) -> int:
+    """h = bf16(x + res), y = RMS norm of h times (weight_offset + weight), row by row. x is fp32 or bf16
+    (by its element size), res and res_out bf16 or None; y_q8_1 is a byte buffer of 36 bytes per 32 outputs."""
+    x32, x16 = (None, x) if x is not None and x.element_size() == 2 else (x, None)
+    return _bind.ix_add_rms_norm(rows, n, x32, x16, res, res_out, weight, weight_offset, eps, y, y_bf16, y_q8_1, s)
+
+
+def kv8_cache(k, v, k_scale, v_scale) -> Kv8:
+    """The description of a cache from its tensors: codes k [n_pages][h_kv][page][d] and v
+    [n_pages][h_kv][d][page] (int8), scales [n_pages][h_kv] (fp32). It holds on to them."""
+    import torch
+    if k.dim() != 4 or tuple(v.shape) != (*k.shape[:2], k.shape[3], k.shape[2]):
+        raise ValueError("baloon_amd: k is [n_pages][h_kv][page][d] and v [n_pages][h_kv][d][page]")
+    if tuple(k_scale.shape) != tuple(k.shape[:2]) or tuple(v_scale.shape) != tuple(k.shape[:2]):
+        raise ValueError("baloon_amd: scales are [n_pages][h_kv]")
+    if k.dtype != torch.int8 or v.dtype != torch.int8 or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise ValueError("baloon_amd: codes are int8, scales fp32")
+    c = Kv8(k.shape[0], k.shape[2], k.shape[1], k.shape[3], _ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale))
+    c.tensors = (k, v, k_scale, v_scale)
+    return c
+
+
+def ix_kv8_append(cache: Kv8, n_seq, total_T, cu_seqlens, kv_len, table, width, k, v, s=None) -> int:
+    """Append total_T new tokens' keys and values to n_seq sequences. k, v are bf16 tensors of rows
+    [h_kv][d] whose first dimension may have any stride (slices of a fused projection)."""
+    return _bind.ix_kv8_append(cache, n_seq, total_T, cu_seqlens, kv_len, table, width, k, v, s)
+
+
+def ix_kv8_read(cache: Kv8, n_seq, total_T, cu_seqlens, kv_len, table, width, k=None, v=None, s=None) -> int:
+    """The cache's values at the batch's positions, as bf16 [total_T][h_kv][d]."""
+    return _bind.ix_kv8_read(cache, n_seq, total_T, cu_seqlens, kv_len, table, width, k, v, s)
 
 
 def version() -> str:

@@ -7,12 +7,14 @@
 // 38 us for 16 us of kernels. Here an argument is read from the tensor's C++ object.
 //
 // Arguments are converted by the C parameter's type: pointers from tensors (plain torch.Tensor or
-// Parameter, on the GPU, contiguous) or None, descriptions from ctypes structures, numbers from ints and
+// Parameter, on the GPU, contiguous) or None, token rows from such tensors of any row stride, descriptions from
+// ctypes structures, numbers from ints and
 // floats, the stream from None (torch's current one), a torch stream or an address. A call with any other argument
 // goes as a whole to the mirror's ctypes path, which reads or refuses it. The mirror hands over the addresses
 // of the library's functions.
 #include <Python.h>
 
+#include <algorithm>
 #include <cstring>
 #include <tuple>
 #include <utility>
@@ -85,9 +87,50 @@ hipStream_t stream(PyObject* o, bool& other) {
     return nullptr;
 }
 
+// What the converted arguments are held in: token rows by value, as they come from a tensor.
+struct Rows {
+    ix_rows r;
+    bool any;
+    operator const ix_rows*() const { return any ? &r : nullptr; }
+};
+template <class T>
+struct Held { typedef T type; };
+template <>
+struct Held<const ix_rows*> { typedef Rows type; };
+
 template <class T>
 struct Arg {                                                 // pointers to device memory
     static T of(PyObject* o, bool& other) { return static_cast<T>(tensor_ptr(o, other)); }
+};
+template <>
+struct Arg<const ix_kv8*> {
+    static const ix_kv8* of(PyObject* o, bool& other) {
+        return o == Py_None ? nullptr : structure<ix_kv8>(o, other);
+    }
+};
+// Rows of a tensor on the GPU: 2-byte elements, dense but for the first dimension.
+template <>
+struct Arg<const ix_rows*> {
+    static Rows of(PyObject* o, bool& other) {
+        if (o == Py_None) return Rows{};
+        if (THPVariable_CheckExact(o)) {
+            const at::Tensor& t = THPVariable_Unpack(o);
+            if (t.is_cuda() && t.layout() == c10::kStrided && t.element_size() == 2 && t.dim() >= 2) {
+                int64_t dense = 1;
+                bool ok = true;
+                for (int64_t i = t.dim() - 1; i >= 1; --i) {
+                    ok = ok && (t.size(i) == 1 || t.stride(i) == dense);
+                    dense *= t.size(i);
+                }
+                if (ok) {
+                    const int64_t st = t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), dense);
+                    return Rows{{static_cast<const uint16_t*>(t.data_ptr()), (long long)st}, true};
+                }
+            }
+        }
+        other = true;
+        return Rows{};
+    }
 };
 template <>
 struct Arg<const ix_gdn_cfg*> {
@@ -136,7 +179,7 @@ template <class... A, size_t... I>
 PyObject* invoke(hipError_t (*fn)(A...), const char* name, PyObject* const* args, std::index_sequence<I...>) {
     bool other = false;
     // Braces: converted from left to right, up to the first that is left to ctypes.
-    const std::tuple<A...> v{(other ? A{} : Arg<A>::of(args[I], other))...};
+    const std::tuple<typename Held<A>::type...> v{(other ? typename Held<A>::type{} : Arg<A>::of(args[I], other))...};
     if (other) return through_ctypes(name, args, (Py_ssize_t)sizeof...(A));
     hipError_t e;
     Py_BEGIN_ALLOW_THREADS
@@ -167,7 +210,8 @@ PyObject* call(hipError_t (*fn)(A...), const char* name, PyObject* const* args, 
     X(ix_gdn_step) X(ix_gdn_conv_step) X(ix_gdn_l2_norm) X(ix_gdn_beta_gate) X(ix_gdn_out_norm) X(ix_gdn_decode) \
     X(ix_gdn_decode_noalloc) X(ix_gdn_decode_gated) X(ix_gdn_prefill) X(ix_gdn_prefill_gated)                    \
     X(ix_gdn_decode_window) X(ix_gdn_decode_window_mfma) X(ix_gdn_commit_window) X(ix_bf16_gemv)                 \
-    X(ix_bf16_gemv_pair) X(ix_bf16_gemv_split) X(ix_mmvq_q8_0) X(ix_q8_1_quantize) X(ix_gdn_in_proj)
+    X(ix_bf16_gemv_pair) X(ix_bf16_gemv_split) X(ix_mmvq_q8_0) X(ix_q8_1_quantize) X(ix_gdn_in_proj)             \
+    X(ix_add_rms_norm) X(ix_kv8_append) X(ix_kv8_read)
 
 #define X(name)                                                                        \
     decltype(&::name) p_##name = nullptr;                                              \

@@ -488,7 +488,7 @@ extern "C" int ix_gdn_channels(const ix_gdn_cfg* c) {
     return c ? 2 * c->h_k * c->d_k + c->h_v * c->d_v : 0;
 }
 
-extern "C" const char* ix_gdn_version(void) { return "ixgdn 0.5.0 gfx950"; }
+extern "C" const char* ix_gdn_version(void) { return "ixgdn 0.6.0 gfx950"; }
 
 // Shared validation of the fused layer description (also used by the prefill).
 extern "C" hipError_t ix_gdn_check_cfg_(const ix_gdn_cfg* c) {

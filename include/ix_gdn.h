@@ -332,8 +332,81 @@ hipError_t ix_gdn_in_proj(const ix_gdn_cfg* cfg, int B, int hidden, const uint16
                           uint16_t* x, uint16_t* z, uint16_t* a, uint16_t* b, float* y,
                           hipStream_t s IX_GDN_DEFAULT_STREAM);
 
-/* Library version string ("ixgdn 0.5.0 gfx950"). 0.5.0: ix_gdn_out_gate ends with y_q8_1, so
- * callers compiled against an older header must be rebuilt. */
+/* ---------------------------------------------------------------------------------------
+ * Between the GDN layers (additions; no reference counterpart)
+ *
+ * A hybrid model has a norm on its residual stream ahead of every layer, and attention
+ * layers among the GDN ones.
+ * --------------------------------------------------------------------------------------- */
+
+/* RMS norm with the residual's addition, row by row:
+ *   h = bf16(x + res),  y = h / sqrt(mean(h^2) + eps) * (weight_offset + weight)
+ *   x [rows][n] fp32 or x_bf16 [rows][n] bf16: exactly one of them
+ *   res [rows][n] bf16, or NULL (h = bf16(x))
+ *   res_out [rows][n] bf16 = h, or NULL; may be res itself or x_bf16
+ *   weight [n] fp32; weight_offset is 0, or 1 where a model stores its weights around zero
+ *   y fp32, y_bf16 (RNE of the fp32 value) [rows][n], y_q8_1 [rows][n/32] q8_1 blocks (the
+ *   activation format of ix_mmvq_q8_0, the bytes that ix_q8_1_quantize gives for y): at least
+ *   one of them. y_bf16 may be x_bf16 or res.
+ * The sum of squares and the norm are fp32. Requires rows >= 0, 0 < n <= 32768, n % 32 == 0
+ * for y_q8_1 (4-byte aligned). n % 8 == 0 with 16-byte aligned operands is faster. */
+hipError_t ix_add_rms_norm(int rows, int n, const float* x, const uint16_t* x_bf16, const uint16_t* res,
+                           uint16_t* res_out, const float* weight, float weight_offset, float eps, float* y,
+                           uint16_t* y_bf16, void* y_q8_1, hipStream_t s IX_GDN_DEFAULT_STREAM);
+
+/* Token rows of bf16 that need not lie packed: row t is at p + t * stride (in elements), dense
+ * within itself, e.g. a slice of the rows of a fused projection. Read on the host at call time. */
+typedef struct ix_rows {
+    const uint16_t* p;
+    long long stride;
+} ix_rows;
+
+/* A key/value cache of one attention layer in 8 bits, in pages (read on the host at call time;
+ * the memory is the caller's). Each page holds `page` tokens of every kv head, and each (page,
+ * head) has one scale for its keys and one for its values: a value stands as scale * code.
+ *   k [n_pages][h_kv][page][d], v [n_pages][h_kv][d][page] int8, 16-byte aligned
+ *   k_scale, v_scale [n_pages][h_kv] fp32
+ * page is 16, 32, 64 or 128, d 64, 128 or 256, 1 <= h_kv <= 1024. New memory needs no
+ * initialisation: a page's first token sets its scales. */
+typedef struct ix_kv8 {
+    int n_pages, page, h_kv, d;
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+} ix_kv8;
+
+/* The batch of the calls below: n_seq sequences (at most 65535), total_T packed new tokens,
+ *   cu_seqlens [n_seq+1] int32 device offsets of their rows (cu_seqlens[0] = 0, non-decreasing;
+ *   a sequence may have none)
+ *   kv_len [n_seq] int32: tokens of each sequence with the new ones, which stand at positions
+ *   kv_len - q .. kv_len - 1 for q new ones
+ *   table [n_seq][width] int32: page p of sequence b, tokens p * page on, is page table[b][p] of
+ *   the cache. Entries behind the last page are not read; a page without a place in the cache
+ *   (an entry outside [0, n_pages), or p >= width) holds nothing: writes to it are dropped, its
+ *   tokens are hidden from every query.
+ * total_T = 0 is a call without work. */
+
+/* Append the batch's keys and values to its sequences: k, v rows of [h_kv][d], stride >= h_kv * d.
+ * Where a page gets new tokens its scale becomes s' = max(s, max|x| / 127), s being its scale if
+ * it holds older tokens of the sequence and 0 if not; where s' > s the older codes become
+ * rint(code * (s / s')); the new codes are rint(x / s') (0 when s' is 0). All in fp32, IEEE
+ * divisions, rint to nearest even. Values must be finite. The new tokens' pages must not be
+ * another sequence's of this batch, or hold anything behind the new tokens. Strides that are
+ * multiples of 8 at 16-byte aligned rows are faster. */
+hipError_t ix_kv8_append(const ix_kv8* cache, int n_seq, int total_T, const int32_t* cu_seqlens,
+                         const int32_t* kv_len, const int32_t* table, int width, const ix_rows* k, const ix_rows* v,
+                         hipStream_t s IX_GDN_DEFAULT_STREAM);
+
+/* What the cache holds at the batch's positions: k, v [total_T][h_kv][d] bf16 (RNE of scale *
+ * code), either of them NULL if not wanted. The inverse of ix_kv8_append on the same batch;
+ * rows of pages without a place in the cache are left as they are. */
+hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_t* cu_seqlens, const int32_t* kv_len,
+                       const int32_t* table, int width, uint16_t* k, uint16_t* v,
+                       hipStream_t s IX_GDN_DEFAULT_STREAM);
+
+/* Library version string ("ixgdn 0.6.0 gfx950"). 0.5.0: ix_gdn_out_gate ends with y_q8_1, so
+ * callers compiled against an older header must be rebuilt. 0.6.0: new entry points only. */
 const char* ix_gdn_version(void);
 
 #ifdef __cplusplus
