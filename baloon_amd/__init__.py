@@ -38,7 +38,7 @@ EXPORTS = (
     "ix_gdn_window_record_size", "ix_gdn_decode_window", "ix_gdn_decode_window_mfma", "ix_gdn_commit_window",
     "ix_bf16_gemv", "ix_bf16_gemv_pair", "ix_bf16_gemv_split", "ix_mmvq_q8_0", "ix_gdn_in_proj_width", "ix_gdn_in_proj",
     "ix_gdn_version", "ix_gdn_decode_noalloc", "ix_q8_1_quantize", "ix_gdn_commit_window_layers",
-    "ix_add_rms_norm", "ix_kv8_append", "ix_kv8_read",
+    "ix_add_rms_norm", "ix_kv8_append", "ix_kv8_read", "ix_kv8_attn_workspace_size", "ix_kv8_attn",
 )
 
 
@@ -130,6 +130,8 @@ _SIGNATURES = {
     "ix_add_rms_norm": ("iipppppffppps", _I),
     "ix_kv8_append": ("kiipppirrs", _I),
     "ix_kv8_read": ("kiipppipps", _I),
+    "ix_kv8_attn_workspace_size": ("kiiii", _Z),
+    "ix_kv8_attn": ("kiiipppirifiirppzs", _I),
 }
 
 _lib = None
@@ -460,6 +462,19 @@ def ix_kv8_append(cache: Kv8, n_seq, total_T, cu_seqlens, kv_len, table, width, 
 def ix_kv8_read(cache: Kv8, n_seq, total_T, cu_seqlens, kv_len, table, width, k=None, v=None, s=None) -> int:
     """The cache's values at the batch's positions, as bf16 [total_T][h_kv][d]."""
     return _bind.ix_kv8_read(cache, n_seq, total_T, cu_seqlens, kv_len, table, width, k, v, s)
+
+
+def ix_kv8_attn_workspace_size(cache: Kv8, n_seq: int, total_T: int, max_q: int, h_q: int) -> int:
+    return lib().ix_kv8_attn_workspace_size(ctypes.byref(cache), n_seq, total_T, max_q, h_q)
+
+
+def ix_kv8_attn(cache: Kv8, n_seq, total_T, max_q, cu_seqlens, kv_len, table, width, q, h_q, scale, window=0, sinks=0,
+                gate=None, o=None, workspace=None, workspace_bytes=0, s=None) -> int:
+    """Attention of total_T new tokens over the cache that holds them: o [total_T][h_q][d] bf16. q and gate
+    are bf16 tensors of rows [h_q][d] whose first dimension may have any stride. With window > 0 a token
+    sees that many positions and the first `sinks`. workspace: ix_kv8_attn_workspace_size(...) bytes."""
+    return _bind.ix_kv8_attn(cache, n_seq, total_T, max_q, cu_seqlens, kv_len, table, width, q, h_q, scale, window, sinks,
+                             gate, o, workspace, workspace_bytes, s)
 
 
 def version() -> str:

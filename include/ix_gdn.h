@@ -405,6 +405,33 @@ hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_
                        const int32_t* table, int width, uint16_t* k, uint16_t* v,
                        hipStream_t s IX_GDN_DEFAULT_STREAM);
 
+/* Bytes of device workspace for ix_kv8_attn on such a batch (partial results of sequences that
+ * several workgroups share; independent of the lengths), or 0 for an invalid request. It needs
+ * no initialisation; calls that share it must be ordered. */
+size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, int max_q, int h_q);
+
+/* Attention of the batch's tokens over the cache, which holds them already (ix_kv8_append):
+ *   o_r = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q_r . k_j)
+ * for every row r = (token at position pos, query head h), over kv head h / (h_q / h_kv) and the
+ * positions j that it sees: j <= pos and, when window > 0, pos - j < window or j < sinks (a
+ * sliding window and a few first tokens that stay visible). A row that sees nothing is 0.
+ *   max_q   at least the new tokens of the longest sequence (rows of longer ones are not written)
+ *   q       rows of [h_q][d]; h_q a multiple of h_kv
+ *   window  0 (everything before) .. 2^30; sinks >= 0, without meaning when window is 0
+ *   gate    rows of [h_q][d], or NULL: o is multiplied by sigmoid(gate)
+ *   o       [total_T][h_q][d] bf16 (RNE); may be the memory of q or gate where those are packed
+ *   workspace  256-byte aligned, workspace_bytes >= ix_kv8_attn_workspace_size(...)
+ * Positions up to 2^30. Scores are formed from 16-bit fixed-point q (of each row's largest
+ * value) and the codes, exactly, softmax sums in fp32, p in fp16 of its running maximum for
+ * the product with the codes of v. Scales that are not finite in
+ * hidden places do not matter. q and gate with strides that are multiples of 8 at
+ * 16-byte aligned rows are faster. The call may be captured into a HIP graph, and kv_len, table
+ * and the rest of the device data may change between its replays. */
+hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens,
+                       const int32_t* kv_len, const int32_t* table, int width, const ix_rows* q, int h_q, float scale,
+                       int window, int sinks, const ix_rows* gate, uint16_t* o, void* workspace,
+                       size_t workspace_bytes, hipStream_t s IX_GDN_DEFAULT_STREAM);
+
 /* Library version string ("ixgdn 0.6.0 gfx950"). 0.5.0: ix_gdn_out_gate ends with y_q8_1, so
  * callers compiled against an older header must be rebuilt. 0.6.0: new entry points only. */
 const char* ix_gdn_version(void);

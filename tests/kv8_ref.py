@@ -56,15 +56,20 @@ class Cache:
         return out, has
 
 
-def attend(q, kv_len, k, v, has, scale, window, sinks, gate=None):
-    """o [q][h_q][d] in 64 bits for one sequence: q rows fp32, k and v [kv_len][h_kv][d]."""
-    n, h_q, d = q.shape
-    G = h_q // k.shape[1] if kv_len else 1
+def seen_by(n, kv_len, has, window, sinks):
+    """[n][kv_len]: which tokens each of a sequence's n queries sees."""
     pos = kv_len - n + np.arange(n)[:, None]
     j = np.arange(kv_len)[None, :]
     seen = (j <= pos) & has[None, :]
     if window > 0:
         seen &= (pos - j < window) | (j < sinks)
+    return seen
+
+
+def attend(q, kv_len, k, v, seen, scale, gate=None):
+    """o [q][h_q][d] in 64 bits for one sequence: q rows fp32, k and v [kv_len][h_kv][d], 0 where no query sees them."""
+    n, h_q, d = q.shape
+    G = h_q // k.shape[1]
     o = np.zeros((n, h_q, d))
     k, v = k.astype(np.float64), v.astype(np.float64)
     for h in range(h_q):
