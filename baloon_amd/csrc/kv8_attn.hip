@@ -29,7 +29,6 @@ struct AttnArgs {
     float* part;              // partial results, see Parts
     float scale2;             // scale * log2(e)
     int h_q, G, window, sinks;
-    bool q_wide, gate_wide, o_wide;
 };
 
 // The kernel's argument (its only one) read from memory again where it is used next: keeping all of it in
@@ -65,26 +64,25 @@ __device__ __forceinline__ u16x2 max_abs_bits(u16x2 m, const uint4& x) {
     return m;
 }
 
-__device__ __forceinline__ uint4 load_row8(const uint16_t* p, bool wide) {
-    if (wide) return *reinterpret_cast<const uint4*>(p);
-    uint32_t u[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = p[2 * e] | ((uint32_t)p[2 * e + 1] << 16);
-    return make_uint4(u[0], u[1], u[2], u[3]);
+// 8 values of a row at any 2-byte address (the target reads and writes words unaligned).
+__device__ __forceinline__ uint4 load_row8(const uint16_t* p) {
+    uint4 x;
+    __builtin_memcpy(&x, p, sizeof(x));
+    return x;
 }
 
-// What the rows of one sequence see together: `ns` tiles of sinks and the tiles lo .. hi - 1.
+// What the rows of one sequence see together: `ns` tiles of sinks and those from `lo` on.
 struct Span {
     int s0, q, kv, first;     // rows s0 .. s0 + q - 1, at positions first ..
     int ns, lo, nt, nrb;      // nt tiles in all (1 where nothing is seen: zeros are written), nrb blocks of rows
     __device__ __forceinline__ int tile(int t) const { return t < ns ? t : lo + t - ns; }
 };
 template <int ROWS, int TOK>
-__device__ __forceinline__ Span span_of(const AttnArgs& A, int b) {
+__device__ __forceinline__ Span span_of(const AttnArgs& A, int s0, int q, int kv) {
     Span s;
-    s.s0 = A.a.start(b);
-    s.q = max(A.a.start(b + 1) - s.s0, 0);
-    s.kv = max(A.a.kv_len[b], 0);
+    s.s0 = s0;
+    s.q = q;
+    s.kv = kv;
     s.first = s.kv - s.q;
     s.lo = A.window > 0 ? max(s.first - A.window + 1, 0) / TOK : 0;
     s.ns = A.window > 0 ? min(A.sinks / TOK + (A.sinks % TOK != 0), s.lo) : 0;
@@ -93,59 +91,99 @@ __device__ __forceinline__ Span span_of(const AttnArgs& A, int b) {
     return s;
 }
 template <int ROWS, int TOK>
-__device__ __forceinline__ long long work_of(const AttnArgs& A, int b) {
-    const Span s = span_of<ROWS, TOK>(A, b);
-    return (long long)s.nrb * s.nt * A.c.h_kv;
+__device__ __forceinline__ Span span_at(const AttnArgs& A, int b) {
+    const int s0 = A.a.start(b);
+    return span_of<ROWS, TOK>(A, s0, max(A.a.start(b + 1) - s0, 0), max(A.a.kv_len[b], 0));
 }
 
-__device__ __forceinline__ long long wave_scan64(long long v, int lane) {
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const long long u = __shfl_up(v, off, kWave);
-        v += lane >= off ? u : 0;
-    }
-    return v;
+// Inclusive sum over lanes 0 .. l (the steps of wave_scan on 64-bit integers).
+template <int Ctrl, int RowMask>
+__device__ __forceinline__ long long dpp_add64(long long v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)v, Ctrl, RowMask, 0xF, RowMask == 0xF);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), Ctrl, RowMask, 0xF, RowMask == 0xF);
+    return v + (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
 }
+__device__ __forceinline__ long long wave_scan64(long long v) {
+    v = dpp_add64<0x111, 0xF>(v);
+    v = dpp_add64<0x112, 0xF>(v);
+    v = dpp_add64<0x114, 0xF>(v);
+    v = dpp_add64<0x118, 0xF>(v);
+    v = dpp_add64<0x142, 0xA>(v);
+    return dpp_add64<0x143, 0xC>(v);
+}
+__device__ __forceinline__ long long lane_of64(long long v, int l) {
+    const unsigned lo = __builtin_amdgcn_readlane((int)v, l), hi = __builtin_amdgcn_readlane((int)(v >> 32), l);
+    return (long long)(((unsigned long long)hi << 32) | lo);
+}
+// a / b for 0 <= a < 2^50, through the correctly rounded division in double.
+__device__ __forceinline__ long long quotient(long long a, int b) { return (long long)((double)a / (double)b); }
 
 // The batch's tiles, numbered through over sequences, kv heads, row blocks and tiles, are shared out evenly:
-// workgroup w takes [w per, (w + 1) per). Every wave works the shares out by itself from the lengths.
+// workgroup w takes [w per, (w + 1) per). Every wave works its share out by itself from the lengths.
 constexpr int kMinShare = 4;          // tiles: one for each wave
-struct Shares {
-    long long total, per;
+struct Share {
+    int per, left;                    // tiles of every workgroup, and of this one
+    int b, e, rb, t0;                 // where it begins
+    Span s;
 };
 template <int ROWS, int TOK>
-__device__ __forceinline__ Shares shares(const AttnArgs& A, int n_wg, int lane) {
-    long long v = 0;
-    for (int b = lane; b < A.a.n_seq; b += kWave) v += work_of<ROWS, TOK>(A, b);
-    Shares s;
-    s.total = __shfl(wave_scan64(v, lane), kWave - 1, kWave);
-    s.per = max((s.total + n_wg - 1) / n_wg, (long long)kMinShare);
-    return s;
-}
-// The sequence that tile `at` belongs to (at < total), and the number of its first tile.
-template <int ROWS, int TOK>
-__device__ __forceinline__ int locate(const AttnArgs& A, long long at, int lane, long long* base) {
-    long long carry = 0;
+__device__ __forceinline__ bool share_of(const AttnArgs& A, int n_wg, int w, int lane, Share* out) {
+    const int n = A.a.n_seq, h_kv = A.c.h_kv;
+    const auto chunk = [&](int b0, Span* s) {                // the work of sequence b0 + lane
+        if (b0 + lane >= n) return 0ll;
+        *s = span_at<ROWS, TOK>(A, b0 + lane);
+        return (long long)s->nrb * s->nt * h_kv;
+    };
+    Span s{};
+    long long v = chunk(0, &s), incl = wave_scan64(v), carry = 0;
+    long long total = lane_of64(incl, kWave - 1);
+    if (n > kWave) {
+        long long rest = 0;
+        Span x;
+        for (int b0 = kWave; b0 < n; b0 += kWave) rest += chunk(b0, &x);
+        total += lane_of64(wave_scan64(rest), kWave - 1);
+    }
+    out->per = (int)max(quotient(total + n_wg - 1, n_wg), (long long)kMinShare);
+    const long long cur = (long long)w * out->per;
+    if (cur >= total) return false;
+    out->left = (int)min((long long)out->per, total - cur);
     for (int b0 = 0;; b0 += kWave) {
-        const long long v = b0 + lane < A.a.n_seq ? work_of<ROWS, TOK>(A, b0 + lane) : 0;
-        const long long incl = wave_scan64(v, lane);
-        const unsigned long long hit = __ballot(carry + incl > at);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            *base = carry + __shfl(incl - v, l, kWave);
-            return b0 + l;
+        if (b0) {
+            v = chunk(b0, &s);
+            incl = wave_scan64(v);
         }
-        carry += __shfl(incl, kWave - 1, kWave);
+        const unsigned long long hit = __ballot(carry + incl > cur);
+        if (hit) {
+            const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
+            const long long rel = cur - carry - lane_of64(incl - v, l);
+            out->b = b0 + l;
+            out->s = span_of<ROWS, TOK>(A, __builtin_amdgcn_readlane(s.s0, l), __builtin_amdgcn_readlane(s.q, l),
+                                        __builtin_amdgcn_readlane(s.kv, l));
+            const int seg = __builtin_amdgcn_readfirstlane((int)quotient(rel, out->s.nt));
+            out->t0 = __builtin_amdgcn_readfirstlane((int)(rel - (long long)seg * out->s.nt));
+            out->e = seg / out->s.nrb;
+            out->rb = seg - out->e * out->s.nrb;
+            return true;
+        }
+        carry += lane_of64(incl, kWave - 1);
     }
 }
 
 // Partial results: workgroup w leaves that of the segment it starts in the middle of (or cuts at both
-// ends) in slot 2 w, that of another one it ends in the middle of in slot 2 w + 1.
+// ends) in slot 2 w, that of another one it ends in the middle of in slot 2 w + 1; and for the segment that lies
+// across the end of its tiles, where its parts are.
+struct Cut {
+    int first, last, slot;            // workgroups first .. last; slot of the first (2 w for the others)
+    int row, e, r0, rows;             // its sequence's first row, kv head, first row of the block, rows of the sequence
+    int any;
+};
 template <int ROWS, int D>
 struct Parts {
     float *o, *ml;
-    __device__ __forceinline__ Parts(float* p, int n_wg) : o(p), ml(p + (size_t)2 * n_wg * ROWS * D) {}
-    static size_t bytes(int n_wg) { return (size_t)2 * n_wg * ROWS * (D + 2) * sizeof(float); }
+    Cut* cut;
+    __device__ __forceinline__ Parts(float* p, int n_wg)
+        : o(p), ml(p + (size_t)2 * n_wg * ROWS * D), cut(reinterpret_cast<Cut*>(ml + (size_t)2 * n_wg * ROWS * 2)) {}
+    static size_t bytes(int n_wg) { return (size_t)2 * n_wg * ROWS * (D + 2) * sizeof(float) + n_wg * sizeof(Cut); }
 };
 
 // The lowest n bits, of a n that may lie anywhere.
@@ -168,25 +206,15 @@ __device__ __forceinline__ f16x8 halves8(uint32_t a, uint32_t b) {
 // Writes 4 outputs of a row, gated.
 __device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d, v4f v) {
     if (A.gate) {
-        const uint16_t* g = A.gate + (long long)t * A.gate_stride + (size_t)h * A.c.d + d;
-        if (A.gate_wide) {
-            const uint2 z = *reinterpret_cast<const uint2*>(g);
-            v[0] *= sigmoid_f(__uint_as_float(z.x << 16));
-            v[1] *= sigmoid_f(__uint_as_float(z.x & 0xffff0000u));
-            v[2] *= sigmoid_f(__uint_as_float(z.y << 16));
-            v[3] *= sigmoid_f(__uint_as_float(z.y & 0xffff0000u));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= sigmoid_f(bf16_to_f32(g[e]));
-        }
+        uint2 z;
+        __builtin_memcpy(&z, A.gate + (long long)t * A.gate_stride + (size_t)h * A.c.d + d, sizeof(z));
+        v[0] *= sigmoid_f(__uint_as_float(z.x << 16));
+        v[1] *= sigmoid_f(__uint_as_float(z.x & 0xffff0000u));
+        v[2] *= sigmoid_f(__uint_as_float(z.y << 16));
+        v[3] *= sigmoid_f(__uint_as_float(z.y & 0xffff0000u));
     }
-    uint16_t* o = A.o + ((size_t)t * A.h_q + h) * A.c.d + d;
-    if (A.o_wide) {
-        *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = f32_to_bf16(v[e]);
-    }
+    const uint2 y = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    __builtin_memcpy(A.o + ((size_t)t * A.h_q + h) * A.c.d + d, &y, sizeof(y));
 }
 
 constexpr int kSplitThreads = 256, kSplitWaves = kSplitThreads / kWave, kSplitRows = 16;
@@ -213,64 +241,23 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     extern __shared__ float lds[];
     float* lo_o = lds;                                        // [waves][16][kPitch]
     float* lo_ml = lds + kSplitWaves * kSplitRows * kPitch;   // [waves][16][2]
-    float* lo_qc = lo_ml + kSplitWaves * kSplitRows * 2;      // [16]
-    uint4* lo_q = reinterpret_cast<uint4*>(lo_qc + kSplitRows);   // [kC][hi, lo][lane]
+    uint32_t* lo_qm = reinterpret_cast<uint32_t*>(lo_ml + kSplitWaves * kSplitRows * 2);   // [waves][16]
+    uint4* lo_q = reinterpret_cast<uint4*>(lo_qm + kSplitWaves * kSplitRows);               // [kC][hi, lo][lane]
     const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int n = lane & 15, g = lane >> 4, mine = 4 * kS * g, keys = 4 * kS * (n >> 2);
-    int b, e, rb, t0, left;
+    int b, e, rb, t0, left, w_per;
     Span s;
     {
         const AttnArgs& Z = args_again();
-        const Shares sh = shares<kSplitRows, kTok>(Z, gridDim.x, lane);
-        const long long cur = blockIdx.x * sh.per;
-        if (cur >= sh.total) return;
-        left = __builtin_amdgcn_readfirstlane((int)min(sh.per, sh.total - cur));
-        long long base;
-        b = __builtin_amdgcn_readfirstlane(locate<kSplitRows, kTok>(Z, cur, lane, &base));
-        s = span_of<kSplitRows, kTok>(Z, b);
-        const long long rel = cur - base;
-        const int seg = (int)(rel / s.nt);
-        t0 = __builtin_amdgcn_readfirstlane((int)(rel - (long long)seg * s.nt));
-        e = __builtin_amdgcn_readfirstlane(seg / s.nrb);
-        rb = __builtin_amdgcn_readfirstlane(seg - seg / s.nrb * s.nrb);
+        Share sh;
+        if (!share_of<kSplitRows, kTok>(Z, gridDim.x, blockIdx.x, lane, &sh)) {
+            if (tid == 0) Parts<kSplitRows, D>(Z.part, gridDim.x).cut[blockIdx.x].any = 0;
+            return;
+        }
+        b = sh.b, e = sh.e, rb = sh.rb, t0 = sh.t0, left = sh.left, w_per = parked(sh.per), s = sh.s;
     }
     for (int piece = 0; left > 0; ++piece) {
         const int t1 = min(s.nt, t0 + left), r0 = rb * kSplitRows, rows = s.q * args_again().G;
-        // q as two int8 of 16 bits: wave c takes channels 64 c + 16 g .. + 15 of every row (row n its lanes')
-        if (w < kC) {
-            const AttnArgs& Z = args_again();
-            const int rc = min(r0 + n, rows - 1), qi = rc / Z.G;
-            const uint16_t* qp = Z.q + (long long)(s.s0 + qi) * Z.q_stride + (size_t)(e * Z.G + rc - qi * Z.G) * D + 16 * g;
-            u16x2 mb = {0, 0};
-            uint4 raw[2];
-#pragma unroll
-            for (int c = 0; c < kC; ++c)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint4 x = load_row8(qp + 64 * c + 8 * k, Z.q_wide);
-                    if (c == w) raw[k] = x;
-                    mb = max_abs_bits(mb, x);
-                }
-            uint32_t mu = max((uint32_t)mb[0], (uint32_t)mb[1]);
-            mu = max(mu, (uint32_t)__shfl_xor((int)mu, 16, kWave));
-            mu = max(mu, (uint32_t)__shfl_xor((int)mu, 32, kWave));
-            const float m = __uint_as_float(mu << 16);        // a row that is not finite gets scores that are none
-            const float inv = m > 1e-33f ? 32639.0f / m : 0.0f;
-            if (w == 0 && g == 0) lo_qc[n] = m * (1.0f / 32639.0f) * Z.scale2;
-            uint32_t hi[4] = {0, 0, 0, 0}, lw[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const uint4& p = raw[x / 8];
-                const uint32_t u = (x & 7) / 2 == 0 ? p.x : (x & 7) / 2 == 1 ? p.y : (x & 7) / 2 == 2 ? p.z : p.w;
-                const float v = __uint_as_float(x & 1 ? u & 0xffff0000u : u << 16);
-                const int q = (int)rintf(v * inv), h = (q + 128) >> 8;
-                hi[x / 4] |= (uint32_t)(h & 255) << (8 * (x & 3));
-                lw[x / 4] |= (uint32_t)((q - 256 * h) & 255) << (8 * (x & 3));
-            }
-            lo_q[(2 * w) * kWave + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            lo_q[(2 * w + 1) * kWave + lane] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
-        }
-        __syncthreads();
         const int w_left = parked(left), w_e = parked(e), w_rb = parked(rb), w_b = parked(b), w_s0 = parked(s.s0),
                   w_nrb = parked(s.nrb), w_nt = parked(s.nt), w_rows = parked(rows), w_t0 = parked(t0), w_t1 = parked(t1),
                   w_piece = parked(piece);
@@ -281,7 +268,6 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         // tiles that every row sees as a whole: those starting at full_lo .. full_hi
         const int full_hi = s.first + r0 / Y.G - kTok + 1;
         const int full_lo = window > 0 ? s.first + (min(r0 + kSplitRows, rows) - 1) / Y.G - window + 1 : 0;
-        const float qc = lo_qc[n];
 
         // A tile's places in the cache: this lane's values, scores and scales are of its tokens `mine` on, its
         // keys of those from `keys` on (both within 16 tokens of a page). A lost page's memory is page 0's,
@@ -311,22 +297,60 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             return vb + (size_t)max(page, 0) * page_bytes + (n << page_log) + slot_of(t, mine);
         };
 
-        v4f acc[kM];
-#pragma unroll
-        for (int m = 0; m < kM; ++m) acc[m] = v4f{0, 0, 0, 0};
-        float mref = -__builtin_inff(), l = 0.0f;
-
         int t = t0 + w;
-        int pv = page_of(t, mine), pk_next = page_of(t + kSplitWaves, keys), pv_next = page_of(t + kSplitWaves, mine);
+        int pk = page_of(t, keys), pv = page_of(t, mine), pk_next = page_of(t + kSplitWaves, keys), pv_next = page_of(t + kSplitWaves, mine);
+        // q as two int8 of 16 bits: wave c takes channels 64 c + 16 g .. + 15 of every row (row n its lanes')
+        uint4 raw[2];
+        if (w < kC) {
+            const AttnArgs& Z = args_again();
+            const int rc = min(r0 + n, rows - 1), qi = rc / Z.G;
+            const uint16_t* qp = Z.q + (long long)(s.s0 + qi) * Z.q_stride + (size_t)(e * Z.G + rc - qi * Z.G) * D + 64 * w + 16 * g;
+            raw[0] = load_row8(qp);
+            raw[1] = load_row8(qp + 8);
+        }
         float ks = 0.0f, vs = 0.0f;
         if (t < t1) {
-            load_k(t, page_of(t, keys));
+            load_k(t, pk);
             const int8_t* p = values_at(t, pv);
 #pragma unroll
             for (int m = 0; m < kM; ++m) vr[m] = *reinterpret_cast<const Codes*>(p + ((size_t)(16 * m) << page_log));
             ks = ksb[(size_t)max(pv, 0) * h_kv];
             vs = vsb[(size_t)max(pv, 0) * h_kv];
         }
+        if (w < kC) {
+            u16x2 mb = max_abs_bits(max_abs_bits(u16x2{0, 0}, raw[0]), raw[1]);
+            uint32_t mu = max((uint32_t)mb[0], (uint32_t)mb[1]);
+            mu = max(mu, (uint32_t)__shfl_xor((int)mu, 16, kWave));
+            mu = max(mu, (uint32_t)__shfl_xor((int)mu, 32, kWave));
+            if (g == 0) lo_qm[w * kSplitRows + n] = mu;
+        }
+        lds_barrier();
+        uint32_t mu = lo_qm[n];
+#pragma unroll
+        for (int c = 1; c < kC; ++c) mu = max(mu, lo_qm[c * kSplitRows + n]);
+        const float qm = __uint_as_float(mu << 16);           // a row that is not finite gets scores that are none
+        const float qc = qm * (1.0f / 32639.0f) * Y.scale2;
+        if (w < kC) {
+            const float inv = qm > 1e-33f ? 32639.0f / qm : 0.0f;
+            uint32_t hi[4] = {0, 0, 0, 0}, lw[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const uint4& p = raw[x / 8];
+                const uint32_t u = (x & 7) / 2 == 0 ? p.x : (x & 7) / 2 == 1 ? p.y : (x & 7) / 2 == 2 ? p.z : p.w;
+                const float v = __uint_as_float(x & 1 ? u & 0xffff0000u : u << 16);
+                const int q = (int)rintf(v * inv), h = (q + 128) >> 8;
+                hi[x / 4] |= (uint32_t)(h & 255) << (8 * (x & 3));
+                lw[x / 4] |= (uint32_t)((q - 256 * h) & 255) << (8 * (x & 3));
+            }
+            lo_q[(2 * w) * kWave + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            lo_q[(2 * w + 1) * kWave + lane] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+        }
+        lds_barrier();
+        v4f acc[kM];
+#pragma unroll
+        for (int m = 0; m < kM; ++m) acc[m] = v4f{0, 0, 0, 0};
+        float mref = -__builtin_inff(), l = 0.0f;
+
         for (; t < t1; t += kSplitWaves) {
             const bool more = t + kSplitWaves < t1;
             const int at = s.tile(t) * kTok;
@@ -415,7 +439,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         }
 #pragma unroll
         for (int m = 0; m < kM; ++m) *reinterpret_cast<v4f*>(lo_o + (w * kSplitRows + n) * kPitch + 16 * m + 4 * g) = acc[m];
-        __syncthreads();
+        lds_barrier();
         const bool whole = t0 == 0 && t1_ == nt;
         const int slot = 2 * blockIdx.x + (piece > 0);
         const Parts<kSplitRows, D> parts(Z.part, gridDim.x);
@@ -444,15 +468,24 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
                 }
             }
         }
-        __syncthreads();                                      // lo_o, lo_ml and lo_q are free again
         left -= t1_ - t0;
+        if (left == 0 && tid == 0) {
+            Cut c{};
+            if (t1_ < nt) {
+                const int w = blockIdx.x, per = taken(w_per), before = (t0 + per - 1) / per;
+                c = Cut{w - before, w + (nt - t1_ + per - 1) / per, before ? 2 * (w - before) + (t0 % per > 0) : slot,
+                        s0, e, r0_, rows_, 1};
+            }
+            parts.cut[blockIdx.x] = c;
+        }
+        lds_barrier();                                      // lo_o, lo_ml and lo_q are free again
         if (t1_ == nt && left > 0) {                         // the next segment: row block, head, sequence
             t0 = 0;
             if (++rb == nrb) {
                 rb = 0;
                 if (++e == Z.c.h_kv) {
                     e = 0;
-                    do s = span_of<kSplitRows, kTok>(Z, ++b);       // left > 0: a sequence with rows follows
+                    do s = span_at<kSplitRows, kTok>(Z, ++b);       // left > 0: a sequence with rows follows
                     while (s.nrb == 0);
                 }
             }
@@ -460,50 +493,61 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     }
 }
 
-// Segments that several workgroups share: the one that lies across the end of workgroup w's tiles, if it
-// began in them. Partial results are joined in the workgroups' order.
+// Segments that several workgroups share. One that lies across n ends of shares has n workgroups here,
+// which take even parts of its outputs (in fours); where those are fewer than the threads, several threads
+// take every so many partial results of an output and are joined in LDS. The order of the sums is fixed.
+constexpr int kJoinThreads = 256;
 template <int D>
-__global__ void __launch_bounds__(256) join_kernel(AttnArgs A, int n_wg) {
-    constexpr int kTok = kSplitTok<D>;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), w = blockIdx.x;
-    const Shares sh = shares<kSplitRows, kTok>(A, n_wg, lane);
-    const long long edge = (w + 1) * sh.per;
-    if (edge >= sh.total) return;
-    long long base;
-    const int b = __builtin_amdgcn_readfirstlane(locate<kSplitRows, kTok>(A, edge, lane, &base));
-    const Span s = span_of<kSplitRows, kTok>(A, b);
-    const int seg = (int)((edge - base) / s.nt);
-    const long long from = base + (long long)seg * s.nt;
-    if (from >= edge || from / sh.per != w) return;
-    const int last = (int)((from + s.nt - 1) / sh.per), first_slot = 2 * w + (from > w * sh.per);
-    const int e = seg / s.nrb, r0 = (seg - e * s.nrb) * kSplitRows, rows = s.q * A.G;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg) {
+    __shared__ v4f lo_o[kJoinThreads];
+    __shared__ float lo_m[kJoinThreads], lo_l[kJoinThreads];
     const Parts<kSplitRows, D> parts(A.part, n_wg);
-    for (int i = tid; i < kSplitRows * D / 4; i += 256) {
-        const int row = i / (D / 4), d = i % (D / 4) * 4;
-        if (r0 + row >= rows) break;
+    const Cut c = parts.cut[blockIdx.x];
+    if (!c.any) return;
+    const int n = c.last - c.first, i = blockIdx.x - c.first;
+    const int all = min(kSplitRows, c.rows - c.r0) * (D / 4);
+    const int from = (int)((long long)all * i / n), to = (int)((long long)all * (i + 1) / n);
+    int wide = 1;                                             // outputs at a time
+    while (wide < to - from && wide < kJoinThreads) wide *= 2;
+    const int ways = kJoinThreads / wide, way = threadIdx.x / wide;
+    for (int x0 = from; x0 < to; x0 += wide) {
+        const int x = min(x0 + (int)(threadIdx.x & (wide - 1)), to - 1), row = x / (D / 4), d = x % (D / 4) * 4;
         float top = -__builtin_inff(), total = 0.0f;
         v4f sum = {0, 0, 0, 0};
-        for (int k = w; k <= last; ++k) {
-            const size_t at = (size_t)(k == w ? first_slot : 2 * k) * kSplitRows + row;
-            const float m = parts.ml[2 * at], lk = parts.ml[2 * at + 1];
-            const v4f o = *reinterpret_cast<const v4f*>(parts.o + at * D + d);
+        const auto add = [&](float m, float l, const v4f& o) {
             const float now = fmaxf(top, m);
             const float f = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - now);
-            const float fk = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
-            total = fmaf(lk, fk, total * f);
-            sum = sum * f + o * fk;
+            const float g = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+            total = fmaf(l, g, total * f);
+            sum = sum * f + o * g;
             top = now;
+        };
+#pragma unroll 4
+        for (int k = c.first + way; k <= c.last; k += ways) {
+            const size_t at = (size_t)(k == c.first ? c.slot : 2 * k) * kSplitRows + row;
+            add(parts.ml[2 * at], parts.ml[2 * at + 1], *reinterpret_cast<const v4f*>(parts.o + at * D + d));
         }
-        const int token = (r0 + row) / A.G;
-        store_out(A, s.s0 + token, e * A.G + r0 + row - token * A.G, d, sum * (total == 0.0f ? 0.0f : 1.0f / total));
+        for (int half = ways / 2; half > 0; half /= 2) {
+            lo_o[threadIdx.x] = sum;
+            lo_m[threadIdx.x] = top;
+            lo_l[threadIdx.x] = total;
+            __syncthreads();
+            const int other = threadIdx.x + half * wide;
+            if (way < half) add(lo_m[other], lo_l[other], lo_o[other]);
+            __syncthreads();
+        }
+        if (way == 0 && x0 + (int)threadIdx.x < to) {
+            const int token = (c.r0 + row) / A.G;
+            store_out(A, c.row + token, c.e * A.G + c.r0 + row - token * A.G, d, sum * (total == 0.0f ? 0.0f : 1.0f / total));
+        }
     }
 }
 
 template <int D>
 void launch_split(const AttnArgs& A, int n_wg, hipStream_t s) {
-    const unsigned lds = (kSplitWaves * kSplitRows * (D + 4 + 2) + kSplitRows) * sizeof(float) + D / 64 * 2 * kWave * sizeof(uint4);
+    const unsigned lds = kSplitWaves * kSplitRows * (D + 4 + 2 + 1) * sizeof(float) + D / 64 * 2 * kWave * sizeof(uint4);
     hipLaunchKernelGGL((split_kernel<D>), dim3((unsigned)n_wg), dim3(kSplitThreads), lds, s, A);
-    if (n_wg > 1) hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)n_wg - 1), dim3(256), 0, s, A, n_wg);
+    if (n_wg > 1) hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)n_wg - 1), dim3(kJoinThreads), 0, s, A, n_wg);
 }
 
 size_t parts_bytes(int d, int n_wg) {
@@ -547,14 +591,11 @@ hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, c
     if (total_T == 0) return hipSuccess;
     A.q = q->p;
     A.q_stride = q->stride;
-    A.q_wide = rows_wide(q);
     if (gate) {
         A.gate = gate->p;
         A.gate_stride = gate->stride;
-        A.gate_wide = rows_wide(gate);
     }
     A.o = o;
-    A.o_wide = ptr_aligned(o, 8);
     A.part = static_cast<float*>(workspace);
     A.scale2 = scale * kLog2e;
     A.h_q = h_q;

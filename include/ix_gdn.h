@@ -424,8 +424,7 @@ size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, i
  * Positions up to 2^30. Scores are formed from 16-bit fixed-point q (of each row's largest
  * value) and the codes, exactly, softmax sums in fp32, p in fp16 of its running maximum for
  * the product with the codes of v. Scales that are not finite in
- * hidden places do not matter. q and gate with strides that are multiples of 8 at
- * 16-byte aligned rows are faster. The call may be captured into a HIP graph, and kv_len, table
+ * hidden places do not matter. The call may be captured into a HIP graph, and kv_len, table
  * and the rest of the device data may change between its replays. */
 hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens,
                        const int32_t* kv_len, const int32_t* table, int width, const ix_rows* q, int h_q, float scale,
