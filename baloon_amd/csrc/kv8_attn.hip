@@ -29,6 +29,7 @@ struct AttnArgs {
     float* part;              // partial results, see Parts
     float scale2;             // scale * log2(e)
     int h_q, G, window, sinks;
+    int small;                // sequences of more (token, head) rows a kv head than this are block_kernel's
 };
 
 // The kernel's argument (its only one) read from memory again where it is used next: keeping all of it in
@@ -71,6 +72,21 @@ __device__ __forceinline__ uint4 load_row8(const uint16_t* p) {
     return x;
 }
 
+// 16 bf16 values (a, b) times inv as 16-bit integers 256 hi + lo of two int8: hi in a, lo in b.
+__device__ __forceinline__ void split_q(uint4& a, uint4& b, float inv) {
+    const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+        const float v = __uint_as_float(x & 1 ? u[x / 2] & 0xffff0000u : u[x / 2] << 16);
+        const int q = (int)rintf(v * inv), h = (q + 128) >> 8;
+        hi[x / 4] |= (uint32_t)(h & 255) << (8 * (x & 3));
+        lo[x / 4] |= (uint32_t)((q - 256 * h) & 255) << (8 * (x & 3));
+    }
+    a = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    b = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+
 // What the rows of one sequence see together: `ns` tiles of sinks and those from `lo` on.
 struct Span {
     int s0, q, kv, first;     // rows s0 .. s0 + q - 1, at positions first ..
@@ -81,9 +97,9 @@ template <int ROWS, int TOK>
 __device__ __forceinline__ Span span_of(const AttnArgs& A, int s0, int q, int kv) {
     Span s;
     s.s0 = s0;
-    s.q = q;
+    s.q = (long long)q * A.G <= A.small ? q : 0;
     s.kv = kv;
-    s.first = s.kv - s.q;
+    s.first = s.kv - q;
     s.lo = A.window > 0 ? max(s.first - A.window + 1, 0) / TOK : 0;
     s.ns = A.window > 0 ? min(A.sinks / TOK + (A.sinks % TOK != 0), s.lo) : 0;
     s.nt = max(s.ns + s.kv / TOK + (s.kv % TOK != 0) - s.lo, 1);
@@ -203,15 +219,20 @@ __device__ __forceinline__ f16x8 halves8(uint32_t a, uint32_t b) {
     return f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
 }
 
+// sigmoid for a bf16 result: v_exp and v_rcp are within an ulp of 32 bits.
+__device__ __forceinline__ float sigmoid_16(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -kLog2e));
+}
+
 // Writes 4 outputs of a row, gated.
 __device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d, v4f v) {
     if (A.gate) {
         uint2 z;
         __builtin_memcpy(&z, A.gate + (long long)t * A.gate_stride + (size_t)h * A.c.d + d, sizeof(z));
-        v[0] *= sigmoid_f(__uint_as_float(z.x << 16));
-        v[1] *= sigmoid_f(__uint_as_float(z.x & 0xffff0000u));
-        v[2] *= sigmoid_f(__uint_as_float(z.y << 16));
-        v[3] *= sigmoid_f(__uint_as_float(z.y & 0xffff0000u));
+        v[0] *= sigmoid_16(__uint_as_float(z.x << 16));
+        v[1] *= sigmoid_16(__uint_as_float(z.x & 0xffff0000u));
+        v[2] *= sigmoid_16(__uint_as_float(z.y << 16));
+        v[3] *= sigmoid_16(__uint_as_float(z.y & 0xffff0000u));
     }
     const uint2 y = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
     __builtin_memcpy(A.o + ((size_t)t * A.h_q + h) * A.c.d + d, &y, sizeof(y));
@@ -332,18 +353,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         const float qc = qm * (1.0f / 32639.0f) * Y.scale2;
         if (w < kC) {
             const float inv = qm > 1e-33f ? 32639.0f / qm : 0.0f;
-            uint32_t hi[4] = {0, 0, 0, 0}, lw[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const uint4& p = raw[x / 8];
-                const uint32_t u = (x & 7) / 2 == 0 ? p.x : (x & 7) / 2 == 1 ? p.y : (x & 7) / 2 == 2 ? p.z : p.w;
-                const float v = __uint_as_float(x & 1 ? u & 0xffff0000u : u << 16);
-                const int q = (int)rintf(v * inv), h = (q + 128) >> 8;
-                hi[x / 4] |= (uint32_t)(h & 255) << (8 * (x & 3));
-                lw[x / 4] |= (uint32_t)((q - 256 * h) & 255) << (8 * (x & 3));
-            }
-            lo_q[(2 * w) * kWave + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            lo_q[(2 * w + 1) * kWave + lane] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+            split_q(raw[0], raw[1], inv);
+            lo_q[(2 * w) * kWave + lane] = raw[0];
+            lo_q[(2 * w + 1) * kWave + lane] = raw[1];
         }
         lds_barrier();
         v4f acc[kM];
@@ -543,11 +555,346 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg
     }
 }
 
+// Blocks of rows: prompts.
+//
+// A workgroup of 8 waves takes 256 (token, head) rows of one sequence and kv head, 32 a wave, and the tiles of
+// 64 tokens that they see one after another through LDS: keys as codes, values as fp16 (converted once for the
+// 256 rows), each 16-byte chunk at a place that 8 consecutive lanes read without a conflict. The products are
+// split_kernel's on the 32 x 32 shapes: S^T = K Q^T in int8 (q in two halves), O^T += V^T P^T in fp16, P where
+// the first product left it, because row 16 s + 8 a + 4 h + b of a key product is token 16 s + 8 h + 4 a + b.
+constexpr int kBlockThreads = 512, kBlockRows = 256, kBlockTok = 64;
+
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ int swap23(int t) { return (t & ~12) | ((t & 4) << 1) | ((t & 8) >> 1); }
+
+// LDS of block_kernel, two buffers of each: keys [64 tokens][D], values [D][64 tokens] fp16, and of each 16
+// tokens ks, log2 vs and 1 / vs.
 template <int D>
-void launch_split(const AttnArgs& A, int n_wg, hipStream_t s) {
+struct BlockLds {
+    static constexpr int kChunks = D / 16;                    // of a token's keys
+    static constexpr int kK = kBlockTok * D, kV = 2 * kBlockTok * D, kS = kBlockTok / 16 * 16;
+    static constexpr int kVAt = 2 * kK, kSAt = kVAt + 2 * kV, kQAt = kSAt + 2 * kS;
+    static constexpr int kQl = D == 256 ? 2 : D / 32, kBytes = kQAt + 8 * (D / 32 - kQl) * kWave * 16;
+    // Byte offset of 16-byte chunk c of token t's keys, and of chunk c (8 tokens) of channel d's values: both are
+    // what they are for c = 0, xor 16 c. A 16-byte read takes 16 lanes at a time over 256 bytes of banks, lanes
+    // 0-3, 12-15, 20-23, 24-27 and the others of a half wave: these put the chunks of each such set at different places.
+    static __device__ __forceinline__ int k_at(int t, int c) {
+        const int r = swap23(t);                              // the lane that reads it
+        return t * D + ((c ^ (D == 64 ? (r >> 2) & 3 : D == 128 ? (r >> 1) & 7 : r & 15)) << 4);
+    }
+    static __device__ __forceinline__ int v_at(int d, int c) { return kVAt + d * 128 + ((c ^ ((d >> 1) & 7)) << 4); }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kBlockThreads, 2) block_kernel(AttnArgs A) {
+    constexpr int kC = D / 32, kM = D / 32, kUnits = kBlockTok * D / 16, kPer = (kUnits + kBlockThreads - 1) / kBlockThreads;
+    typedef BlockLds<D> Lds;
+    constexpr int kQl = Lds::kQl, kSubs = D == 256 ? 1 : 2;   // 32-token products at a time
+    extern __shared__ __align__(16) uint8_t block_lds[];
+    uint8_t* lds = block_lds;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int n = lane & 31, h = lane >> 5;
+
+    // Block j of the grid, from the last: of the causal blocks the longest start first. Sequence b owns the
+    // blocks from cu[b] G / 256 + b on; consecutive workgroups, which different XCDs take, are different heads.
+    const int e = blockIdx.x % A.c.h_kv, j = gridDim.x / A.c.h_kv - 1 - blockIdx.x / A.c.h_kv;
+    const auto key = [&](int b) { return (int)((long long)A.a.start(b) * A.G / kBlockRows) + b; };
+    const int b = wave_search(A.a.n_seq, j, lane, key);
+    const int s0 = A.a.start(b), q = A.a.start(b + 1) - s0, r0 = (j - key(b)) * kBlockRows, rows = max(q, 0) * A.G;
+    if (rows <= A.small || r0 >= rows) return;
+    const int kv = max(A.a.kv_len[b], 0), first = kv - q;
+
+    // q of row n of the wave, channels 32 c + 16 h .. + 15
+    const int r = r0 + 32 * w + n;
+    uint4 qh[kC], ql[kC];                                     // of ql, the registers hold kQl chunks and LDS the others
+    float qc;
+    {
+        const int rc = min(r, rows - 1), qi = rc / A.G;
+        const uint16_t* qp = A.q + (long long)(s0 + qi) * A.q_stride + (size_t)(e * A.G + rc - qi * A.G) * D + 16 * h;
+        u16x2 mb = {0, 0};
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            qh[c] = load_row8(qp + 32 * c);
+            ql[c] = load_row8(qp + 32 * c + 8);
+            mb = max_abs_bits(max_abs_bits(mb, qh[c]), ql[c]);
+        }
+        uint32_t mu = max((uint32_t)mb[0], (uint32_t)mb[1]);
+        mu = max(mu, (uint32_t)__shfl_xor((int)mu, 32, kWave));
+        const float m = __uint_as_float(mu << 16), inv = m > 1e-33f ? 32639.0f / m : 0.0f;
+        qc = m * (1.0f / 32639.0f) * A.scale2;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            split_q(qh[c], ql[c], inv);
+            if (c >= kQl) *reinterpret_cast<uint4*>(lds + Lds::kQAt + ((w * (kC - kQl) + c - kQl) * kWave + lane) * 16) = ql[c];
+        }
+    }
+    const int pos = r < rows ? first + r / A.G : -1;
+    // Of the wave's positions wave_first .. wave_last: tokens from full_lo to full_hi start products that every row
+    // sees as a whole, those below some_lo (the sinks aside) and above wave_last ones that none does.
+    const int wave_first = first + min(r0 + 32 * w, rows - 1) / A.G, wave_last = first + (min(r0 + 32 * w + 32, rows) - 1) / A.G;
+    const int full_hi = wave_first - 32 * kSubs + 1, full_lo = A.window > 0 ? wave_last - A.window + 1 : 0;
+    const int some_lo = A.window > 0 ? wave_first - A.window + 1 - 32 * kSubs + 1 : 0;
+
+    // the block's tiles
+    const int block_first = first + r0 / A.G, block_last = first + (min(r0 + kBlockRows, rows) - 1) / A.G;
+    const int lo = A.window > 0 ? max(block_first - A.window + 1, 0) / kBlockTok : 0;
+    const int ns = A.window > 0 ? min(A.sinks / kBlockTok + (A.sinks % kBlockTok != 0), lo) : 0;
+    const int nt = block_last < 0 ? 0 : ns + block_last / kBlockTok + 1 - lo;
+    const auto tile = [&](int t) { return (t < ns ? t : lo + t - ns) * kBlockTok; };
+
+    // A thread copies kPer chunks of keys and as many of values (16 tokens of a channel): those of one wave
+    // instruction are in one page. Places are worked out anew for each tile: there are no registers to keep them.
+    const int page_log = A.c.page_log, gpp_log = min(page_log, 6) - 4;      // 16 tokens in a tile's page
+    const int32_t* tab = A.a.table + (size_t)b * A.a.width;
+    const int kv_held = (int)min((long long)kv, (long long)A.a.width << page_log);
+    // Lane g of 0 .. 3 holds the page of the tile's tokens 16 g .. + 15, loaded a tile ahead of its use.
+    const auto pages = [&](int at) {
+        const int x = at + 16 * (lane & 3);
+        const int id = x < kv_held ? tab[x >> page_log] : -1;
+        return (unsigned)id < (unsigned)A.c.n_pages ? id : -1;
+    };
+    const auto memory = [&](const int8_t* p, int id) {        // this head's of a page
+        return p + (((size_t)max(id, 0) * A.c.h_kv + e) << page_log) * D;
+    };
+    const auto unit = [&](int i) {
+        int u = tid;
+        asm volatile("" : "+v"(u));
+        return u + i * kBlockThreads;
+    };
+    const bool copies = kUnits >= kBlockThreads || w < kUnits / kWave;
+    constexpr bool kTwice = D == 256;                         // keys and values one after the other through the same registers
+    uint4 held[kPer], held_v[kPer];
+    const auto load_k = [&](int at, int ids) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int u = unit(i), t = u / Lds::kChunks, c = u % Lds::kChunks;
+            const int id = __builtin_amdgcn_readlane(ids, (w * kWave + i * kBlockThreads) / Lds::kChunks / 16 & 3);
+            if (copies)
+                held[i] = *reinterpret_cast<const uint4*>(memory(A.c.k, id) + (uint32_t)(((at + t) & ((1 << page_log) - 1)) * D + 16 * c));
+        }
+    };
+    const auto store_k = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int u = unit(i), t = u / Lds::kChunks, c = u % Lds::kChunks;
+            if (copies) *reinterpret_cast<uint4*>(lds + buf * Lds::kK + Lds::k_at(t, c)) = held[i];
+        }
+    };
+    // unit u of the values: sub-page u / (D gpp), then channel by channel its 16 tokens
+    const auto place_v = [&](int u, int& d, int& g) {
+        const int sp = u >> (gpp_log + (D == 64 ? 6 : D == 128 ? 7 : 8)), x = u & ((D << gpp_log) - 1);
+        d = x >> gpp_log;
+        g = (sp << gpp_log) + (x & ((1 << gpp_log) - 1));
+    };
+    int page_v[kPer];
+    const auto pages_v = [&](int ids) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            page_v[i] = __builtin_amdgcn_readlane(ids, (w * kWave + i * kBlockThreads) >> (gpp_log + (D == 64 ? 6 : D == 128 ? 7 : 8)) << gpp_log & 3);
+    };
+    const auto load_v = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            int d, g;
+            place_v(unit(i), d, g);
+            if (copies)
+                (kTwice ? held : held_v)[i] = *reinterpret_cast<const uint4*>(memory(A.c.v, page_v[i]) + (uint32_t)((d << page_log) + ((at + 16 * g) & ((1 << page_log) - 1))));
+        }
+    };
+    const auto store_v = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            int d, g;
+            place_v(unit(i), d, g);
+            if (copies) {
+                *reinterpret_cast<f16x8*>(lds + buf * Lds::kV + Lds::v_at(d, 2 * g)) = halves8((kTwice ? held : held_v)[i].x, (kTwice ? held : held_v)[i].y);
+                *reinterpret_cast<f16x8*>(lds + buf * Lds::kV + Lds::v_at(d, 2 * g + 1)) = halves8((kTwice ? held : held_v)[i].z, (kTwice ? held : held_v)[i].w);
+            }
+        }
+    };
+    // Scales of 16 tokens by one thread each. A lost page's tokens get the logarithm of 0.
+    float ks = 0.0f, vs = 0.0f;
+    const auto load_scale = [&](int ids) {
+        if (tid < kBlockTok / 16) {
+            ks = A.c.k_scale[(size_t)max(ids, 0) * A.c.h_kv + e];
+            vs = A.c.v_scale[(size_t)max(ids, 0) * A.c.h_kv + e];
+            if (ids < 0) vs = -1.0f;                          // no scale is negative
+        }
+    };
+    const auto store_scale = [&](int buf) {
+        if (tid < kBlockTok / 16) {
+            const v4f s = {vs < 0.0f ? 0.0f : ks, vs < 0.0f ? -__builtin_inff() : vs == 0.0f ? 0.0f : log2f(vs),
+                           vs > 0.0f && vs < __builtin_inff() ? 1.0f / vs : 1.0f, 0.0f};
+            *reinterpret_cast<v4f*>(lds + Lds::kSAt + buf * Lds::kS + 16 * tid) = s;
+        }
+    };
+    const int k0 = Lds::k_at(swap23(n), h), v0 = Lds::v_at(n, h);
+
+    f32x16 acc[kM];
+#pragma unroll
+    for (int m = 0; m < kM; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[m][i] = 0.0f;
+    // p is taken relative to 2^ref; a lane whose row gets a score over `limit` of it moves ref to that score.
+    float ref = 0.0f, limit = -__builtin_inff(), l = 0.0f;
+
+    int ids = pages(tile(0));
+    if (nt > 0) {
+        load_k(tile(0), ids);
+        store_k(0);
+        pages_v(ids);
+        load_v(tile(0));
+        load_scale(ids);
+        store_v(0);
+        store_scale(0);
+    }
+    ids = pages(tile(min(1, max(nt - 1, 0))));
+    lds_barrier();
+    for (int t = 0; t < nt; ++t) {
+        const int buf = t & 1, at0 = tile(t), next = tile(min(t + 1, nt - 1));
+        const int kt = buf * Lds::kK + k0, vt = buf * Lds::kV + v0;      // bits 4 to 7 are k0's and v0's
+        load_k(next, ids);
+        pages_v(ids);
+        if (!kTwice) load_v(next);
+        load_scale(ids);
+        ids = pages(tile(min(t + 2, nt - 1)));
+#pragma unroll
+        for (int part = 0; part < 2 / kSubs; ++part) {
+            const int at = at0 + 32 * kSubs * part;
+            if (at <= wave_last && (at >= some_lo || at < A.sinks)) {
+                i32x16 hi[kSubs], lw[kSubs];
+#pragma unroll
+                for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) hi[u][i] = lw[u][i] = 0;
+#pragma unroll
+                for (int c = 0; c < kC; ++c)
+#pragma unroll
+                    for (int u = 0; u < kSubs; ++u) {
+                        const i32x4 k = *reinterpret_cast<const i32x4*>(lds + (kt ^ (32 * c)) + 32 * (kSubs * part + u) * D);
+                        hi[u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, __builtin_bit_cast(i32x4, qh[c]), hi[u], 0, 0, 0);
+                        const i32x4 q1 = c < kQl ? __builtin_bit_cast(i32x4, ql[c < kQl ? c : 0])
+                                                 : *reinterpret_cast<const i32x4*>(lds + Lds::kQAt + ((w * (kC - kQl) + c - kQl) * kWave + lane) * 16);
+                        lw[u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, q1, lw[u], 0, 0, 0);
+                        if (D == 256 && c % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                    }
+                // lane: row n, tokens at + 32 u + 16 s + 8 h + x, of 16 tokens with one pair of scales
+                float p[kSubs][16], iv[kSubs][2], top = -__builtin_inff();
+#pragma unroll
+                for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const v4f sc = *reinterpret_cast<const v4f*>(lds + Lds::kSAt + buf * Lds::kS + 16 * (2 * (kSubs * part + u) + s));
+                        const float cs = qc * sc[0], lv = sc[1] - ref;
+                        iv[u][s] = sc[2];
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) p[u][8 * s + x] = fmaf((float)((hi[u][8 * s + x] << 8) + lw[u][8 * s + x]), cs, lv);
+                    }
+                if (at < full_lo || at > full_hi) {
+#pragma unroll
+                    for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            const int j0 = at + 32 * u + 16 * s + 8 * h;
+                            const int from = A.window > 0 ? pos - A.window + 1 : 0;
+                            const uint32_t seen = low_bits(pos - j0 + 1) & (low_bits(A.sinks - j0) | ~low_bits(from - j0));
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) p[u][8 * s + x] = (seen >> x) & 1 ? p[u][8 * s + x] : -__builtin_inff();
+                        }
+                }
+#pragma unroll
+                for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, p[u][i]);
+                top = pair_max32(top);
+                if (__ballot(top > limit)) {
+                    const float mref = limit == -__builtin_inff() ? limit : ref + kLift;
+                    const float now = fmaxf(mref, top + ref), to = now == -__builtin_inff() ? 0.0f : now - kLift;
+                    const float f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mref - now);
+#pragma unroll
+                    for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) p[u][i] += ref - to;
+                    ref = to;
+                    limit = now == -__builtin_inff() ? now : kLift + kLag;
+                    l *= f;
+#pragma unroll
+                    for (int m = 0; m < kM; ++m)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[m][i] *= f;
+                }
+#pragma unroll
+                for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        f16x2 pf[4];
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            pf[x] = f16x2{(_Float16)__builtin_amdgcn_exp2f(p[u][8 * s + 2 * x]), (_Float16)__builtin_amdgcn_exp2f(p[u][8 * s + 2 * x + 1])};
+                            sum = __builtin_amdgcn_fdot2(pf[x], f16x2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+                        }
+                        l = fmaf(sum, iv[u][s], l);           // of the rounded p, as the values' product
+                        if (D == 256) __builtin_amdgcn_sched_barrier(0);
+                        const f16x8 b = {pf[0][0], pf[0][1], pf[1][0], pf[1][1], pf[2][0], pf[2][1], pf[3][0], pf[3][1]};
+#pragma unroll
+                        for (int m = 0; m < kM; ++m)
+                            acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                                *reinterpret_cast<const f16x8*>(lds + (vt ^ (64 * (kSubs * part + u) + 32 * s)) + 32 * m * 128), b, acc[m], 0, 0, 0);
+                    }
+            }
+            if (kTwice && part == 0) {
+                store_k(buf ^ 1);
+                load_v(next);
+            }
+        }
+        if (!kTwice) store_k(buf ^ 1);
+        store_v(buf ^ 1);
+        store_scale(buf ^ 1);
+        lds_barrier();
+    }
+
+    l = pair_sum32(l);
+    int thread = tid;
+    asm volatile("" : "+v"(thread));                          // worked out again: nothing of it waits in registers
+    const int ro = r0 + 32 * w + (thread & 31), qo = ro / A.G;
+    if (ro < rows) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                store_out(A, s0 + qo, e * A.G + ro - qo * A.G, 32 * m + 2 * i + 4 * (thread >> 5 & 1),
+                          v4f{acc[m][i], acc[m][i + 1], acc[m][i + 2], acc[m][i + 3]} * inv);
+    }
+}
+
+// Sequences of at most kSplitMost rows a kv head are split_kernel's in any case, and so are all where the blocks
+// are fewer than kBlockLeast.
+constexpr int kSplitMost = 64, kBlockLeast = 64;
+
+template <int D>
+hipError_t launch_attn(AttnArgs& A, int max_q, int n_wg, hipStream_t s) {
+    // Blocks of 256 rows where they occupy a quarter of the chip: block_kernel is about four times as fast a
+    // workgroup as split_kernel on the same rows, which spreads over all of it.
+    const long long blocks = ((long long)A.a.T * A.G / kBlockRows + A.a.n_seq) * A.c.h_kv;
+    const long long longest = (long long)max_q * A.G;
+    const bool block = longest > kSplitMost && (long long)A.a.T * A.G / kBlockRows * A.c.h_kv >= kBlockLeast;
+    A.small = block ? kSplitMost : 0x7fffffff;
+    if (block) {
+        static const hipError_t ready =
+            hipFuncSetAttribute(reinterpret_cast<const void*>(&block_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                BlockLds<D>::kBytes);
+        if (ready != hipSuccess) return ready;
+        hipLaunchKernelGGL((block_kernel<D>), dim3((unsigned)blocks), dim3(kBlockThreads), BlockLds<D>::kBytes, s, A);
+        if (A.a.n_seq == 1) return hipGetLastError();         // its only sequence is a long one
+    }
     const unsigned lds = kSplitWaves * kSplitRows * (D + 4 + 2 + 1) * sizeof(float) + D / 64 * 2 * kWave * sizeof(uint4);
     hipLaunchKernelGGL((split_kernel<D>), dim3((unsigned)n_wg), dim3(kSplitThreads), lds, s, A);
     if (n_wg > 1) hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)n_wg - 1), dim3(kJoinThreads), 0, s, A, n_wg);
+    return hipGetLastError();
 }
 
 size_t parts_bytes(int d, int n_wg) {
@@ -604,11 +951,10 @@ hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, c
     A.sinks = sinks;
     const int n_wg = split_groups(s);
     switch (A.c.d) {
-        case 64: launch_split<64>(A, n_wg, s); break;
-        case 128: launch_split<128>(A, n_wg, s); break;
-        default: launch_split<256>(A, n_wg, s); break;
+        case 64: return launch_attn<64>(A, max_q, n_wg, s);
+        case 128: return launch_attn<128>(A, max_q, n_wg, s);
+        default: return launch_attn<256>(A, max_q, n_wg, s);
     }
-    return hipGetLastError();
 }
 
 }  // extern "C"

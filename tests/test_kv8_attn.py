@@ -150,6 +150,55 @@ def test_drafts_and_prompts(d, G):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("G", [1, 3, 8])
+def test_long_prompts(d, page, G):
+    """Batches of enough rows for blocks of 256: prompts from the start and behind cached tokens, of lengths around the
+    blocks', with single tokens and empty sequences among them."""
+    n = 64 * 256 // (8 * G)
+    q = [n // 2 + 5, 1, 0, 256 // G + 1, n // 3, 64, 256 // G, n // 6 + 40]
+    kv = [q[0], 700, 3, q[3] + 200, q[4] + 77, 64, q[6] + 1, q[7] + 1000]
+    Problem(q, kv, page, 8, d, G, seed=G).both(gate=G == 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (100, 3), (300, 200), (64, 0), (2000, 4), (5, 2 ** 31 - 1)])
+def test_long_prompts_in_a_window(d, window, sinks):
+    Problem([900, 3, 700], [900, 2000, 1900], 16, 8, d, 2, seed=window).both(window=window, sinks=sinks)
+    Problem([3000], [3100], 64, 8, 64, 1, seed=sinks % 999, q_std=1.0).both(window=window, sinks=sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_long_prompts_that_see_little(d):
+    """Pages that are gone, tokens before the start, scales that are not numbers in hidden places, and edges of scales and
+    scores, in blocks of 256 rows."""
+    P = Problem([1500, 700, 40], [1400, 720, 30], 16, 8, d, 2, seed=1, spare=8)
+    ref = P.p.ref
+    P.tables[0, 5:9] = [-1, 1 << 30, -7, -1]
+    P.tables[1, :] = -5
+    used = set(P.tables[(P.tables >= 0) & (P.tables < ref.n_pages)].tolist())
+    for i in set(range(ref.n_pages)) - used:
+        for n in "kv":
+            ref.codes[n][i] = -128
+            ref.scale[n][i] = [np.nan, np.inf][i % 2]
+    for n in "kv":
+        ref.codes[n][P.tables[0, 2]] = 0
+        ref.scale[n][P.tables[0, 2]] = 0
+        for p in range(20, 40):
+            ref.scale[n][P.tables[0, p]] *= np.float32(10.0 ** (p % 5 - 3))
+    ref.scale["k"][P.tables[0, 60:]] *= 30
+    P.q[100:200] = 0
+    P.q[300:400, :, 5] *= 50
+    P.q_bits = bf16.from_f32(P.q)
+    P.q = bf16.to_f32(P.q_bits)
+    P.both(gate=True)
+    P.both(scale=-0.05)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (63, 0), (64, 100), (100, 17), (300, 1), (5000, 4), (7, 2 ** 31 - 1),
                                          (2 ** 30, 4)])
 def test_window_and_sinks(d, window, sinks):
@@ -246,7 +295,7 @@ def test_flat_long_context_with_a_sink():
 @pytest.mark.gpu
 def test_rows_not_finite_stay_alone():
     """A query that is not a number spoils its own row only."""
-    for q in (1, 130):
+    for q in (1, 130, 600):
         P = Problem([q, q], [q + 70, q + 9], 16, 2, 128, 8, seed=q)
         clean = P.run()
         P.q[0, 3] = np.nan
@@ -263,8 +312,8 @@ def test_rows_not_finite_stay_alone():
 def test_operands_and_repeats():
     """q and gate as slices of wider rows, of odd strides, o over q; the same bits each time."""
     import torch
-    for q in ([1, 1, 1], [5, 200, 3]):
-        P = Problem(q, [40, 900, 3], 16, 2, 128, 4, seed=4)
+    for q in ([1, 1, 1], [5, 200, 3], [5, 2200, 3]):
+        P = Problem(q, [40, 900 if q[1] < 900 else 2300, 3], 16, 2, 128, 4, seed=4)
         n, d = 8, 128
         want = P.run(gate=True)
         P.check(want, gate=True)
@@ -319,7 +368,7 @@ def test_graph_replays_with_other_lengths():
 def test_offsets_past_32_bits():
     import torch
     n_pages, page, h, d = 700_000, 16, 2, 256
-    P = Problem([1, 2], [40, 300], page, h, d, 4, seed=9)
+    P = Problem([1, 2, 2100], [40, 300, 2200], page, h, d, 4, seed=9)
     big = [torch.empty(n_pages, h, page, d, dtype=torch.int8, device="cuda"), torch.empty(n_pages, h, d, page, dtype=torch.int8, device="cuda")]
     big += [torch.empty(n_pages, h, device="cuda") for _ in "kv"]
     P.upload()
@@ -329,7 +378,7 @@ def test_offsets_past_32_bits():
     a = list(P.args())
     a[0] = bx.kv8_cache(*big)
     a[6] = torch.where(a[6] >= 0, a[6] + (n_pages - m), -1).to(torch.int32)
-    o = torch.empty(3, h * 4, d, dtype=torch.bfloat16, device="cuda")
+    o = torch.empty(P.T, h * 4, d, dtype=torch.bfloat16, device="cuda")
     n = bx.ix_kv8_attn_workspace_size(a[0], *a[1:4], h * 4)
     ws = torch.empty(n, dtype=torch.uint8, device="cuda")
     assert bx.ix_kv8_attn(*a, bf(P.q_bits), h * 4, P.scale, 0, 0, None, o, ws, n) == 0
