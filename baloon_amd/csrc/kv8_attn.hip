@@ -11,6 +11,7 @@ namespace ixg {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -224,11 +225,14 @@ __device__ __forceinline__ float sigmoid_16(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -kLog2e));
 }
 
-// Writes 4 outputs of a row, gated.
-__device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d, v4f v) {
+__device__ __forceinline__ uint2 load_gate(const AttnArgs& A, int t, int h, int d) {
+    uint2 z = make_uint2(0, 0);
+    if (A.gate) __builtin_memcpy(&z, A.gate + (long long)t * A.gate_stride + (size_t)h * A.c.d + d, sizeof(z));
+    return z;
+}
+// Writes 4 outputs of a row, gated by z.
+__device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d, v4f v, uint2 z) {
     if (A.gate) {
-        uint2 z;
-        __builtin_memcpy(&z, A.gate + (long long)t * A.gate_stride + (size_t)h * A.c.d + d, sizeof(z));
         v[0] *= sigmoid_16(__uint_as_float(z.x << 16));
         v[1] *= sigmoid_16(__uint_as_float(z.x & 0xffff0000u));
         v[2] *= sigmoid_16(__uint_as_float(z.y << 16));
@@ -236,6 +240,9 @@ __device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d
     }
     const uint2 y = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
     __builtin_memcpy(A.o + ((size_t)t * A.h_q + h) * A.c.d + d, &y, sizeof(y));
+}
+__device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d, v4f v) {
+    store_out(A, t, h, d, v, load_gate(A, t, h, d));
 }
 
 constexpr int kSplitThreads = 256, kSplitWaves = kSplitThreads / kWave, kSplitRows = 16;
@@ -392,6 +399,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
                 vs = vsb[(size_t)max(pv_next, 0) * h_kv];
             }
             if (at < full_lo || at > full_hi || __ballot(pv_now < 0)) {
+                asm volatile("");                             // a branch: most tiles are seen as a whole
                 // of the lane's tokens j0 + y
                 const int j0 = at + mine;
                 const int last = pv_now < 0 ? -1 : pos - j0;
@@ -557,17 +565,15 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg
 
 // Blocks of rows: prompts.
 //
-// A workgroup of 8 waves takes 256 (token, head) rows of one sequence and kv head, 32 a wave, and the tiles of
-// 64 tokens that they see one after another through LDS: keys as codes, values as fp16 (converted once for the
-// 256 rows), each 16-byte chunk at a place that 8 consecutive lanes read without a conflict. The products are
-// split_kernel's on the 32 x 32 shapes: S^T = K Q^T in int8 (q in two halves), O^T += V^T P^T in fp16, P where
-// the first product left it, because row 16 s + 8 a + 4 h + b of a key product is token 16 s + 8 h + 4 a + b.
-constexpr int kBlockThreads = 512, kBlockRows = 256, kBlockTok = 64;
-
-typedef int i32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-__device__ __forceinline__ int swap23(int t) { return (t & ~12) | ((t & 4) << 1) | ((t & 8) >> 1); }
+// A workgroup of 8 waves takes 128 (token, head) rows of one sequence and kv head, 16 a wave, and the tiles of 64
+// tokens that they see one after another through LDS: keys as codes, values as fp16 (converted once for all the
+// rows). The products are split_kernel's: S^T = K Q^T in int8 (q in two halves), O^T += V^T P^T in fp16, P where
+// the first product left it, because row 4 g + i of key product t is token 16 g + 4 t + i.
+//
+// 256 rows, 32 a wave on the 32 x 32 shapes, read half as much of LDS but took 231 us for a prompt of 4,096 tokens
+// (16 heads over 2 of 256) against 176: it is 256 blocks of 1 to 64 tiles then, one to a CU, and the sums leave no
+// registers to read ahead. At D <= 128 two workgroups share a CU.
+constexpr int kBlockThreads = 512, kBlockTok = 64, kBlockRows = 128;
 
 // LDS of block_kernel, two buffers of each: keys [64 tokens][D], values [D][64 tokens] fp16, and of each 16
 // tokens ks, log2 vs and 1 / vs.
@@ -575,30 +581,37 @@ template <int D>
 struct BlockLds {
     static constexpr int kChunks = D / 16;                    // of a token's keys
     static constexpr int kK = kBlockTok * D, kV = 2 * kBlockTok * D, kS = kBlockTok / 16 * 16;
-    static constexpr int kVAt = 2 * kK, kSAt = kVAt + 2 * kV, kQAt = kSAt + 2 * kS;
-    static constexpr int kQl = D == 256 ? 2 : D / 32, kBytes = kQAt + 8 * (D / 32 - kQl) * kWave * 16;
+    static constexpr int kVAt = 2 * kK, kSAt = kVAt + 2 * kV, kBytes = kSAt + 2 * kS;
     // Byte offset of 16-byte chunk c of token t's keys, and of chunk c (8 tokens) of channel d's values: both are
     // what they are for c = 0, xor 16 c. A 16-byte read takes 16 lanes at a time over 256 bytes of banks, lanes
-    // 0-3, 12-15, 20-23, 24-27 and the others of a half wave: these put the chunks of each such set at different places.
+    // 0-3, 12-15, 20-23, 24-27 and the others of a half wave: these put the chunks of each such set at different places
+    // (with chunks placed for sets of 8 lanes 40% of the LDS cycles were conflicts).
     static __device__ __forceinline__ int k_at(int t, int c) {
-        const int r = swap23(t);                              // the lane that reads it
-        return t * D + ((c ^ (D == 64 ? (r >> 2) & 3 : D == 128 ? (r >> 1) & 7 : r & 15)) << 4);
+        const int r = (t >> 2 & 12) | (t & 3);                // the row of its product
+        return t * D + ((c ^ (D == 64 ? (r >> 2) + 3 & 3 : D == 128 ? r >> 1 : r)) << 4);
     }
-    static __device__ __forceinline__ int v_at(int d, int c) { return kVAt + d * 128 + ((c ^ ((d >> 1) & 7)) << 4); }
+    static __device__ __forceinline__ int v_at(int d, int c) { return kVAt + d * 128 + ((c ^ ((d >> 1) + 6 & 7)) << 4); }
 };
 
+// f of 0 and, if there are two, of 1, as constants.
+template <int N, class F>
+__device__ __forceinline__ void each(F f) {
+    f(std::integral_constant<int, 0>{});
+    if constexpr (N == 2) f(std::integral_constant<int, 1>{});
+}
+
 template <int D>
-__global__ void __launch_bounds__(kBlockThreads, 2) block_kernel(AttnArgs A) {
-    constexpr int kC = D / 32, kM = D / 32, kUnits = kBlockTok * D / 16, kPer = (kUnits + kBlockThreads - 1) / kBlockThreads;
+__global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(AttnArgs A) {
+    constexpr int kC = D / 64, kM = D / 16;
+    constexpr int kUnits = kBlockTok * D / 16, kPer = (kUnits + kBlockThreads - 1) / kBlockThreads;
     typedef BlockLds<D> Lds;
-    constexpr int kQl = Lds::kQl, kSubs = D == 256 ? 1 : 2;   // 32-token products at a time
     extern __shared__ __align__(16) uint8_t block_lds[];
     uint8_t* lds = block_lds;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int n = lane & 31, h = lane >> 5;
+    const int n = lane & 15, g = lane >> 4;
 
     // Block j of the grid, from the last: of the causal blocks the longest start first. Sequence b owns the
-    // blocks from cu[b] G / 256 + b on; consecutive workgroups, which different XCDs take, are different heads.
+    // blocks from cu[b] G / 128 + b on; consecutive workgroups, which different XCDs take, are different heads.
     const int e = blockIdx.x % A.c.h_kv, j = gridDim.x / A.c.h_kv - 1 - blockIdx.x / A.c.h_kv;
     const auto key = [&](int b) { return (int)((long long)A.a.start(b) * A.G / kBlockRows) + b; };
     const int b = wave_search(A.a.n_seq, j, lane, key);
@@ -606,36 +619,35 @@ __global__ void __launch_bounds__(kBlockThreads, 2) block_kernel(AttnArgs A) {
     if (rows <= A.small || r0 >= rows) return;
     const int kv = max(A.a.kv_len[b], 0), first = kv - q;
 
-    // q of row n of the wave, channels 32 c + 16 h .. + 15
-    const int r = r0 + 32 * w + n;
-    uint4 qh[kC], ql[kC];                                     // of ql, the registers hold kQl chunks and LDS the others
+    // q of row n of the wave, channels 64 c + 16 g .. + 15
+    const int w0 = r0 + 16 * w;
+    int pos;                                                  // taken from here, the places of the wave below stay scalar
+    uint4 qh[kC], ql[kC];
     float qc;
     {
-        const int rc = min(r, rows - 1), qi = rc / A.G;
-        const uint16_t* qp = A.q + (long long)(s0 + qi) * A.q_stride + (size_t)(e * A.G + rc - qi * A.G) * D + 16 * h;
+        const int r = w0 + n, rc = min(r, rows - 1), qi = rc / A.G;
+        pos = r < rows ? first + qi : -1;
+        const uint16_t* qp = A.q + (long long)(s0 + qi) * A.q_stride + (size_t)(e * A.G + rc - qi * A.G) * D + 16 * g;
         u16x2 mb = {0, 0};
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
-            qh[c] = load_row8(qp + 32 * c);
-            ql[c] = load_row8(qp + 32 * c + 8);
+            qh[c] = load_row8(qp + 64 * c);
+            ql[c] = load_row8(qp + 64 * c + 8);
             mb = max_abs_bits(max_abs_bits(mb, qh[c]), ql[c]);
         }
         uint32_t mu = max((uint32_t)mb[0], (uint32_t)mb[1]);
+        mu = max(mu, (uint32_t)__shfl_xor((int)mu, 16, kWave));
         mu = max(mu, (uint32_t)__shfl_xor((int)mu, 32, kWave));
         const float m = __uint_as_float(mu << 16), inv = m > 1e-33f ? 32639.0f / m : 0.0f;
         qc = m * (1.0f / 32639.0f) * A.scale2;
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
-            split_q(qh[c], ql[c], inv);
-            if (c >= kQl) *reinterpret_cast<uint4*>(lds + Lds::kQAt + ((w * (kC - kQl) + c - kQl) * kWave + lane) * 16) = ql[c];
-        }
+        for (int c = 0; c < kC; ++c) split_q(qh[c], ql[c], inv);
     }
-    const int pos = r < rows ? first + r / A.G : -1;
-    // Of the wave's positions wave_first .. wave_last: tokens from full_lo to full_hi start products that every row
-    // sees as a whole, those below some_lo (the sinks aside) and above wave_last ones that none does.
-    const int wave_first = first + min(r0 + 32 * w, rows - 1) / A.G, wave_last = first + (min(r0 + 32 * w + 32, rows) - 1) / A.G;
-    const int full_hi = wave_first - 32 * kSubs + 1, full_lo = A.window > 0 ? wave_last - A.window + 1 : 0;
-    const int some_lo = A.window > 0 ? wave_first - A.window + 1 - 32 * kSubs + 1 : 0;
+    // Of the wave's positions wave_first .. wave_last: tiles that start from full_lo to full_hi every row sees as a
+    // whole, those below some_lo (the sinks aside) and above wave_last none does.
+    const int wave_first = first + min(w0, rows - 1) / A.G, wave_last = first + (min(w0 + 16, rows) - 1) / A.G;
+    const int full_hi = wave_first - kBlockTok + 1, full_lo = A.window > 0 ? wave_last - A.window + 1 : 0;
+    const int some_lo = A.window > 0 ? wave_first - A.window + 1 - kBlockTok + 1 : 0;
 
     // the block's tiles
     const int block_first = first + r0 / A.G, block_last = first + (min(r0 + kBlockRows, rows) - 1) / A.G;
@@ -644,9 +656,10 @@ __global__ void __launch_bounds__(kBlockThreads, 2) block_kernel(AttnArgs A) {
     const int nt = block_last < 0 ? 0 : ns + block_last / kBlockTok + 1 - lo;
     const auto tile = [&](int t) { return (t < ns ? t : lo + t - ns) * kBlockTok; };
 
-    // A thread copies kPer chunks of keys and as many of values (16 tokens of a channel): those of one wave
-    // instruction are in one page. Places are worked out anew for each tile: there are no registers to keep them.
-    const int page_log = A.c.page_log, gpp_log = min(page_log, 6) - 4;      // 16 tokens in a tile's page
+    // Copies of a tile: 16-byte pieces 512 i + tid of its keys, token by token, and of its values, page by page
+    // and in a page (or 64 tokens of it) channel by channel. The pieces of one wave's i are in one page.
+    const int page_log = A.c.page_log, part_log = min(page_log, 6);
+    constexpr int kDLog = D == 64 ? 6 : D == 128 ? 7 : 8;
     const int32_t* tab = A.a.table + (size_t)b * A.a.width;
     const int kv_held = (int)min((long long)kv, (long long)A.a.width << page_log);
     // Lane g of 0 .. 3 holds the page of the tile's tokens 16 g .. + 15, loaded a tile ahead of its use.
@@ -658,61 +671,49 @@ __global__ void __launch_bounds__(kBlockThreads, 2) block_kernel(AttnArgs A) {
     const auto memory = [&](const int8_t* p, int id) {        // this head's of a page
         return p + (((size_t)max(id, 0) * A.c.h_kv + e) << page_log) * D;
     };
-    const auto unit = [&](int i) {
-        int u = tid;
-        asm volatile("" : "+v"(u));
-        return u + i * kBlockThreads;
-    };
     const bool copies = kUnits >= kBlockThreads || w < kUnits / kWave;
-    constexpr bool kTwice = D == 256;                         // keys and values one after the other through the same registers
-    uint4 held[kPer], held_v[kPer];
-    const auto load_k = [&](int at, int ids) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int u = unit(i), t = u / Lds::kChunks, c = u % Lds::kChunks;
-            const int id = __builtin_amdgcn_readlane(ids, (w * kWave + i * kBlockThreads) / Lds::kChunks / 16 & 3);
-            if (copies)
-                held[i] = *reinterpret_cast<const uint4*>(memory(A.c.k, id) + (uint32_t)(((at + t) & ((1 << page_log) - 1)) * D + 16 * c));
-        }
+    u32x4 held[kPer], held_v[kPer];
+    const auto pages_of = [&](int ids, int (&page_k)[kPer], int (&page_v)[kPer]) {
+        each<kPer>([&](auto i) {
+            const int first = (w * kWave + i * kBlockThreads) * 16;
+            page_k[i] = __builtin_amdgcn_readlane(ids, first >> (kDLog + 4) & 3);
+            page_v[i] = __builtin_amdgcn_readlane(ids, first >> (kDLog + part_log) << (part_log - 4) & 3);
+        });
+    };
+    const auto load_k = [&](int at, const int (&page_k)[kPer]) {
+        const uint32_t off = (16 * tid) & ((D << part_log) - 1);
+        each<kPer>([&](auto i) {
+            const int8_t* p = memory(A.c.k, page_k[i]) + (at & ((1 << page_log) - 1)) * D + ((i * kBlockThreads * 16) & ((D << part_log) - 1));
+            if (copies) held[i] = *reinterpret_cast<const u32x4*>(p + off);
+        });
     };
     const auto store_k = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int u = unit(i), t = u / Lds::kChunks, c = u % Lds::kChunks;
-            if (copies) *reinterpret_cast<uint4*>(lds + buf * Lds::kK + Lds::k_at(t, c)) = held[i];
-        }
+        const int u = tid, to = Lds::k_at(u / Lds::kChunks, u % Lds::kChunks) + buf * Lds::kK;
+        each<kPer>([&](auto i) {
+            if (copies) *reinterpret_cast<u32x4*>(lds + ((to + i * kBlockThreads * 16) ^ (i * 128))) = held[i];      // 32 tokens on: rows 8 on
+        });
     };
-    // unit u of the values: sub-page u / (D gpp), then channel by channel its 16 tokens
-    const auto place_v = [&](int u, int& d, int& g) {
-        const int sp = u >> (gpp_log + (D == 64 ? 6 : D == 128 ? 7 : 8)), x = u & ((D << gpp_log) - 1);
-        d = x >> gpp_log;
-        g = (sp << gpp_log) + (x & ((1 << gpp_log) - 1));
-    };
-    int page_v[kPer];
-    const auto pages_v = [&](int ids) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            page_v[i] = __builtin_amdgcn_readlane(ids, (w * kWave + i * kBlockThreads) >> (gpp_log + (D == 64 ? 6 : D == 128 ? 7 : 8)) << gpp_log & 3);
-    };
-    const auto load_v = [&](int at) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            int d, g;
-            place_v(unit(i), d, g);
-            if (copies)
-                (kTwice ? held : held_v)[i] = *reinterpret_cast<const uint4*>(memory(A.c.v, page_v[i]) + (uint32_t)((d << page_log) + ((at + 16 * g) & ((1 << page_log) - 1))));
-        }
+    const auto load_v = [&](int at, const int (&page_v)[kPer]) {
+        const uint32_t y = (16 * tid) & ((D << part_log) - 1), off = y + (page_log == 7 ? y & ~63u : 0u);
+        each<kPer>([&](auto i) {
+            const uint32_t step = ((i * kBlockThreads * 16) & ((D << part_log) - 1)) << (page_log - part_log);   // more channels
+            const int8_t* p = memory(A.c.v, page_v[i]) + (at & ((1 << page_log) - 1)) + step;
+            if (copies) held_v[i] = *reinterpret_cast<const u32x4*>(p + off);
+        });
     };
     const auto store_v = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            int d, g;
-            place_v(unit(i), d, g);
+        const uint32_t u = 16 * tid, y = u & ((D << part_log) - 1);
+        const int d = y >> part_log, g = ((u >> (kDLog + part_log)) << (part_log - 4)) + (y >> 4 & ((1 << (part_log - 4)) - 1));
+        const int to = Lds::v_at(d, 2 * g) + buf * Lds::kV;
+        const int more_d = part_log == 6 ? 128 * (kBlockThreads / 4) : 0, more_t = part_log == 6 ? 0 : 64;
+        each<kPer>([&](auto i) {
+            // the second piece: channels 128 on, or tokens 32 on
+            const int at = (to + i * more_d) ^ (i * more_t);
             if (copies) {
-                *reinterpret_cast<f16x8*>(lds + buf * Lds::kV + Lds::v_at(d, 2 * g)) = halves8((kTwice ? held : held_v)[i].x, (kTwice ? held : held_v)[i].y);
-                *reinterpret_cast<f16x8*>(lds + buf * Lds::kV + Lds::v_at(d, 2 * g + 1)) = halves8((kTwice ? held : held_v)[i].z, (kTwice ? held : held_v)[i].w);
+                *reinterpret_cast<f16x8*>(lds + at) = halves8(held_v[i][0], held_v[i][1]);
+                *reinterpret_cast<f16x8*>(lds + (at ^ 16)) = halves8(held_v[i][2], held_v[i][3]);
             }
-        }
+        });
     };
     // Scales of 16 tokens by one thread each. A lost page's tokens get the logarithm of 0.
     float ks = 0.0f, vs = 0.0f;
@@ -730,144 +731,110 @@ __global__ void __launch_bounds__(kBlockThreads, 2) block_kernel(AttnArgs A) {
             *reinterpret_cast<v4f*>(lds + Lds::kSAt + buf * Lds::kS + 16 * tid) = s;
         }
     };
-    const int k0 = Lds::k_at(swap23(n), h), v0 = Lds::v_at(n, h);
+    const int k0 = Lds::k_at((n >> 2) * 16 + (n & 3), g), v0 = Lds::v_at(n, 2 * g);
 
-    f32x16 acc[kM];
+    v4f acc[kM];
 #pragma unroll
-    for (int m = 0; m < kM; ++m)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[m][i] = 0.0f;
+    for (int m = 0; m < kM; ++m) acc[m] = v4f{0, 0, 0, 0};
     // p is taken relative to 2^ref; a lane whose row gets a score over `limit` of it moves ref to that score.
     float ref = 0.0f, limit = -__builtin_inff(), l = 0.0f;
 
-    int ids = pages(tile(0));
+    int ids = pages(tile(0)), page_k[kPer], page_v[kPer];
+    pages_of(ids, page_k, page_v);
     if (nt > 0) {
-        load_k(tile(0), ids);
-        store_k(0);
-        pages_v(ids);
-        load_v(tile(0));
+        load_k(tile(0), page_k);
+        load_v(tile(0), page_v);
         load_scale(ids);
+        store_k(0);
         store_v(0);
         store_scale(0);
     }
     ids = pages(tile(min(1, max(nt - 1, 0))));
     lds_barrier();
     for (int t = 0; t < nt; ++t) {
-        const int buf = t & 1, at0 = tile(t), next = tile(min(t + 1, nt - 1));
+        const int buf = t & 1, at = tile(t), next = tile(min(t + 1, nt - 1));
         const int kt = buf * Lds::kK + k0, vt = buf * Lds::kV + v0;      // bits 4 to 7 are k0's and v0's
-        load_k(next, ids);
-        pages_v(ids);
-        if (!kTwice) load_v(next);
+        pages_of(ids, page_k, page_v);
+        load_k(next, page_k);
+        load_v(next, page_v);
         load_scale(ids);
         ids = pages(tile(min(t + 2, nt - 1)));
+        if (at <= wave_last && (at >= some_lo || at < A.sinks)) {
+            const v4f sc = *reinterpret_cast<const v4f*>(lds + Lds::kSAt + buf * Lds::kS + 16 * g);
+            float p[16], top = -__builtin_inff();             // lane: row n, tokens at + 16 g + y
+            const float cs = qc * sc[0], lv = sc[1] - ref;
 #pragma unroll
-        for (int part = 0; part < 2 / kSubs; ++part) {
-            const int at = at0 + 32 * kSubs * part;
-            if (at <= wave_last && (at >= some_lo || at < A.sinks)) {
-                i32x16 hi[kSubs], lw[kSubs];
+            for (int i = 0; i < 4; ++i) {
+                i32x4 hi = {0, 0, 0, 0}, lw = {0, 0, 0, 0};
 #pragma unroll
-                for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) hi[u][i] = lw[u][i] = 0;
-#pragma unroll
-                for (int c = 0; c < kC; ++c)
-#pragma unroll
-                    for (int u = 0; u < kSubs; ++u) {
-                        const i32x4 k = *reinterpret_cast<const i32x4*>(lds + (kt ^ (32 * c)) + 32 * (kSubs * part + u) * D);
-                        hi[u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, __builtin_bit_cast(i32x4, qh[c]), hi[u], 0, 0, 0);
-                        const i32x4 q1 = c < kQl ? __builtin_bit_cast(i32x4, ql[c < kQl ? c : 0])
-                                                 : *reinterpret_cast<const i32x4*>(lds + Lds::kQAt + ((w * (kC - kQl) + c - kQl) * kWave + lane) * 16);
-                        lw[u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, q1, lw[u], 0, 0, 0);
-                        if (D == 256 && c % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-                    }
-                // lane: row n, tokens at + 32 u + 16 s + 8 h + x, of 16 tokens with one pair of scales
-                float p[kSubs][16], iv[kSubs][2], top = -__builtin_inff();
-#pragma unroll
-                for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const v4f sc = *reinterpret_cast<const v4f*>(lds + Lds::kSAt + buf * Lds::kS + 16 * (2 * (kSubs * part + u) + s));
-                        const float cs = qc * sc[0], lv = sc[1] - ref;
-                        iv[u][s] = sc[2];
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) p[u][8 * s + x] = fmaf((float)((hi[u][8 * s + x] << 8) + lw[u][8 * s + x]), cs, lv);
-                    }
-                if (at < full_lo || at > full_hi) {
-#pragma unroll
-                    for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            const int j0 = at + 32 * u + 16 * s + 8 * h;
-                            const int from = A.window > 0 ? pos - A.window + 1 : 0;
-                            const uint32_t seen = low_bits(pos - j0 + 1) & (low_bits(A.sinks - j0) | ~low_bits(from - j0));
-#pragma unroll
-                            for (int x = 0; x < 8; ++x) p[u][8 * s + x] = (seen >> x) & 1 ? p[u][8 * s + x] : -__builtin_inff();
-                        }
+                for (int c = 0; c < kC; ++c) {
+                    const i32x4 k = *reinterpret_cast<const i32x4*>(lds + (kt ^ (64 * c)) + 4 * i * D);
+                    hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, __builtin_bit_cast(i32x4, qh[c]), hi, 0, 0, 0);
+                    lw = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, __builtin_bit_cast(i32x4, ql[c]), lw, 0, 0, 0);
                 }
 #pragma unroll
-                for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) top = fmaxf(top, p[u][i]);
-                top = pair_max32(top);
-                if (__ballot(top > limit)) {
-                    const float mref = limit == -__builtin_inff() ? limit : ref + kLift;
-                    const float now = fmaxf(mref, top + ref), to = now == -__builtin_inff() ? 0.0f : now - kLift;
-                    const float f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mref - now);
-#pragma unroll
-                    for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) p[u][i] += ref - to;
-                    ref = to;
-                    limit = now == -__builtin_inff() ? now : kLift + kLag;
-                    l *= f;
-#pragma unroll
-                    for (int m = 0; m < kM; ++m)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[m][i] *= f;
-                }
-#pragma unroll
-                for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        f16x2 pf[4];
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            pf[x] = f16x2{(_Float16)__builtin_amdgcn_exp2f(p[u][8 * s + 2 * x]), (_Float16)__builtin_amdgcn_exp2f(p[u][8 * s + 2 * x + 1])};
-                            sum = __builtin_amdgcn_fdot2(pf[x], f16x2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
-                        }
-                        l = fmaf(sum, iv[u][s], l);           // of the rounded p, as the values' product
-                        if (D == 256) __builtin_amdgcn_sched_barrier(0);
-                        const f16x8 b = {pf[0][0], pf[0][1], pf[1][0], pf[1][1], pf[2][0], pf[2][1], pf[3][0], pf[3][1]};
-#pragma unroll
-                        for (int m = 0; m < kM; ++m)
-                            acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                                *reinterpret_cast<const f16x8*>(lds + (vt ^ (64 * (kSubs * part + u) + 32 * s)) + 32 * m * 128), b, acc[m], 0, 0, 0);
-                    }
+                for (int y = 0; y < 4; ++y) p[4 * i + y] = fmaf((float)((hi[y] << 8) + lw[y]), cs, lv);
             }
-            if (kTwice && part == 0) {
-                store_k(buf ^ 1);
-                load_v(next);
+            if (at < full_lo || at > full_hi) {
+                asm volatile("");                             // a branch: most tiles are seen as a whole
+                const int j0 = at + 16 * g, from = A.window > 0 ? pos - A.window + 1 : 0;
+                const uint32_t seen = low_bits(pos - j0 + 1) & (low_bits(A.sinks - j0) | ~low_bits(from - j0));
+#pragma unroll
+                for (int y = 0; y < 16; ++y) p[y] = (seen >> y) & 1 ? p[y] : -__builtin_inff();
             }
+#pragma unroll
+            for (int y = 0; y < 16; ++y) top = fmaxf(top, p[y]);
+            top = pair_max32(pair_max16(top));
+            if (__ballot(top > limit)) {
+                const float mref = limit == -__builtin_inff() ? limit : ref + kLift;
+                const float now = fmaxf(mref, top + ref), to = now == -__builtin_inff() ? 0.0f : now - kLift;
+                const float f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mref - now);
+#pragma unroll
+                for (int y = 0; y < 16; ++y) p[y] += ref - to;
+                ref = to;
+                limit = now == -__builtin_inff() ? now : kLift + kLag;
+                l *= f;
+#pragma unroll
+                for (int m = 0; m < kM; ++m) acc[m] *= f;
+            }
+            f16x8 pf[2];
+            float sum = 0.0f;
+#pragma unroll
+            for (int y = 0; y < 16; y += 2) {
+                const f16x2 two = {(_Float16)__builtin_amdgcn_exp2f(p[y]), (_Float16)__builtin_amdgcn_exp2f(p[y + 1])};
+                sum = __builtin_amdgcn_fdot2(two, f16x2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+                pf[y / 8][y & 7] = two[0];
+                pf[y / 8][(y & 7) + 1] = two[1];
+            }
+            l = fmaf(sum, sc[2], l);                          // of the rounded p, as the values' product
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int m = 0; m < kM; ++m)
+                    acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        *reinterpret_cast<const f16x8*>(lds + (vt ^ (16 * s)) + 16 * m * 128), pf[s], acc[m], 0, 0, 0);
         }
-        if (!kTwice) store_k(buf ^ 1);
+        store_k(buf ^ 1);
         store_v(buf ^ 1);
         store_scale(buf ^ 1);
         lds_barrier();
     }
 
-    l = pair_sum32(l);
+    l = pair_sum32(pair_sum16(l));
     int thread = tid;
-    asm volatile("" : "+v"(thread));                          // worked out again: nothing of it waits in registers
-    const int ro = r0 + 32 * w + (thread & 31), qo = ro / A.G;
-    if (ro < rows) {
+    asm volatile("" : "+v"(thread));                          // the row is worked out again: it does not wait in registers
+    const int r = w0 + (thread & 15), qi = r / A.G, head = e * A.G + r - qi * A.G, d0 = 4 * (thread >> 4 & 3);
+    if (r < rows) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        constexpr int kN = kM < 8 ? kM : 8;                   // pieces of 4 channels, their gates on the way together
 #pragma unroll
-        for (int m = 0; m < kM; ++m)
+        for (int m0 = 0; m0 < kM; m0 += kN) {
+            uint2 z[kN];
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                store_out(A, s0 + qo, e * A.G + ro - qo * A.G, 32 * m + 2 * i + 4 * (thread >> 5 & 1),
-                          v4f{acc[m][i], acc[m][i + 1], acc[m][i + 2], acc[m][i + 3]} * inv);
+            for (int i = 0; i < kN; ++i) z[i] = load_gate(A, s0 + qi, head, 16 * (m0 + i) + d0);
+#pragma unroll
+            for (int i = 0; i < kN; ++i) store_out(A, s0 + qi, head, 16 * (m0 + i) + d0, acc[m0 + i] * inv, z[i]);
+        }
     }
 }
 
@@ -877,11 +844,11 @@ constexpr int kSplitMost = 64, kBlockLeast = 64;
 
 template <int D>
 hipError_t launch_attn(AttnArgs& A, int max_q, int n_wg, hipStream_t s) {
-    // Blocks of 256 rows where they occupy a quarter of the chip: block_kernel is about four times as fast a
+    // Blocks of rows where they occupy a quarter of the chip: block_kernel is about four times as fast a
     // workgroup as split_kernel on the same rows, which spreads over all of it.
-    const long long blocks = ((long long)A.a.T * A.G / kBlockRows + A.a.n_seq) * A.c.h_kv;
+    const long long full = (long long)A.a.T * A.G / kBlockRows * A.c.h_kv, blocks = full + (long long)A.a.n_seq * A.c.h_kv;
     const long long longest = (long long)max_q * A.G;
-    const bool block = longest > kSplitMost && (long long)A.a.T * A.G / kBlockRows * A.c.h_kv >= kBlockLeast;
+    const bool block = longest > kSplitMost && full >= kBlockLeast;
     A.small = block ? kSplitMost : 0x7fffffff;
     if (block) {
         static const hipError_t ready =
