@@ -30,6 +30,7 @@ struct AttnArgs {
     float* part;              // partial results, see Parts
     float scale2;             // scale * log2(e)
     int h_q, G, window, sinks;
+    int narrow;               // the batch has fewer than 2^31 tiles for split_kernel
     int small;                // sequences of more (token, head) rows a kv head than this are block_kernel's
 };
 
@@ -73,16 +74,23 @@ __device__ __forceinline__ uint4 load_row8(const uint16_t* p) {
     return x;
 }
 
-// 16 bf16 values (a, b) times inv as 16-bit integers 256 hi + lo of two int8: hi in a, lo in b.
+// 16 bf16 values (a, b) times inv, at most 32639 of them, as 16-bit integers 256 hi + lo of two int8: hi in a, lo
+// in b. 1.5 2^23 added to a number leaves its nearest integer in the sum's low bits.
 __device__ __forceinline__ void split_q(uint4& a, uint4& b, float inv) {
+    constexpr float kMagic = 12582912.0f;
     const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+    uint32_t hi[4], lo[4], two[2];
 #pragma unroll
-    for (int x = 0; x < 16; ++x) {
-        const float v = __uint_as_float(x & 1 ? u[x / 2] & 0xffff0000u : u[x / 2] << 16);
-        const int q = (int)rintf(v * inv), h = (q + 128) >> 8;
-        hi[x / 4] |= (uint32_t)(h & 255) << (8 * (x & 3));
-        lo[x / 4] |= (uint32_t)((q - 256 * h) & 255) << (8 * (x & 3));
+    for (int x = 0; x < 8; ++x) {
+        const uint32_t q0 = __float_as_uint(fmaf(__uint_as_float(u[x] << 16), inv, kMagic));
+        const uint32_t q1 = __float_as_uint(fmaf(__uint_as_float(u[x] & 0xffff0000u), inv, kMagic));
+        two[x & 1] = __builtin_amdgcn_perm(q1, q0, 0x05040100u);
+        if (x & 1) {
+            lo[x / 2] = __builtin_amdgcn_perm(two[1], two[0], 0x06040200u);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) two[y] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, two[y]) + u16x2{128, 128});
+            hi[x / 2] = __builtin_amdgcn_perm(two[1], two[0], 0x07050301u);
+        }
     }
     a = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     b = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -103,7 +111,8 @@ __device__ __forceinline__ Span span_of(const AttnArgs& A, int s0, int q, int kv
     s.first = s.kv - q;
     s.lo = A.window > 0 ? max(s.first - A.window + 1, 0) / TOK : 0;
     s.ns = A.window > 0 ? min(A.sinks / TOK + (A.sinks % TOK != 0), s.lo) : 0;
-    s.nt = max(s.ns + s.kv / TOK + (s.kv % TOK != 0) - s.lo, 1);
+    const int held = (int)min((long long)kv, (long long)A.a.width << A.c.page_log);      // what the table has places for
+    s.nt = max(s.ns + max(held / TOK + (held % TOK != 0) - s.lo, 0), 1);
     s.nrb = (int)(((long long)s.q * A.G + ROWS - 1) / ROWS);
     return s;
 }
@@ -113,77 +122,88 @@ __device__ __forceinline__ Span span_at(const AttnArgs& A, int b) {
     return span_of<ROWS, TOK>(A, s0, max(A.a.start(b + 1) - s0, 0), max(A.a.kv_len[b], 0));
 }
 
-// Inclusive sum over lanes 0 .. l (the steps of wave_scan on 64-bit integers).
+// Inclusive sum over lanes 0 .. l (the steps of wave_scan), and a lane's value in all, for 32 and 64 bits.
 template <int Ctrl, int RowMask>
-__device__ __forceinline__ long long dpp_add64(long long v) {
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, Ctrl, RowMask, 0xF, RowMask == 0xF);
+}
+template <int Ctrl, int RowMask>
+__device__ __forceinline__ long long dpp_add(long long v) {
     const int lo = __builtin_amdgcn_update_dpp(0, (int)v, Ctrl, RowMask, 0xF, RowMask == 0xF);
     const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), Ctrl, RowMask, 0xF, RowMask == 0xF);
     return v + (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
 }
-__device__ __forceinline__ long long wave_scan64(long long v) {
-    v = dpp_add64<0x111, 0xF>(v);
-    v = dpp_add64<0x112, 0xF>(v);
-    v = dpp_add64<0x114, 0xF>(v);
-    v = dpp_add64<0x118, 0xF>(v);
-    v = dpp_add64<0x142, 0xA>(v);
-    return dpp_add64<0x143, 0xC>(v);
+template <class Int>
+__device__ __forceinline__ Int wave_scan_int(Int v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    return dpp_add<0x143, 0xC>(v);
 }
-__device__ __forceinline__ long long lane_of64(long long v, int l) {
+__device__ __forceinline__ int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+__device__ __forceinline__ long long lane_of(long long v, int l) {
     const unsigned lo = __builtin_amdgcn_readlane((int)v, l), hi = __builtin_amdgcn_readlane((int)(v >> 32), l);
     return (long long)(((unsigned long long)hi << 32) | lo);
 }
-// a / b for 0 <= a < 2^50, through the correctly rounded division in double.
+// a / b for a >= 0: in 64 bits (below 2^50) through the correctly rounded division in double.
+__device__ __forceinline__ int quotient(int a, int b) { return (int)((unsigned)a / (unsigned)b); }
 __device__ __forceinline__ long long quotient(long long a, int b) { return (long long)((double)a / (double)b); }
 
 // The batch's tiles, numbered through over sequences, kv heads, row blocks and tiles, are shared out evenly:
-// workgroup w takes [w per, (w + 1) per). Every wave works its share out by itself from the lengths.
+// workgroup w takes [w per, (w + 1) per). Every wave works its share out by itself from the lengths, in 32 bits where
+// the batch cannot have 2^31 tiles (each launch fetches its instructions anew: 250 of them took 1.3 us).
 constexpr int kMinShare = 4;          // tiles: one for each wave
 struct Share {
     int per, left;                    // tiles of every workgroup, and of this one
     int b, e, rb, t0;                 // where it begins
     Span s;
 };
-template <int ROWS, int TOK>
-__device__ __forceinline__ bool share_of(const AttnArgs& A, int n_wg, int w, int lane, Share* out) {
+template <int ROWS, int TOK, class Int>
+__device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int lane, Share* out) {
     const int n = A.a.n_seq, h_kv = A.c.h_kv;
     const auto chunk = [&](int b0, Span* s) {                // the work of sequence b0 + lane
-        if (b0 + lane >= n) return 0ll;
+        if (b0 + lane >= n) return (Int)0;
         *s = span_at<ROWS, TOK>(A, b0 + lane);
-        return (long long)s->nrb * s->nt * h_kv;
+        return (Int)s->nrb * s->nt * h_kv;
     };
     Span s{};
-    long long v = chunk(0, &s), incl = wave_scan64(v), carry = 0;
-    long long total = lane_of64(incl, kWave - 1);
+    Int v = chunk(0, &s), incl = wave_scan_int(v), carry = 0;
+    Int total = lane_of(incl, kWave - 1);
     if (n > kWave) {
-        long long rest = 0;
+        Int rest = 0;
         Span x;
         for (int b0 = kWave; b0 < n; b0 += kWave) rest += chunk(b0, &x);
-        total += lane_of64(wave_scan64(rest), kWave - 1);
+        total += lane_of(wave_scan_int(rest), kWave - 1);
     }
-    out->per = (int)max(quotient(total + n_wg - 1, n_wg), (long long)kMinShare);
-    const long long cur = (long long)w * out->per;
+    out->per = (int)max(quotient((Int)(total + n_wg - 1), n_wg), (Int)kMinShare);
+    const Int cur = (Int)w * out->per;
     if (cur >= total) return false;
-    out->left = (int)min((long long)out->per, total - cur);
+    out->left = (int)min((Int)out->per, (Int)(total - cur));
     for (int b0 = 0;; b0 += kWave) {
         if (b0) {
             v = chunk(b0, &s);
-            incl = wave_scan64(v);
+            incl = wave_scan_int(v);
         }
         const unsigned long long hit = __ballot(carry + incl > cur);
         if (hit) {
             const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
-            const long long rel = cur - carry - lane_of64(incl - v, l);
+            const Int rel = cur - carry - lane_of((Int)(incl - v), l);
             out->b = b0 + l;
-            out->s = span_of<ROWS, TOK>(A, __builtin_amdgcn_readlane(s.s0, l), __builtin_amdgcn_readlane(s.q, l),
-                                        __builtin_amdgcn_readlane(s.kv, l));
+            out->s = span_of<ROWS, TOK>(A, lane_of(s.s0, l), lane_of(s.q, l), lane_of(s.kv, l));
             const int seg = __builtin_amdgcn_readfirstlane((int)quotient(rel, out->s.nt));
-            out->t0 = __builtin_amdgcn_readfirstlane((int)(rel - (long long)seg * out->s.nt));
-            out->e = seg / out->s.nrb;
+            out->t0 = __builtin_amdgcn_readfirstlane((int)(rel - (Int)seg * out->s.nt));
+            out->e = quotient(seg, out->s.nrb);
             out->rb = seg - out->e * out->s.nrb;
             return true;
         }
-        carry += lane_of64(incl, kWave - 1);
+        carry += lane_of(incl, kWave - 1);
     }
+}
+template <int ROWS, int TOK>
+__device__ __forceinline__ bool share_of(const AttnArgs& A, int n_wg, int w, int lane, Share* out) {
+    return A.narrow ? share_in<ROWS, TOK, int>(A, n_wg, w, lane, out) : share_in<ROWS, TOK, long long>(A, n_wg, w, lane, out);
 }
 
 // Partial results: workgroup w leaves that of the segment it starts in the middle of (or cuts at both
@@ -289,6 +309,15 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         const int w_left = parked(left), w_e = parked(e), w_rb = parked(rb), w_b = parked(b), w_s0 = parked(s.s0),
                   w_nrb = parked(s.nrb), w_nt = parked(s.nt), w_rows = parked(rows), w_t0 = parked(t0), w_t1 = parked(t1),
                   w_piece = parked(piece);
+        // q as two int8 of 16 bits: wave c takes channels 64 c + 16 g .. + 15 of every row (row n its lanes')
+        uint4 raw[2];
+        if (w < kC) {
+            const AttnArgs& Z = args_again();
+            const int rc = min(r0 + n, rows - 1), qi = rc / Z.G;
+            const uint16_t* qp = Z.q + (long long)(s.s0 + qi) * Z.q_stride + (size_t)(e * Z.G + rc - qi * Z.G) * D + 64 * w + 16 * g;
+            raw[0] = load_row8(qp);
+            raw[1] = load_row8(qp + 8);
+        }
         const AttnArgs& Y = args_again();
         const int page_log = Y.c.page_log, window = Y.window, sinks = Y.sinks;
         const int pos = r0 + n < rows ? s.first + (r0 + n) / Y.G : -1;
@@ -327,15 +356,6 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
 
         int t = t0 + w;
         int pk = page_of(t, keys), pv = page_of(t, mine), pk_next = page_of(t + kSplitWaves, keys), pv_next = page_of(t + kSplitWaves, mine);
-        // q as two int8 of 16 bits: wave c takes channels 64 c + 16 g .. + 15 of every row (row n its lanes')
-        uint4 raw[2];
-        if (w < kC) {
-            const AttnArgs& Z = args_again();
-            const int rc = min(r0 + n, rows - 1), qi = rc / Z.G;
-            const uint16_t* qp = Z.q + (long long)(s.s0 + qi) * Z.q_stride + (size_t)(e * Z.G + rc - qi * Z.G) * D + 64 * w + 16 * g;
-            raw[0] = load_row8(qp);
-            raw[1] = load_row8(qp + 8);
-        }
         float ks = 0.0f, vs = 0.0f;
         if (t < t1) {
             load_k(t, pk);
@@ -850,6 +870,10 @@ hipError_t launch_attn(AttnArgs& A, int max_q, int n_wg, hipStream_t s) {
     const long long longest = (long long)max_q * A.G;
     const bool block = longest > kSplitMost && full >= kBlockLeast;
     A.small = block ? kSplitMost : 0x7fffffff;
+    // tiles: at most those of a whole table for each block of rows, and n_wg - 1 and a workgroup's share more in sums
+    const long long row_blocks = (long long)A.a.T * A.G / kSplitRows + A.a.n_seq;
+    const long long tiles = ((long long)A.a.width << A.c.page_log) / kSplitTok<D> + 1;
+    A.narrow = row_blocks < (1ll << 31) / tiles / A.c.h_kv / 2 - n_wg;
     if (block) {
         static const hipError_t ready =
             hipFuncSetAttribute(reinterpret_cast<const void*>(&block_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize,
