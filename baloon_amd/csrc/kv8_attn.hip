@@ -152,48 +152,54 @@ __device__ __forceinline__ int quotient(int a, int b) { return (int)((unsigned)a
 __device__ __forceinline__ long long quotient(long long a, int b) { return (long long)((double)a / (double)b); }
 
 // The batch's tiles, numbered through over sequences, kv heads, row blocks and tiles, are shared out evenly:
-// workgroup w takes [w per, (w + 1) per). Every wave works its share out by itself from the lengths, in 32 bits where
-// the batch cannot have 2^31 tiles (each launch fetches its instructions anew: 250 of them took 1.3 us).
+// workgroup w takes [w per, (w + 1) per). In front of each segment's tiles `start` more are counted for what a
+// workgroup does to begin one, where the shares are long enough for it to matter (37 sequences of 8 kv heads, 296
+// segments over 512 workgroups, took 52 us without and 40 with 3 or 6). Every wave works its share out by itself from the
+// lengths, in 32 bits where the batch cannot have 2^31 tiles (each launch fetches its instructions anew: 250 of them
+// took 1.3 us).
 constexpr int kMinShare = 4;          // tiles: one for each wave
+constexpr int kStart = 6;             // tiles of 16 KiB in the time of a segment's start
 struct Share {
-    int per, left;                    // tiles of every workgroup, and of this one
-    int b, e, rb, t0;                 // where it begins
+    int per, left, start;             // counts of every workgroup and of this one, and in front of a segment
+    int b, e, rb, v0;                 // where it begins: count v0 of a segment
     Span s;
 };
 template <int ROWS, int TOK, class Int>
 __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int lane, Share* out) {
     const int n = A.a.n_seq, h_kv = A.c.h_kv;
-    const auto chunk = [&](int b0, Span* s) {                // the work of sequence b0 + lane
-        if (b0 + lane >= n) return (Int)0;
-        *s = span_at<ROWS, TOK>(A, b0 + lane);
-        return (Int)s->nrb * s->nt * h_kv;
-    };
     Span s{};
-    Int v = chunk(0, &s), incl = wave_scan_int(v), carry = 0;
-    Int total = lane_of(incl, kWave - 1);
-    if (n > kWave) {
-        Int rest = 0;
-        Span x;
-        for (int b0 = kWave; b0 < n; b0 += kWave) rest += chunk(b0, &x);
-        total += lane_of(wave_scan_int(rest), kWave - 1);
+    const auto span = [&](int b0) {                          // of sequence b0 + lane; no rows behind the last
+        s.nrb = 0;
+        if (b0 + lane < n) s = span_at<ROWS, TOK>(A, b0 + lane);
+    };
+    Int tiles = 0, segments = 0;
+    for (int b0 = (n - 1) & ~(kWave - 1); b0 >= 0; b0 -= kWave) {
+        span(b0);
+        tiles += (Int)s.nrb * s.nt * h_kv;
+        segments += (Int)s.nrb * h_kv;
     }
+    tiles = lane_of(wave_scan_int(tiles), kWave - 1);
+    segments = lane_of(wave_scan_int(segments), kWave - 1);
+    int start = (int)min((Int)kStart, quotient(tiles, 2 * n_wg));
+    if (segments * start < n_wg) start = 0;                   // less than a tile for each
+    const Int total = tiles + segments * start;
+    out->start = start;
     out->per = (int)max(quotient((Int)(total + n_wg - 1), n_wg), (Int)kMinShare);
     const Int cur = (Int)w * out->per;
     if (cur >= total) return false;
     out->left = (int)min((Int)out->per, (Int)(total - cur));
+    Int carry = 0;
     for (int b0 = 0;; b0 += kWave) {
-        if (b0) {
-            v = chunk(b0, &s);
-            incl = wave_scan_int(v);
-        }
+        if (b0) span(b0);
+        const Int v = (Int)s.nrb * (s.nt + start) * h_kv, incl = wave_scan_int(v);
         const unsigned long long hit = __ballot(carry + incl > cur);
         if (hit) {
             const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
             const Int rel = cur - carry - lane_of((Int)(incl - v), l);
             out->b = b0 + l;
             out->s = span_of<ROWS, TOK>(A, lane_of(s.s0, l), lane_of(s.q, l), lane_of(s.kv, l));
-            const int seg = __builtin_amdgcn_readfirstlane((int)quotient(rel, out->s.nt));
-            out->t0 = __builtin_amdgcn_readfirstlane((int)(rel - (Int)seg * out->s.nt));
+            const int seg = __builtin_amdgcn_readfirstlane((int)quotient(rel, out->s.nt + start));
+            out->v0 = __builtin_amdgcn_readfirstlane((int)(rel - (Int)seg * (out->s.nt + start)));
             out->e = quotient(seg, out->s.nrb);
             out->rb = seg - out->e * out->s.nrb;
             return true;
@@ -293,7 +299,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     uint4* lo_q = reinterpret_cast<uint4*>(lo_qm + kSplitWaves * kSplitRows);               // [kC][hi, lo][lane]
     const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int n = lane & 15, g = lane >> 4, mine = 4 * kS * g, keys = 4 * kS * (n >> 2);
-    int b, e, rb, t0, left, w_per;
+    int b, e, rb, v0, left, w_per, start;
     Span s;
     {
         const AttnArgs& Z = args_again();
@@ -302,30 +308,29 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             if (tid == 0) Parts<kSplitRows, D>(Z.part, gridDim.x).cut[blockIdx.x].any = 0;
             return;
         }
-        b = sh.b, e = sh.e, rb = sh.rb, t0 = sh.t0, left = sh.left, w_per = parked(sh.per), s = sh.s;
+        b = sh.b, e = sh.e, rb = sh.rb, v0 = sh.v0, left = sh.left, w_per = parked(sh.per), start = sh.start, s = sh.s;
     }
-    for (int piece = 0; left > 0; ++piece) {
-        const int t1 = min(s.nt, t0 + left), r0 = rb * kSplitRows, rows = s.q * args_again().G;
-        const int w_left = parked(left), w_e = parked(e), w_rb = parked(rb), w_b = parked(b), w_s0 = parked(s.s0),
-                  w_nrb = parked(s.nrb), w_nt = parked(s.nt), w_rows = parked(rows), w_t0 = parked(t0), w_t1 = parked(t1),
-                  w_piece = parked(piece);
-        // q as two int8 of 16 bits: wave c takes channels 64 c + 16 g .. + 15 of every row (row n its lanes')
-        uint4 raw[2];
-        if (w < kC) {
-            const AttnArgs& Z = args_again();
-            const int rc = min(r0 + n, rows - 1), qi = rc / Z.G;
-            const uint16_t* qp = Z.q + (long long)(s.s0 + qi) * Z.q_stride + (size_t)(e * Z.G + rc - qi * Z.G) * D + 64 * w + 16 * g;
-            raw[0] = load_row8(qp);
-            raw[1] = load_row8(qp + 8);
+
+    // The sums of a piece (the part of a segment in this share), for rows n: of 2^(kLift - mref) p v / vs, and of p.
+    v4f acc[kM];
+    float mref, l;
+    // What is left to do for the piece whose sums these are, in vector registers: the main loop needs the scalar ones.
+    int o_e = 0, o_r0 = 0, o_rows = 0, o_s0 = 0, o_slot = 0;        // o_slot -1: the whole segment
+    bool open = false;
+    int pieces = 0;
+    Cut cut{};
+    for (;;) {
+        // The next piece, whose first loads are on their way while the last one's waves are joined.
+        int t0 = 0, t1 = 0;
+        if (left > 0) {
+            t0 = max(v0 - start, 0);
+            t1 = min(s.nt, t0 + left - max(start - v0, 0));         // t1 <= t0: only counts of its start are left
         }
+        const bool any = t1 > t0;
+        if (!any && !open) break;
+        const int r0 = rb * kSplitRows, rows = s.q * args_again().G;
         const AttnArgs& Y = args_again();
         const int page_log = Y.c.page_log, window = Y.window, sinks = Y.sinks;
-        const int pos = r0 + n < rows ? s.first + (r0 + n) / Y.G : -1;
-        const int from = window > 0 ? pos - window + 1 : 0;   // the row sees from .. pos, and the sinks
-        // tiles that every row sees as a whole: those starting at full_lo .. full_hi
-        const int full_hi = s.first + r0 / Y.G - kTok + 1;
-        const int full_lo = window > 0 ? s.first + (min(r0 + kSplitRows, rows) - 1) / Y.G - window + 1 : 0;
-
         // A tile's places in the cache: this lane's values, scores and scales are of its tokens `mine` on, its
         // keys of those from `keys` on (both within 16 tokens of a page). A lost page's memory is page 0's,
         // hidden below.
@@ -353,18 +358,72 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         const auto values_at = [&](int t, int page) {
             return vb + (size_t)max(page, 0) * page_bytes + (n << page_log) + slot_of(t, mine);
         };
-
+        // q: wave c takes channels 64 c + 16 g .. + 15 of every row (row n its lanes')
+        uint4 raw[2];
         int t = t0 + w;
-        int pk = page_of(t, keys), pv = page_of(t, mine), pk_next = page_of(t + kSplitWaves, keys), pv_next = page_of(t + kSplitWaves, mine);
+        int pk = -1, pv = -1, pk_next = -1, pv_next = -1;
         float ks = 0.0f, vs = 0.0f;
-        if (t < t1) {
-            load_k(t, pk);
-            const int8_t* p = values_at(t, pv);
+        if (any) {
+            if (w < kC) {
+                const AttnArgs& Z = args_again();
+                const int rc = min(r0 + n, rows - 1), qi = rc / Z.G;
+                const uint16_t* qp = Z.q + (long long)(s.s0 + qi) * Z.q_stride + (size_t)(e * Z.G + rc - qi * Z.G) * D + 64 * w + 16 * g;
+                raw[0] = load_row8(qp);
+                raw[1] = load_row8(qp + 8);
+            }
+            pk = page_of(t, keys), pv = page_of(t, mine), pk_next = page_of(t + kSplitWaves, keys), pv_next = page_of(t + kSplitWaves, mine);
+            if (t < t1) {
+                load_k(t, pk);
+                const int8_t* p = values_at(t, pv);
 #pragma unroll
-            for (int m = 0; m < kM; ++m) vr[m] = *reinterpret_cast<const Codes*>(p + ((size_t)(16 * m) << page_log));
-            ks = ksb[(size_t)max(pv, 0) * h_kv];
-            vs = vsb[(size_t)max(pv, 0) * h_kv];
+                for (int m = 0; m < kM; ++m) vr[m] = *reinterpret_cast<const Codes*>(p + ((size_t)(16 * m) << page_log));
+                ks = ksb[(size_t)max(pv, 0) * h_kv];
+                vs = vsb[(size_t)max(pv, 0) * h_kv];
+            }
         }
+
+        if (open) {                                           // the four waves' parts of the last piece together
+            const AttnArgs& Z = args_again();
+            const int x_r0 = taken(o_r0), x_rows = taken(o_rows), x_slot = taken(o_slot);
+            l = pair_sum32(pair_sum16(l));
+            if (g == 0) {
+                lo_ml[(w * kSplitRows + n) * 2] = mref;
+                lo_ml[(w * kSplitRows + n) * 2 + 1] = l;
+            }
+#pragma unroll
+            for (int m = 0; m < kM; ++m) *reinterpret_cast<v4f*>(lo_o + (w * kSplitRows + n) * kPitch + 16 * m + 4 * g) = acc[m];
+            lds_barrier();
+            const Parts<kSplitRows, D> parts(Z.part, gridDim.x);
+            for (int i = tid; i < kSplitRows * D / 4; i += kSplitThreads) {
+                const int row = i / (D / 4), d = i % (D / 4) * 4;
+                if (x_r0 + row >= x_rows) break;
+                float top = -__builtin_inff(), total = 0.0f;
+                v4f sum = {0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < kSplitWaves; ++k) top = fmaxf(top, lo_ml[(k * kSplitRows + row) * 2]);
+#pragma unroll
+                for (int k = 0; k < kSplitWaves; ++k) {
+                    const float m = lo_ml[(k * kSplitRows + row) * 2];
+                    const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+                    total = fmaf(lo_ml[(k * kSplitRows + row) * 2 + 1], f, total);
+                    sum += *reinterpret_cast<const v4f*>(lo_o + (k * kSplitRows + row) * kPitch + d) * f;
+                }
+                if (x_slot < 0) {
+                    const int token = (x_r0 + row) / Z.G;
+                    store_out(Z, taken(o_s0) + token, taken(o_e) * Z.G + x_r0 + row - token * Z.G, d, sum * (total == 0.0f ? 0.0f : 1.0f / total));
+                } else {
+                    *reinterpret_cast<v4f*>(parts.o + ((size_t)x_slot * kSplitRows + row) * D + d) = sum;
+                    if (d == 0) {
+                        parts.ml[((size_t)x_slot * kSplitRows + row) * 2] = top;
+                        parts.ml[((size_t)x_slot * kSplitRows + row) * 2 + 1] = total;
+                    }
+                }
+            }
+            lds_barrier();                                    // lo_o and lo_ml are free again
+        }
+        if (!any) break;
+
+        // q as two int8 of 16 bits
         if (w < kC) {
             u16x2 mb = max_abs_bits(max_abs_bits(u16x2{0, 0}, raw[0]), raw[1]);
             uint32_t mu = max((uint32_t)mb[0], (uint32_t)mb[1]);
@@ -384,11 +443,28 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             lo_q[(2 * w) * kWave + lane] = raw[0];
             lo_q[(2 * w + 1) * kWave + lane] = raw[1];
         }
+        const int pos = r0 + n < rows ? s.first + (r0 + n) / Y.G : -1;
+        const int from = window > 0 ? pos - window + 1 : 0;   // the row sees from .. pos, and the sinks
+        // tiles that every row sees as a whole: those starting at full_lo .. full_hi
+        const int full_hi = s.first + r0 / Y.G - kTok + 1;
+        const int full_lo = window > 0 ? s.first + (min(r0 + kSplitRows, rows) - 1) / Y.G - window + 1 : 0;
         lds_barrier();
-        v4f acc[kM];
 #pragma unroll
         for (int m = 0; m < kM; ++m) acc[m] = v4f{0, 0, 0, 0};
-        float mref = -__builtin_inff(), l = 0.0f;
+        mref = -__builtin_inff(), l = 0.0f;
+
+        // Where its parts go, and whether it is cut at its end.
+        o_e = parked(e), o_r0 = parked(r0), o_rows = parked(rows), o_s0 = parked(s.s0);
+        o_slot = parked(t0 == 0 && t1 == s.nt ? -1 : 2 * (int)blockIdx.x + (pieces > 0));
+        open = true;
+        ++pieces;
+        if (t1 < s.nt && tid == 0) {
+            const int x = blockIdx.x, per = taken(w_per), before = v0 > start ? (v0 - start + per - 1) / per : 0;
+            // the first part is its workgroup's only one so far where the segment began at or before the share
+            cut = Cut{x - before, x + (s.nt + start - (t1 + start) + per - 1) / per, before ? 2 * (x - before) + (v0 < before * per) : o_slot,
+                      s.s0, e, r0, rows, 1};
+        }
+        const int n_left = parked(left - (s.nt + start - v0)), n_rb = parked(rb), n_b = parked(b), n_nrb = parked(s.nrb), n_start = parked(start);
 
         for (; t < t1; t += kSplitWaves) {
             const bool more = t + kSplitWaves < t1;
@@ -468,69 +544,21 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             }
         }
 
-        // the four waves' parts together
-        left = taken(w_left), e = taken(w_e), rb = taken(w_rb), b = taken(w_b), t0 = taken(w_t0), piece = taken(w_piece);
-        const int s0 = taken(w_s0), nrb = taken(w_nrb), nt = taken(w_nt), rows_ = taken(w_rows), t1_ = taken(w_t1), r0_ = rb * kSplitRows;
-        const AttnArgs& Z = args_again();
-        l = pair_sum32(pair_sum16(l));
-        if (g == 0) {
-            lo_ml[(w * kSplitRows + n) * 2] = mref;
-            lo_ml[(w * kSplitRows + n) * 2 + 1] = l;
-        }
-#pragma unroll
-        for (int m = 0; m < kM; ++m) *reinterpret_cast<v4f*>(lo_o + (w * kSplitRows + n) * kPitch + 16 * m + 4 * g) = acc[m];
-        lds_barrier();
-        const bool whole = t0 == 0 && t1_ == nt;
-        const int slot = 2 * blockIdx.x + (piece > 0);
-        const Parts<kSplitRows, D> parts(Z.part, gridDim.x);
-        for (int i = tid; i < kSplitRows * D / 4; i += kSplitThreads) {
-            const int row = i / (D / 4), d = i % (D / 4) * 4;
-            if (r0_ + row >= rows_) break;
-            float top = -__builtin_inff(), total = 0.0f;
-            v4f sum = {0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < kSplitWaves; ++k) top = fmaxf(top, lo_ml[(k * kSplitRows + row) * 2]);
-#pragma unroll
-            for (int k = 0; k < kSplitWaves; ++k) {
-                const float m = lo_ml[(k * kSplitRows + row) * 2];
-                const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-                total = fmaf(lo_ml[(k * kSplitRows + row) * 2 + 1], f, total);
-                sum += *reinterpret_cast<const v4f*>(lo_o + (k * kSplitRows + row) * kPitch + d) * f;
-            }
-            if (whole) {
-                const int token = (r0_ + row) / Z.G;
-                store_out(Z, s0 + token, e * Z.G + r0_ + row - token * Z.G, d, sum * (total == 0.0f ? 0.0f : 1.0f / total));
-            } else {
-                *reinterpret_cast<v4f*>(parts.o + ((size_t)slot * kSplitRows + row) * D + d) = sum;
-                if (d == 0) {
-                    parts.ml[((size_t)slot * kSplitRows + row) * 2] = top;
-                    parts.ml[((size_t)slot * kSplitRows + row) * 2 + 1] = total;
-                }
-            }
-        }
-        left -= t1_ - t0;
-        if (left == 0 && tid == 0) {
-            Cut c{};
-            if (t1_ < nt) {
-                const int w = blockIdx.x, per = taken(w_per), before = (t0 + per - 1) / per;
-                c = Cut{w - before, w + (nt - t1_ + per - 1) / per, before ? 2 * (w - before) + (t0 % per > 0) : slot,
-                        s0, e, r0_, rows_, 1};
-            }
-            parts.cut[blockIdx.x] = c;
-        }
-        lds_barrier();                                      // lo_o, lo_ml and lo_q are free again
-        if (t1_ == nt && left > 0) {                         // the next segment: row block, head, sequence
-            t0 = 0;
-            if (++rb == nrb) {
-                rb = 0;
-                if (++e == Z.c.h_kv) {
-                    e = 0;
-                    do s = span_at<kSplitRows, kTok>(Z, ++b);       // left > 0: a sequence with rows follows
-                    while (s.nrb == 0);
-                }
+
+        // the next segment: row block, head, sequence
+        left = taken(n_left), rb = taken(n_rb) + 1, b = taken(n_b), e = taken(o_e), start = taken(n_start);
+        v0 = 0;
+        if (left > 0 && rb == taken(n_nrb)) {
+            const AttnArgs& Z = args_again();
+            rb = 0;
+            if (++e == Z.c.h_kv) {
+                e = 0;
+                do s = span_at<kSplitRows, kTok>(Z, ++b);     // left > 0: a sequence with rows follows
+                while (s.nrb == 0);
             }
         }
     }
+    if (tid == 0) Parts<kSplitRows, D>(args_again().part, gridDim.x).cut[blockIdx.x] = cut;
 }
 
 // Segments that several workgroups share. One that lies across n ends of shares has n workgroups here,
