@@ -46,7 +46,6 @@ inline bool make_batch(int n_seq, int T, const int32_t* cu, const int32_t* kv_le
 inline bool rows_ok(const ix_rows* r, long long least) {
     return r && r->p && ptr_aligned(r->p, 2) && r->stride >= least;
 }
-inline bool rows_wide(const ix_rows* r) { return ptr_aligned(r->p, 16) && r->stride % 8 == 0; }
 
 // The last b in [0, n) with key(b) <= j, for a key that does not fall and key(0) <= j: each step the wave's
 // lanes try 64 places (one load's latency for 64 sequences, two for 4,096). The same in every lane.

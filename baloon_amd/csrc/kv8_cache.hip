@@ -51,8 +51,45 @@ __device__ __forceinline__ float max_abs(const uint4& x) {
     return m;
 }
 
-__device__ __forceinline__ uint32_t code_of(float x, float s) {
-    return (uint8_t)(int8_t)(int)fminf(fmaxf(rintf(x / s), -127.0f), 127.0f);
+// Eight codes rint(x / s) by the reciprocal y of s: q = x y is within an ulp of the quotient, and q + (x - q s) y
+// is the quotient correctly rounded (Markstein: y is the reciprocal correctly rounded, and the remainder exact where
+// nothing underflows; a division is 10 instructions). 1.5 2^23 added to a number leaves its nearest integer, to even,
+// in the sum's low bits.
+constexpr float kMagic = 12582912.0f, kLeast = 1e-30f;
+__device__ __forceinline__ float code_bits(float x, float s, float y) {
+    const float q = x * y;
+    return fmaf(fmaf(-q, s, x), y, q) + kMagic;
+}
+__device__ __forceinline__ uint2 codes_of(const uint4& x, float s, float y) {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+    uint32_t two[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        two[e] = __builtin_amdgcn_perm(__float_as_uint(code_bits(__uint_as_float(u[e] & 0xffff0000u), s, y)),
+                                       __float_as_uint(code_bits(__uint_as_float(u[e] << 16), s, y)), 0x0c0c0400u);
+    return make_uint2(__builtin_amdgcn_perm(two[1], two[0], 0x05040100u), __builtin_amdgcn_perm(two[3], two[2], 0x05040100u));
+}
+// The same where s is under kLeast.
+__device__ __forceinline__ uint2 codes_of_small(const uint4& x, float s) {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+    uint32_t q[2] = {0, 0};
+    if (s > 0.0f)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
+            q[e / 4] |= (uint32_t)(uint8_t)(int8_t)(int)fminf(fmaxf(rintf(v / s), -127.0f), 127.0f) << (8 * (e & 3));
+        }
+    return make_uint2(q[0], q[1]);
+}
+
+// 4 x 4 bytes: row i of the results is byte i of each operand.
+__device__ __forceinline__ void transpose4(uint32_t (&x)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), b = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u), d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+    x[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    x[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    x[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    x[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
 // Four codes times r, each rounded again.
@@ -66,50 +103,64 @@ __device__ __forceinline__ uint32_t recode4(uint32_t c, float r) {
     return out;
 }
 
-// 8 values of a row, bf16.
-__device__ __forceinline__ uint4 load8(const uint16_t* p, bool wide) {
-    if (wide) return *reinterpret_cast<const uint4*>(p);
-    uint32_t u[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = p[2 * e] | ((uint32_t)p[2 * e + 1] << 16);
-    return make_uint4(u[0], u[1], u[2], u[3]);
+// The first `keep` of four codes, and four of which the first `keep` are older ones.
+__device__ __forceinline__ uint32_t first_mask(int keep) { return keep <= 0 ? 0u : keep >= 4 ? ~0u : (1u << (8 * keep)) - 1; }
+__device__ __forceinline__ uint32_t first(uint32_t q, int keep) { return q & first_mask(keep); }
+__device__ __forceinline__ uint32_t older(uint32_t was, uint32_t now, float r, int keep) {
+    return first(recode4(was, r), keep) | (now & ~first_mask(keep));
 }
 
-// LDS tile of a page's values, [d][page] with rows 4 bytes longer.
-constexpr int kTilePad = 4;
+// 8 values of a row, bf16, at any 2-byte address (the target reads words unaligned).
+__device__ __forceinline__ uint4 load8(const uint16_t* p) {
+    uint4 x;
+    __builtin_memcpy(&x, p, sizeof(x));
+    return x;
+}
 
-// Thread t holds the 8 channels 8 (t % (d/8)) .. + 7 of NC consecutive slots of the page, from slot
-// NC (t / (d/8)) on: one 16-byte load a slot, and NC codes of a channel side by side for the values' tile.
-template <int NC>
+// A page's values pass through LDS slot by slot. A lane takes 4 channels of 16 slots, which it turns 4 x 4 bytes at
+// a time; consecutive lanes take the 16s of the same channels, which lie side by side in the page.
+struct Turn {
+    int ch, s0;                                               // channels ch .. + 3, slots s0 .. + 15
+};
+__device__ __forceinline__ Turn turn_of(int i, int span_log) {
+    return Turn{(i >> span_log) * 4, (i & ((1 << span_log) - 1)) * 16};
+}
+
+// Two passes over the page's new rows, in chunks of 8 channels: the largest value, then the codes. LDS holds a slot's
+// chunks of 16 bytes in between; a chunk's codes take its first or, in odd 16s of slots, second half (the turn reads
+// the 16s together). The second pass is a rolled loop: every launch begins with an empty instruction cache, and with it
+// unrolled 8, 4 and 2 times a single token for 64 sequences took 7.9, 6.6 and 5.5 us of the kernel's time.
+constexpr int kBatch = 4;
 __global__ void __launch_bounds__(kCacheThreads)
 append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_stride, const uint16_t* __restrict__ vr,
-              long long v_stride, bool k_wide, bool v_wide) {
-    extern __shared__ uint8_t tile[];
+              long long v_stride) {
+    extern __shared__ uint4 raw[];
     __shared__ float red[kCacheThreads / kWave];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), h = blockIdx.y;
     const bool is_v = blockIdx.z;
     PageJob job;
     if (!page_job(a, c, blockIdx.x, lane, &job)) return;
-    const int per = c.d / 8, col = (tid % per) * 8, slot0 = tid / per * NC;
-    const uint16_t* rows = is_v ? vr : kr;
+    const int per_log = c.d == 64 ? 3 : c.d == 128 ? 4 : 5, chunks = (job.end - job.held) << per_log;
     const long long stride = is_v ? v_stride : k_stride;
-    const bool wide = is_v ? v_wide : k_wide;
+    const uint16_t* rows = (is_v ? vr : kr) + (long long)job.row * stride + (size_t)h * c.d;
     const size_t ph = (size_t)job.id * c.h_kv + h;
     float* scale = (is_v ? c.v_scale : c.k_scale) + ph;
     int8_t* codes = (is_v ? c.v : c.k) + ph * c.page * c.d;
+    const auto load = [&](int i) { return load8(rows + (i >> per_log) * stride + ((i & ((1 << per_log) - 1)) << 3)); };
 
-    uint4 x[NC];
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int slot = slot0 + i;
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (slot >= job.held && slot < job.end)
-            x[i] = load8(rows + (long long)(job.row + slot - job.held) * stride + (size_t)h * c.d + col, wide);
-    }
     const float old = job.held > 0 ? *scale : 0.0f;
+    float m = 0.0f;
+    uint4* held = raw + (job.held << per_log);
+    for (int i0 = tid; i0 < chunks; i0 += kBatch * kCacheThreads) {
+        uint4 x[kBatch];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) m = fmaxf(m, max_abs(x[i]));
+        for (int y = 0; y < kBatch; ++y) x[y] = i0 + y * kCacheThreads < chunks ? load(i0 + y * kCacheThreads) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int y = 0; y < kBatch; ++y) {
+            m = fmaxf(m, max_abs(x[y]));
+            if (i0 + y * kCacheThreads < chunks) held[i0 + y * kCacheThreads] = x[y];
+        }
+    }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
     if (lane == 0) red[tid / kWave] = m;
@@ -117,29 +168,17 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float s = fmaxf(old, m / 127.0f);
     const bool grown = job.held > 0 && s > old;
-    const float ratio = grown ? old / s : 1.0f;
+    const float ratio = grown ? old / s : 1.0f, inv = 1.0f / s;
     if (tid == 0) *scale = s;
 
-    uint32_t q[NC][2];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        q[i][0] = q[i][1] = 0;
-        if (s > 0.0f && slot0 + i >= job.held && slot0 + i < job.end)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t two = code_of(__uint_as_float(u[e] << 16), s) |
-                                     code_of(__uint_as_float(u[e] & 0xffff0000u), s) << 8;
-                q[i][e / 2] |= two << (16 * (e & 1));
-            }
+#pragma unroll 1
+    for (int i = tid; i < chunks; i += kCacheThreads) {       // a thread's own chunks
+        const int slot = job.held + (i >> per_log);
+        const uint2 q = s < kLeast ? codes_of_small(held[i], s) : codes_of(held[i], s, inv);
+        if (is_v) reinterpret_cast<uint2*>(held + i)[slot >> 4 & 1] = q;
+        else *reinterpret_cast<uint2*>(codes + slot * c.d + ((i & ((1 << per_log) - 1)) << 3)) = q;
     }
     if (!is_v) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int slot = slot0 + i;
-            if (slot >= job.held && slot < job.end)
-                *reinterpret_cast<uint2*>(codes + slot * c.d + col) = make_uint2(q[i][0], q[i][1]);
-        }
         if (grown) {
             uint4* p = reinterpret_cast<uint4*>(codes);
             for (int i = tid; i < job.held * c.d / 16; i += kCacheThreads) {
@@ -149,40 +188,38 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
         }
         return;
     }
-    const int pitch = c.page + kTilePad;
-    if (slot0 < c.page) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int i = 0; i < NC; ++i) tile[(col + e) * pitch + slot0 + i] = (uint8_t)(q[i][e / 4] >> (8 * (e & 3)));
-    }
     __syncthreads();
     // Channel rows of 16 slots: whole ones at once (slots behind the new tokens hold nothing yet, and get
     // zeros), the one with older tokens in it by bytes, or as a whole where the older ones change too.
-    const int spans = c.page / 16;
-    for (int i = tid; i < c.d * spans; i += kCacheThreads) {
-        const int ch = i / spans, s0 = (i - ch * spans) * 16;
-        if (s0 >= job.end || (s0 + 16 <= job.held && !grown)) continue;
-        const uint8_t* from = tile + ch * pitch + s0;
-        int8_t* to = codes + ch * c.page + s0;
-        uint32_t n[4];
+    const int span_log = c.page_log - 4;
+    for (int i = tid; i < (c.d / 4) << span_log; i += kCacheThreads) {
+        const Turn u = turn_of(i, span_log);
+        if (u.s0 >= job.end || (u.s0 + 16 <= job.held && !grown)) continue;
+        const int keep = job.end - u.s0;                      // slots that hold tokens
+        const uint8_t* tile = reinterpret_cast<const uint8_t*>(raw) + (u.ch >> 3) * 16 + (u.s0 >> 4 & 1) * 8 + (u.ch & 7);
+        uint32_t n[4][4];                                     // [4 slots][channel]
 #pragma unroll
-        for (int e = 0; e < 4; ++e) n[e] = *reinterpret_cast<const uint32_t*>(from + 4 * e);
-        if (s0 < job.held) {
-            if (!grown) {
-                for (int e = job.held - s0; e < min(16, job.end - s0); ++e) to[e] = (int8_t)from[e];
+        for (int y = 0; y < 4; ++y) {
+#pragma unroll
+            for (int z = 0; z < 4; ++z) n[y][z] = *reinterpret_cast<const uint32_t*>(tile + (u.s0 + 4 * y + z) * c.d * 2);
+            transpose4(n[y]);
+        }
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+            int8_t* to = codes + ((u.ch + z) << c.page_log) + u.s0;
+            if (u.s0 < job.held && !grown) {
+                for (int y = job.held - u.s0; y < min(16, job.end - u.s0); ++y)
+                    to[y] = (int8_t)tile[(u.s0 + y) * c.d * 2 + z];
                 continue;
             }
-            const uint4 o = *reinterpret_cast<const uint4*>(to);
-            const uint32_t was[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int keep = min(max(job.held - s0 - 4 * e, 0), 4);          // older slots among these four
-                const uint32_t mask = keep == 4 ? 0xffffffffu : (1u << (8 * keep)) - 1;
-                n[e] = (recode4(was[e], ratio) & mask) | (n[e] & ~mask);
+            uint4 v = make_uint4(first(n[0][z], keep), first(n[1][z], keep - 4), first(n[2][z], keep - 8), first(n[3][z], keep - 12));
+            if (u.s0 < job.held) {
+                const uint4 o = *reinterpret_cast<const uint4*>(to);
+                v = make_uint4(older(o.x, v.x, ratio, job.held - u.s0), older(o.y, v.y, ratio, job.held - u.s0 - 4),
+                               older(o.z, v.z, ratio, job.held - u.s0 - 8), older(o.w, v.w, ratio, job.held - u.s0 - 12));
             }
+            *reinterpret_cast<uint4*>(to) = v;
         }
-        *reinterpret_cast<uint4*>(to) = make_uint4(n[0], n[1], n[2], n[3]);
     }
 }
 
@@ -204,13 +241,23 @@ read_kernel(Kv8 c, Batch a, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo
     const size_t ph = (size_t)job.id * c.h_kv + h;
     const float s = (is_v ? c.v_scale : c.k_scale)[ph];
     const int8_t* codes = (is_v ? c.v : c.k) + ph * c.page * c.d;
-    const int per = c.d / 8, pitch = c.page + kTilePad, spans = c.page / 16;
+    const int per = c.d / 8, pitch = c.d + 4, span_log = c.page_log - 4;      // rows of slots 4 bytes longer: 16 slots on, other banks
     if (is_v) {
-        for (int i = tid; i < c.d * spans; i += kCacheThreads) {
-            const int ch = i / spans, s0 = (i - ch * spans) * 16;
-            const uint4 o = *reinterpret_cast<const uint4*>(codes + ch * c.page + s0);
-            uint32_t* to = reinterpret_cast<uint32_t*>(tile + ch * pitch + s0);
-            to[0] = o.x; to[1] = o.y; to[2] = o.z; to[3] = o.w;
+        for (int i = tid; i < (c.d / 4) << span_log; i += kCacheThreads) {
+            const Turn u = turn_of(i, span_log);
+            if (u.s0 >= job.end || u.s0 + 16 <= job.held) continue;
+            uint32_t n[4][4];                                 // [4 slots][channel]
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                const uint4 o = *reinterpret_cast<const uint4*>(codes + ((u.ch + z) << c.page_log) + u.s0);
+                n[0][z] = o.x; n[1][z] = o.y; n[2][z] = o.z; n[3][z] = o.w;
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                transpose4(n[y]);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) *reinterpret_cast<uint32_t*>(tile + (u.s0 + 4 * y + z) * pitch + u.ch) = n[y][z];
+            }
         }
         __syncthreads();
     }
@@ -218,10 +265,8 @@ read_kernel(Kv8 c, Batch a, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo
         const int slot = i / per, col = (i - slot * per) * 8;
         uint2 q;
         if (is_v) {
-            uint32_t u[2] = {0, 0};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) u[e / 4] |= (uint32_t)tile[(col + e) * pitch + slot] << (8 * (e & 3));
-            q = make_uint2(u[0], u[1]);
+            const uint32_t* p = reinterpret_cast<const uint32_t*>(tile + slot * pitch + col);
+            q = make_uint2(p[0], p[1]);
         } else {
             q = *reinterpret_cast<const uint2*>(codes + slot * c.d + col);
         }
@@ -241,12 +286,6 @@ dim3 page_grid(const Kv8& c, const Batch& a) {
     return dim3((unsigned)(a.T >> c.page_log) + 2u * (unsigned)a.n_seq, (unsigned)c.h_kv, 2);
 }
 
-template <int NC>
-void launch_append(const Kv8& c, const Batch& a, const ix_rows* k, const ix_rows* v, hipStream_t s) {
-    hipLaunchKernelGGL((append_kernel<NC>), page_grid(c, a), dim3(kCacheThreads), c.d * (c.page + kTilePad), s, c, a, k->p,
-                       k->stride, v->p, v->stride, rows_wide(k), rows_wide(v));
-}
-
 }  // namespace
 }  // namespace ixg
 
@@ -260,14 +299,11 @@ hipError_t ix_kv8_append(const ix_kv8* cache, int n_seq, int total_T, const int3
     if (!make_kv8(cache, &c) || !make_batch(n_seq, total_T, cu_seqlens, kv_len, table, width, &a)) return hipErrorInvalidValue;
     if (!rows_ok(k, (long long)c.h_kv * c.d) || !rows_ok(v, (long long)c.h_kv * c.d)) return hipErrorInvalidValue;
     if (total_T == 0) return hipSuccess;
-    switch (c.page * c.d / 8 / kCacheThreads) {
-        case 0: launch_append<1>(c, a, k, v, s); break;       // 16 x 64: half the threads
-        case 1: launch_append<1>(c, a, k, v, s); break;
-        case 2: launch_append<2>(c, a, k, v, s); break;
-        case 4: launch_append<4>(c, a, k, v, s); break;
-        case 8: launch_append<8>(c, a, k, v, s); break;
-        default: launch_append<16>(c, a, k, v, s); break;
-    }
+    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(&append_kernel),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 256 * sizeof(uint16_t));
+    if (ready != hipSuccess) return ready;
+    hipLaunchKernelGGL(append_kernel, page_grid(c, a), dim3(kCacheThreads), c.page * c.d * sizeof(uint16_t), s, c, a, k->p, k->stride,
+                       v->p, v->stride);
     return hipGetLastError();
 }
 
@@ -279,7 +315,7 @@ hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_
     if (!make_kv8(cache, &c) || !make_batch(n_seq, total_T, cu_seqlens, kv_len, table, width, &a)) return hipErrorInvalidValue;
     if ((!k && !v) || !ptr_aligned(k, 2) || !ptr_aligned(v, 2)) return hipErrorInvalidValue;
     if (total_T == 0) return hipSuccess;
-    hipLaunchKernelGGL(read_kernel, page_grid(c, a), dim3(kCacheThreads), c.d * (c.page + kTilePad), s, c, a, k, v,
+    hipLaunchKernelGGL(read_kernel, page_grid(c, a), dim3(kCacheThreads), c.page * (c.d + 4), s, c, a, k, v,
                        ptr_aligned(k, 16) && ptr_aligned(v, 16));
     return hipGetLastError();
 }

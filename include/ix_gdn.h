@@ -392,8 +392,7 @@ typedef struct ix_kv8 {
  * it holds older tokens of the sequence and 0 if not; where s' > s the older codes become
  * rint(code * (s / s')); the new codes are rint(x / s') (0 when s' is 0). All in fp32, IEEE
  * divisions, rint to nearest even. Values must be finite. The new tokens' pages must not be
- * another sequence's of this batch, or hold anything behind the new tokens. Strides that are
- * multiples of 8 at 16-byte aligned rows are faster. */
+ * another sequence's of this batch, or hold anything behind the new tokens. */
 hipError_t ix_kv8_append(const ix_kv8* cache, int n_seq, int total_T, const int32_t* cu_seqlens,
                          const int32_t* kv_len, const int32_t* table, int width, const ix_rows* k, const ix_rows* v,
                          hipStream_t s IX_GDN_DEFAULT_STREAM);
