@@ -3,6 +3,7 @@
 //   o_r = sum_j p_rj v_j / sum_j p_rj,  p_rj = exp(scale q_r . k_j)  over the tokens j that row r sees
 //
 // with k_j = ks c_j and v_j = vs d_j, c and d the codes and ks, vs the scales of the token's page.
+#include <algorithm>
 #include <type_traits>
 
 #include "kv8.h"
@@ -32,6 +33,8 @@ struct AttnArgs {
     int h_q, G, window, sinks;
     int narrow;               // the batch has fewer than 2^31 tiles for split_kernel
     int small;                // sequences of more (token, head) rows a kv head than this are block_kernel's
+    float* block_part;        // partial results of its blocks, see BlockParts
+    int slots, items;         // workgroups of it that the chip holds, and parts of blocks at most
 };
 
 // The kernel's argument (its only one) read from memory again where it is used next: keeping all of it in
@@ -561,20 +564,15 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     if (tid == 0) Parts<kSplitRows, D>(args_again().part, gridDim.x).cut[blockIdx.x] = cut;
 }
 
-// Segments that several workgroups share. One that lies across n ends of shares has n workgroups here,
-// which take even parts of its outputs (in fours); where those are fewer than the threads, several threads
-// take every so many partial results of an output and are joined in LDS. The order of the sums is fixed.
+// Outputs from .. to - 1 (in fours, row by row) of a segment whose partial results are k0 .. k1, the rows of k at at(k).
+// Where the outputs are fewer than the threads, several threads take every so many partial results of one and are
+// joined in LDS. The order of the sums is fixed.
 constexpr int kJoinThreads = 256;
-template <int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg) {
+template <int D, class At>
+__device__ __forceinline__ void join_outputs(const AttnArgs& A, const float* po, const float* ml, int k0, int k1, At at_part, int from,
+                                             int to, int s0, int e, int r0) {
     __shared__ v4f lo_o[kJoinThreads];
     __shared__ float lo_m[kJoinThreads], lo_l[kJoinThreads];
-    const Parts<kSplitRows, D> parts(A.part, n_wg);
-    const Cut c = parts.cut[blockIdx.x];
-    if (!c.any) return;
-    const int n = c.last - c.first, i = blockIdx.x - c.first;
-    const int all = min(kSplitRows, c.rows - c.r0) * (D / 4);
-    const int from = (int)((long long)all * i / n), to = (int)((long long)all * (i + 1) / n);
     int wide = 1;                                             // outputs at a time
     while (wide < to - from && wide < kJoinThreads) wide *= 2;
     const int ways = kJoinThreads / wide, way = threadIdx.x / wide;
@@ -591,9 +589,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg
             top = now;
         };
 #pragma unroll 4
-        for (int k = c.first + way; k <= c.last; k += ways) {
-            const size_t at = (size_t)(k == c.first ? c.slot : 2 * k) * kSplitRows + row;
-            add(parts.ml[2 * at], parts.ml[2 * at + 1], *reinterpret_cast<const v4f*>(parts.o + at * D + d));
+        for (int k = k0 + way; k <= k1; k += ways) {
+            const size_t at = at_part(k) + row;
+            add(ml[2 * at], ml[2 * at + 1], *reinterpret_cast<const v4f*>(po + at * D + d));
         }
         for (int half = ways / 2; half > 0; half /= 2) {
             lo_o[threadIdx.x] = sum;
@@ -605,10 +603,24 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg
             __syncthreads();
         }
         if (way == 0 && x0 + (int)threadIdx.x < to) {
-            const int token = (c.r0 + row) / A.G;
-            store_out(A, c.row + token, c.e * A.G + c.r0 + row - token * A.G, d, sum * (total == 0.0f ? 0.0f : 1.0f / total));
+            const int token = (r0 + row) / A.G;
+            store_out(A, s0 + token, e * A.G + r0 + row - token * A.G, d, sum * (total == 0.0f ? 0.0f : 1.0f / total));
         }
     }
+}
+
+// Segments that several workgroups share. One that lies across n ends of shares has n workgroups here,
+// which take even parts of its outputs.
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg) {
+    const Parts<kSplitRows, D> parts(A.part, n_wg);
+    const Cut c = parts.cut[blockIdx.x];
+    if (!c.any) return;
+    const int n = c.last - c.first, i = blockIdx.x - c.first;
+    const int all = min(kSplitRows, c.rows - c.r0) * (D / 4);
+    const int from = (int)((long long)all * i / n), to = (int)((long long)all * (i + 1) / n);
+    const auto at = [&](int k) { return (size_t)(k == c.first ? c.slot : 2 * k) * kSplitRows; };
+    join_outputs<D>(A, parts.o, parts.ml, c.first, c.last, at, from, to, c.row, c.e, c.r0);
 }
 
 // Blocks of rows: prompts.
@@ -648,7 +660,72 @@ __device__ __forceinline__ void each(F f) {
     if constexpr (N == 2) f(std::integral_constant<int, 1>{});
 }
 
+// Where the blocks are fewer than the workgroups that the chip holds, several workgroups take parts of a block's tiles,
+// as many for each block as fill the chip best, and block_join_kernel joins them: 512 tokens of 32 heads over 8 of 128
+// behind 16,384, 128 blocks, took 356 us whole and take 170.
+struct BlockCut {
+    int first, parts, step;                                   // partial results first, first + step ..
+    int s0, e, r0, rows, unused;                              // as in Cut
+};
 template <int D>
+struct BlockParts {
+    float *o, *ml;
+    BlockCut* cut;
+    __device__ __forceinline__ BlockParts(float* p, int slots)
+        : o(p), ml(p + (size_t)2 * slots * kBlockRows * D),
+          cut(reinterpret_cast<BlockCut*>(ml + (size_t)2 * slots * kBlockRows * 2)) {}
+    static size_t bytes(int slots) {
+        return (size_t)2 * slots * kBlockRows * (D + 2) * sizeof(float) + (size_t)slots * sizeof(BlockCut);
+    }
+};
+// The largest of all lanes' v.
+template <int Ctrl, int RowMask>
+__device__ __forceinline__ int dpp_max(int v) {
+    return max(v, __builtin_amdgcn_update_dpp(v, v, Ctrl, RowMask, 0xF, false));
+}
+__device__ __forceinline__ int wave_max_int(int v) {
+    v = dpp_max<0x111, 0xF>(v);
+    v = dpp_max<0x112, 0xF>(v);
+    v = dpp_max<0x114, 0xF>(v);
+    v = dpp_max<0x118, 0xF>(v);
+    v = dpp_max<0x142, 0xA>(v);
+    return lane_of(dpp_max<0x143, 0xC>(v), kWave - 1);
+}
+// The blocks of a sequence.
+__device__ __forceinline__ int blocks_of(const AttnArgs& A, int b) {
+    if (b >= A.a.n_seq) return 0;
+    const int rows = max(A.a.start(b + 1) - A.a.start(b), 0) * A.G;
+    return rows > A.small ? (rows + kBlockRows - 1) / kBlockRows : 0;
+}
+// The blocks of all sequences and heads, and in how many parts each is taken: lane p - 1 knows the time of p, in tiles,
+// from the rounds of workgroups and the longest block's tiles.
+struct Blocks {
+    int n, parts;
+};
+template <int D>
+constexpr float kPartCost = D == 256 ? 4.0f : 8.0f;           // tiles in the time of a part's start, its sums and their joining
+constexpr int kLeastPart = 4;         // tiles
+template <int D>
+__device__ __forceinline__ Blocks all_blocks(const AttnArgs& A, int lane) {
+    int sum = 0, kv = 0;
+    for (int b0 = 0; b0 < A.a.n_seq; b0 += kWave) {
+        const int v = blocks_of(A, b0 + lane);
+        sum += v;
+        if (v > 0) kv = max(kv, A.a.kv_len[b0 + lane]);
+    }
+    Blocks out;
+    out.n = lane_of(wave_scan_int(sum), kWave - 1) * A.c.h_kv;
+    kv = wave_max_int(kv);
+    if (A.window > 0) kv = min(kv, A.window + min(A.sinks, kv) + kBlockRows / A.G);
+    const int p = lane + 1, rounds = (out.n * p + A.slots - 1) / A.slots;
+    float cost = (float)rounds * ((float)kv / (float)(kBlockTok * p) + (p > 1 ? kPartCost<D> : 0.0f));
+    if (p > 1 && (long long)out.n * p > A.items) cost = __builtin_inff();
+    const int least = -wave_max_int(-__float_as_int(cost));   // numbers >= 0 are in the order of their bits
+    out.parts = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(__float_as_int(cost) == least))) + 1;
+    return out;
+}
+
+template <int D, bool kCut>
 __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(AttnArgs A) {
     constexpr int kC = D / 64, kM = D / 16;
     constexpr int kUnits = kBlockTok * D / 16, kPer = (kUnits + kBlockThreads - 1) / kBlockThreads;
@@ -660,11 +737,34 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
 
     // Block j of the grid, from the last: of the causal blocks the longest start first. Sequence b owns the
     // blocks from cu[b] G / 128 + b on; consecutive workgroups, which different XCDs take, are different heads.
-    const int e = blockIdx.x % A.c.h_kv, j = gridDim.x / A.c.h_kv - 1 - blockIdx.x / A.c.h_kv;
-    const auto key = [&](int b) { return (int)((long long)A.a.start(b) * A.G / kBlockRows) + b; };
-    const int b = wave_search(A.a.n_seq, j, lane, key);
-    const int s0 = A.a.start(b), q = A.a.start(b + 1) - s0, r0 = (j - key(b)) * kBlockRows, rows = max(q, 0) * A.G;
-    if (rows <= A.small || r0 >= rows) return;
+    const int e = blockIdx.x % A.c.h_kv;
+    int b, rb, parts = 1, part = 0;
+    if constexpr (kCut) {
+        const Blocks all = all_blocks<D>(A, lane);
+        if (blockIdx.x >= all.n * all.parts) return;
+        const int i = blockIdx.x / A.c.h_kv;
+        parts = all.parts;
+        part = i % parts;
+        rb = all.n / A.c.h_kv - 1 - i / parts;
+        for (int b0 = 0;; b0 += kWave) {
+            const int v = blocks_of(A, b0 + lane), incl = wave_scan_int(v);
+            const unsigned long long hit = __ballot(incl > rb);
+            if (hit) {
+                const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
+                b = b0 + l;
+                rb -= lane_of(incl - v, l);
+                break;
+            }
+            rb -= lane_of(incl, kWave - 1);
+        }
+    } else {
+        const int j = gridDim.x / A.c.h_kv - 1 - blockIdx.x / A.c.h_kv;
+        const auto key = [&](int b) { return (int)((long long)A.a.start(b) * A.G / kBlockRows) + b; };
+        b = wave_search(A.a.n_seq, j, lane, key);
+        rb = j - key(b);
+    }
+    const int s0 = A.a.start(b), q = A.a.start(b + 1) - s0, r0 = rb * kBlockRows, rows = max(q, 0) * A.G;
+    if (!kCut && (rows <= A.small || r0 >= rows)) return;
     const int kv = max(A.a.kv_len[b], 0), first = kv - q;
 
     // q of row n of the wave, channels 64 c + 16 g .. + 15
@@ -701,8 +801,20 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     const int block_first = first + r0 / A.G, block_last = first + (min(r0 + kBlockRows, rows) - 1) / A.G;
     const int lo = A.window > 0 ? max(block_first - A.window + 1, 0) / kBlockTok : 0;
     const int ns = A.window > 0 ? min(A.sinks / kBlockTok + (A.sinks % kBlockTok != 0), lo) : 0;
-    const int nt = block_last < 0 ? 0 : ns + block_last / kBlockTok + 1 - lo;
-    const auto tile = [&](int t) { return (t < ns ? t : lo + t - ns) * kBlockTok; };
+    const int all = block_last < 0 ? 0 : ns + block_last / kBlockTok + 1 - lo;
+    int begin = 0, nt = all;                                  // this part's: tiles begin .. begin + nt - 1
+    if constexpr (kCut) {
+        if (parts > 1) {
+            const int i = blockIdx.x / A.c.h_kv / parts;
+            parts = min(parts, max(all / kLeastPart, 1));
+            if (part == 0 && tid == 0)
+                BlockParts<D>(A.block_part, A.slots).cut[i * A.c.h_kv + e] = BlockCut{(int)blockIdx.x, parts, A.c.h_kv, s0, e, r0, rows, 0};
+            if (part >= parts) return;
+            begin = all / parts * part + min(part, all % parts);
+            nt = all / parts + (part < all % parts);
+        }
+    }
+    const auto tile = [&](int t) { return (begin + t < ns ? begin + t : lo + begin + t - ns) * kBlockTok; };
 
     // Copies of a tile: 16-byte pieces 512 i + tid of its keys, token by token, and of its values, page by page
     // and in a page (or 64 tokens of it) channel by channel. The pieces of one wave's i are in one page.
@@ -872,6 +984,16 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     int thread = tid;
     asm volatile("" : "+v"(thread));                          // the row is worked out again: it does not wait in registers
     const int r = w0 + (thread & 15), qi = r / A.G, head = e * A.G + r - qi * A.G, d0 = 4 * (thread >> 4 & 3);
+    if (kCut && parts > 1) {
+        const BlockParts<D> to(A.block_part, A.slots);
+        const size_t at = (size_t)blockIdx.x * kBlockRows + (r - r0);
+        if (r < rows) {
+            if (d0 == 0) *reinterpret_cast<float2*>(to.ml + 2 * at) = make_float2(l == 0.0f ? -__builtin_inff() : ref, l);
+#pragma unroll
+            for (int m = 0; m < kM; ++m) *reinterpret_cast<v4f*>(to.o + at * D + 16 * m + d0) = acc[m];
+        }
+        return;
+    }
     if (r < rows) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         constexpr int kN = kM < 8 ? kM : 8;                   // pieces of 4 channels, their gates on the way together
@@ -886,28 +1008,83 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     }
 }
 
-// Sequences of at most kSplitMost rows a kv head are split_kernel's in any case, and so are all where the blocks
-// are fewer than kBlockLeast.
-constexpr int kSplitMost = 64, kBlockLeast = 64;
+// Every block's outputs are shared out over as many workgroups as there are for each.
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) block_join_kernel(AttnArgs A) {
+    const Blocks blocks = all_blocks<D>(A, threadIdx.x & (kWave - 1));
+    if (blocks.parts == 1) return;
+    const int n = (int)gridDim.x / blocks.n, k = blockIdx.x % blocks.n, i = blockIdx.x / blocks.n;
+    if (i >= n) return;
+    const BlockParts<D> parts(A.block_part, A.slots);
+    const BlockCut c = parts.cut[k];
+    if (c.parts == 1) return;
+    const int all = min(kBlockRows, c.rows - c.r0) * (D / 4);
+    const auto at = [&](int k) { return (size_t)(c.first + k * c.step) * kBlockRows; };
+    join_outputs<D>(A, parts.o, parts.ml, 0, c.parts - 1, at, (int)((long long)all * i / n), (int)((long long)all * (i + 1) / n),
+                    c.s0, c.e, c.r0);
+}
+
+// Sequences of at most kSplitMost (token, head) rows a kv head are split_kernel's in any case, and so are all where the
+// batch's rows fill fewer than least_blocks(D) blocks. A block takes the same time with 1 row and with 128, and
+// split_kernel that of its 16s: 128 sequences over 4 kv heads of 128, 4,096 tokens each, take with 32, 48 and 64 rows
+// 193, 283 and 371 us there and 187, 187 and 194 here, with 512 tokens 32, 43 and 54 to 36, 40 and 42. Few blocks are few
+// workgroups, or parts that must be joined: 16, 32 and 64 blocks of one sequence take, at D = 128 behind 16,384 tokens,
+// 60, 104 and 186 us there and 44, 61 and 96 here, behind 2,048 tokens 19, 28 and 35 to 28, 30 and 31, and behind none 9,
+// 10 and 11 to 15; at D = 256 16 blocks 130, 33 and 15 to 60, 30 and 22, at D = 64 64 blocks 106, 21 and 9 to 69, 23 and 12.
+constexpr int kSplitMost = 32;
+constexpr int least_blocks(int d) { return 4096 / d; }
+
+struct Plan {
+    bool block, cut;          // block_kernel for sequences of more than kSplitMost rows; in parts
+    int n_wg, slots;          // workgroups that the chip holds: of split_kernel two a CU, of block_kernel one or two
+    long long full;           // whole blocks that the batch's rows fill
+};
+Plan plan_of(int d, int h_kv, int G, int T, int max_q, hipStream_t s) {
+    Plan p;
+    const int n_cu = device_cu_count(s);
+    p.n_wg = 2 * n_cu;
+    p.slots = d == 256 ? n_cu : 2 * n_cu;
+    p.full = (long long)T * G / kBlockRows * h_kv;
+    p.block = (long long)max_q * G > kSplitMost && p.full >= least_blocks(d);
+    p.cut = p.block && p.full < p.slots;
+    return p;
+}
 
 template <int D>
-hipError_t launch_attn(AttnArgs& A, int max_q, int n_wg, hipStream_t s) {
-    // Blocks of rows where they occupy a quarter of the chip: block_kernel is about four times as fast a
-    // workgroup as split_kernel on the same rows, which spreads over all of it.
-    const long long full = (long long)A.a.T * A.G / kBlockRows * A.c.h_kv, blocks = full + (long long)A.a.n_seq * A.c.h_kv;
-    const long long longest = (long long)max_q * A.G;
-    const bool block = longest > kSplitMost && full >= kBlockLeast;
-    A.small = block ? kSplitMost : 0x7fffffff;
+size_t split_bytes(const Plan& p) { return (Parts<kSplitRows, D>::bytes(p.n_wg) + 255) / 256 * 256; }
+template <int D>
+size_t attn_bytes(const Plan& p) { return split_bytes<D>(p) + (p.cut ? BlockParts<D>::bytes(p.slots) : 0); }
+
+template <int D, bool kCut>
+hipError_t launch_blocks(const AttnArgs& A, long long n, hipStream_t s) {
+    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(&block_kernel<D, kCut>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, BlockLds<D>::kBytes);
+    if (ready == hipSuccess)
+        hipLaunchKernelGGL((block_kernel<D, kCut>), dim3((unsigned)n), dim3(kBlockThreads), BlockLds<D>::kBytes, s, A);
+    return ready;
+}
+
+template <int D>
+hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
+    const int n_wg = p.n_wg;
+    A.small = p.block ? kSplitMost : 0x7fffffff;
     // tiles: at most those of a whole table for each block of rows, and n_wg - 1 and a workgroup's share more in sums
     const long long row_blocks = (long long)A.a.T * A.G / kSplitRows + A.a.n_seq;
     const long long tiles = ((long long)A.a.width << A.c.page_log) / kSplitTok<D> + 1;
     A.narrow = row_blocks < (1ll << 31) / tiles / A.c.h_kv / 2 - n_wg;
-    if (block) {
-        static const hipError_t ready =
-            hipFuncSetAttribute(reinterpret_cast<const void*>(&block_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                BlockLds<D>::kBytes);
-        if (ready != hipSuccess) return ready;
-        hipLaunchKernelGGL((block_kernel<D>), dim3((unsigned)blocks), dim3(kBlockThreads), BlockLds<D>::kBytes, s, A);
+    if (p.block) {
+        const long long blocks = p.full + (long long)A.a.n_seq * A.c.h_kv;
+        hipError_t e;
+        if (p.cut) {
+            A.slots = p.slots;
+            A.items = 2 * p.slots;
+            A.block_part = A.part + split_bytes<D>(p) / sizeof(float);
+            e = launch_blocks<D, true>(A, std::max(blocks, (long long)A.items), s);
+            if (e == hipSuccess) hipLaunchKernelGGL((block_join_kernel<D>), dim3((unsigned)(2 * n_wg)), dim3(kJoinThreads), 0, s, A);
+        } else {
+            e = launch_blocks<D, false>(A, blocks, s);
+        }
+        if (e != hipSuccess) return e;
         if (A.a.n_seq == 1) return hipGetLastError();         // its only sequence is a long one
     }
     const unsigned lds = kSplitWaves * kSplitRows * (D + 4 + 2 + 1) * sizeof(float) + D / 64 * 2 * kWave * sizeof(uint4);
@@ -916,18 +1093,10 @@ hipError_t launch_attn(AttnArgs& A, int max_q, int n_wg, hipStream_t s) {
     return hipGetLastError();
 }
 
-size_t parts_bytes(int d, int n_wg) {
-    return d == 64 ? Parts<kSplitRows, 64>::bytes(n_wg) : d == 128 ? Parts<kSplitRows, 128>::bytes(n_wg)
-                                                                   : Parts<kSplitRows, 256>::bytes(n_wg);
-}
-
 bool attn_shape_ok(const Kv8& c, int n_seq, int T, int max_q, int h_q) {
     return n_seq > 0 && n_seq <= 65535 && T >= 0 && max_q >= 0 && (T == 0 || max_q > 0) && h_q > 0 && h_q % c.h_kv == 0 &&
            h_q <= 65536;
 }
-
-// Two workgroups a CU.
-int split_groups(hipStream_t s) { return 2 * device_cu_count(s); }
 
 }  // namespace
 }  // namespace ixg
@@ -938,7 +1107,8 @@ size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, i
     using namespace ixg;
     Kv8 c;
     if (!make_kv8(cache, &c) || !attn_shape_ok(c, n_seq, total_T, max_q, h_q)) return 0;
-    return parts_bytes(c.d, split_groups(nullptr));
+    const Plan p = plan_of(c.d, c.h_kv, h_q / c.h_kv, total_T, max_q, nullptr);
+    return c.d == 64 ? attn_bytes<64>(p) : c.d == 128 ? attn_bytes<128>(p) : attn_bytes<256>(p);
 }
 
 hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens,
@@ -968,11 +1138,11 @@ hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, c
     A.G = h_q / A.c.h_kv;
     A.window = window;
     A.sinks = sinks;
-    const int n_wg = split_groups(s);
+    const Plan p = plan_of(A.c.d, A.c.h_kv, A.G, total_T, max_q, s);
     switch (A.c.d) {
-        case 64: return launch_attn<64>(A, max_q, n_wg, s);
-        case 128: return launch_attn<128>(A, max_q, n_wg, s);
-        default: return launch_attn<256>(A, max_q, n_wg, s);
+        case 64: return launch_attn<64>(A, p, s);
+        case 128: return launch_attn<128>(A, p, s);
+        default: return launch_attn<256>(A, p, s);
     }
 }
 

@@ -51,10 +51,11 @@ __device__ __forceinline__ float max_abs(const uint4& x) {
     return m;
 }
 
-// Eight codes rint(x / s) by the reciprocal y of s: q = x y is within an ulp of the quotient, and q + (x - q s) y
-// is the quotient correctly rounded (Markstein: y is the reciprocal correctly rounded, and the remainder exact where
-// nothing underflows; a division is 10 instructions). 1.5 2^23 added to a number leaves its nearest integer, to even,
-// in the sum's low bits.
+// Eight codes rint(x / s) by the correctly rounded reciprocal y of s and one correction, q + (x - q s) y with q = x y (a
+// division is 10 instructions). Before its last rounding that is within 2^-21 ulp of x / s, so it can only be rounded
+// otherwise, and the code with it, where x / s lies that near half an ulp from a tie n + 1/2. x has 8 significant bits:
+// x = (n + 1/2)(1 +- 2^-k) s + that little has no solution but s = 2^e (1 - 2^-24), x = s rounded up / 2, which comes
+// out right. 1.5 2^23 added to a number leaves its nearest integer, to even, in the sum's low bits.
 constexpr float kMagic = 12582912.0f, kLeast = 1e-30f;
 __device__ __forceinline__ float code_bits(float x, float s, float y) {
     const float q = x * y;

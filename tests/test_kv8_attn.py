@@ -383,3 +383,47 @@ def test_offsets_past_32_bits():
     ws = torch.empty(n, dtype=torch.uint8, device="cuda")
     assert bx.ix_kv8_attn(*a, bf(P.q_bits), h * 4, P.scale, 0, 0, None, o, ws, n) == 0
     P.check(o.float().cpu().numpy())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,page", [(64, 16), (64, 128), (128, 32), (128, 64), (256, 16), (256, 128)])
+def test_blocks_in_parts(d, page):
+    """So few blocks of rows that several workgroups share one: each block's parts are joined, those in which nothing is
+    seen among them, and blocks that are too short for parts stand beside them."""
+    P = Problem([256], [256 + 2900], page, 4, d, 8, seed=d + page)
+    P.both(gate=True)
+    P.both(window=1111, sinks=70)
+    got = P.run()
+    assert np.array_equal(P.run(), got)
+    P = Problem([1, 140, 3, 0, 145, 37, 20], [900, 1500, 70, 40, 145, 2000, 10], page, 4, d, 8, seed=d * page)
+    P.tables[1, :1100 // page] = -1                              # parts without a token
+    P.tables[5, 700 // page:] = -1
+    P.both()
+    P.both(window=64, sinks=129, gate=True)
+    P.both(window=1200, sinks=0, max_q=3000)
+
+
+@pytest.mark.gpu
+def test_blocks_in_parts_of_many_sequences():
+    """More sequences than lanes, blocks among them from the first to the last."""
+    q = [1 + 7 * (i % 5 == 0) for i in range(150)]
+    q[0], q[63], q[64], q[149] = 70, 65, 33, 90
+    P = Problem(q, [n + 37 * i % 600 for i, n in enumerate(q)], 16, 2, 256, 8, seed=11)
+    P.both()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,h,width", [(1, 1024, 1 << 22), (70, 64, 1 << 20)])
+def test_tables_with_places_for_more_than_32_bits_of_tiles(n, h, width):
+    """The same bits with a table of so many places that counts of tiles could pass 32 bits."""
+    import torch
+    P = Problem([1 + i % 3 for i in range(n)], [3 + (41 * i) % 150 for i in range(n)], 16, h, 64, 1, seed=n)
+    want = P.run()
+    P.check(want)
+    wide = torch.full((n, width), -1, dtype=torch.int32, device="cuda")
+    wide[:, :P.tables.shape[1]] = ints(P.tables)
+    c, b, T, max_q, cu, kv, _, _ = P.args()
+    size = bx.ix_kv8_attn_workspace_size(c, b, T, max_q, h)
+    ws, o = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty(T, h, 64, dtype=torch.bfloat16, device="cuda")
+    assert bx.ix_kv8_attn(c, b, T, max_q, cu, kv, wide, width, bf(P.q_bits), h, P.scale, 0, 0, None, o, ws, size) == 0
+    assert np.array_equal(o.float().cpu().numpy(), want)
