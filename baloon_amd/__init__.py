@@ -481,4 +481,4 @@ def version() -> str:
     return lib().ix_gdn_version().decode()
 
 
-from .layer import GdnLayer  # noqa: E402,F401
+from .layer import AttnLayer, GdnLayer  # noqa: E402,F401

@@ -716,7 +716,7 @@ __device__ __forceinline__ Blocks all_blocks(const AttnArgs& A, int lane) {
     Blocks out;
     out.n = lane_of(wave_scan_int(sum), kWave - 1) * A.c.h_kv;
     kv = wave_max_int(kv);
-    if (A.window > 0) kv = min(kv, A.window + min(A.sinks, kv) + kBlockRows / A.G);
+    if (A.window > 0 && A.window < kv) kv = A.window + min(A.sinks, kv - A.window);
     const int p = lane + 1, rounds = (out.n * p + A.slots - 1) / A.slots;
     float cost = (float)rounds * ((float)kv / (float)(kBlockTok * p) + (p > 1 ? kPartCost<D> : 0.0f));
     if (p > 1 && (long long)out.n * p > A.items) cost = __builtin_inff();

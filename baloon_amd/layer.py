@@ -1,18 +1,21 @@
-"""GdnLayer: device-resident parameters and per-sequence states for one GDN layer.
+"""GdnLayer and AttnLayer: device-resident parameters and per-sequence states of one layer.
 
-A thin host object over the C ABI: it owns the conv weights, A_log, dt_bias, the recurrent
+GdnLayer is a thin host object over the C ABI: it owns the conv weights, A_log, dt_bias, the recurrent
 state block [n][h_v][d_v][d_k] fp32 (each head's state stored column by column), the conv
 state [n][C][d_conv-1] bf16, the gated output norm's weight ssm_norm [d_v] fp32 and the
 zeroed decode workspace, and calls ``ix_gdn_decode`` / ``ix_gdn_prefill`` (or their gated
 variants, when a gate input z is passed) on the current stream. Allocation happens here, at
 construction (and for the prefill workspace, on first use of a given size), never inside the
 library calls.
+
+AttnLayer is the same for the softmax attention layers that stand between GDN layers: it owns a paged 8-bit
+cache of keys and values and the lengths of its sequences, and calls ``ix_kv8_append`` and ``ix_kv8_attn``.
 """
 from __future__ import annotations
 
 import torch
 
-from . import (Cfg, check, ix_gdn_decode, ix_gdn_decode_gated, ix_gdn_decode_workspace_size, ix_gdn_prefill,
+from . import (Cfg, check, ix_kv8_append, ix_kv8_attn, ix_kv8_attn_workspace_size, kv8_cache, ix_gdn_decode, ix_gdn_decode_gated, ix_gdn_decode_workspace_size, ix_gdn_prefill,
                ix_gdn_prefill_gated, ix_gdn_prefill_gated_workspace_size, ix_gdn_prefill_workspace_size, make_cfg,
                out_gate)
 
@@ -62,3 +65,58 @@ class GdnLayer:
         else:
             g = out_gate(z, self.ssm_norm, self.norm_eps, y, y_bf16, y_q8_1)
             check("ix_gdn_prefill_gated", ix_gdn_prefill_gated(*args, g, self._ws, self._ws.numel(), stream))
+
+
+class AttnLayer:
+    """Attention of n_slots sequences of at most max_len tokens, h_q query heads over h_kv cached ones of d channels.
+
+    Slot i has pages i * width .. of the cache to itself; with n_pages the caller keeps the pages instead and fills
+    `table` [n_slots][width] int32 before they are needed. kv_len [n_slots] int32 counts the tokens held: setting it to 0
+    empties a slot, to fewer tokens drops the last ones (rejected drafts). Tokens behind max_len are dropped."""
+
+    def __init__(self, n_slots: int, max_len: int, h_q=16, h_kv=2, d=256, page=64, n_pages=None, window=0, sinks=0,
+                 scale=None, device="cuda"):
+        self.n_slots, self.h_q, self.h_kv, self.d = n_slots, h_q, h_kv, d
+        self.window, self.sinks, self.scale = window, sinks, d ** -0.5 if scale is None else scale
+        self.device = torch.device(device)
+        self.width = -(-max_len // page)
+
+        def tensor(*shape, dtype):
+            return torch.zeros(*shape, dtype=dtype, device=self.device)
+
+        pages = n_slots * self.width if n_pages is None else n_pages
+        self.cache = kv8_cache(tensor(pages, h_kv, page, d, dtype=torch.int8), tensor(pages, h_kv, d, page, dtype=torch.int8),
+                               tensor(pages, h_kv, dtype=torch.float32), tensor(pages, h_kv, dtype=torch.float32))
+        self.table = tensor(n_slots, self.width, dtype=torch.int32)
+        if n_pages is None:
+            self.table.copy_(torch.arange(pages, dtype=torch.int32).view(n_slots, self.width))
+        else:
+            self.table.fill_(-1)
+        self.kv_len = tensor(n_slots, dtype=torch.int32)
+        self._one_each = torch.arange(n_slots + 1, dtype=torch.int32, device=self.device)
+        self._ws = None
+
+    def prefill(self, cu_seqlens, max_q, q, k, v, gate=None, o=None, stream=None):
+        """Appends packed new tokens (cu_seqlens int32 [n_slots + 1] on the device, at most max_q of a sequence) and
+        returns their attention o [T][h_q][d] bf16. q and gate are rows of [h_q][d], k and v of [h_kv][d], bf16, with any
+        stride between rows; gate multiplies by its sigmoid. The lengths are advanced on torch's current stream."""
+        self.kv_len += cu_seqlens.diff()
+        return self._attend(cu_seqlens, max_q, q, k, v, gate, o, stream)
+
+    def decode(self, q, k, v, gate=None, o=None, stream=None):
+        """The same for one token of every sequence."""
+        self.kv_len += 1
+        return self._attend(self._one_each, 1, q, k, v, gate, o, stream)
+
+    def _attend(self, cu_seqlens, max_q, q, k, v, gate, o, stream):
+        T = q.shape[0]
+        if o is None:
+            o = torch.empty(T, self.h_q, self.d, dtype=torch.bfloat16, device=self.device)
+        need = ix_kv8_attn_workspace_size(self.cache, self.n_slots, T, max_q, self.h_q)
+        if self._ws is None or self._ws.numel() < need:
+            self._ws = torch.empty(max(need, 256), dtype=torch.uint8, device=self.device)
+        where = (cu_seqlens, self.kv_len, self.table, self.width)
+        check("ix_kv8_append", ix_kv8_append(self.cache, self.n_slots, T, *where, k, v, stream))
+        check("ix_kv8_attn", ix_kv8_attn(self.cache, self.n_slots, T, max_q, *where, q, self.h_q, self.scale, self.window,
+                                         self.sinks, gate, o, self._ws, self._ws.numel(), stream))
+        return o
