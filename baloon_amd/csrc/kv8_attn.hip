@@ -1040,6 +1040,7 @@ struct Plan {
     bool block, cut;          // block_kernel for sequences of more than kSplitMost rows; in parts
     int n_wg, slots;          // workgroups that the chip holds: of split_kernel two a CU, of block_kernel one or two
     long long full;           // whole blocks that the batch's rows fill
+    int max_q;
 };
 Plan plan_of(int d, int h_kv, int G, int T, int max_q, hipStream_t s) {
     Plan p;
@@ -1047,6 +1048,7 @@ Plan plan_of(int d, int h_kv, int G, int T, int max_q, hipStream_t s) {
     p.n_wg = 2 * n_cu;
     p.slots = d == 256 ? n_cu : 2 * n_cu;
     p.full = (long long)T * G / kBlockRows * h_kv;
+    p.max_q = max_q;
     p.block = (long long)max_q * G > kSplitMost && p.full >= least_blocks(d);
     p.cut = p.block && p.full < p.slots;
     return p;
@@ -1087,7 +1089,9 @@ hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
             e = launch_blocks<D, false>(A, blocks, s);
         }
         if (e != hipSuccess) return e;
-        if (A.a.n_seq == 1) return hipGetLastError();         // its only sequence is a long one
+        // With at most max_q new tokens in each other one, a sequence has at least these.
+        const long long shortest = A.a.T - (long long)(A.a.n_seq - 1) * p.max_q;
+        if (shortest * A.G > kSplitMost) return hipGetLastError();
     }
     const unsigned lds = kSplitWaves * kSplitRows * (D + 4 + 2 + 1) * sizeof(float) + D / 64 * 2 * kWave * sizeof(uint4);
     hipLaunchKernelGGL((split_kernel<D>), dim3((unsigned)n_wg), dim3(kSplitThreads), lds, s, A);
