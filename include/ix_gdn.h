@@ -404,9 +404,9 @@ hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_
                        const int32_t* table, int width, uint16_t* k, uint16_t* v,
                        hipStream_t s IX_GDN_DEFAULT_STREAM);
 
-/* Bytes of device workspace for ix_kv8_attn on such a batch (partial results of sequences that
- * several workgroups share; independent of the lengths), or 0 for an invalid request. It needs
- * no initialisation; calls that share it must be ordered. */
+/* Bytes of device workspace for ix_kv8_attn on such a batch (partial results of what several
+ * workgroups share; independent of the lengths, at most 81 MiB on 256 CUs), or 0 for an invalid
+ * request. It needs no initialisation; calls that share it must be ordered. */
 size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, int max_q, int h_q);
 
 /* Attention of the batch's tokens over the cache, which holds them already (ix_kv8_append):

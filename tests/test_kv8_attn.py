@@ -427,3 +427,12 @@ def test_tables_with_places_for_more_than_32_bits_of_tiles(n, h, width):
     ws, o = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty(T, h, 64, dtype=torch.bfloat16, device="cuda")
     assert bx.ix_kv8_attn(c, b, T, max_q, cu, kv, wide, width, bf(P.q_bits), h, P.scale, 0, 0, None, o, ws, size) == 0
     assert np.array_equal(o.float().cpu().numpy(), want)
+
+
+def test_workspace_sizes():
+    """Of the sizes only: single tokens need little, and any batch a bounded size."""
+    for d, few, most in ((64, 5, 38), (128, 9, 74), (256, 17, 81)):
+        c = desc(h=8, d=d)
+        assert bx.ix_kv8_attn_workspace_size(c, 1, 1, 1, 8) == bx.ix_kv8_attn_workspace_size(c, 500, 500, 1, 64) <= few << 20
+        for n, T, max_q in ((1, 1 << 20, 1 << 20), (1, 512, 512), (64, 64 * 512, 512), (65535, 1 << 20, 4000), (3, 130, 100)):
+            assert 0 < bx.ix_kv8_attn_workspace_size(c, n, T, max_q, 64) <= most << 20
