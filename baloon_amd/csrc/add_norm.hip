@@ -44,12 +44,35 @@ __device__ __forceinline__ void q81_store8(const float (&v)[8], int lane, uint8_
     }
     const float sum = ((s[0] + s[4]) + (s[2] + s[6])) + ((s[1] + s[5]) + (s[3] + s[7]));
     const float d = fminf(m / 127.0f, kHalfMax);
-    uint32_t q[2] = {0, 0};
+    // rint, halves away from 0, of v / d by its correctly rounded reciprocal and two corrections, which leave the quotient
+    // correctly rounded (Markstein; the second is needed where the first product is more than an ulp off), and 1/2 less half
+    // an ulp of it: a division and roundf for each value are 3 times the instructions, and the kernel takes 4.0 us for 8
+    // rows of 4,096 with them.
+    const auto bounded = [](float x, float most) { return fminf(fmaxf(x, -most), most); };
+    const float inv = 1.0f / d;
+    float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const int c = d == 0.0f ? 0 : (int)fminf(fmaxf(roundf(v[e] / d), -127.0f), 127.0f);
-        q[e / 4] |= (uint32_t)(uint8_t)(int8_t)c << (8 * (e & 3));
+        x[e] = bounded(v[e] * inv, 200.0f);
+        x[e] = bounded(fmaf(fmaf(-x[e], d, v[e]), inv, x[e]), 200.0f);
+        x[e] = bounded(fmaf(fmaf(-x[e], d, v[e]), inv, x[e]), 127.0f);
     }
+    if (d < 1e-30f) {                                         // 1 / d or the remainders could leave the floats' range
+        asm volatile("");
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+            float y = 0.0f;
+#pragma unroll
+            for (int f = 0; f < 8; ++f) y = f == e ? v[f] : y;
+            y = d == 0.0f ? 0.0f : bounded(y / d, 127.0f);
+#pragma unroll
+            for (int f = 0; f < 8; ++f) x[f] = f == e ? y : x[f];
+        }
+    }
+    uint32_t q[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        q[e / 4] |= (uint32_t)(uint8_t)(int8_t)(int)(x[e] + copysignf(0x1.fffffep-2f, x[e])) << (8 * (e & 3));
     if (!blk) return;
     uint32_t* to = reinterpret_cast<uint32_t*>(blk + 4 + 8 * (lane & 3));    // blocks are 36 bytes: 4-byte stores
     to[0] = q[0];
