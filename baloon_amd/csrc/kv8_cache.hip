@@ -14,15 +14,15 @@
 //
 // One workgroup per (page with new tokens, head, K or V): it alone reads and writes that scale and those
 // codes, reads the rows once into LDS, and turns the values there. 16 sequences of 1 to 2,048 new tokens, 2 heads of
-// 256, 15,059 tokens in all: 46 MB in 16.8 us, 2.8 TB/s of a copy's 5.3. A workgroup's pass is a chain (its place, the
-// rows, their largest value, the codes), 4 workgroups a CU of it side by side; a read of the same tokens takes 11.6 us.
-// One token for each of 64 sequences: 5.4 and 4.2 us, launches and that chain.
+// 256, 15,059 tokens in all: 46 MB in 15 us, 3.1 TB/s of a copy's 5.3. A workgroup's pass is a chain (its place, the
+// rows, their largest value, the codes), 3 workgroups a CU of it side by side; a read of the same tokens takes 10 to 11 us.
+// One token for each of 64 sequences: 5.2 and 4.2 us, launches and that chain.
+#include <type_traits>
+
 #include "kv8.h"
 
 namespace ixg {
 namespace {
-
-constexpr int kCacheThreads = 256;
 
 // The page that slot j of the grid stands for. Sequence b owns the slots from cu[b] / page + 2 b on: at most
 // q / page + 2 pages hold its q new tokens, so no prefix sum over the sequences is needed.
@@ -135,11 +135,12 @@ __device__ __forceinline__ Turn turn_of(int i, int span_log) {
 // the 16s together). The second pass is a rolled loop: every launch begins with an empty instruction cache, and with it
 // unrolled 8, 4 and 2 times a single token for 64 sequences took 7.9, 6.6 and 5.5 us of the kernel's time.
 constexpr int kBatch = 4;
-__global__ void __launch_bounds__(kCacheThreads)
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads)
 append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_stride, const uint16_t* __restrict__ vr,
               long long v_stride) {
     extern __shared__ uint4 raw[];
-    __shared__ float red[kCacheThreads / kWave];
+    __shared__ float red[kThreads / kWave];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), h = blockIdx.y;
     const bool is_v = blockIdx.z;
     PageJob job;
@@ -155,28 +156,29 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
     const float old = job.held > 0 ? *scale : 0.0f;
     float m = 0.0f;
     uint4* held = raw + (job.held << per_log);
-    for (int i0 = tid; i0 < chunks; i0 += kBatch * kCacheThreads) {
+    for (int i0 = tid; i0 < chunks; i0 += kBatch * kThreads) {
         uint4 x[kBatch];
 #pragma unroll
-        for (int y = 0; y < kBatch; ++y) x[y] = i0 + y * kCacheThreads < chunks ? load(i0 + y * kCacheThreads) : make_uint4(0, 0, 0, 0);
+        for (int y = 0; y < kBatch; ++y) x[y] = i0 + y * kThreads < chunks ? load(i0 + y * kThreads) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int y = 0; y < kBatch; ++y) {
             m = fmaxf(m, max_abs(x[y]));
-            if (i0 + y * kCacheThreads < chunks) held[i0 + y * kCacheThreads] = x[y];
+            if (i0 + y * kThreads < chunks) held[i0 + y * kThreads] = x[y];
         }
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
     if (lane == 0) red[tid / kWave] = m;
     __syncthreads();                                          // every thread has read the old scale, too
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+    for (int i = 0; i < kThreads / kWave; ++i) m = fmaxf(m, red[i]);
     const float s = fmaxf(old, m / 127.0f);
     const bool grown = job.held > 0 && s > old;
     const float ratio = grown ? old / s : 1.0f, inv = 1.0f / s;
     if (tid == 0) *scale = s;
 
 #pragma unroll 1
-    for (int i = tid; i < chunks; i += kCacheThreads) {       // a thread's own chunks
+    for (int i = tid; i < chunks; i += kThreads) {       // a thread's own chunks
         const int slot = job.held + (i >> per_log);
         const uint2 q = s < kLeast ? codes_of_small(held[i], s) : codes_of(held[i], s, inv);
         if (is_v) reinterpret_cast<uint2*>(held + i)[slot >> 4 & 1] = q;
@@ -185,7 +187,7 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
     if (!is_v) {
         if (grown) {
             uint4* p = reinterpret_cast<uint4*>(codes);
-            for (int i = tid; i < job.held * c.d / 16; i += kCacheThreads) {
+            for (int i = tid; i < job.held * c.d / 16; i += kThreads) {
                 const uint4 o = p[i];
                 p[i] = make_uint4(recode4(o.x, ratio), recode4(o.y, ratio), recode4(o.z, ratio), recode4(o.w, ratio));
             }
@@ -196,7 +198,7 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
     // Channel rows of 16 slots: whole ones at once (slots behind the new tokens hold nothing yet, and get
     // zeros), the one with older tokens in it by bytes, or as a whole where the older ones change too.
     const int span_log = c.page_log - 4;
-    for (int i = tid; i < (c.d / 4) << span_log; i += kCacheThreads) {
+    for (int i = tid; i < (c.d / 4) << span_log; i += kThreads) {
         const Turn u = turn_of(i, span_log);
         if (u.s0 >= job.end || (u.s0 + 16 <= job.held && !grown)) continue;
         const int keep = job.end - u.s0;                      // slots that hold tokens
@@ -234,8 +236,9 @@ __device__ __forceinline__ uint4 values8(uint32_t lo, uint32_t hi, float s) {
     return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-__global__ void __launch_bounds__(kCacheThreads)
-read_kernel(Kv8 c, Batch a, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo, bool wide) {
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads)
+read_kernel(Kv8 c, Batch a, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo) {
     extern __shared__ uint8_t tile[];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), h = blockIdx.y;
     const bool is_v = blockIdx.z;
@@ -245,9 +248,9 @@ read_kernel(Kv8 c, Batch a, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo
     const size_t ph = (size_t)job.id * c.h_kv + h;
     const float s = (is_v ? c.v_scale : c.k_scale)[ph];
     const int8_t* codes = (is_v ? c.v : c.k) + ph * c.page * c.d;
-    const int per = c.d / 8, pitch = c.d + 4, span_log = c.page_log - 4;      // rows of slots 4 bytes longer: 16 slots on, other banks
+    const int per_log = c.d == 64 ? 3 : c.d == 128 ? 4 : 5, pitch = c.d + 4, span_log = c.page_log - 4;      // rows of slots 4 bytes longer: 16 slots on, other banks
     if (is_v) {
-        for (int i = tid; i < (c.d / 4) << span_log; i += kCacheThreads) {
+        for (int i = tid; i < (c.d / 4) << span_log; i += kThreads) {
             const Turn u = turn_of(i, span_log);
             if (u.s0 >= job.end || u.s0 + 16 <= job.held) continue;
             uint32_t n[4][4];                                 // [4 slots][channel]
@@ -265,8 +268,8 @@ read_kernel(Kv8 c, Batch a, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo
         }
         __syncthreads();
     }
-    for (int i = tid + job.held * per; i < job.end * per; i += kCacheThreads) {
-        const int slot = i / per, col = (i - slot * per) * 8;
+    for (int i = tid + (job.held << per_log); i < job.end << per_log; i += kThreads) {
+        const int slot = i >> per_log, col = (i & ((1 << per_log) - 1)) << 3;
         uint2 q;
         if (is_v) {
             const uint32_t* p = reinterpret_cast<const uint32_t*>(tile + slot * pitch + col);
@@ -276,18 +279,43 @@ read_kernel(Kv8 c, Batch a, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo
         }
         const uint4 v = values8(q.x, q.y, s);
         uint16_t* to = out + ((size_t)(job.row + slot - job.held) * c.h_kv + h) * c.d + col;
-        if (wide) {
-            *reinterpret_cast<uint4*>(to) = v;
-        } else {
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) to[e] = (uint16_t)(u[e / 2] >> (16 * (e & 1)));
-        }
+        __builtin_memcpy(to, &v, sizeof(v));                  // at any 2-byte address
     }
 }
 
 dim3 page_grid(const Kv8& c, const Batch& a) {
     return dim3((unsigned)(a.T >> c.page_log) + 2u * (unsigned)a.n_seq, (unsigned)c.h_kv, 2);
+}
+
+// A thread for 32 values of a page; in appends for 64 where the sequences have less than a page of new tokens each. A
+// workgroup is bound by the chain of its reads: more threads make it shorter where there is work for them, and keep other
+// workgroups from the CU where not. With 16, 32, 64 and 128 values a thread an append takes, us: 16 x 1,024 tokens on 8 heads
+// of 128, pages of 64, 32, 24, 26, 30; on 2 heads of 256, pages of 16, 16, 14, 15, 15; 64 x 16 tokens on the former 10.7,
+// 9.2, 8.1, 9.7; 256 single tokens 16.7, 14.2, 14.2, 14.8, and on 2 heads of 256, pages of 64, 9.9, 8.7, 8.6, 9.7. A read of
+// the first takes 17.9, 17.7, 17.9, 17.6, of 64 pages of 16 tokens on 2 heads of 256 3.3, 3.5, 3.6, 3.6, of 1 x 4,096 4.5,
+// 4.6, 5.2, 5.2.
+template <class F>
+hipError_t with_threads(int n, F launch) {
+    if (n <= 64) return launch(std::integral_constant<int, 64>{});
+    if (n <= 128) return launch(std::integral_constant<int, 128>{});
+    if (n <= 256) return launch(std::integral_constant<int, 256>{});
+    return launch(std::integral_constant<int, 512>{});
+}
+
+template <int kThreads>
+hipError_t launch_append(const Kv8& c, const Batch& a, const ix_rows* k, const ix_rows* v, hipStream_t s) {
+    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(&append_kernel<kThreads>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 256 * sizeof(uint16_t));
+    if (ready != hipSuccess) return ready;
+    hipLaunchKernelGGL((append_kernel<kThreads>), page_grid(c, a), dim3(kThreads), c.page * c.d * sizeof(uint16_t), s, c, a,
+                       k->p, k->stride, v->p, v->stride);
+    return hipGetLastError();
+}
+
+template <int kThreads>
+hipError_t launch_read(const Kv8& c, const Batch& a, uint16_t* k, uint16_t* v, hipStream_t s) {
+    hipLaunchKernelGGL((read_kernel<kThreads>), page_grid(c, a), dim3(kThreads), c.page * (c.d + 4), s, c, a, k, v);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -303,12 +331,8 @@ hipError_t ix_kv8_append(const ix_kv8* cache, int n_seq, int total_T, const int3
     if (!make_kv8(cache, &c) || !make_batch(n_seq, total_T, cu_seqlens, kv_len, table, width, &a)) return hipErrorInvalidValue;
     if (!rows_ok(k, (long long)c.h_kv * c.d) || !rows_ok(v, (long long)c.h_kv * c.d)) return hipErrorInvalidValue;
     if (total_T == 0) return hipSuccess;
-    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(&append_kernel),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 256 * sizeof(uint16_t));
-    if (ready != hipSuccess) return ready;
-    hipLaunchKernelGGL(append_kernel, page_grid(c, a), dim3(kCacheThreads), c.page * c.d * sizeof(uint16_t), s, c, a, k->p, k->stride,
-                       v->p, v->stride);
-    return hipGetLastError();
+    const int few = a.T < (long long)c.page * a.n_seq ? 2 : 1;
+    return with_threads(c.page * c.d / 32 / few, [&](auto n) { return launch_append<n>(c, a, k, v, s); });
 }
 
 hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_t* cu_seqlens, const int32_t* kv_len,
@@ -319,9 +343,7 @@ hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_
     if (!make_kv8(cache, &c) || !make_batch(n_seq, total_T, cu_seqlens, kv_len, table, width, &a)) return hipErrorInvalidValue;
     if ((!k && !v) || !ptr_aligned(k, 2) || !ptr_aligned(v, 2)) return hipErrorInvalidValue;
     if (total_T == 0) return hipSuccess;
-    hipLaunchKernelGGL(read_kernel, page_grid(c, a), dim3(kCacheThreads), c.page * (c.d + 4), s, c, a, k, v,
-                       ptr_aligned(k, 16) && ptr_aligned(v, 16));
-    return hipGetLastError();
+    return with_threads(c.page * c.d / 32, [&](auto n) { return launch_read<n>(c, a, k, v, s); });
 }
 
 }  // extern "C"
