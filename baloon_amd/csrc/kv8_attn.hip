@@ -160,7 +160,7 @@ __device__ __forceinline__ long long quotient(long long a, int b) { return (long
 // segments over 512 workgroups, took 52 us without and 40 with 3 or 6). Every wave works its share out by itself from the
 // lengths, in 32 bits where the batch cannot have 2^31 tiles (each launch fetches its instructions anew: 250 of them
 // took 1.3 us).
-constexpr int kMinShare = 4;          // tiles: one for each wave
+constexpr int kMinShare = 4;          // tiles
 constexpr int kStart = 6;             // tiles of 16 KiB in the time of a segment's start
 struct Share {
     int per, left, start;             // counts of every workgroup and of this one, and in front of a segment
@@ -187,7 +187,9 @@ __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int
     if (segments * start < n_wg) start = 0;                   // less than a tile for each
     const Int total = tiles + segments * start;
     out->start = start;
-    out->per = (int)max(quotient((Int)(total + n_wg - 1), n_wg), (Int)kMinShare);
+    // At least a tile for each wave, but not several segments for want of them.
+    const int least = segments * kMinShare > tiles ? 1 : kMinShare;
+    out->per = max((int)quotient((Int)(total + n_wg - 1), n_wg), least);
     const Int cur = (Int)w * out->per;
     if (cur >= total) return false;
     out->left = (int)min((Int)out->per, (Int)(total - cur));
