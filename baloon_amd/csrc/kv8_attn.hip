@@ -160,7 +160,12 @@ __device__ __forceinline__ long long quotient(long long a, int b) { return (long
 // segments over 512 workgroups, took 52 us without and 40 with 3 or 6). Every wave works its share out by itself from the
 // lengths, in 32 bits where the batch cannot have 2^31 tiles (each launch fetches its instructions anew: 250 of them
 // took 1.3 us).
-constexpr int kMinShare = 4;          // tiles
+//
+// A share is at least kMinShare tiles, one for each wave, but a segment where those have fewer on average, and where
+// up to kWhole tiles make segments that a quarter of the workgroups can take: 16 sequences over 8 heads of 128 take, us, with
+// 1 token each 8.4 (18.6 as 4 tiles), 100 8.6 (12.2) and 300 10.3 (13.3); 64 over 2 of 256, 300 each, 13.3 (18.2), but 4 drafts
+// of 8 heads each there, 256 segments, 27.0 (22.7); one of 1,000 over 8 of 128, 16 tiles, 13.4 (10.3).
+constexpr int kMinShare = 4, kWhole = 10;
 constexpr int kStart = 6;             // tiles of 16 KiB in the time of a segment's start
 struct Share {
     int per, left, start;             // counts of every workgroup and of this one, and in front of a segment
@@ -187,8 +192,8 @@ __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int
     if (segments * start < n_wg) start = 0;                   // less than a tile for each
     const Int total = tiles + segments * start;
     out->start = start;
-    // At least a tile for each wave, but not several segments for want of them.
-    const int least = segments * kMinShare > tiles ? 1 : kMinShare;
+    const int mean = (int)min((Int)(kWhole + 1), quotient((Int)(tiles + segments - 1), (int)max(segments, (Int)1)));
+    const int least = mean <= kMinShare || (mean <= kWhole && 4 * segments <= n_wg) ? mean : kMinShare;
     out->per = max((int)quotient((Int)(total + n_wg - 1), n_wg), least);
     const Int cur = (Int)w * out->per;
     if (cur >= total) return false;
