@@ -727,10 +727,11 @@ constexpr int kLeastPart = 4;         // tiles
 template <int D>
 __device__ __forceinline__ Blocks all_blocks(const AttnArgs& A, int lane) {
     int sum = 0, kv = 0;
+#pragma unroll 4
     for (int b0 = 0; b0 < A.a.n_seq; b0 += kWave) {
-        const int v = blocks_of(A, b0 + lane);
+        const int v = blocks_of(A, b0 + lane), held = A.a.kv_len[min(b0 + lane, A.a.n_seq - 1)];
         sum += v;
-        if (v > 0) kv = max(kv, A.a.kv_len[b0 + lane]);
+        kv = max(kv, v > 0 ? held : 0);
     }
     Blocks out;
     out.n = lane_of(wave_scan_int(sum), kWave - 1) * A.c.h_kv;
@@ -1094,16 +1095,17 @@ hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
     const long long tiles = ((long long)A.a.width << A.c.page_log) / kSplitTok<D> + 1;
     A.narrow = row_blocks < (1ll << 31) / tiles / A.c.h_kv / 2 - n_wg;
     if (p.block) {
-        const long long blocks = p.full + (long long)A.a.n_seq * A.c.h_kv;
         hipError_t e;
         if (p.cut) {
+            // a sequence has at most one block that is not full, and more than kSplitMost rows
+            const long long blocks = p.full + std::min((long long)A.a.n_seq, (long long)A.a.T * A.G / kSplitMost) * A.c.h_kv;
             A.slots = p.slots;
             A.items = 2 * p.slots;
             A.block_part = A.part + split_bytes<D>(p) / sizeof(float);
             e = launch_blocks<D, true>(A, std::max(blocks, (long long)A.items), s);
             if (e == hipSuccess) hipLaunchKernelGGL((block_join_kernel<D>), dim3((unsigned)(2 * n_wg)), dim3(kJoinThreads), 0, s, A);
         } else {
-            e = launch_blocks<D, false>(A, blocks, s);
+            e = launch_blocks<D, false>(A, p.full + (long long)A.a.n_seq * A.c.h_kv, s);
         }
         if (e != hipSuccess) return e;
         // With at most max_q new tokens in each other one, a sequence has at least these.
