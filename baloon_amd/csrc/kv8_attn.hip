@@ -162,10 +162,11 @@ __device__ __forceinline__ long long quotient(long long a, int b) { return (long
 // took 1.3 us).
 //
 // A share is at least kMinShare tiles, one for each wave, but a segment where those have fewer on average, and where
-// up to kWhole tiles make segments that a quarter of the workgroups can take: 16 sequences over 8 heads of 128 take, us, with
-// 1 token each 8.4 (18.6 as 4 tiles), 100 8.6 (12.2) and 300 10.3 (13.3); 64 over 2 of 256, 300 each, 13.3 (18.2), but 4 drafts
-// of 8 heads each there, 256 segments, 27.0 (22.7); one of 1,000 over 8 of 128, 16 tiles, 13.4 (10.3).
-constexpr int kMinShare = 4, kWhole = 10;
+// there is a workgroup for each and they have up to kWhole: joining costs more than a few tiles one after another. 64
+// sequences over 8 heads of 128 take, us, with 1 token each 9.3 (18.6 as 4 tiles), 32 with 300 10.2 (15.3) and with 800 16.0
+// (18.0); 128 over 2 of 256 with 200 12.9 (20.1) and with 450, 15 tiles, 18.3 (23.5). From 16 tiles on few segments are
+// slower whole: 8 sequences over 8 heads of 128, 1,020 tokens each, 13.6 (10.7).
+constexpr int kMinShare = 4, kWhole = 15;
 constexpr int kStart = 6;             // tiles of 16 KiB in the time of a segment's start
 struct Share {
     int per, left, start;             // counts of every workgroup and of this one, and in front of a segment
@@ -181,6 +182,7 @@ __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int
         if (b0 + lane < n) s = span_at<ROWS, TOK>(A, b0 + lane);
     };
     Int tiles = 0, segments = 0;
+#pragma unroll 4
     for (int b0 = (n - 1) & ~(kWave - 1); b0 >= 0; b0 -= kWave) {
         span(b0);
         tiles += (Int)s.nrb * s.nt * h_kv;
@@ -193,7 +195,7 @@ __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int
     const Int total = tiles + segments * start;
     out->start = start;
     const int mean = (int)min((Int)(kWhole + 1), quotient((Int)(tiles + segments - 1), (int)max(segments, (Int)1)));
-    const int least = mean <= kMinShare || (mean <= kWhole && 4 * segments <= n_wg) ? mean : kMinShare;
+    const int least = mean <= kMinShare || (mean <= kWhole && segments <= n_wg) ? mean + start : kMinShare;
     out->per = max((int)quotient((Int)(total + n_wg - 1), n_wg), least);
     const Int cur = (Int)w * out->per;
     if (cur >= total) return false;
