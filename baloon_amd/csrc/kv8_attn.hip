@@ -763,7 +763,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     int b, rb, parts = 1, part = 0;
     if constexpr (kCut) {
         const Blocks all = all_blocks<D>(A, lane);
-        if (blockIdx.x >= all.n * all.parts) return;
+        if ((int)blockIdx.x >= all.n * all.parts) return;
         const int i = blockIdx.x / A.c.h_kv;
         parts = all.parts;
         part = i % parts;

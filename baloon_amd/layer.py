@@ -15,9 +15,9 @@ from __future__ import annotations
 
 import torch
 
-from . import (Cfg, check, ix_kv8_append, ix_kv8_attn, ix_kv8_attn_workspace_size, kv8_cache, ix_gdn_decode, ix_gdn_decode_gated, ix_gdn_decode_workspace_size, ix_gdn_prefill,
-               ix_gdn_prefill_gated, ix_gdn_prefill_gated_workspace_size, ix_gdn_prefill_workspace_size, make_cfg,
-               out_gate)
+from . import (Cfg, IxGdnError, check, ix_gdn_decode, ix_gdn_decode_gated, ix_gdn_decode_workspace_size, ix_gdn_prefill,
+               ix_gdn_prefill_gated, ix_gdn_prefill_gated_workspace_size, ix_gdn_prefill_workspace_size,
+               ix_kv8_append, ix_kv8_attn, ix_kv8_attn_workspace_size, kv8_cache, make_cfg, out_gate)
 
 
 class GdnLayer:
@@ -100,23 +100,32 @@ class AttnLayer:
         """Appends packed new tokens (cu_seqlens int32 [n_slots + 1] on the device, at most max_q of a sequence) and
         returns their attention o [T][h_q][d] bf16. q and gate are rows of [h_q][d], k and v of [h_kv][d], bf16, with any
         stride between rows; gate multiplies by its sigmoid. The lengths are advanced on torch's current stream."""
-        self.kv_len += cu_seqlens.diff()
-        return self._attend(cu_seqlens, max_q, q, k, v, gate, o, stream)
+        if cu_seqlens.shape != (self.n_slots + 1,):
+            raise ValueError("baloon_amd: cu_seqlens has an offset for each sequence and one more")
+        return self._attend(cu_seqlens.diff(), cu_seqlens, max_q, q, k, v, gate, o, stream)
 
     def decode(self, q, k, v, gate=None, o=None, stream=None):
         """The same for one token of every sequence."""
-        self.kv_len += 1
-        return self._attend(self._one_each, 1, q, k, v, gate, o, stream)
+        if q.shape[0] != self.n_slots:
+            raise ValueError("baloon_amd: one token for each sequence")
+        return self._attend(1, self._one_each, 1, q, k, v, gate, o, stream)
 
-    def _attend(self, cu_seqlens, max_q, q, k, v, gate, o, stream):
+    def _attend(self, new, cu_seqlens, max_q, q, k, v, gate, o, stream):
         T = q.shape[0]
+        if k.shape[0] != T or v.shape[0] != T or (gate is not None and gate.shape[0] != T):
+            raise ValueError("baloon_amd: q, k, v and gate have a row for each token")
         if o is None:
             o = torch.empty(T, self.h_q, self.d, dtype=torch.bfloat16, device=self.device)
         need = ix_kv8_attn_workspace_size(self.cache, self.n_slots, T, max_q, self.h_q)
         if self._ws is None or self._ws.numel() < need:
             self._ws = torch.empty(max(need, 256), dtype=torch.uint8, device=self.device)
         where = (cu_seqlens, self.kv_len, self.table, self.width)
-        check("ix_kv8_append", ix_kv8_append(self.cache, self.n_slots, T, *where, k, v, stream))
-        check("ix_kv8_attn", ix_kv8_attn(self.cache, self.n_slots, T, max_q, *where, q, self.h_q, self.scale, self.window,
-                                         self.sinks, gate, o, self._ws, self._ws.numel(), stream))
+        self.kv_len += new
+        try:
+            check("ix_kv8_append", ix_kv8_append(self.cache, self.n_slots, T, *where, k, v, stream))
+            check("ix_kv8_attn", ix_kv8_attn(self.cache, self.n_slots, T, max_q, *where, q, self.h_q, self.scale, self.window,
+                                             self.sinks, gate, o, self._ws, self._ws.numel(), stream))
+        except IxGdnError:
+            self.kv_len -= new                                # a refused call leaves the lengths as they were
+            raise
         return o

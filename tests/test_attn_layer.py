@@ -65,6 +65,21 @@ def test_prompts_drafts_tokens(own_pages, window, sinks):
             assert np.all(np.abs(got[cu[b]:cu[b + 1]] - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -9 * (np.abs(vv).max() if m else 0))
 
 
+def test_refusals():
+    import torch
+    layer = bx.AttnLayer(2, 64, 4, 2, 64, 16)
+    q, k = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 2, 64, dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: layer.decode(q[:1], k[:1], k[:1]), lambda: layer.decode(q, k[:1], k), lambda: layer.decode(q, k, k, q[:1]),
+                 lambda: layer.prefill(ints([0, 2]), 2, q, k, k)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(bx.IxGdnError):
+        layer.prefill(ints([0, 1, 2]), 0, q, k, k)              # no new tokens at most
+    assert layer.kv_len.tolist() == [0, 0]
+    with pytest.raises(bx.IxGdnError):
+        bx.AttnLayer(2, 64, 5, 2, 64, 16).decode(torch.zeros(2, 5, 64, dtype=torch.bfloat16, device="cuda"), k, k)
+
+
 def test_hybrid_stack():
     """Generated token by token, the stack ends where one prompt of all the tokens ends. The two differ by roundings of the
     layers' bf16 outputs and of pages' scales that grow in different steps, 2^-9 and 2^-8 of a value each over 4 layers of
