@@ -1091,7 +1091,11 @@ hipError_t launch_blocks(const AttnArgs& A, long long n, hipStream_t s) {
 template <int D>
 hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
     const int n_wg = p.n_wg;
-    A.small = p.block ? kSplitMost : 0x7fffffff;
+    // With at most max_q new tokens in each other one, a sequence of the batch has at least these. Where that is more than
+    // kSplitMost rows all are block_kernel's (also those of a batch whose offsets end before T), and it is the only launch.
+    const long long shortest = A.a.T - (long long)(A.a.n_seq - 1) * p.max_q;
+    const bool only = p.block && shortest * A.G > kSplitMost;
+    A.small = only ? 0 : p.block ? kSplitMost : 0x7fffffff;
     // tiles: at most those of a whole table for each block of rows, and n_wg - 1 and a workgroup's share more in sums
     const long long row_blocks = (long long)A.a.T * A.G / kSplitRows + A.a.n_seq;
     const long long tiles = ((long long)A.a.width << A.c.page_log) / kSplitTok<D> + 1;
@@ -1100,7 +1104,8 @@ hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
         hipError_t e;
         if (p.cut) {
             // a sequence has at most one block that is not full, and more than kSplitMost rows
-            const long long blocks = p.full + std::min((long long)A.a.n_seq, (long long)A.a.T * A.G / kSplitMost) * A.c.h_kv;
+            const long long most = only ? A.a.n_seq : std::min((long long)A.a.n_seq, (long long)A.a.T * A.G / kSplitMost);
+            const long long blocks = p.full + most * A.c.h_kv;
             A.slots = p.slots;
             A.items = 2 * p.slots;
             A.block_part = A.part + split_bytes<D>(p) / sizeof(float);
@@ -1110,9 +1115,7 @@ hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
             e = launch_blocks<D, false>(A, p.full + (long long)A.a.n_seq * A.c.h_kv, s);
         }
         if (e != hipSuccess) return e;
-        // With at most max_q new tokens in each other one, a sequence has at least these.
-        const long long shortest = A.a.T - (long long)(A.a.n_seq - 1) * p.max_q;
-        if (shortest * A.G > kSplitMost) return hipGetLastError();
+        if (only) return hipGetLastError();
     }
     const unsigned lds = kSplitWaves * kSplitRows * (D + 4 + 2 + 1) * sizeof(float) + D / 64 * 2 * kWave * sizeof(uint4);
     hipLaunchKernelGGL((split_kernel<D>), dim3((unsigned)n_wg), dim3(kSplitThreads), lds, s, A);

@@ -436,3 +436,22 @@ def test_workspace_sizes():
         assert bx.ix_kv8_attn_workspace_size(c, 1, 1, 1, 8) == bx.ix_kv8_attn_workspace_size(c, 500, 500, 1, 64) <= few << 20
         for n, T, max_q in ((1, 1 << 20, 1 << 20), (1, 512, 512), (64, 64 * 512, 512), (65535, 1 << 20, 4000), (3, 130, 100)):
             assert 0 < bx.ix_kv8_attn_workspace_size(c, n, T, max_q, 64) <= most << 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[3, 2, 1], [200, 1, 0], [0, 0, 256], [90, 90, 90]])
+def test_offsets_that_end_before_the_rows(lens):
+    """Room for 256 rows a sequence, as a captured call keeps it, of which the offsets use fewer: the rest is not written."""
+    import torch
+    P = Problem(lens, [n + 700 for n in lens], 16, 4, 256, 8, seed=sum(lens))
+    P.upload()
+    c, n, T, _, cu, kv, table, width = P.args()
+    room = 3 * 256
+    q = torch.zeros(room, 32, 256, dtype=torch.bfloat16, device="cuda")
+    q[:T] = bf(P.q_bits)[:T]
+    o = torch.full_like(q, 7)
+    size = bx.ix_kv8_attn_workspace_size(c, n, room, 256, 32)
+    ws = torch.full((size,), 0xFF, dtype=torch.uint8, device="cuda")
+    assert bx.ix_kv8_attn(c, n, room, 256, cu, kv, table, width, q, 32, P.scale, 0, 0, None, o, ws, size) == 0
+    P.check(o[:T].float().cpu().numpy())
+    assert bool((o[T:] == 7).all())
