@@ -61,6 +61,47 @@ __device__ __forceinline__ float pair_max32(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// A page's value scale vs weighs its values, not its tokens, so the sum of p has a reference of its own. The values'
+// product takes p' = p vs = 2^(score + log2 vs) relative to the largest of those; the sum takes p = 2^score relative to a
+// score of the lane's own tokens, which is at most 2^kFar below another. A lane's tokens of a tile are of one page, so p is p' times
+// one factor for all of them. Where that would pass 2^kFar (the page's values next to nothing beside others) p' may be
+// gone from 32 bits, and p is worked out by itself.
+constexpr float kFar = 60.0f;
+// log2 of a page's scale. A page of zeros has none and only takes part in the sum: 2^kNoValue is so far under the least
+// scale, 2^-149, that what the product loses when such a page's p' is its largest is under any bf16 number.
+constexpr float kNoValue = -200.0f;
+__device__ __forceinline__ float log2_scale(float vs) { return vs == 0.0f ? kNoValue : log2f(vs); }
+
+// The sum of a lane's p: l 2^ref.
+struct LaneSum {
+    float l = 0.0f, ref = -__builtin_inff();
+    // Before tokens of which the largest score is `most`, -inf where none is seen.
+    __device__ __forceinline__ void raise(float most) {
+        if (most > ref + kFar) {
+            l *= __builtin_amdgcn_exp2f(ref - most);
+            ref = most;
+        }
+    }
+    // Adds tokens with scores x[] + shift, the largest of them `most`, whose p' relative to 2^to have this sum.
+    template <int N>
+    __device__ __forceinline__ void add(const float (&x)[N], float shift, float most, float sum, float to, float lv) {
+        const float e = to - ref - lv;                        // to and ref, nearly the same or both large, first
+        if (e > kFar && most > -__builtin_inff()) {
+            asm volatile("");                                 // a branch: hardly ever taken
+#pragma unroll
+            for (int y = 0; y < N; ++y) l += __builtin_amdgcn_exp2f(x[y] + (shift - ref));
+        } else {
+            l = fmaf(sum, __builtin_amdgcn_exp2f(fminf(e, kFar)), l);      // of a hidden page's scale, whatever it is: 0 times that
+        }
+    }
+    // log2 of the sum of a row's four lanes.
+    __device__ __forceinline__ float log2_row() const {
+        const float top = pair_max32(pair_max16(ref));
+        const float f = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - top);
+        return top + __builtin_amdgcn_logf(pair_sum32(pair_sum16(l * f)));
+    }
+};
+
 // The largest |x| among bf16 pairs as bits, on which NaN is above infinity.
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ u16x2 max_abs_bits(u16x2 m, const uint4& x) {
@@ -268,6 +309,38 @@ __device__ __forceinline__ uint2 load_gate(const AttnArgs& A, int t, int h, int 
     if (A.gate) __builtin_memcpy(&z, A.gate + (long long)t * A.gate_stride + (size_t)h * A.c.d + d, sizeof(z));
     return z;
 }
+// 4 outputs of a row from its sum of p' and its sum of p, 2^m o and 2^lse: o 2^(m - lse), of which the power alone can leave the
+// floats' range.
+__device__ __forceinline__ v4f outputs(v4f o, float m, float lse) {
+    if (lse == -__builtin_inff()) return v4f{0, 0, 0, 0};
+    const float f = __builtin_amdgcn_exp2f(0.5f * (m - lse));
+    return o * f * f;
+}
+// Partial results of a row put together: sums of p' relative to 2^m, and logarithms of the sums of p.
+struct Joined {
+    float m = -__builtin_inff(), top = -__builtin_inff(), total = 0.0f;      // total 2^top: the sum of p
+    v4f o = {0, 0, 0, 0};
+    static __device__ __forceinline__ float power(float x, float to) {       // 2^(x - to), 0 for x = -inf
+        return x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x - to);
+    }
+    // The references, before what is added is.
+    __device__ __forceinline__ void meet(float pm, float lse) {
+        m = fmaxf(m, pm);
+        top = fmaxf(top, lse);
+    }
+    __device__ __forceinline__ void add(float pm, float lse, const v4f& po) {
+        total += power(lse, top);
+        o += po * power(pm, m);
+    }
+    __device__ __forceinline__ void more(float pm, float lse, const v4f& po) {
+        const float was_m = m, was_top = top;
+        meet(pm, lse);
+        total *= power(was_top, top);
+        o *= power(was_m, m);
+        add(pm, lse, po);
+    }
+    __device__ __forceinline__ float log2_sum() const { return top + __builtin_amdgcn_logf(total); }
+};
 // Writes 4 outputs of a row, gated by z.
 __device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d, v4f v, uint2 z) {
     if (A.gate) {
@@ -300,8 +373,7 @@ constexpr int kSplitTok = D == 256 ? 32 : 64;
 //   P in fp16, its rows where the products left them: a lane's S x 4 scores are 4 S consecutive tokens of
 //     one row, because row 4 g + i of product t is made token 4 S g + 4 t + i;
 //   O^T += V^T P^T on v_mfma_f32_16x16x32_f16, V's codes converted on the way.
-// The page's value scale goes into the exponent (p' = p vs, held relative to its own maximum), and 1 / vs
-// into the sum of p.
+// The page's value scale goes into the exponent (p' = p vs, held relative to its own maximum); the sum of p is LaneSum's.
 //
 // Bound by memory: 128 tokens over 8,000 each, 32 heads over 8 of 128, read 2.1 GB in 360 us, 5.8 of the 6.2 TB/s that reads
 // reach, 64 over 1 to 8,192, 16 heads over 2 of 256, 252 MB in 54 and join_kernel's 6. Short contexts are bound by the way to
@@ -330,9 +402,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         b = sh.b, e = sh.e, rb = sh.rb, v0 = sh.v0, left = sh.left, w_per = parked(sh.per), start = sh.start, s = sh.s;
     }
 
-    // The sums of a piece (the part of a segment in this share), for rows n: of 2^(kLift - mref) p v / vs, and of p.
+    // The sums of a piece (the part of a segment in this share), for rows n: of 2^(kLift - mref) p' v / vs, and of p.
     v4f acc[kM];
-    float mref, l;
+    float mref;
+    LaneSum sum;
     // What is left to do for the piece whose sums these are, in vector registers: the main loop needs the scalar ones.
     int o_e = 0, o_r0 = 0, o_rows = 0, o_s0 = 0, o_slot = 0;        // o_slot -1: the whole segment
     bool open = false;
@@ -404,10 +477,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         if (open) {                                           // the four waves' parts of the last piece together
             const AttnArgs& Z = args_again();
             const int x_r0 = taken(o_r0), x_rows = taken(o_rows), x_slot = taken(o_slot);
-            l = pair_sum32(pair_sum16(l));
+            const float lse = sum.log2_row();
             if (g == 0) {
-                lo_ml[(w * kSplitRows + n) * 2] = mref;
-                lo_ml[(w * kSplitRows + n) * 2 + 1] = l;
+                lo_ml[(w * kSplitRows + n) * 2] = mref - kLift;
+                lo_ml[(w * kSplitRows + n) * 2 + 1] = lse;
             }
 #pragma unroll
             for (int m = 0; m < kM; ++m) *reinterpret_cast<v4f*>(lo_o + (w * kSplitRows + n) * kPitch + 16 * m + 4 * g) = acc[m];
@@ -416,25 +489,21 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             for (int i = tid; i < kSplitRows * D / 4; i += kSplitThreads) {
                 const int row = i / (D / 4), d = i % (D / 4) * 4;
                 if (x_r0 + row >= x_rows) break;
-                float top = -__builtin_inff(), total = 0.0f;
-                v4f sum = {0, 0, 0, 0};
+                Joined to;
 #pragma unroll
-                for (int k = 0; k < kSplitWaves; ++k) top = fmaxf(top, lo_ml[(k * kSplitRows + row) * 2]);
+                for (int k = 0; k < kSplitWaves; ++k) to.meet(lo_ml[(k * kSplitRows + row) * 2], lo_ml[(k * kSplitRows + row) * 2 + 1]);
 #pragma unroll
-                for (int k = 0; k < kSplitWaves; ++k) {
-                    const float m = lo_ml[(k * kSplitRows + row) * 2];
-                    const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-                    total = fmaf(lo_ml[(k * kSplitRows + row) * 2 + 1], f, total);
-                    sum += *reinterpret_cast<const v4f*>(lo_o + (k * kSplitRows + row) * kPitch + d) * f;
-                }
+                for (int k = 0; k < kSplitWaves; ++k)
+                    to.add(lo_ml[(k * kSplitRows + row) * 2], lo_ml[(k * kSplitRows + row) * 2 + 1],
+                           *reinterpret_cast<const v4f*>(lo_o + (k * kSplitRows + row) * kPitch + d));
                 if (x_slot < 0) {
                     const int token = (x_r0 + row) / Z.G;
-                    store_out(Z, taken(o_s0) + token, taken(o_e) * Z.G + x_r0 + row - token * Z.G, d, sum * (total == 0.0f ? 0.0f : 1.0f / total));
+                    store_out(Z, taken(o_s0) + token, taken(o_e) * Z.G + x_r0 + row - token * Z.G, d, outputs(to.o, to.m, to.log2_sum()));
                 } else {
-                    *reinterpret_cast<v4f*>(parts.o + ((size_t)x_slot * kSplitRows + row) * D + d) = sum;
+                    *reinterpret_cast<v4f*>(parts.o + ((size_t)x_slot * kSplitRows + row) * D + d) = to.o;
                     if (d == 0) {
-                        parts.ml[((size_t)x_slot * kSplitRows + row) * 2] = top;
-                        parts.ml[((size_t)x_slot * kSplitRows + row) * 2 + 1] = total;
+                        parts.ml[((size_t)x_slot * kSplitRows + row) * 2] = to.m;
+                        parts.ml[((size_t)x_slot * kSplitRows + row) * 2 + 1] = to.log2_sum();
                     }
                 }
             }
@@ -470,7 +539,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         lds_barrier();
 #pragma unroll
         for (int m = 0; m < kM; ++m) acc[m] = v4f{0, 0, 0, 0};
-        mref = -__builtin_inff(), l = 0.0f;
+        mref = -__builtin_inff(), sum = LaneSum{};
 
         // Where its parts go, and whether it is cut at its end.
         o_e = parked(e), o_r0 = parked(r0), o_rows = parked(rows), o_s0 = parked(s.s0);
@@ -489,11 +558,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             const bool more = t + kSplitWaves < t1;
             const int at = s.tile(t) * kTok;
             asm volatile("" ::: "memory");                    // q is read from LDS again: there are no registers to keep it
-            // A block of zeros has scale 0, and its codes are 0.
-            const float lv = vs == 0.0f ? 0.0f : log2f(vs);
-            const float iv = vs > 0.0f && vs < __builtin_inff() ? 1.0f / vs : 1.0f;
+            const float lv = log2_scale(vs);
             const float cs = qc * ks;
-            float p[4 * kS], top = -__builtin_inff();
+            float p[4 * kS], most = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < kS; ++i) {
                 i32x4 h = {0, 0, 0, 0}, lw = {0, 0, 0, 0};
@@ -523,24 +590,26 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
                 for (int y = 0; y < 4 * kS; ++y) p[y] = (seen >> y) & 1 ? p[y] : -__builtin_inff();
             }
 #pragma unroll
-            for (int y = 0; y < 4 * kS; ++y) top = fmaxf(top, p[y]);
-            top = pair_max32(pair_max16(top));
+            for (int y = 0; y < 4 * kS; ++y) most = fmaxf(most, p[y]);
+            const float top = pair_max32(pair_max16(most));
+            sum.raise(most - lv);
             if (__ballot(top > mref + kLag)) {
                 const float now = fmaxf(mref, top);
                 const float f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mref - now);
                 mref = now;
-                l *= f;
 #pragma unroll
                 for (int m = 0; m < kM; ++m) acc[m] *= f;
             }
             const float ref = mref == -__builtin_inff() ? 0.0f : mref - kLift;
             f16x8 pf[kS / 2];
+            float of_tile = 0.0f;
 #pragma unroll
             for (int y = 0; y < 4 * kS; ++y) {
                 const float v = __builtin_amdgcn_exp2f(p[y] - ref);
-                l = fmaf(v, iv, l);
+                of_tile += v;
                 pf[y / 8][y & 7] = (_Float16)v;
             }
+            sum.add(p, -lv, most, of_tile, ref, lv);
             pv = pv_next;
             const int8_t* vp = values_at(t + kSplitWaves, pv);
             pk_next = page_of(t + 2 * kSplitWaves, keys);
@@ -594,33 +663,24 @@ __device__ __forceinline__ void join_outputs(const AttnArgs& A, const float* po,
     const int ways = kJoinThreads / wide, way = threadIdx.x / wide;
     for (int x0 = from; x0 < to; x0 += wide) {
         const int x = min(x0 + (int)(threadIdx.x & (wide - 1)), to - 1), row = x / (D / 4), d = x % (D / 4) * 4;
-        float top = -__builtin_inff(), total = 0.0f;
-        v4f sum = {0, 0, 0, 0};
-        const auto add = [&](float m, float l, const v4f& o) {
-            const float now = fmaxf(top, m);
-            const float f = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - now);
-            const float g = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
-            total = fmaf(l, g, total * f);
-            sum = sum * f + o * g;
-            top = now;
-        };
+        Joined sum;
 #pragma unroll 4
         for (int k = k0 + way; k <= k1; k += ways) {
             const size_t at = at_part(k) + row;
-            add(ml[2 * at], ml[2 * at + 1], *reinterpret_cast<const v4f*>(po + at * D + d));
+            sum.more(ml[2 * at], ml[2 * at + 1], *reinterpret_cast<const v4f*>(po + at * D + d));
         }
         for (int half = ways / 2; half > 0; half /= 2) {
-            lo_o[threadIdx.x] = sum;
-            lo_m[threadIdx.x] = top;
-            lo_l[threadIdx.x] = total;
+            lo_o[threadIdx.x] = sum.o;
+            lo_m[threadIdx.x] = sum.m;
+            lo_l[threadIdx.x] = sum.log2_sum();
             __syncthreads();
             const int other = threadIdx.x + half * wide;
-            if (way < half) add(lo_m[other], lo_l[other], lo_o[other]);
+            if (way < half) sum.more(lo_m[other], lo_l[other], lo_o[other]);
             __syncthreads();
         }
         if (way == 0 && x0 + (int)threadIdx.x < to) {
             const int token = (r0 + row) / A.G;
-            store_out(A, s0 + token, e * A.G + r0 + row - token * A.G, d, sum * (total == 0.0f ? 0.0f : 1.0f / total));
+            store_out(A, s0 + token, e * A.G + r0 + row - token * A.G, d, outputs(sum.o, sum.m, sum.log2_sum()));
         }
     }
 }
@@ -1010,7 +1070,8 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         const BlockParts<D> to(A.block_part, A.slots);
         const size_t at = (size_t)blockIdx.x * kBlockRows + (r - r0);
         if (r < rows) {
-            if (d0 == 0) *reinterpret_cast<float2*>(to.ml + 2 * at) = make_float2(l == 0.0f ? -__builtin_inff() : ref, l);
+            if (d0 == 0)
+                *reinterpret_cast<float2*>(to.ml + 2 * at) = make_float2(l == 0.0f ? -__builtin_inff() : ref, ref + __builtin_amdgcn_logf(l));
 #pragma unroll
             for (int m = 0; m < kM; ++m) *reinterpret_cast<v4f*>(to.o + at * D + 16 * m + d0) = acc[m];
         }
