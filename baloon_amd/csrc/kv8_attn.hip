@@ -62,10 +62,10 @@ __device__ __forceinline__ float pair_max32(float v) {
 }
 
 // A page's value scale vs weighs its values, not its tokens, so the sum of p has a reference of its own. The values'
-// product takes p' = p vs = 2^(score + log2 vs) relative to the largest of those; the sum takes p = 2^score relative to a
-// score of the lane's own tokens, which is at most 2^kFar below another. A lane's tokens of a tile are of one page, so p is p' times
-// one factor for all of them. Where that would pass 2^kFar (the page's values next to nothing beside others) p' may be
-// gone from 32 bits, and p is worked out by itself.
+// product takes p' = p vs = 2^(score + log2 vs) relative to the largest of those; the sum takes p = 2^score relative to 2^kFar
+// of a score among the lane's own tokens, so that it can grow by 2^kFar. A lane's tokens of a tile are of one page: p is p' times
+// one factor for all of them. Where that would be above 1 (the page's values next to nothing beside others) p' may be
+// gone from 32 bits, and p is worked out by itself; else what 32 bits lose of p' is under 2^(kFar - 126) of the sum.
 constexpr float kFar = 60.0f;
 // log2 of a page's scale. A page of zeros has none and only takes part in the sum: 2^kNoValue is so far under the least
 // scale, 2^-149, that what the product loses when such a page's p' is its largest is under any bf16 number.
@@ -75,24 +75,28 @@ __device__ __forceinline__ float log2_scale(float vs) { return vs == 0.0f ? kNoV
 // The sum of a lane's p: l 2^ref.
 struct LaneSum {
     float l = 0.0f, ref = -__builtin_inff();
-    // Before tokens of which the largest score is `most`, -inf where none is seen.
-    __device__ __forceinline__ void raise(float most) {
-        if (most > ref + kFar) {
-            l *= __builtin_amdgcn_exp2f(ref - most);
-            ref = most;
-        }
-    }
-    // Adds tokens with scores x[] + shift, the largest of them `most`, whose p' relative to 2^to have this sum.
+    // What the sum of a tile's p' counts in l. The lane's tokens have p' = 2^(x[] - from) relative to 2^to, the largest of them 2^most
+    // (0 where none is seen); lv is log2 vs. 6 instructions and a power for most tiles.
     template <int N>
-    __device__ __forceinline__ void add(const float (&x)[N], float shift, float most, float sum, float to, float lv) {
-        const float e = to - ref - lv;                        // to and ref, nearly the same or both large, first
-        if (e > kFar && most > -__builtin_inff()) {
-            asm volatile("");                                 // a branch: hardly ever taken
+    __device__ __forceinline__ float factor(const float (&x)[N], float from, float most, float to, float lv) {
+        float a = ref - to + lv;                              // p' is p relative to 2^ref times 2^a
+        float f = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(-a), 0.0f, 1.0f);
+        // more than the least that is rare: a if that is >= 0, else next to everything
+        if (most > fminf(a, a * 0x1p100f)) {
+            asm volatile("");                                 // a branch: taken at a lane's first tokens, then hardly ever
+            if (most > a) {
+                const float was = a;
+                ref = most + kFar - lv + to;
+                a = ref - to + lv;
+                l *= __builtin_amdgcn_exp2f(was - a);
+            }
+            f = a < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-a);
+            if (a < 0.0f) {
 #pragma unroll
-            for (int y = 0; y < N; ++y) l += __builtin_amdgcn_exp2f(x[y] + (shift - ref));
-        } else {
-            l = fmaf(sum, __builtin_amdgcn_exp2f(fminf(e, kFar)), l);      // of a hidden page's scale, whatever it is: 0 times that
+                for (int y = 0; y < N; ++y) l += __builtin_amdgcn_exp2f(x[y] - from - a);
+            }
         }
+        return f;
     }
     // log2 of the sum of a row's four lanes.
     __device__ __forceinline__ float log2_row() const {
@@ -592,7 +596,6 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
 #pragma unroll
             for (int y = 0; y < 4 * kS; ++y) most = fmaxf(most, p[y]);
             const float top = pair_max32(pair_max16(most));
-            sum.raise(most - lv);
             if (__ballot(top > mref + kLag)) {
                 const float now = fmaxf(mref, top);
                 const float f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mref - now);
@@ -601,15 +604,14 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
                 for (int m = 0; m < kM; ++m) acc[m] *= f;
             }
             const float ref = mref == -__builtin_inff() ? 0.0f : mref - kLift;
+            const float counts = sum.factor(p, ref, most - ref, ref, lv);
             f16x8 pf[kS / 2];
-            float of_tile = 0.0f;
 #pragma unroll
             for (int y = 0; y < 4 * kS; ++y) {
                 const float v = __builtin_amdgcn_exp2f(p[y] - ref);
-                of_tile += v;
+                sum.l = fmaf(v, counts, sum.l);
                 pf[y / 8][y & 7] = (_Float16)v;
             }
-            sum.add(p, -lv, most, of_tile, ref, lv);
             pv = pv_next;
             const int8_t* vp = values_at(t + kSplitWaves, pv);
             pk_next = page_of(t + 2 * kSplitWaves, keys);
@@ -717,11 +719,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg
 constexpr int kBlockThreads = 512, kBlockTok = 64, kBlockRows = 128;
 
 // LDS of block_kernel, two buffers of each: keys [64 tokens][D], values [D][64 tokens] fp16, and of each 16
-// tokens ks, log2 vs and 1 / vs.
+// tokens ks and log2 vs.
 template <int D>
 struct BlockLds {
     static constexpr int kChunks = D / 16;                    // of a token's keys
-    static constexpr int kK = kBlockTok * D, kV = 2 * kBlockTok * D, kS = kBlockTok / 16 * 16;
+    static constexpr int kK = kBlockTok * D, kV = 2 * kBlockTok * D, kS = kBlockTok / 16 * 8;
     static constexpr int kVAt = 2 * kK, kSAt = kVAt + 2 * kV, kBytes = kSAt + 2 * kS;
     // Byte offset of 16-byte chunk c of token t's keys, and of chunk c (8 tokens) of channel d's values: both are
     // what they are for c = 0, xor 16 c. A 16-byte read takes 16 lanes at a time over 256 bytes of banks, lanes
@@ -968,9 +970,8 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     };
     const auto store_scale = [&](int buf) {
         if (tid < kBlockTok / 16) {
-            const v4f s = {vs < 0.0f ? 0.0f : ks, vs < 0.0f ? -__builtin_inff() : vs == 0.0f ? 0.0f : log2f(vs),
-                           vs > 0.0f && vs < __builtin_inff() ? 1.0f / vs : 1.0f, 0.0f};
-            *reinterpret_cast<v4f*>(lds + Lds::kSAt + buf * Lds::kS + 16 * tid) = s;
+            *reinterpret_cast<float2*>(lds + Lds::kSAt + buf * Lds::kS + 8 * tid) =
+                make_float2(vs < 0.0f ? 0.0f : ks, vs < 0.0f ? -__builtin_inff() : log2_scale(vs));
         }
     };
     const int k0 = Lds::k_at((n >> 2) * 16 + (n & 3), g), v0 = Lds::v_at(n, 2 * g);
@@ -978,8 +979,9 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     v4f acc[kM];
 #pragma unroll
     for (int m = 0; m < kM; ++m) acc[m] = v4f{0, 0, 0, 0};
-    // p is taken relative to 2^ref; a lane whose row gets a score over `limit` of it moves ref to that score.
-    float ref = 0.0f, limit = -__builtin_inff(), l = 0.0f;
+    // p' is taken relative to 2^ref; a lane whose row gets one over 2^limit of it moves ref there.
+    float ref = 0.0f, limit = -__builtin_inff();
+    LaneSum sum;
 
     int ids = pages(tile(0)), page_k[kPer], page_v[kPer];
     pages_of(ids, page_k, page_v);
@@ -1002,9 +1004,9 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         load_scale(ids);
         ids = pages(tile(min(t + 2, nt - 1)));
         if (at <= wave_last && (at >= some_lo || at < A.sinks)) {
-            const v4f sc = *reinterpret_cast<const v4f*>(lds + Lds::kSAt + buf * Lds::kS + 16 * g);
-            float p[16], top = -__builtin_inff();             // lane: row n, tokens at + 16 g + y
-            const float cs = qc * sc[0], lv = sc[1] - ref;
+            const float2 sc = *reinterpret_cast<const float2*>(lds + Lds::kSAt + buf * Lds::kS + 8 * g);
+            float p[16], most = -__builtin_inff();            // lane: row n, tokens at + 16 g + y
+            const float cs = qc * sc.x, lv = sc.y - ref;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 i32x4 hi = {0, 0, 0, 0}, lw = {0, 0, 0, 0};
@@ -1025,30 +1027,30 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
                 for (int y = 0; y < 16; ++y) p[y] = (seen >> y) & 1 ? p[y] : -__builtin_inff();
             }
 #pragma unroll
-            for (int y = 0; y < 16; ++y) top = fmaxf(top, p[y]);
-            top = pair_max32(pair_max16(top));
+            for (int y = 0; y < 16; ++y) most = fmaxf(most, p[y]);
+            const float top = pair_max32(pair_max16(most));
             if (__ballot(top > limit)) {
                 const float mref = limit == -__builtin_inff() ? limit : ref + kLift;
                 const float now = fmaxf(mref, top + ref), to = now == -__builtin_inff() ? 0.0f : now - kLift;
                 const float f = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mref - now);
 #pragma unroll
                 for (int y = 0; y < 16; ++y) p[y] += ref - to;
+                most += ref - to;
                 ref = to;
                 limit = now == -__builtin_inff() ? now : kLift + kLag;
-                l *= f;
 #pragma unroll
                 for (int m = 0; m < kM; ++m) acc[m] *= f;
             }
+            const float counts = sum.factor(p, 0.0f, most, ref, sc.y);
             f16x8 pf[2];
-            float sum = 0.0f;
+            float of_tile = 0.0f;
 #pragma unroll
-            for (int y = 0; y < 16; y += 2) {
-                const f16x2 two = {(_Float16)__builtin_amdgcn_exp2f(p[y]), (_Float16)__builtin_amdgcn_exp2f(p[y + 1])};
-                sum = __builtin_amdgcn_fdot2(two, f16x2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
-                pf[y / 8][y & 7] = two[0];
-                pf[y / 8][(y & 7) + 1] = two[1];
+            for (int y = 0; y < 16; ++y) {
+                const float v = __builtin_amdgcn_exp2f(p[y]);
+                of_tile += v;                                 // before its rounding: a small page's p' loses bits by it
+                pf[y / 8][y & 7] = (_Float16)v;
             }
-            l = fmaf(sum, sc[2], l);                          // of the rounded p, as the values' product
+            sum.l = fmaf(of_tile, counts, sum.l);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -1062,7 +1064,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         lds_barrier();
     }
 
-    l = pair_sum32(pair_sum16(l));
+    const float lse = sum.log2_row(), m_ref = limit == -__builtin_inff() ? limit : ref;
     int thread = tid;
     asm volatile("" : "+v"(thread));                          // the row is worked out again: it does not wait in registers
     const int r = w0 + (thread & 15), qi = r / A.G, head = e * A.G + r - qi * A.G, d0 = 4 * (thread >> 4 & 3);
@@ -1070,15 +1072,13 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         const BlockParts<D> to(A.block_part, A.slots);
         const size_t at = (size_t)blockIdx.x * kBlockRows + (r - r0);
         if (r < rows) {
-            if (d0 == 0)
-                *reinterpret_cast<float2*>(to.ml + 2 * at) = make_float2(l == 0.0f ? -__builtin_inff() : ref, ref + __builtin_amdgcn_logf(l));
+            if (d0 == 0) *reinterpret_cast<float2*>(to.ml + 2 * at) = make_float2(m_ref, lse);
 #pragma unroll
             for (int m = 0; m < kM; ++m) *reinterpret_cast<v4f*>(to.o + at * D + 16 * m + d0) = acc[m];
         }
         return;
     }
     if (r < rows) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         constexpr int kN = kM < 8 ? kM : 8;                   // pieces of 4 channels, their gates on the way together
 #pragma unroll
         for (int m0 = 0; m0 < kM; m0 += kN) {
@@ -1086,7 +1086,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
 #pragma unroll
             for (int i = 0; i < kN; ++i) z[i] = load_gate(A, s0 + qi, head, 16 * (m0 + i) + d0);
 #pragma unroll
-            for (int i = 0; i < kN; ++i) store_out(A, s0 + qi, head, 16 * (m0 + i) + d0, acc[m0 + i] * inv, z[i]);
+            for (int i = 0; i < kN; ++i) store_out(A, s0 + qi, head, 16 * (m0 + i) + d0, outputs(acc[m0 + i], m_ref, lse), z[i]);
         }
     }
 }

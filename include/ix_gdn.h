@@ -421,9 +421,12 @@ size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, i
  *   o       [total_T][h_q][d] bf16 (RNE); may be the memory of q or gate where those are packed
  *   workspace  256-byte aligned, workspace_bytes >= ix_kv8_attn_workspace_size(...)
  * Positions up to 2^30. Scores are formed from 16-bit fixed-point q (of each row's largest
- * value) and the codes, exactly, softmax sums in fp32, p in fp16 of its running maximum for
- * the product with the codes of v. Scales that are not finite in
- * hidden places do not matter. The call may be captured into a HIP graph, and kv_len, table
+ * value) and the codes, exactly, softmax sums in fp32, and p times the page's value scale in
+ * fp16 relative to the running maximum of that product for the one with the codes of v. So a
+ * row is exact to about 2^-11 of the largest p |v| it sums, and channels of q far below the
+ * row's largest have fewer bits than bf16 gives them (under 2^-8 of it). Pages' scales may
+ * be any finite numbers >= 0, however far apart; what stands in places that a row does not
+ * see, codes or scales of any bits, does not matter. The call may be captured into a HIP graph, and kv_len, table
  * and the rest of the device data may change between its replays. */
 hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens,
                        const int32_t* kv_len, const int32_t* table, int width, const ix_rows* q, int h_q, float scale,

@@ -49,8 +49,8 @@ def free_page_0(P):
     return sorted(other)
 
 
-# (new tokens, sequences, heads): single tokens and drafts
-SHAPES = [(1, 3, 2), (3, 3, 2)]
+# (new tokens, sequences, heads): a token and drafts by the wave, blocks of rows, and those in parts
+SHAPES = [(1, 3, 2), (3, 3, 2), (500, 2, 8)]
 
 
 @pytest.mark.gpu
