@@ -168,9 +168,10 @@ def _rows(t):
     """``ix_rows`` of a bf16 CUDA tensor whose rows (its first dimension) are dense (None for None)."""
     if t is None or isinstance(t, ctypes.Structure):
         return t
+    import torch
     if not t.is_cuda:
         raise ValueError("baloon_amd: tensors must be on the GPU")
-    if t.element_size() != 2 or t.dim() < 2:
+    if t.dtype != torch.bfloat16 or t.dim() < 2:
         raise ValueError("baloon_amd: token rows are bf16 tensors of two dimensions or more")
     dense = 1
     for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
@@ -433,8 +434,16 @@ def ix_gdn_in_proj(cfg: Cfg, B, hidden, h, w, x, z, a, b, y=None, s=None) -> int
 def ix_add_rms_norm(rows, n, x, res, res_out, weight, weight_offset, eps, y=None, y_bf16=None, y_q8_1=None,
                     s=None) -> int:
     """h = bf16(x + res), y = RMS norm of h times (weight_offset + weight), row by row. x is fp32 or bf16
-    (by its element size), res and res_out bf16 or None; y_q8_1 is a byte buffer of 36 bytes per 32 outputs."""
-    x32, x16 = (None, x) if x is not None and x.element_size() == 2 else (x, None)
+    (by its type), res and res_out bf16 or None; y_q8_1 is a byte buffer of 36 bytes per 32 outputs."""
+    import torch
+    x32 = x16 = None
+    if x is not None:
+        if x.dtype == torch.bfloat16:
+            x16 = x
+        elif x.dtype == torch.float32:
+            x32 = x
+        else:
+            raise ValueError("baloon_amd: x is fp32 or bf16")
     return _bind.ix_add_rms_norm(rows, n, x32, x16, res, res_out, weight, weight_offset, eps, y, y_bf16, y_q8_1, s)
 
 

@@ -108,14 +108,14 @@ struct Arg<const ix_kv8*> {
         return o == Py_None ? nullptr : structure<ix_kv8>(o, other);
     }
 };
-// Rows of a tensor on the GPU: 2-byte elements, dense but for the first dimension.
+// Rows of a tensor on the GPU: bf16, dense but for the first dimension.
 template <>
 struct Arg<const ix_rows*> {
     static Rows of(PyObject* o, bool& other) {
         if (o == Py_None) return Rows{};
         if (THPVariable_CheckExact(o)) {
             const at::Tensor& t = THPVariable_Unpack(o);
-            if (t.is_cuda() && t.layout() == c10::kStrided && t.element_size() == 2 && t.dim() >= 2) {
+            if (t.is_cuda() && t.layout() == c10::kStrided && t.scalar_type() == at::kBFloat16 && t.dim() >= 2) {
                 int64_t dense = 1;
                 bool ok = true;
                 for (int64_t i = t.dim() - 1; i >= 1; --i) {
