@@ -217,13 +217,12 @@ extern "C" hipError_t ix_add_rms_norm(int rows, int n, const float* x, const uin
                                       uint16_t* res_out, const float* weight, float weight_offset, float eps, float* y,
                                       uint16_t* y_bf16, void* y_q8_1, hipStream_t s) {
     using namespace ixg;
-    if (rows < 0 || n <= 0 || n > kNormMax || !x == !x_bf16 || !weight || (!y && !y_bf16 && !y_q8_1))
-        return hipErrorInvalidValue;
-    if (y_q8_1 && n % 32) return hipErrorInvalidValue;
+    if (rows < 0 || n <= 0 || n > kNormMax || (y_q8_1 && n % 32)) return hipErrorInvalidValue;
+    if (rows == 0) return hipSuccess;                         // of tensors without elements, whose addresses may be 0
+    if (!x == !x_bf16 || !weight || (!y && !y_bf16 && !y_q8_1)) return hipErrorInvalidValue;
     if (!aligned(x, 4) || !aligned(x_bf16, 2) || !aligned(res, 2) || !aligned(res_out, 2) || !aligned(weight, 4) ||
         !aligned(y, 4) || !aligned(y_bf16, 2) || !aligned(y_q8_1, 4))
         return hipErrorInvalidValue;
-    if (rows == 0) return hipSuccess;
     const NormIo io{x, x_bf16, res, res_out, weight, weight_offset, eps, y, y_bf16, static_cast<uint8_t*>(y_q8_1), rows, n};
     // A chunk a thread, as few threads as hold the row: one row takes 1.9 to 2.6 us up to 8,192 values (2.6 to 3.8 with 4
     // chunks a thread), and 128 MB 25 to 27 (27 to 29).

@@ -1210,12 +1210,12 @@ hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, c
     AttnArgs A{};
     if (!make_kv8(cache, &A.c) || !make_batch(n_seq, total_T, cu_seqlens, kv_len, table, width, &A.a)) return hipErrorInvalidValue;
     if (!attn_shape_ok(A.c, n_seq, total_T, max_q, h_q) || window < 0 || window > 1 << 30 || sinks < 0) return hipErrorInvalidValue;
+    if (total_T == 0) return hipSuccess;                      // of tensors without elements, whose addresses may be 0
     if (!rows_ok(q, (long long)h_q * A.c.d) || (gate && !rows_ok(gate, (long long)h_q * A.c.d))) return hipErrorInvalidValue;
     if (!o || !ptr_aligned(o, 2)) return hipErrorInvalidValue;
     if (!workspace || !ptr_aligned(workspace, 256) ||
         workspace_bytes < ix_kv8_attn_workspace_size(cache, n_seq, total_T, max_q, h_q))
         return hipErrorInvalidValue;
-    if (total_T == 0) return hipSuccess;
     A.q = q->p;
     A.q_stride = q->stride;
     if (gate) {

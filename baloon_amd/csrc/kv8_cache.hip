@@ -329,8 +329,8 @@ hipError_t ix_kv8_append(const ix_kv8* cache, int n_seq, int total_T, const int3
     Kv8 c;
     Batch a;
     if (!make_kv8(cache, &c) || !make_batch(n_seq, total_T, cu_seqlens, kv_len, table, width, &a)) return hipErrorInvalidValue;
+    if (total_T == 0) return hipSuccess;                      // of tensors without elements, whose addresses may be 0
     if (!rows_ok(k, (long long)c.h_kv * c.d) || !rows_ok(v, (long long)c.h_kv * c.d)) return hipErrorInvalidValue;
-    if (total_T == 0) return hipSuccess;
     const int few = a.T < (long long)c.page * a.n_seq ? 2 : 1;
     return with_threads(c.page * c.d / 32 / few, [&](auto n) { return launch_append<n>(c, a, k, v, s); });
 }
@@ -341,8 +341,8 @@ hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_
     Kv8 c;
     Batch a;
     if (!make_kv8(cache, &c) || !make_batch(n_seq, total_T, cu_seqlens, kv_len, table, width, &a)) return hipErrorInvalidValue;
-    if ((!k && !v) || !ptr_aligned(k, 2) || !ptr_aligned(v, 2)) return hipErrorInvalidValue;
     if (total_T == 0) return hipSuccess;
+    if ((!k && !v) || !ptr_aligned(k, 2) || !ptr_aligned(v, 2)) return hipErrorInvalidValue;
     return with_threads(c.page * c.d / 32, [&](auto n) { return launch_read<n>(c, a, k, v, s); });
 }
 

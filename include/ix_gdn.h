@@ -348,7 +348,8 @@ hipError_t ix_gdn_in_proj(const ix_gdn_cfg* cfg, int B, int hidden, const uint16
  *   y fp32, y_bf16 (RNE of the fp32 value) [rows][n], y_q8_1 [rows][n/32] q8_1 blocks (the
  *   activation format of ix_mmvq_q8_0, the bytes that ix_q8_1_quantize gives for y): at least
  *   one of them. y_bf16 may be x_bf16 or res.
- * The sum of squares and the norm are fp32. Requires rows >= 0, 0 < n <= 32768, n % 32 == 0
+ * The sum of squares and the norm are fp32. rows = 0 is a call without work, whose operands may
+ * be NULL. Requires rows >= 0, 0 < n <= 32768, n % 32 == 0
  * for y_q8_1 (4-byte aligned). n % 8 == 0 with 16-byte aligned operands is faster. */
 hipError_t ix_add_rms_norm(int rows, int n, const float* x, const uint16_t* x_bf16, const uint16_t* res,
                            uint16_t* res_out, const float* weight, float weight_offset, float eps, float* y,
@@ -385,7 +386,7 @@ typedef struct ix_kv8 {
  *   the cache. Entries behind the last page are not read; a page without a place in the cache
  *   (an entry outside [0, n_pages), or p >= width) holds nothing: writes to it are dropped, its
  *   tokens are hidden from every query.
- * total_T = 0 is a call without work. */
+ * total_T = 0 is a call without work, whose rows and outputs may be NULL. */
 
 /* Append the batch's keys and values to its sequences: k, v rows of [h_kv][d], stride >= h_kv * d.
  * Where a page gets new tokens its scale becomes s' = max(s, max|x| / 127), s being its scale if
