@@ -202,10 +202,23 @@ __global__ void __launch_bounds__(T) norm_kernel(NormIo io) {
 }
 
 template <int T, int N>
-void launch_norm(const NormIo& io, hipStream_t s) {
-    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)io.rows), dim3(T), 0, s, io); };
-    if (io.n % 8) io.x ? launch(&norm_kernel<T, N, true, true>) : launch(&norm_kernel<T, N, false, true>);
-    else io.x ? launch(&norm_kernel<T, N, true, false>) : launch(&norm_kernel<T, N, false, false>);
+hipError_t launch_norm(const NormIo& io, hipStream_t s) {
+    return launch_in_pieces(io.rows, T, [&](long long first, unsigned rows) {
+        const size_t at = (size_t)first * io.n;
+        NormIo p = io;
+        if (first > 0) {
+            if (p.x) p.x += at;
+            if (p.x16) p.x16 += at;
+            if (p.res) p.res += at;
+            if (p.res_out) p.res_out += at;
+            if (p.y) p.y += at;
+            if (p.y16) p.y16 += at;
+            if (p.q81) p.q81 += at / 32 * kQ81Bytes;
+        }
+        const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(rows), dim3(T), 0, s, p); };
+        if (io.n % 8) io.x ? launch(&norm_kernel<T, N, true, true>) : launch(&norm_kernel<T, N, false, true>);
+        else io.x ? launch(&norm_kernel<T, N, true, false>) : launch(&norm_kernel<T, N, false, false>);
+    });
 }
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -227,11 +240,10 @@ extern "C" hipError_t ix_add_rms_norm(int rows, int n, const float* x, const uin
     // A chunk a thread, as few threads as hold the row: one row takes 1.9 to 2.6 us up to 8,192 values (2.6 to 3.8 with 4
     // chunks a thread), and 128 MB 25 to 27 (27 to 29).
     const int chunks = (n + 7) / 8;
-    if (chunks <= 64) launch_norm<64, 1>(io, s);
-    else if (chunks <= 256) launch_norm<256, 1>(io, s);
-    else if (chunks <= 512) launch_norm<512, 1>(io, s);
-    else if (chunks <= 1024) launch_norm<1024, 1>(io, s);
-    else if (chunks <= 2048) launch_norm<1024, 2>(io, s);
-    else launch_norm<1024, 4>(io, s);
-    return hipGetLastError();
+    if (chunks <= 64) return launch_norm<64, 1>(io, s);
+    if (chunks <= 256) return launch_norm<256, 1>(io, s);
+    if (chunks <= 512) return launch_norm<512, 1>(io, s);
+    if (chunks <= 1024) return launch_norm<1024, 1>(io, s);
+    if (chunks <= 2048) return launch_norm<1024, 2>(io, s);
+    return launch_norm<1024, 4>(io, s);
 }

@@ -7,6 +7,7 @@
 // (gate from A_log/dt_bias, beta = sigmoid(b), optional SiLU after the conv, the
 // contiguous head map) are selected by ix_gdn_cfg.
 #pragma once
+#include <algorithm>
 #include <atomic>
 #include "ix_gdn.h"
 #include "wave64.h"
@@ -152,6 +153,19 @@ inline int device_cu_count(hipStream_t s) {
         cached[dev].store(n, std::memory_order_relaxed);
     }
     return n;
+}
+
+// Workgroups first .. of `n` in launches of as many as a grid's first dimension can have: 2^32 - 1 threads, beyond which it is
+// taken modulo 2^32 without an error.
+template <class F>
+inline hipError_t launch_in_pieces(long long n, int threads, F launch) {
+    const long long most = 0xffffffffLL / threads;
+    for (long long first = 0; first < n; first += most) {
+        launch(first, (unsigned)std::min(most, n - first));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // q8_1 block (36 bytes: half d, half s, int8 qs[32]; the activation format of the Q8_0 product,

@@ -35,6 +35,7 @@ struct AttnArgs {
     int small;                // sequences of more (token, head) rows a kv head than this are block_kernel's
     float* block_part;        // partial results of its blocks, see BlockParts
     int slots, items;         // workgroups of it that the chip holds, and parts of blocks at most
+    int first, blocks;        // where a launch of it begins, and its workgroups in all launches
 };
 
 // The kernel's argument (its only one) read from memory again where it is used next: keeping all of it in
@@ -821,7 +822,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
 
     // Block j of the grid, from the last: of the causal blocks the longest start first. Sequence b owns the
     // blocks from cu[b] G / 128 + b on; consecutive workgroups, which different XCDs take, are different heads.
-    const int e = blockIdx.x % A.c.h_kv;
+    const int block = kCut ? (int)blockIdx.x : A.first + (int)blockIdx.x, e = block % A.c.h_kv;
     int b, rb, parts = 1, part = 0;
     if constexpr (kCut) {
         const Blocks all = all_blocks<D>(A, lane);
@@ -842,7 +843,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
             rb -= lane_of(incl, kWave - 1);
         }
     } else {
-        const int j = gridDim.x / A.c.h_kv - 1 - blockIdx.x / A.c.h_kv;
+        const int j = A.blocks / A.c.h_kv - 1 - block / A.c.h_kv;
         const auto key = [&](int b) { return (int)((long long)A.a.start(b) * A.G / kBlockRows) + b; };
         b = wave_search(A.a.n_seq, j, lane, key);
         rb = j - key(b);
@@ -1141,12 +1142,15 @@ template <int D>
 size_t attn_bytes(const Plan& p) { return split_bytes<D>(p) + (p.cut ? BlockParts<D>::bytes(p.slots) : 0); }
 
 template <int D, bool kCut>
-hipError_t launch_blocks(const AttnArgs& A, long long n, hipStream_t s) {
+hipError_t launch_blocks(AttnArgs& A, long long n, hipStream_t s) {
     static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(&block_kernel<D, kCut>),
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, BlockLds<D>::kBytes);
-    if (ready == hipSuccess)
-        hipLaunchKernelGGL((block_kernel<D, kCut>), dim3((unsigned)n), dim3(kBlockThreads), BlockLds<D>::kBytes, s, A);
-    return ready;
+    if (ready != hipSuccess) return ready;
+    A.blocks = (int)n;
+    return launch_in_pieces(n, kBlockThreads, [&](long long first, unsigned count) {      // one, of blocks in parts
+        A.first = (int)first;
+        hipLaunchKernelGGL((block_kernel<D, kCut>), dim3(count), dim3(kBlockThreads), BlockLds<D>::kBytes, s, A);
+    });
 }
 
 template <int D>
@@ -1184,9 +1188,10 @@ hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
     return hipGetLastError();
 }
 
+// The blocks of the batch are numbered in 31 bits.
 bool attn_shape_ok(const Kv8& c, int n_seq, int T, int max_q, int h_q) {
     return n_seq > 0 && n_seq <= 65535 && T >= 0 && max_q >= 0 && (T == 0 || max_q > 0) && h_q > 0 && h_q % c.h_kv == 0 &&
-           h_q <= 65536;
+           h_q <= 65536 && (long long)T * h_q <= 1ll << 37;
 }
 
 }  // namespace

@@ -138,13 +138,13 @@ constexpr int kBatch = 4;
 template <int kThreads>
 __global__ void __launch_bounds__(kThreads)
 append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_stride, const uint16_t* __restrict__ vr,
-              long long v_stride) {
+              long long v_stride, int first_slot) {
     extern __shared__ uint4 raw[];
     __shared__ float red[kThreads / kWave];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), h = blockIdx.y;
     const bool is_v = blockIdx.z;
     PageJob job;
-    if (!page_job(a, c, blockIdx.x, lane, &job)) return;
+    if (!page_job(a, c, first_slot + (int)blockIdx.x, lane, &job)) return;
     const int per_log = c.d == 64 ? 3 : c.d == 128 ? 4 : 5, chunks = (job.end - job.held) << per_log;
     const long long stride = is_v ? v_stride : k_stride;
     const uint16_t* rows = (is_v ? vr : kr) + (long long)job.row * stride + (size_t)h * c.d;
@@ -238,13 +238,13 @@ __device__ __forceinline__ uint4 values8(uint32_t lo, uint32_t hi, float s) {
 
 template <int kThreads>
 __global__ void __launch_bounds__(kThreads)
-read_kernel(Kv8 c, Batch a, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo) {
+read_kernel(Kv8 c, Batch a, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo, int first_slot) {
     extern __shared__ uint8_t tile[];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), h = blockIdx.y;
     const bool is_v = blockIdx.z;
     uint16_t* out = is_v ? vo : ko;
     PageJob job;
-    if (!out || !page_job(a, c, blockIdx.x, lane, &job)) return;
+    if (!out || !page_job(a, c, first_slot + (int)blockIdx.x, lane, &job)) return;
     const size_t ph = (size_t)job.id * c.h_kv + h;
     const float s = (is_v ? c.v_scale : c.k_scale)[ph];
     const int8_t* codes = (is_v ? c.v : c.k) + ph * c.page * c.d;
@@ -283,9 +283,7 @@ read_kernel(Kv8 c, Batch a, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo
     }
 }
 
-dim3 page_grid(const Kv8& c, const Batch& a) {
-    return dim3((unsigned)(a.T >> c.page_log) + 2u * (unsigned)a.n_seq, (unsigned)c.h_kv, 2);
-}
+long long page_slots(const Kv8& c, const Batch& a) { return (a.T >> c.page_log) + 2ll * a.n_seq; }
 
 // A thread for 32 values of a page; in appends for 64 where the sequences have less than a page of new tokens each. A
 // workgroup is bound by the chain of its reads: more threads make it shorter where there is work for them, and keep other
@@ -307,15 +305,18 @@ hipError_t launch_append(const Kv8& c, const Batch& a, const ix_rows* k, const i
     static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(&append_kernel<kThreads>),
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 256 * sizeof(uint16_t));
     if (ready != hipSuccess) return ready;
-    hipLaunchKernelGGL((append_kernel<kThreads>), page_grid(c, a), dim3(kThreads), c.page * c.d * sizeof(uint16_t), s, c, a,
-                       k->p, k->stride, v->p, v->stride);
-    return hipGetLastError();
+    return launch_in_pieces(page_slots(c, a), kThreads, [&](long long first, unsigned n) {
+        hipLaunchKernelGGL((append_kernel<kThreads>), dim3(n, (unsigned)c.h_kv, 2), dim3(kThreads), c.page * c.d * sizeof(uint16_t), s,
+                           c, a, k->p, k->stride, v->p, v->stride, (int)first);
+    });
 }
 
 template <int kThreads>
 hipError_t launch_read(const Kv8& c, const Batch& a, uint16_t* k, uint16_t* v, hipStream_t s) {
-    hipLaunchKernelGGL((read_kernel<kThreads>), page_grid(c, a), dim3(kThreads), c.page * (c.d + 4), s, c, a, k, v);
-    return hipGetLastError();
+    return launch_in_pieces(page_slots(c, a), kThreads, [&](long long first, unsigned n) {
+        hipLaunchKernelGGL((read_kernel<kThreads>), dim3(n, (unsigned)c.h_kv, 2), dim3(kThreads), c.page * (c.d + 4), s, c, a, k, v,
+                           (int)first);
+    });
 }
 
 }  // namespace

@@ -416,7 +416,7 @@ size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, i
  * positions j that it sees: j <= pos and, when window > 0, pos - j < window or j < sinks (a
  * sliding window and a few first tokens that stay visible). A row that sees nothing is 0.
  *   max_q   at least the new tokens of the longest sequence (rows of longer ones are not written)
- *   q       rows of [h_q][d]; h_q a multiple of h_kv
+ *   q       rows of [h_q][d]; h_q a multiple of h_kv, at most 65536, total_T * h_q at most 2^37
  *   window  0 (everything before) .. 2^30; sinks >= 0, without meaning when window is 0
  *   gate    rows of [h_q][d], or NULL: o is multiplied by sigmoid(gate)
  *   o       [total_T][h_q][d] bf16 (RNE); may be the memory of q or gate where those are packed
