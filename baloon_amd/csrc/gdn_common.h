@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <atomic>
 #include "ix_gdn.h"
+#include "per_device.h"
 #include "wave64.h"
 
 namespace ixg {
@@ -133,26 +134,48 @@ inline OutGate make_out_gate(const ix_gdn_out_gate* g) {
     return o;
 }
 
+// The device of a stream, the current one for the null stream.
+inline hipError_t stream_device(hipStream_t s, int* dev) {
+    if (!s) return hipGetDevice(dev);
+    hipDevice_t d = 0;
+    const hipError_t e = hipStreamGetDevice(s, &d);
+    *dev = (int)d;
+    return e;
+}
+
 // Compute units of the device that stream s launches on (the calling thread's current device
 // for the null stream), queried once per device (256 on MI355X).
 inline int device_cu_count(hipStream_t s) {
     constexpr int kMaxDev = 64;
     static std::atomic<int> cached[kMaxDev];
     int dev = 0;
-    if (s) {
-        hipDevice_t d = 0;
-        if (hipStreamGetDevice(s, &d) != hipSuccess) return 256;
-        dev = (int)d;
-    } else if (hipGetDevice(&dev) != hipSuccess) {
-        return 256;
-    }
-    if (dev < 0 || dev >= kMaxDev) return 256;
+    if (stream_device(s, &dev) != hipSuccess || dev < 0 || dev >= kMaxDev) return 256;
     int n = cached[dev].load(std::memory_order_relaxed);
     if (n <= 0) {
         if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
         cached[dev].store(n, std::memory_order_relaxed);
     }
     return n;
+}
+
+// Lets a kernel's launches on the stream's device have `bytes` of dynamic LDS. `once` is that kernel's.
+template <class Kernel>
+inline hipError_t allow_lds(OncePerDevice& once, Kernel kernel, int bytes, hipStream_t s) {
+    int dev = 0;
+    const hipError_t e = stream_device(s, &dev);
+    if (e != hipSuccess) return e;
+    return once(dev, [&] {
+        int now = dev;                                        // the attribute is the current device's
+        hipError_t r = hipGetDevice(&now);
+        if (r == hipSuccess && now != dev) r = hipSetDevice(dev);
+        if (r != hipSuccess) return r;
+        r = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (now != dev) {
+            const hipError_t back = hipSetDevice(now);
+            if (r == hipSuccess) r = back;
+        }
+        return r;
+    });
 }
 
 // Workgroups first .. of `n` in launches of as many as a grid's first dimension can have: 2^32 - 1 threads, beyond which it is

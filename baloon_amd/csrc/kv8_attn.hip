@@ -1143,8 +1143,8 @@ size_t attn_bytes(const Plan& p) { return split_bytes<D>(p) + (p.cut ? BlockPart
 
 template <int D, bool kCut>
 hipError_t launch_blocks(AttnArgs& A, long long n, hipStream_t s) {
-    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(&block_kernel<D, kCut>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, BlockLds<D>::kBytes);
+    static OncePerDevice once;
+    const hipError_t ready = allow_lds(once, &block_kernel<D, kCut>, BlockLds<D>::kBytes, s);
     if (ready != hipSuccess) return ready;
     A.blocks = (int)n;
     return launch_in_pieces(n, kBlockThreads, [&](long long first, unsigned count) {      // one, of blocks in parts

@@ -302,8 +302,8 @@ hipError_t with_threads(int n, F launch) {
 
 template <int kThreads>
 hipError_t launch_append(const Kv8& c, const Batch& a, const ix_rows* k, const ix_rows* v, hipStream_t s) {
-    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(&append_kernel<kThreads>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 256 * sizeof(uint16_t));
+    static OncePerDevice once;
+    const hipError_t ready = allow_lds(once, &append_kernel<kThreads>, 128 * 256 * sizeof(uint16_t), s);
     if (ready != hipSuccess) return ready;
     return launch_in_pieces(page_slots(c, a), kThreads, [&](long long first, unsigned n) {
         hipLaunchKernelGGL((append_kernel<kThreads>), dim3(n, (unsigned)c.h_kv, 2), dim3(kThreads), c.page * c.d * sizeof(uint16_t), s,
