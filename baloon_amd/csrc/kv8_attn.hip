@@ -1138,8 +1138,10 @@ Plan plan_of(int d, int h_kv, int G, int T, int max_q, hipStream_t s) {
 
 template <int D>
 size_t split_bytes(const Plan& p) { return (Parts<kSplitRows, D>::bytes(p.n_wg) + 255) / 256 * 256; }
+// Also where this batch's blocks stay whole: those of a smaller one, which the workspace has to do for as well, may not.
 template <int D>
-size_t attn_bytes(const Plan& p) { return split_bytes<D>(p) + (p.cut ? BlockParts<D>::bytes(p.slots) : 0); }
+size_t attn_bytes(const Plan& p) { return split_bytes<D>(p) + (p.block ? BlockParts<D>::bytes(p.slots) : 0); }
+size_t attn_bytes(int d, const Plan& p) { return d == 64 ? attn_bytes<64>(p) : d == 128 ? attn_bytes<128>(p) : attn_bytes<256>(p); }
 
 template <int D, bool kCut>
 hipError_t launch_blocks(AttnArgs& A, long long n, hipStream_t s) {
@@ -1203,8 +1205,7 @@ size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, i
     using namespace ixg;
     Kv8 c;
     if (!make_kv8(cache, &c) || !attn_shape_ok(c, n_seq, total_T, max_q, h_q)) return 0;
-    const Plan p = plan_of(c.d, c.h_kv, h_q / c.h_kv, total_T, max_q, nullptr);
-    return c.d == 64 ? attn_bytes<64>(p) : c.d == 128 ? attn_bytes<128>(p) : attn_bytes<256>(p);
+    return attn_bytes(c.d, plan_of(c.d, c.h_kv, h_q / c.h_kv, total_T, max_q, nullptr));
 }
 
 hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens,
@@ -1218,9 +1219,8 @@ hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, c
     if (total_T == 0) return hipSuccess;                      // of tensors without elements, whose addresses may be 0
     if (!rows_ok(q, (long long)h_q * A.c.d) || (gate && !rows_ok(gate, (long long)h_q * A.c.d))) return hipErrorInvalidValue;
     if (!o || !ptr_aligned(o, 2)) return hipErrorInvalidValue;
-    if (!workspace || !ptr_aligned(workspace, 256) ||
-        workspace_bytes < ix_kv8_attn_workspace_size(cache, n_seq, total_T, max_q, h_q))
-        return hipErrorInvalidValue;
+    const Plan p = plan_of(A.c.d, A.c.h_kv, h_q / A.c.h_kv, total_T, max_q, s);
+    if (!workspace || !ptr_aligned(workspace, 256) || workspace_bytes < attn_bytes(A.c.d, p)) return hipErrorInvalidValue;
     A.q = q->p;
     A.q_stride = q->stride;
     if (gate) {
@@ -1234,7 +1234,6 @@ hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, c
     A.G = h_q / A.c.h_kv;
     A.window = window;
     A.sinks = sinks;
-    const Plan p = plan_of(A.c.d, A.c.h_kv, A.G, total_T, max_q, s);
     switch (A.c.d) {
         case 64: return launch_attn<64>(A, p, s);
         case 128: return launch_attn<128>(A, p, s);

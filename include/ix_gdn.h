@@ -407,7 +407,9 @@ hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_
 
 /* Bytes of device workspace for ix_kv8_attn on such a batch (partial results of what several
  * workgroups share; independent of the lengths, at most 81 MiB on 256 CUs), or 0 for an invalid
- * request. It needs no initialisation; calls that share it must be ordered. */
+ * request. It does for every batch of the same cache and h_q with no more tokens in all and no
+ * larger max_q, of any n_seq: a program may size it once, for the largest. It needs no
+ * initialisation; calls that share it must be ordered. */
 size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, int max_q, int h_q);
 
 /* Attention of the batch's tokens over the cache, which holds them already (ix_kv8_append):
