@@ -15,7 +15,7 @@ from __future__ import annotations
 
 import torch
 
-from . import (Cfg, IxGdnError, check, ix_gdn_decode, ix_gdn_decode_gated, ix_gdn_decode_workspace_size, ix_gdn_prefill,
+from . import (HIP_ERROR_INVALID_VALUE, Cfg, _rows, check, ix_gdn_decode, ix_gdn_decode_gated, ix_gdn_decode_workspace_size, ix_gdn_prefill,
                ix_gdn_prefill_gated, ix_gdn_prefill_gated_workspace_size, ix_gdn_prefill_workspace_size,
                ix_kv8_append, ix_kv8_attn, ix_kv8_attn_workspace_size, kv8_cache, make_cfg, out_gate)
 
@@ -67,6 +67,14 @@ class GdnLayer:
             check("ix_gdn_prefill_gated", ix_gdn_prefill_gated(*args, g, self._ws, self._ws.numel(), stream))
 
 
+def _check_rows(t, T, n):
+    """Raises unless t is on the GPU as rows [T] of n bf16 values or more, dense but for the stride between them."""
+    if t.dim() != 2 or t.stride(1) != 1 or t.dtype is not torch.bfloat16 or not t.is_cuda:
+        _rows(t)
+    if t.numel() < T * n or (T > 1 and t.stride(0) < n):
+        raise ValueError("baloon_amd: rows are [heads][d], one behind the other")
+
+
 class AttnLayer:
     """Attention of n_slots sequences of at most max_len tokens, h_q query heads over h_kv cached ones of d channels.
 
@@ -102,6 +110,8 @@ class AttnLayer:
         stride between rows; gate multiplies by its sigmoid. The lengths are advanced on torch's current stream."""
         if cu_seqlens.shape != (self.n_slots + 1,):
             raise ValueError("baloon_amd: cu_seqlens has an offset for each sequence and one more")
+        if cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_cuda or not cu_seqlens.is_contiguous():
+            raise ValueError("baloon_amd: cu_seqlens is int32, contiguous and on the GPU")
         return self._attend(cu_seqlens.diff(), cu_seqlens, max_q, q, k, v, gate, o, stream)
 
     def decode(self, q, k, v, gate=None, o=None, stream=None):
@@ -111,12 +121,20 @@ class AttnLayer:
         return self._attend(1, self._one_each, 1, q, k, v, gate, o, stream)
 
     def _attend(self, new, cu_seqlens, max_q, q, k, v, gate, o, stream):
+        # What the calls below would refuse, or read and write beside the operands, is refused before anything is done.
         T = q.shape[0]
         if k.shape[0] != T or v.shape[0] != T or (gate is not None and gate.shape[0] != T):
             raise ValueError("baloon_amd: q, k, v and gate have a row for each token")
+        for t, heads in ((q, self.h_q), (k, self.h_kv), (v, self.h_kv), (gate, self.h_q)):
+            if t is not None:
+                _check_rows(t, T, heads * self.d)
         if o is None:
             o = torch.empty(T, self.h_q, self.d, dtype=torch.bfloat16, device=self.device)
+        elif o.dtype != torch.bfloat16 or not o.is_cuda or not o.is_contiguous() or o.numel() < T * self.h_q * self.d:
+            raise ValueError("baloon_amd: o is bf16 [T][h_q][d], contiguous and on the GPU")
         need = ix_kv8_attn_workspace_size(self.cache, self.n_slots, T, max_q, self.h_q)
+        if need == 0:
+            check("ix_kv8_attn", HIP_ERROR_INVALID_VALUE)
         if self._ws is None or self._ws.numel() < need:
             self._ws = torch.empty(max(need, 256), dtype=torch.uint8, device=self.device)
         where = (cu_seqlens, self.kv_len, self.table, self.width)
@@ -125,7 +143,7 @@ class AttnLayer:
             check("ix_kv8_append", ix_kv8_append(self.cache, self.n_slots, T, *where, k, v, stream))
             check("ix_kv8_attn", ix_kv8_attn(self.cache, self.n_slots, T, max_q, *where, q, self.h_q, self.scale, self.window,
                                              self.sinks, gate, o, self._ws, self._ws.numel(), stream))
-        except IxGdnError:
-            self.kv_len -= new                                # a refused call leaves the lengths as they were
+        except BaseException:
+            self.kv_len -= new                                # a call that raises leaves the lengths as they were
             raise
         return o
