@@ -80,7 +80,11 @@ class AttnLayer:
 
     Slot i has pages i * width .. of the cache to itself; with n_pages the caller keeps the pages instead and fills
     `table` [n_slots][width] int32 before they are needed. kv_len [n_slots] int32 counts the tokens held: setting it to 0
-    empties a slot, to fewer tokens drops the last ones (rejected drafts). Tokens behind max_len are dropped."""
+    empties a slot, to fewer tokens drops the last ones (rejected drafts). Tokens behind max_len are dropped.
+
+    All of a call is on one stream, the lengths and a new o among it: `stream` (a torch stream or an address), or torch's
+    current one. The caller orders calls on different streams, and what else it does with the layer's tensors. The workspace
+    is allocated here for any batch (38 to 81 MiB), so a captured call's stays where it is."""
 
     def __init__(self, n_slots: int, max_len: int, h_q=16, h_kv=2, d=256, page=64, n_pages=None, window=0, sinks=0,
                  scale=None, device="cuda"):
@@ -102,25 +106,35 @@ class AttnLayer:
             self.table.fill_(-1)
         self.kv_len = tensor(n_slots, dtype=torch.int32)
         self._one_each = torch.arange(n_slots + 1, dtype=torch.int32, device=self.device)
-        self._ws = None
+        most = min(2 ** 31 - 1, 2 ** 37 // max(h_q, 1))       # tokens of a call
+        self._ws_bytes = ix_kv8_attn_workspace_size(self.cache, n_slots, most, most, h_q)
+        self._ws = torch.empty(max(self._ws_bytes, 256), dtype=torch.uint8, device=self.device)
 
     def prefill(self, cu_seqlens, max_q, q, k, v, gate=None, o=None, stream=None):
         """Appends packed new tokens (cu_seqlens int32 [n_slots + 1] on the device, at most max_q of a sequence) and
         returns their attention o [T][h_q][d] bf16. q and gate are rows of [h_q][d], k and v of [h_kv][d], bf16, with any
-        stride between rows; gate multiplies by its sigmoid. The lengths are advanced on torch's current stream."""
+        stride between rows; gate multiplies by its sigmoid."""
         if cu_seqlens.shape != (self.n_slots + 1,):
             raise ValueError("baloon_amd: cu_seqlens has an offset for each sequence and one more")
         if cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_cuda or not cu_seqlens.is_contiguous():
             raise ValueError("baloon_amd: cu_seqlens is int32, contiguous and on the GPU")
-        return self._attend(cu_seqlens.diff(), cu_seqlens, max_q, q, k, v, gate, o, stream)
+        return self._on(stream, cu_seqlens, max_q, q, k, v, gate, o)
 
     def decode(self, q, k, v, gate=None, o=None, stream=None):
         """The same for one token of every sequence."""
         if q.shape[0] != self.n_slots:
             raise ValueError("baloon_amd: one token for each sequence")
-        return self._attend(1, self._one_each, 1, q, k, v, gate, o, stream)
+        return self._on(stream, self._one_each, 1, q, k, v, gate, o)
 
-    def _attend(self, new, cu_seqlens, max_q, q, k, v, gate, o, stream):
+    def _on(self, stream, *args):
+        if stream is None:
+            return self._attend(*args)
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(getattr(stream, "cuda_stream", stream), self.device)
+        with torch.cuda.stream(stream):
+            return self._attend(*args)
+
+    def _attend(self, cu_seqlens, max_q, q, k, v, gate, o):
         # What the calls below would refuse, or read and write beside the operands, is refused before anything is done.
         T = q.shape[0]
         if k.shape[0] != T or v.shape[0] != T or (gate is not None and gate.shape[0] != T):
@@ -132,17 +146,15 @@ class AttnLayer:
             o = torch.empty(T, self.h_q, self.d, dtype=torch.bfloat16, device=self.device)
         elif o.dtype != torch.bfloat16 or not o.is_cuda or not o.is_contiguous() or o.numel() < T * self.h_q * self.d:
             raise ValueError("baloon_amd: o is bf16 [T][h_q][d], contiguous and on the GPU")
-        need = ix_kv8_attn_workspace_size(self.cache, self.n_slots, T, max_q, self.h_q)
-        if need == 0:
+        if not self._ws_bytes or max_q < min(T, 1) or max_q >= 2 ** 31:
             check("ix_kv8_attn", HIP_ERROR_INVALID_VALUE)
-        if self._ws is None or self._ws.numel() < need:
-            self._ws = torch.empty(max(need, 256), dtype=torch.uint8, device=self.device)
+        new = 1 if cu_seqlens is self._one_each else cu_seqlens.diff()
         where = (cu_seqlens, self.kv_len, self.table, self.width)
         self.kv_len += new
         try:
-            check("ix_kv8_append", ix_kv8_append(self.cache, self.n_slots, T, *where, k, v, stream))
+            check("ix_kv8_append", ix_kv8_append(self.cache, self.n_slots, T, *where, k, v))
             check("ix_kv8_attn", ix_kv8_attn(self.cache, self.n_slots, T, max_q, *where, q, self.h_q, self.scale, self.window,
-                                             self.sinks, gate, o, self._ws, self._ws.numel(), stream))
+                                             self.sinks, gate, o, self._ws, self._ws.numel()))
         except BaseException:
             self.kv_len -= new                                # a call that raises leaves the lengths as they were
             raise
