@@ -47,7 +47,7 @@ inline bool rows_ok(const ix_rows* r, long long least) {
     return r && r->p && ptr_aligned(r->p, 2) && r->stride >= least;
 }
 
-// The last b in [0, n) with key(b) <= j, for a key that does not fall and key(0) <= j: each step the wave's
+// The last b in [0, n) with key(b) <= j, or 0 where there is none, for a key that does not fall: each step the wave's
 // lanes try 64 places (one load's latency for 64 sequences, two for 4,096). The same in every lane.
 template <class Key>
 __device__ __forceinline__ int wave_search(int n, int j, int lane, Key key) {

@@ -849,7 +849,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         rb = j - key(b);
     }
     const int s0 = A.a.start(b), q = A.a.start(b + 1) - s0, r0 = rb * kBlockRows, rows = max(q, 0) * A.G;
-    if (!kCut && (rows <= A.small || r0 >= rows)) return;
+    if (!kCut && (rows <= A.small || rb < 0 || r0 >= rows)) return;      // rb < 0: before the first sequence's rows
     const int kv = max(A.a.kv_len[b], 0), first = kv - q;
 
     // q of row n of the wave, channels 64 c + 16 g .. + 15

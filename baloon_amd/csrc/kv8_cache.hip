@@ -33,8 +33,9 @@ __device__ __forceinline__ bool page_job(const Batch& a, const Kv8& c, int j, in
     const int b = wave_search(a.n_seq, j, lane, [&](int i) { return (a.start(i) >> c.page_log) + 2 * i; });
     const int s0 = a.start(b), q = a.start(b + 1) - s0, kv = a.kv_len[b];
     const int first = kv - q, from = max(first, 0);         // tokens before position 0 are not held
-    const int p = (from >> c.page_log) + j - ((s0 >> c.page_log) + 2 * b);
-    if (q <= 0 || kv <= 0 || p > (kv - 1) >> c.page_log) return false;
+    const int slot = j - ((s0 >> c.page_log) + 2 * b);      // negative before the first sequence's rows
+    const int p = (from >> c.page_log) + slot;
+    if (q <= 0 || kv <= 0 || slot < 0 || p > (kv - 1) >> c.page_log) return false;
     const int at = p << c.page_log;
     const int lo = max(from, at);
     out->b = b;

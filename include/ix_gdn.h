@@ -378,8 +378,8 @@ typedef struct ix_kv8 {
 } ix_kv8;
 
 /* The batch of the calls below: n_seq sequences (at most 65535), total_T packed new tokens,
- *   cu_seqlens [n_seq+1] int32 device offsets of their rows (cu_seqlens[0] = 0, non-decreasing;
- *   a sequence may have none; rows behind the last offset are neither read nor written)
+ *   cu_seqlens [n_seq+1] int32 device offsets of their rows (non-decreasing; a sequence may have
+ *   none; rows before the first offset and behind the last are neither read nor written)
  *   kv_len [n_seq] int32: tokens of each sequence with the new ones, which stand at positions
  *   kv_len - q .. kv_len - 1 for q new ones
  *   table [n_seq][width] int32: page p of sequence b, tokens p * page on, is page table[b][p] of
