@@ -323,25 +323,23 @@ __device__ __forceinline__ v4f outputs(v4f o, float m, float lse) {
 }
 // Partial results of a row put together: sums of p' relative to 2^m, and logarithms of the sums of p.
 struct Joined {
-    float m = -__builtin_inff(), top = -__builtin_inff(), total = 0.0f;      // total 2^top: the sum of p
+    // below every reference but -inf, and finite: 2^(-inf - it) is 0, without a question for each
+    float m = -__FLT_MAX__, top = -__FLT_MAX__, total = 0.0f;      // total 2^top: the sum of p
     v4f o = {0, 0, 0, 0};
-    static __device__ __forceinline__ float power(float x, float to) {       // 2^(x - to), 0 for x = -inf
-        return x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x - to);
-    }
     // The references, before what is added is.
     __device__ __forceinline__ void meet(float pm, float lse) {
         m = fmaxf(m, pm);
         top = fmaxf(top, lse);
     }
     __device__ __forceinline__ void add(float pm, float lse, const v4f& po) {
-        total += power(lse, top);
-        o += po * power(pm, m);
+        total += __builtin_amdgcn_exp2f(lse - top);
+        o += po * __builtin_amdgcn_exp2f(pm - m);
     }
     __device__ __forceinline__ void more(float pm, float lse, const v4f& po) {
         const float was_m = m, was_top = top;
         meet(pm, lse);
-        total *= power(was_top, top);
-        o *= power(was_m, m);
+        total *= __builtin_amdgcn_exp2f(was_top - top);
+        o *= __builtin_amdgcn_exp2f(was_m - m);
         add(pm, lse, po);
     }
     __device__ __forceinline__ float log2_sum() const { return top + __builtin_amdgcn_logf(total); }
