@@ -211,7 +211,10 @@ __device__ __forceinline__ long long quotient(long long a, int b) { return (long
 // there is a workgroup for each and they have up to kWhole: joining costs more than a few tiles one after another. 64
 // sequences over 8 heads of 128 take, us, with 1 token each 9.3 (18.6 as 4 tiles), 32 with 300 10.2 (15.3) and with 800 16.0
 // (18.0); 128 over 2 of 256 with 200 12.9 (20.1) and with 450, 15 tiles, 18.3 (23.5). From 16 tiles on few segments are
-// slower whole: 8 sequences over 8 heads of 128, 1,020 tokens each, 13.6 (10.7).
+// slower whole: 8 sequences over 8 heads of 128, 1,020 tokens each, 13.6 (10.7). Where the limit lies depends on how many
+// workgroups are free, which the rule asks only as yes or no. Neither rule keeps a share from lying across two
+// segments and beginning both: lengths that a share's tiles do not divide can take more than longer ones that they do (1
+// sequence over 2 heads of 256: 900 tokens 13.9, 1,001 11.3, 1,100 14.9).
 constexpr int kMinShare = 4, kWhole = 15;
 constexpr int kStart = 6;             // tiles of 16 KiB in the time of a segment's start
 struct Share {
@@ -381,7 +384,7 @@ constexpr int kSplitTok = D == 256 ? 32 : 64;
 // Bound by memory: 128 tokens over 8,000 each, 32 heads over 8 of 128, read 2.1 GB in 360 us, 5.8 of the 6.2 TB/s that reads
 // reach, 64 over 1 to 8,192, 16 heads over 2 of 256, 252 MB in 54 and join_kernel's 6. Short contexts are bound by the way to
 // the first tile (lengths, pages, codes: about 5 us with the launch), by whole tiles for each of four waves, and by the
-// second launch: 48 windows of 1,028 tokens over 4 heads of 128, 51 MB, take 20.4 us where reading takes 8.2.
+// second launch: 48 windows of 1,028 tokens over 4 heads of 128, 51 MB, take 21.0 us where reading takes 8.2.
 template <int D>
 __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     constexpr int kC = D / 64, kM = D / 16, kPitch = D + 4, kTok = kSplitTok<D>, kS = kTok / 16;
@@ -711,8 +714,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg
 // (16 heads over 2 of 256) against 176: it is 256 blocks of 1 to 64 tiles then, one to a CU, and the sums leave no
 // registers to read ahead. At D <= 128 two workgroups share a CU.
 //
-// Those 176 us are 780 TFLOP/s (a large bf16 product reaches 1,240), with the matrix units busy for 34% of it, vector
-// instructions issued in 39% and LDS in 37%: the waves of a workgroup pass through products and exponentials together.
+// Those 176 us are 780 TFLOP/s (a large bf16 product reaches 1,240), with the matrix units busy for 33% of it, vector
+// instructions issued in 41% and LDS in 36%: the waves of a workgroup pass through products and exponentials together.
 // Half of them half a tile behind, with two barriers a tile, took 236 us, the next tile's scores between a tile's
 // exponentials and its second product 204 to 212.
 constexpr int kBlockThreads = 512, kBlockTok = 64, kBlockRows = 128;
