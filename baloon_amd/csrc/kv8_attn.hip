@@ -99,11 +99,12 @@ struct LaneSum {
         }
         return f;
     }
-    // log2 of the sum of a row's four lanes.
-    __device__ __forceinline__ float log2_row() const {
+    // log2 of the sum of a row's four lanes, less `to` (finite, near to ref or far below all): itself a score is as large as it likes,
+    // and a power of its rounding would be in the result.
+    __device__ __forceinline__ float log2_row(float to) const {
         const float top = pair_max32(pair_max16(ref));
         const float f = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - top);
-        return top + __builtin_amdgcn_logf(pair_sum32(pair_sum16(l * f)));
+        return top - to + __builtin_amdgcn_logf(pair_sum32(pair_sum16(l * f)));
     }
 };
 
@@ -317,32 +318,32 @@ __device__ __forceinline__ uint2 load_gate(const AttnArgs& A, int t, int h, int 
     if (A.gate) __builtin_memcpy(&z, A.gate + (long long)t * A.gate_stride + (size_t)h * A.c.d + d, sizeof(z));
     return z;
 }
-// 4 outputs of a row from its sum of p' and its sum of p, 2^m o and 2^lse: o 2^(m - lse), of which the power alone can leave the
-// floats' range.
-__device__ __forceinline__ v4f outputs(v4f o, float m, float lse) {
+// 4 outputs of a row from its sum of p', o 2^m, and the logarithm of its sum of p, m + lse: o 2^-lse, of which the power alone can
+// leave the floats' range.
+__device__ __forceinline__ v4f outputs(v4f o, float lse) {
     if (lse == -__builtin_inff()) return v4f{0, 0, 0, 0};
-    const float f = __builtin_amdgcn_exp2f(0.5f * (m - lse));
+    const float f = __builtin_amdgcn_exp2f(-0.5f * lse);
     return o * f * f;
 }
-// Partial results of a row put together: sums of p' relative to 2^m, and logarithms of the sums of p.
+constexpr float kNone = -__FLT_MAX__;      // m of a part without a token: finite, so that lse, -inf, is 0 as a power, without a question
+// Partial results (m, lse, o) of a row put together.
 struct Joined {
-    // below every reference but -inf, and finite: 2^(-inf - it) is 0, without a question for each
-    float m = -__FLT_MAX__, top = -__FLT_MAX__, total = 0.0f;      // total 2^top: the sum of p
+    float m = kNone, top = kNone, total = 0.0f;              // total 2^(m + top): the sum of p
     v4f o = {0, 0, 0, 0};
-    // The references, before what is added is.
-    __device__ __forceinline__ void meet(float pm, float lse) {
-        m = fmaxf(m, pm);
-        top = fmaxf(top, lse);
-    }
+    // Several that are at hand: m of all, then top of all, then what they add.
+    __device__ __forceinline__ void meet_m(float pm) { m = fmaxf(m, pm); }
+    __device__ __forceinline__ void meet_sum(float pm, float lse) { top = fmaxf(top, pm - m + lse); }
     __device__ __forceinline__ void add(float pm, float lse, const v4f& po) {
-        total += __builtin_amdgcn_exp2f(lse - top);
+        total += __builtin_amdgcn_exp2f(pm - m + lse - top);
         o += po * __builtin_amdgcn_exp2f(pm - m);
     }
+    // One more.
     __device__ __forceinline__ void more(float pm, float lse, const v4f& po) {
-        const float was_m = m, was_top = top;
-        meet(pm, lse);
-        total *= __builtin_amdgcn_exp2f(was_top - top);
-        o *= __builtin_amdgcn_exp2f(was_m - m);
+        const float now = fmaxf(m, pm), was = m - now + top;
+        o *= __builtin_amdgcn_exp2f(m - now);
+        m = now;
+        top = fmaxf(fmaxf(was, pm - m + lse), kNone);
+        total *= __builtin_amdgcn_exp2f(was - top);
         add(pm, lse, po);
     }
     __device__ __forceinline__ float log2_sum() const { return top + __builtin_amdgcn_logf(total); }
@@ -483,9 +484,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         if (open) {                                           // the four waves' parts of the last piece together
             const AttnArgs& Z = args_again();
             const int x_r0 = taken(o_r0), x_rows = taken(o_rows), x_slot = taken(o_slot);
-            const float lse = sum.log2_row();
+            const float m = mref == -__builtin_inff() ? kNone : mref - kLift, lse = sum.log2_row(m);
             if (g == 0) {
-                lo_ml[(w * kSplitRows + n) * 2] = mref - kLift;
+                lo_ml[(w * kSplitRows + n) * 2] = m;
                 lo_ml[(w * kSplitRows + n) * 2 + 1] = lse;
             }
 #pragma unroll
@@ -497,14 +498,16 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
                 if (x_r0 + row >= x_rows) break;
                 Joined to;
 #pragma unroll
-                for (int k = 0; k < kSplitWaves; ++k) to.meet(lo_ml[(k * kSplitRows + row) * 2], lo_ml[(k * kSplitRows + row) * 2 + 1]);
+                for (int k = 0; k < kSplitWaves; ++k) to.meet_m(lo_ml[(k * kSplitRows + row) * 2]);
+#pragma unroll
+                for (int k = 0; k < kSplitWaves; ++k) to.meet_sum(lo_ml[(k * kSplitRows + row) * 2], lo_ml[(k * kSplitRows + row) * 2 + 1]);
 #pragma unroll
                 for (int k = 0; k < kSplitWaves; ++k)
                     to.add(lo_ml[(k * kSplitRows + row) * 2], lo_ml[(k * kSplitRows + row) * 2 + 1],
                            *reinterpret_cast<const v4f*>(lo_o + (k * kSplitRows + row) * kPitch + d));
                 if (x_slot < 0) {
                     const int token = (x_r0 + row) / Z.G;
-                    store_out(Z, taken(o_s0) + token, taken(o_e) * Z.G + x_r0 + row - token * Z.G, d, outputs(to.o, to.m, to.log2_sum()));
+                    store_out(Z, taken(o_s0) + token, taken(o_e) * Z.G + x_r0 + row - token * Z.G, d, outputs(to.o, to.log2_sum()));
                 } else {
                     *reinterpret_cast<v4f*>(parts.o + ((size_t)x_slot * kSplitRows + row) * D + d) = to.o;
                     if (d == 0) {
@@ -684,7 +687,7 @@ __device__ __forceinline__ void join_outputs(const AttnArgs& A, const float* po,
         }
         if (way == 0 && x0 + (int)threadIdx.x < to) {
             const int token = (r0 + row) / A.G;
-            store_out(A, s0 + token, e * A.G + r0 + row - token * A.G, d, outputs(sum.o, sum.m, sum.log2_sum()));
+            store_out(A, s0 + token, e * A.G + r0 + row - token * A.G, d, outputs(sum.o, sum.log2_sum()));
         }
     }
 }
@@ -1066,7 +1069,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         lds_barrier();
     }
 
-    const float lse = sum.log2_row(), m_ref = limit == -__builtin_inff() ? limit : ref;
+    const float m_ref = limit == -__builtin_inff() ? kNone : ref, lse = sum.log2_row(m_ref);
     int thread = tid;
     asm volatile("" : "+v"(thread));                          // the row is worked out again: it does not wait in registers
     const int r = w0 + (thread & 15), qi = r / A.G, head = e * A.G + r - qi * A.G, d0 = 4 * (thread >> 4 & 3);
@@ -1088,7 +1091,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
 #pragma unroll
             for (int i = 0; i < kN; ++i) z[i] = load_gate(A, s0 + qi, head, 16 * (m0 + i) + d0);
 #pragma unroll
-            for (int i = 0; i < kN; ++i) store_out(A, s0 + qi, head, 16 * (m0 + i) + d0, outputs(acc[m0 + i], m_ref, lse), z[i]);
+            for (int i = 0; i < kN; ++i) store_out(A, s0 + qi, head, 16 * (m0 + i) + d0, outputs(acc[m0 + i], lse), z[i]);
         }
     }
 }

@@ -171,3 +171,29 @@ def test_rows_keep_their_bits_beside_others():
         for t, hh in ((0, 3), (1, 15)):
             got[t, hh] = clean[t, hh]
         assert np.array_equal(got, clean)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("q,n,h", SHAPES)
+@pytest.mark.parametrize("first,others", [(3e4, 0), (0, -3e4), (-1e6, -2e6), (1e6, -1e6), (2e7, 1e7)])
+def test_one_token_far_above_the_others(d, q, n, h, first, others):
+    """Scores far from 0 of which the first token's is so much larger that it has all of the weight: the result is its value, and the
+    scores' size is no part of the tolerance (2^-11 for p in fp16 and 2^-8 for the result's half ulp, as in the module's)."""
+    P = Problem([q] * n, [q + 203 * b + 9 for b in range(n)], 16, h, d, 4, seed=7)
+    ref = P.p.ref
+    P.q[:] = 0
+    P.q[:, :, 0] = 8
+    P.q_bits = bf16.from_f32(P.q)
+    unit = 1e4 if max(abs(first), abs(others)) < 1e6 else 1e6
+    ref.codes["k"][:] = 0
+    ref.codes["k"][:, :, :, 0] = int(others / unit)
+    for b in range(n):
+        ref.codes["k"][P.tables[b, 0], :, 0, 0] = int(first / unit)
+    ref.scale["k"][:] = 1
+    got, at = P.run(scale=unit / 8), 0
+    for b, m in enumerate(P.q_len):
+        v, _ = ref.tokens("v", 1, P.tables[b])
+        want = v[0].astype(np.float64).repeat(4, 0)[None]
+        assert np.all(np.abs(got[at:at + m] - want) <= (2.0 ** -11 + 2.0 ** -8) * np.abs(want) + 2.0 ** -33 * np.abs(v).max())
+        at += m
