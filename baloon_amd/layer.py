@@ -130,7 +130,9 @@ class AttnLayer:
         if stream is None:
             return self._attend(*args)
         if not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(getattr(stream, "cuda_stream", stream), self.device)
+            address = getattr(stream, "cuda_stream", getattr(stream, "value", stream)) or 0      # also a ctypes.c_void_p
+            # torch takes an ExternalStream of address 0 for one that it is to choose
+            stream = torch.cuda.ExternalStream(address, self.device) if address else torch.cuda.default_stream(self.device)
         with torch.cuda.stream(stream):
             return self._attend(*args)
 

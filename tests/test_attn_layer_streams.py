@@ -1,5 +1,7 @@
 """AttnLayer on another stream than torch's current one, and captured: a call's lengths, kernels and outputs are in its stream's order,
 and its workspace stays where it is."""
+import ctypes
+
 import pytest
 
 import baloon_amd as bx
@@ -50,6 +52,29 @@ def test_a_stream_that_is_behind(as_address, own_o):
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     assert layer.kv_len.tolist() == other.kv_len.tolist() == [44, 8, 207]
+
+
+@pytest.mark.parametrize("null", [0, "c_void_p", "default"])
+def test_the_null_stream_by_its_address(null):
+    """While torch's current stream is another one and the null stream is busy."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(6)
+    layer, other = layers()
+    todo = steps(g)
+    want = [call(other, s) for s in todo]
+    side, busy = torch.cuda.Stream(), torch.randn(4096, 4096, device="cuda")
+    default = torch.cuda.default_stream()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        busy = busy @ busy * 1e-3
+    with torch.cuda.stream(side):
+        stream = {0: 0, "c_void_p": ctypes.c_void_p(0), "default": default}[null]
+        got = [call(layer, s, stream=stream) for s in todo]
+    side_done, behind = side.query(), not default.query()
+    torch.cuda.synchronize()
+    assert side_done and behind
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
 
 
 def test_streams_in_turn():
