@@ -15,6 +15,7 @@ missing; the other symbols are bound with ctypes.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -28,6 +29,8 @@ HEAD_MOD = 0   # src = h mod h_k (reference pairing, src/ix_gdn.cu:38)
 HEAD_DIV = 1   # src = h / (h_v / h_k)
 ACT_NONE = 0   # conv output used as is (reference, src/ix_gdn.cu:64-67)
 ACT_SILU = 1
+ROPE_HALVES = 0   # channel i turns with i + rot / 2
+ROPE_PAIRS = 1    # channel 2 i with 2 i + 1
 
 # Every symbol include/ix_gdn.h declares.
 EXPORTS = (
@@ -39,6 +42,7 @@ EXPORTS = (
     "ix_bf16_gemv", "ix_bf16_gemv_pair", "ix_bf16_gemv_split", "ix_mmvq_q8_0", "ix_gdn_in_proj_width", "ix_gdn_in_proj",
     "ix_gdn_version", "ix_gdn_decode_noalloc", "ix_q8_1_quantize", "ix_gdn_commit_window_layers",
     "ix_add_rms_norm", "ix_kv8_append", "ix_kv8_read", "ix_kv8_attn_workspace_size", "ix_kv8_attn",
+    "ix_rope_rows", "ix_kv8_append_rope",
 )
 
 
@@ -87,15 +91,24 @@ class Rows(ctypes.Structure):
     _fields_ = [("p", ctypes.c_void_p), ("stride", ctypes.c_longlong)]
 
 
+class Rope(ctypes.Structure):
+    """``ix_rope`` (include/ix_gdn.h): rotary positions of a head's row, and its norm; see :func:`rope`."""
+
+    _fields_ = [
+        ("rot", ctypes.c_int), ("layout", ctypes.c_int), ("freq", ctypes.c_void_p), ("amplitude", ctypes.c_float),
+        ("norm", ctypes.c_void_p), ("norm_offset", ctypes.c_float), ("eps", ctypes.c_float),
+    ]
+
+
 def make_cfg(h_k=16, h_v=32, d_k=128, d_v=128, d_conv=4, head_map=HEAD_MOD, conv_act=ACT_NONE,
              q_scale=1.0, l2_eps=1e-6) -> Cfg:
     """Layer description; defaults are the reference's semantics at the Qwen3-Next shape."""
     return Cfg(h_k, h_v, d_k, d_v, d_conv, head_map, conv_act, q_scale, l2_eps)
 
 
-# Arguments of every symbol: a layer description (c), output gate (g) or cache (k) by reference, token rows (r), a
+# Arguments of every symbol: a layer description (c), output gate (g) or cache (k) or positions (t) by reference, token rows (r), a
 # tensor's address (p), the stream (s); i, l, z and f are an int, a long long, a size_t and a float.
-_TYPES = {**dict.fromkeys("cgkrps", ctypes.c_void_p), "i": ctypes.c_int, "l": ctypes.c_longlong, "z": ctypes.c_size_t,
+_TYPES = {**dict.fromkeys("cgktrps", ctypes.c_void_p), "i": ctypes.c_int, "l": ctypes.c_longlong, "z": ctypes.c_size_t,
           "f": ctypes.c_float}
 _I, _Z = ctypes.c_int, ctypes.c_size_t
 _SIGNATURES = {
@@ -132,6 +145,8 @@ _SIGNATURES = {
     "ix_kv8_read": ("kiipppipps", _I),
     "ix_kv8_attn_workspace_size": ("kiiii", _Z),
     "ix_kv8_attn": ("kiiipppirifiirppzs", _I),
+    "ix_rope_rows": ("tiippriips", _I),
+    "ix_kv8_append_rope": ("kiipppirrtritps", _I),
 }
 
 _lib = None
@@ -202,7 +217,7 @@ def _through_ctypes(name, args) -> int:
     """A launcher's call with ctypes' conversions: for arguments that the extension leaves to it (anything but
     plain tensors, ints, floats, structures and streams), and for every call where there is no extension."""
     convert = {"c": lambda v: _byref(v, Cfg), "g": lambda v: None if v is None else _byref(v, OutGate),
-               "k": lambda v: None if v is None else _byref(v, Kv8),
+               "k": lambda v: None if v is None else _byref(v, Kv8), "t": lambda v: None if v is None else _byref(v, Rope),
                "r": lambda v: None if v is None else _byref(_rows(v), Rows), "p": _ptr, "s": _stream}
     fn = getattr(lib(), name)
     args = [convert[t](v) if t in convert else v for t, v in zip(_SIGNATURES[name][0], args)]
@@ -471,6 +486,77 @@ def ix_kv8_append(cache: Kv8, n_seq, total_T, cu_seqlens, kv_len, table, width, 
 def ix_kv8_read(cache: Kv8, n_seq, total_T, cu_seqlens, kv_len, table, width, k=None, v=None, s=None) -> int:
     """The cache's values at the batch's positions, as bf16 [total_T][h_kv][d]."""
     return _bind.ix_kv8_read(cache, n_seq, total_T, cu_seqlens, kv_len, table, width, k, v, s)
+
+
+def rope_freq(rot, base=10000.0, scaling="none", factor=1.0, trained=None, slow=1.0, fast=32.0):
+    """Frequencies of :func:`rope` for `rot` turned channels, fp32 [rot/2] on the CPU, and the factor of cosine and sine (1 but
+    for "parts"): base ** (-2 i / rot), made fit for contexts of `factor` times the length that a model was trained on:
+
+        "none"    as they are
+        "linear"  all divided by factor
+        "base"    base * factor ** (rot / (rot - 2)): the slowest divided by factor, the fastest kept
+        "parts"   those that went round less than `slow` times in `trained` tokens divided by factor, those that did more than
+                  `fast` times kept, those between in proportion; cosine and sine times 0.1 ln(factor) + 1
+    """
+    import torch
+    if rot < 2 or rot % 2:
+        raise ValueError("baloon_amd: rot is even and at least 2")
+    if factor < 1 or base <= 1:
+        raise ValueError("baloon_amd: base is above 1, factor at least 1")
+    if scaling == "base" and rot > 2:
+        base = base * factor ** (rot / (rot - 2))
+    freq = base ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    amplitude = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "parts":
+        if not trained or fast <= slow:
+            raise ValueError("baloon_amd: scaling by parts needs the length trained on, and fast > slow")
+        keep = ((freq * trained / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+        freq = freq * (keep + (1 - keep) / factor)
+        amplitude = 0.1 * math.log(factor) + 1
+    elif scaling not in ("none", "base"):
+        raise ValueError(f"baloon_amd: no scaling {scaling!r}")
+    return freq.float(), amplitude
+
+
+def rope(freq, layout=ROPE_HALVES, amplitude=1.0, norm=None, norm_offset=0.0, eps=1e-6) -> Rope:
+    """The description of a head's rotary positions: freq [rot/2] fp32 radians a position (None: nothing is turned), layout
+    ROPE_HALVES or ROPE_PAIRS; norm [d] fp32 the weight of the head's RMS norm ahead of them, less norm_offset, or None. It
+    holds on to the tensors."""
+    import torch
+    for t in (freq, norm):
+        if t is not None and (t.dtype != torch.float32 or t.dim() != 1):
+            raise ValueError("baloon_amd: freq and norm are fp32 tensors of one dimension")
+    r = Rope(0 if freq is None else 2 * freq.numel(), layout, _ptr(freq), amplitude, _ptr(norm), norm_offset, eps)
+    r.tensors = (freq, norm)
+    return r
+
+
+def _check_norm(r, d):
+    """The library cannot see how long a norm's tensor is."""
+    norm = getattr(r, "tensors", (None, None))[1]
+    if norm is not None and norm.numel() != d:
+        raise ValueError("baloon_amd: the norm has a weight for each of the head's channels")
+
+
+def ix_rope_rows(rope: Rope, n_seq, total_T, cu_seqlens, kv_len, x, heads, d, y, s=None) -> int:
+    """y [total_T][heads][d] bf16: the rows x normed and turned by their tokens' positions, kv_len - q .. kv_len - 1 for a
+    sequence's q new ones. x is a bf16 tensor of rows [heads][d] whose first dimension may have any stride; y may be x where
+    that is packed."""
+    _check_norm(rope, d)
+    return _bind.ix_rope_rows(rope, n_seq, total_T, cu_seqlens, kv_len, x, heads, d, y, s)
+
+
+def ix_kv8_append_rope(cache: Kv8, n_seq, total_T, cu_seqlens, kv_len, table, width, k, v, rope_k, q=None, h_q=0, rope_q=None,
+                       q_out=None, s=None) -> int:
+    """ix_kv8_append with keys that are normed and turned on the way, and in the same launch the queries: q_out
+    [total_T][h_q][d] bf16 is what ix_rope_rows makes of q with rope_q. q is a bf16 tensor of rows [h_q][d] of any stride."""
+    if cache is not None:
+        _check_norm(rope_k, cache.d)
+        if q is not None:
+            _check_norm(rope_q, cache.d)
+    return _bind.ix_kv8_append_rope(cache, n_seq, total_T, cu_seqlens, kv_len, table, width, k, v, rope_k, q, h_q, rope_q, q_out, s)
 
 
 def ix_kv8_attn_workspace_size(cache: Kv8, n_seq: int, total_T: int, max_q: int, h_q: int) -> int:

@@ -108,6 +108,12 @@ struct Arg<const ix_kv8*> {
         return o == Py_None ? nullptr : structure<ix_kv8>(o, other);
     }
 };
+template <>
+struct Arg<const ix_rope*> {
+    static const ix_rope* of(PyObject* o, bool& other) {
+        return o == Py_None ? nullptr : structure<ix_rope>(o, other);
+    }
+};
 // Rows of a tensor on the GPU: bf16, dense but for the first dimension.
 template <>
 struct Arg<const ix_rows*> {
@@ -211,7 +217,8 @@ PyObject* call(hipError_t (*fn)(A...), const char* name, PyObject* const* args, 
     X(ix_gdn_decode_noalloc) X(ix_gdn_decode_gated) X(ix_gdn_prefill) X(ix_gdn_prefill_gated)                    \
     X(ix_gdn_decode_window) X(ix_gdn_decode_window_mfma) X(ix_gdn_commit_window) X(ix_bf16_gemv)                 \
     X(ix_bf16_gemv_pair) X(ix_bf16_gemv_split) X(ix_mmvq_q8_0) X(ix_q8_1_quantize) X(ix_gdn_in_proj)             \
-    X(ix_add_rms_norm) X(ix_kv8_append) X(ix_kv8_read) X(ix_kv8_attn)
+    X(ix_add_rms_norm) X(ix_kv8_append) X(ix_kv8_read) X(ix_kv8_attn)                                       \
+    X(ix_rope_rows) X(ix_kv8_append_rope)
 
 #define X(name)                                                                        \
     decltype(&::name) p_##name = nullptr;                                              \

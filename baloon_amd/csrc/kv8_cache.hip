@@ -19,7 +19,7 @@
 // One token for each of 64 sequences: 5.2 and 4.2 us, launches and that chain.
 #include <type_traits>
 
-#include "kv8.h"
+#include "rope.h"
 
 namespace ixg {
 namespace {
@@ -28,6 +28,7 @@ namespace {
 // q / page + 2 pages hold its q new tokens, so no prefix sum over the sequences is needed.
 struct PageJob {
     int b, id, held, end, row;      // slots held .. end - 1 of page id take the rows from `row` on
+    int pos;                        // position of slot 0
 };
 __device__ __forceinline__ bool page_job(const Batch& a, const Kv8& c, int j, int lane, PageJob* out) {
     const int b = wave_search(a.n_seq, j, lane, [&](int i) { return (a.start(i) >> c.page_log) + 2 * i; });
@@ -43,6 +44,7 @@ __device__ __forceinline__ bool page_job(const Batch& a, const Kv8& c, int j, in
     out->held = lo - at;
     out->end = min(kv - at, c.page);
     out->row = s0 + lo - first;
+    out->pos = at;
     return out->id >= 0;
 }
 
@@ -135,15 +137,42 @@ __device__ __forceinline__ Turn turn_of(int i, int span_log) {
 // chunks of 16 bytes in between; a chunk's codes take its first or, in odd 16s of slots, second half (the turn reads
 // the 16s together). The second pass is a rolled loop: every launch begins with an empty instruction cache, and with it
 // unrolled 8, 4 and 2 times a single token for 64 sequences took 7.9, 6.6 and 5.5 us of the kernel's time.
+//
+// With positions (Turned; ix_kv8_append_rope) the keys are normed, turned and rounded to bf16 where they lie in LDS, each wave
+// its own rows, so the codes are those of rows that ix_rope_rows has turned, bit for bit. The queries are the third part of
+// the grid, item by item (rope.h).
 constexpr int kBatch = 4;
-template <int kThreads>
+struct Plain {
+    static constexpr bool any = false;
+};
+struct Turned {
+    static constexpr bool any = true;
+    Rope k;
+    RopeRows q;                   // q.x NULL: no queries
+    int table;                    // pairs of a wave's table
+    long long wgs;                // of each part of the grid in all launches
+};
+template <int kThreads, class Pos>
 __global__ void __launch_bounds__(kThreads)
 append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_stride, const uint16_t* __restrict__ vr,
-              long long v_stride, int first_slot) {
+              long long v_stride, int first_slot, Pos turn) {
     extern __shared__ uint4 raw[];
     __shared__ float red[kThreads / kWave];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), h = blockIdx.y;
-    const bool is_v = blockIdx.z;
+    const bool is_v = blockIdx.z == 1;
+    [[maybe_unused]] float2* table = nullptr;
+    if constexpr (Pos::any) {
+        const int w = __builtin_amdgcn_readfirstlane(tid / kWave);
+        table = reinterpret_cast<float2*>(raw + c.page * c.d / 8) + w * turn.table;
+        if (blockIdx.z == 2) {
+            const long long wg = ((long long)first_slot + blockIdx.x) * c.h_kv + h, items = (long long)a.T * turn.q.groups;
+            for (long long i = wg * (kThreads / kWave) + w; i < items; i += turn.wgs * (kThreads / kWave)) {
+                const int t = (int)(i / turn.q.groups);
+                rope_item(turn.q, a, t, (int)(i - (long long)t * turn.q.groups), lane, table);
+            }
+            return;
+        }
+    }
     PageJob job;
     if (!page_job(a, c, first_slot + (int)blockIdx.x, lane, &job)) return;
     const int per_log = c.d == 64 ? 3 : c.d == 128 ? 4 : 5, chunks = (job.end - job.held) << per_log;
@@ -163,10 +192,40 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
         for (int y = 0; y < kBatch; ++y) x[y] = i0 + y * kThreads < chunks ? load(i0 + y * kThreads) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int y = 0; y < kBatch; ++y) {
-            m = fmaxf(m, max_abs(x[y]));
+            if (!Pos::any || is_v) m = fmaxf(m, max_abs(x[y]));
             if (i0 + y * kThreads < chunks) held[i0 + y * kThreads] = x[y];
         }
     }
+    if constexpr (Pos::any)
+        if (!is_v) {
+            const Rope& r = turn.k;
+            RopeLane L;
+            L.begin(r, lane);
+            const int rows_log = 6 - per_log, n = r.half << rows_log;
+            wave_lds_sync();
+#pragma unroll 1
+            for (int i0 = tid - lane; i0 < chunks; i0 += kThreads) {                      // the wave's own chunks, whole rows of them
+                const int i = i0 + lane, first = job.pos + job.held + (i0 >> per_log);
+#pragma unroll 1
+                for (int j = lane; j < n; j += kWave) {
+                    const int row = (int)((unsigned)j / (unsigned)r.half);
+                    table[j] = cos_sin(r, first + row, r.freq[j - row * r.half]);
+                }
+                wave_lds_sync();
+                uint4 x = make_uint4(0, 0, 0, 0), other = x;
+                if (i < chunks) {
+                    x = held[i];
+                    other = L.load_other(r, reinterpret_cast<const uint16_t*>(held + (i >> per_log << per_log)),
+                                         [](const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); });
+                }
+                float C[8], S[8];
+                L.factors(r, table + (lane >> per_log) * r.half, C, S);
+                x = L.turned(r, x, other, C, S);
+                m = fmaxf(m, max_abs(x));
+                wave_lds_sync();
+                if (i < chunks) held[i] = x;
+            }
+        }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
     if (lane == 0) red[tid / kWave] = m;
@@ -301,14 +360,24 @@ hipError_t with_threads(int n, F launch) {
     return launch(std::integral_constant<int, 512>{});
 }
 
-template <int kThreads>
-hipError_t launch_append(const Kv8& c, const Batch& a, const ix_rows* k, const ix_rows* v, hipStream_t s) {
+template <int kThreads, class Pos>
+hipError_t launch_append(const Kv8& c, const Batch& a, const ix_rows* k, const ix_rows* v, Pos turn, hipStream_t s) {
     static OncePerDevice once;
-    const hipError_t ready = allow_lds(once, &append_kernel<kThreads>, 128 * 256 * sizeof(uint16_t), s);
+    size_t lds = c.page * c.d * sizeof(uint16_t);
+    int most = 128 * 256 * sizeof(uint16_t);
+    unsigned parts = 2;
+    const long long slots = page_slots(c, a);
+    if constexpr (Pos::any) {
+        lds += kThreads / kWave * turn.table * sizeof(float2);
+        most += kThreads / kWave * kWave * 8 / 2 * sizeof(float2);                        // a pair for two of a wave's values
+        turn.wgs = slots * c.h_kv;
+        if (turn.q.x) parts = 3;
+    }
+    const hipError_t ready = allow_lds(once, &append_kernel<kThreads, Pos>, most, s);
     if (ready != hipSuccess) return ready;
-    return launch_in_pieces(page_slots(c, a), kThreads, [&](long long first, unsigned n) {
-        hipLaunchKernelGGL((append_kernel<kThreads>), dim3(n, (unsigned)c.h_kv, 2), dim3(kThreads), c.page * c.d * sizeof(uint16_t), s,
-                           c, a, k->p, k->stride, v->p, v->stride, (int)first);
+    return launch_in_pieces(slots, kThreads, [&](long long first, unsigned n) {
+        hipLaunchKernelGGL((append_kernel<kThreads, Pos>), dim3(n, (unsigned)c.h_kv, parts), dim3(kThreads), lds, s, c, a, k->p, k->stride,
+                           v->p, v->stride, (int)first, turn);
     });
 }
 
@@ -334,7 +403,26 @@ hipError_t ix_kv8_append(const ix_kv8* cache, int n_seq, int total_T, const int3
     if (total_T == 0) return hipSuccess;                      // of tensors without elements, whose addresses may be 0
     if (!rows_ok(k, (long long)c.h_kv * c.d) || !rows_ok(v, (long long)c.h_kv * c.d)) return hipErrorInvalidValue;
     const int few = a.T < (long long)c.page * a.n_seq ? 2 : 1;
-    return with_threads(c.page * c.d / 32 / few, [&](auto n) { return launch_append<n>(c, a, k, v, s); });
+    return with_threads(c.page * c.d / 32 / few, [&](auto n) { return launch_append<n>(c, a, k, v, Plain{}, s); });
+}
+
+hipError_t ix_kv8_append_rope(const ix_kv8* cache, int n_seq, int total_T, const int32_t* cu_seqlens, const int32_t* kv_len,
+                              const int32_t* table, int width, const ix_rows* k, const ix_rows* v, const ix_rope* rope_k,
+                              const ix_rows* q, int h_q, const ix_rope* rope_q, uint16_t* q_out, hipStream_t s) {
+    using namespace ixg;
+    Kv8 c;
+    Batch a;
+    Turned turn{};
+    Rope rope;
+    if (!make_kv8(cache, &c) || !make_batch(n_seq, total_T, cu_seqlens, kv_len, table, width, &a)) return hipErrorInvalidValue;
+    if (!make_rope(rope_k, c.d, &turn.k)) return hipErrorInvalidValue;
+    if (q && (h_q <= 0 || h_q > 65536 || !make_rope(rope_q, c.d, &rope))) return hipErrorInvalidValue;
+    if (total_T == 0) return hipSuccess;                      // of tensors without elements, whose addresses may be 0
+    if (!rows_ok(k, (long long)c.h_kv * c.d) || !rows_ok(v, (long long)c.h_kv * c.d)) return hipErrorInvalidValue;
+    if (q && !make_rope_rows(rope_q, q, h_q, c.d, q_out, &turn.q)) return hipErrorInvalidValue;
+    turn.table = std::max(turn.k.half << (6 - turn.k.per_log), q ? turn.q.r.half : 0);
+    const int few = a.T < (long long)c.page * a.n_seq ? 2 : 1;
+    return with_threads(c.page * c.d / 32 / few, [&](auto n) { return launch_append<n>(c, a, k, v, turn, s); });
 }
 
 hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_t* cu_seqlens, const int32_t* kv_len,

@@ -412,6 +412,37 @@ hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_
  * initialisation; calls that share it must be ordered. */
 size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, int max_q, int h_q);
 
+/* Rotary positions of a head's row of d channels, and the RMS norm that may come before them (read on the host at call
+ * time, the arrays are on the device): with f = x, or x / sqrt(mean(x^2) + eps) * (norm_offset + norm), each pair (a, b) of
+ * the first `rot` channels is turned by its angle, the token's position times freq[i],
+ *   y_a = amplitude * (f_a cos - f_b sin),  y_b = amplitude * (f_b cos + f_a sin)
+ * and the channels behind them are f. Pair i is (i, i + rot / 2) in IX_ROPE_HALVES, (2 i, 2 i + 1) in IX_ROPE_PAIRS. However
+ * positions are scaled for long contexts is in freq and amplitude; angles are exact to 2^-22 at any position. */
+enum { IX_ROPE_HALVES = 0, IX_ROPE_PAIRS = 1 };
+typedef struct ix_rope {
+    int rot;                  /* even, 0 (none) .. d */
+    int layout;
+    const float* freq;        /* [rot/2] radians a position; may be NULL where rot is 0 */
+    float amplitude;          /* 1, or what a model's scaling asks for */
+    const float* norm;        /* [d], or NULL: no norm */
+    float norm_offset, eps;   /* norm_offset is 1 where a model stores its weights around zero */
+} ix_rope;
+
+/* Rows of heads turned by their tokens' positions, which are those of the batch (kv_len - q .. kv_len - 1 for a sequence's
+ * q new tokens): y [total_T][heads][d] bf16 (RNE; all in fp32 before it), x rows of [heads][d]. y may be the memory of x
+ * where that is packed. Rows of no sequence are neither read nor written. Requires d % 8 == 0, d <= 512, 1 <= heads <= 65536. */
+hipError_t ix_rope_rows(const ix_rope* rope, int n_seq, int total_T, const int32_t* cu_seqlens, const int32_t* kv_len,
+                        const ix_rows* x, int heads, int d, uint16_t* y, hipStream_t s IX_GDN_DEFAULT_STREAM);
+
+/* ix_kv8_append with keys that are turned on the way, and the batch's queries turned beside them, in one launch. The codes
+ * and scales are those of ix_kv8_append on the rows that ix_rope_rows would make of k (bf16), bit for bit; q_out
+ * [total_T][h_q][d] is what it makes of q (rows of [h_q][d]) with rope_q. q may be NULL: then h_q, rope_q and q_out have no
+ * meaning. q_out may be the memory of q where that is packed, but not of k or v. */
+hipError_t ix_kv8_append_rope(const ix_kv8* cache, int n_seq, int total_T, const int32_t* cu_seqlens, const int32_t* kv_len,
+                              const int32_t* table, int width, const ix_rows* k, const ix_rows* v, const ix_rope* rope_k,
+                              const ix_rows* q, int h_q, const ix_rope* rope_q, uint16_t* q_out,
+                              hipStream_t s IX_GDN_DEFAULT_STREAM);
+
 /* Attention of the batch's tokens over the cache, which holds them already (ix_kv8_append):
  *   o_r = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q_r . k_j)
  * for every row r = (token at position pos, query head h), over kv head h / (h_q / h_kv) and the
