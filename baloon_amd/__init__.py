@@ -42,7 +42,7 @@ EXPORTS = (
     "ix_bf16_gemv", "ix_bf16_gemv_pair", "ix_bf16_gemv_split", "ix_mmvq_q8_0", "ix_gdn_in_proj_width", "ix_gdn_in_proj",
     "ix_gdn_version", "ix_gdn_decode_noalloc", "ix_q8_1_quantize", "ix_gdn_commit_window_layers",
     "ix_add_rms_norm", "ix_kv8_append", "ix_kv8_read", "ix_kv8_attn_workspace_size", "ix_kv8_attn",
-    "ix_rope_rows", "ix_kv8_append_rope",
+    "ix_rope_rows", "ix_kv8_append_rope", "ix_kv8_attn_shared_workspace_size", "ix_kv8_attn_shared",
 )
 
 
@@ -147,6 +147,8 @@ _SIGNATURES = {
     "ix_kv8_attn": ("kiiipppirifiirppzs", _I),
     "ix_rope_rows": ("tiippriips", _I),
     "ix_kv8_append_rope": ("kiipppirrtritps", _I),
+    "ix_kv8_attn_shared_workspace_size": ("kiiiii", _Z),
+    "ix_kv8_attn_shared": ("kiiipppiipprifrppzs", _I),
 }
 
 _lib = None
@@ -570,6 +572,19 @@ def ix_kv8_attn(cache: Kv8, n_seq, total_T, max_q, cu_seqlens, kv_len, table, wi
     sees that many positions and the first `sinks`. workspace: ix_kv8_attn_workspace_size(...) bytes."""
     return _bind.ix_kv8_attn(cache, n_seq, total_T, max_q, cu_seqlens, kv_len, table, width, q, h_q, scale, window, sinks,
                              gate, o, workspace, workspace_bytes, s)
+
+
+def ix_kv8_attn_shared_workspace_size(cache: Kv8, n_seq: int, total_T: int, max_q: int, n_groups: int, h_q: int) -> int:
+    return lib().ix_kv8_attn_shared_workspace_size(ctypes.byref(cache), n_seq, total_T, max_q, n_groups, h_q)
+
+
+def ix_kv8_attn_shared(cache: Kv8, n_seq, total_T, max_q, cu_seqlens, kv_len, table, width, n_groups, groups, shared_len, q, h_q, scale,
+                       gate=None, o=None, workspace=None, workspace_bytes=0, s=None) -> int:
+    """ix_kv8_attn of a batch in which sequences groups[g] .. groups[g + 1] - 1 (groups [n_groups + 1] int32) have their first
+    shared_len[g] tokens (int32) in common, none of them new: they are read once for the group, from the pages of its first
+    sequence. workspace: ix_kv8_attn_shared_workspace_size(...) bytes."""
+    return _bind.ix_kv8_attn_shared(cache, n_seq, total_T, max_q, cu_seqlens, kv_len, table, width, n_groups, groups, shared_len, q, h_q,
+                                    scale, gate, o, workspace, workspace_bytes, s)
 
 
 def version() -> str:

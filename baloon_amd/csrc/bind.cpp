@@ -218,7 +218,7 @@ PyObject* call(hipError_t (*fn)(A...), const char* name, PyObject* const* args, 
     X(ix_gdn_decode_window) X(ix_gdn_decode_window_mfma) X(ix_gdn_commit_window) X(ix_bf16_gemv)                 \
     X(ix_bf16_gemv_pair) X(ix_bf16_gemv_split) X(ix_mmvq_q8_0) X(ix_q8_1_quantize) X(ix_gdn_in_proj)             \
     X(ix_add_rms_norm) X(ix_kv8_append) X(ix_kv8_read) X(ix_kv8_attn)                                       \
-    X(ix_rope_rows) X(ix_kv8_append_rope)
+    X(ix_rope_rows) X(ix_kv8_append_rope) X(ix_kv8_attn_shared)
 
 #define X(name)                                                                        \
     decltype(&::name) p_##name = nullptr;                                              \

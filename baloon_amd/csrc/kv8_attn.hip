@@ -36,6 +36,44 @@ struct AttnArgs {
     float* block_part;        // partial results of its blocks, see BlockParts
     int slots, items;         // workgroups of it that the chip holds, and parts of blocks at most
     int first, blocks;        // where a launch of it begins, and its workgroups in all launches
+    const int32_t *groups, *shared;      // sequences groups[g] .. groups[g + 1] - 1 have their first shared[g] tokens in common
+    int n_groups;
+    float *row_o, *row_ml;    // of kShared's rows: sums [T][h_q][d], and (m, lse) [T][h_q][2], as Joined takes them
+};
+
+// Which tokens a launch is about. kAll is attention as it is. Where the sequences of a group have their first tokens in common it
+// is two: kShared takes the rows of a group as those of one sequence, which see all of the shared tokens, and leaves a partial
+// result for each row; kOwn takes each sequence's tokens behind them, and adds that.
+enum Tokens { kAll, kShared, kOwn };
+// What stands for the batch: its sequences, or for kShared its groups.
+template <Tokens P>
+struct Seqs {
+    static __device__ __forceinline__ int n(const AttnArgs& A) { return P == kShared ? A.n_groups : A.a.n_seq; }
+    static __device__ __forceinline__ int first_of(const AttnArgs& A, int g) { return min(max(A.groups[g], 0), A.a.n_seq); }
+    static __device__ __forceinline__ int start(const AttnArgs& A, int b) { return A.a.start(P == kShared ? first_of(A, b) : b); }
+    static __device__ __forceinline__ int kv(const AttnArgs& A, int b) {
+        if constexpr (P == kShared) return (int)min((long long)max(A.shared[b], 0), (long long)A.a.width << A.c.page_log);
+        return max(A.a.kv_len[b], 0);
+    }
+    // New tokens; of a group that shares nothing none, kOwn does all for it.
+    static __device__ __forceinline__ int rows(const AttnArgs& A, int b, int s0, int kv) {
+        return P == kShared && kv == 0 ? 0 : max(start(A, b + 1) - s0, 0);
+    }
+    static __device__ __forceinline__ const int32_t* table(const AttnArgs& A, int b) {
+        return A.a.table + (size_t)(P == kShared ? first_of(A, b) : b) * A.a.width;
+    }
+    // The first token that kOwn takes.
+    static __device__ __forceinline__ int from(const AttnArgs& A, int b) {
+        if constexpr (P != kOwn) return 0;
+        int lo = 0, n = A.n_groups;                           // the last group that begins at b or before
+        while (n > 1) {
+            const int half = n / 2;
+            const bool right = A.groups[lo + half] <= b;
+            lo += right ? half : 0;
+            n = right ? n - half : half;
+        }
+        return b >= A.groups[lo] && b < A.groups[lo + 1] ? max(A.shared[lo], 0) : 0;
+    }
 };
 
 // The kernel's argument (its only one) read from memory again where it is used next: keeping all of it in
@@ -150,26 +188,28 @@ __device__ __forceinline__ void split_q(uint4& a, uint4& b, float inv) {
 struct Span {
     int s0, q, kv, first;     // rows s0 .. s0 + q - 1, at positions first ..
     int ns, lo, nt, nrb;      // nt tiles in all (1 where nothing is seen: zeros are written), nrb blocks of rows
+    int from;                 // the first token of all (kOwn)
     __device__ __forceinline__ int tile(int t) const { return t < ns ? t : lo + t - ns; }
 };
-template <int ROWS, int TOK>
-__device__ __forceinline__ Span span_of(const AttnArgs& A, int s0, int q, int kv) {
+template <int ROWS, int TOK, Tokens P>
+__device__ __forceinline__ Span span_of(const AttnArgs& A, int s0, int q, int kv, int from) {
     Span s;
+    s.from = from;
     s.s0 = s0;
     s.q = (long long)q * A.G <= A.small ? q : 0;
     s.kv = kv;
     s.first = s.kv - q;
-    s.lo = A.window > 0 ? max(s.first - A.window + 1, 0) / TOK : 0;
-    s.ns = A.window > 0 ? min(A.sinks / TOK + (A.sinks % TOK != 0), s.lo) : 0;
+    s.lo = P == kOwn ? from / TOK : P == kAll && A.window > 0 ? max(s.first - A.window + 1, 0) / TOK : 0;
+    s.ns = P == kAll && A.window > 0 ? min(A.sinks / TOK + (A.sinks % TOK != 0), s.lo) : 0;
     const int held = (int)min((long long)kv, (long long)A.a.width << A.c.page_log);      // what the table has places for
     s.nt = max(s.ns + max(held / TOK + (held % TOK != 0) - s.lo, 0), 1);
     s.nrb = (int)(((long long)s.q * A.G + ROWS - 1) / ROWS);
     return s;
 }
-template <int ROWS, int TOK>
+template <int ROWS, int TOK, Tokens P>
 __device__ __forceinline__ Span span_at(const AttnArgs& A, int b) {
-    const int s0 = A.a.start(b);
-    return span_of<ROWS, TOK>(A, s0, max(A.a.start(b + 1) - s0, 0), max(A.a.kv_len[b], 0));
+    const int s0 = Seqs<P>::start(A, b), kv = Seqs<P>::kv(A, b);
+    return span_of<ROWS, TOK, P>(A, s0, Seqs<P>::rows(A, b, s0, kv), kv, Seqs<P>::from(A, b));
 }
 
 // Inclusive sum over lanes 0 .. l (the steps of wave_scan), and a lane's value in all, for 32 and 64 bits.
@@ -223,13 +263,13 @@ struct Share {
     int b, e, rb, v0;                 // where it begins: count v0 of a segment
     Span s;
 };
-template <int ROWS, int TOK, class Int>
+template <int ROWS, int TOK, Tokens P, class Int>
 __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int lane, Share* out) {
-    const int n = A.a.n_seq, h_kv = A.c.h_kv;
+    const int n = Seqs<P>::n(A), h_kv = A.c.h_kv;
     Span s{};
     const auto span = [&](int b0) {                          // of sequence b0 + lane; no rows behind the last
         s.nrb = 0;
-        if (b0 + lane < n) s = span_at<ROWS, TOK>(A, b0 + lane);
+        if (b0 + lane < n) s = span_at<ROWS, TOK, P>(A, b0 + lane);
     };
     Int tiles = 0, segments = 0;
 #pragma unroll 4
@@ -259,7 +299,7 @@ __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int
             const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
             const Int rel = cur - carry - lane_of((Int)(incl - v), l);
             out->b = b0 + l;
-            out->s = span_of<ROWS, TOK>(A, lane_of(s.s0, l), lane_of(s.q, l), lane_of(s.kv, l));
+            out->s = span_of<ROWS, TOK, P>(A, lane_of(s.s0, l), lane_of(s.q, l), lane_of(s.kv, l), P == kOwn ? lane_of(s.from, l) : 0);
             const int seg = __builtin_amdgcn_readfirstlane((int)quotient(rel, out->s.nt + start));
             out->v0 = __builtin_amdgcn_readfirstlane((int)(rel - (Int)seg * (out->s.nt + start)));
             out->e = quotient(seg, out->s.nrb);
@@ -269,9 +309,9 @@ __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int
         carry += lane_of(incl, kWave - 1);
     }
 }
-template <int ROWS, int TOK>
+template <int ROWS, int TOK, Tokens P>
 __device__ __forceinline__ bool share_of(const AttnArgs& A, int n_wg, int w, int lane, Share* out) {
-    return A.narrow ? share_in<ROWS, TOK, int>(A, n_wg, w, lane, out) : share_in<ROWS, TOK, long long>(A, n_wg, w, lane, out);
+    return A.narrow ? share_in<ROWS, TOK, P, int>(A, n_wg, w, lane, out) : share_in<ROWS, TOK, P, long long>(A, n_wg, w, lane, out);
 }
 
 // Partial results: workgroup w leaves that of the segment it starts in the middle of (or cuts at both
@@ -280,7 +320,7 @@ __device__ __forceinline__ bool share_of(const AttnArgs& A, int n_wg, int w, int
 struct Cut {
     int first, last, slot;            // workgroups first .. last; slot of the first (2 w for the others)
     int row, e, r0, rows;             // its sequence's first row, kv head, first row of the block, rows of the sequence
-    int any;
+    int any;                          // 0: there is none; 2: of a sequence with shared tokens (kOwn)
 };
 template <int ROWS, int D>
 struct Parts {
@@ -363,6 +403,28 @@ __device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d
     store_out(A, t, h, d, v, load_gate(A, t, h, d));
 }
 
+// What kShared has left for 4 channels of a row.
+struct RowPart {
+    float m, lse;
+    v4f o;
+};
+__device__ __forceinline__ RowPart row_part(const AttnArgs& A, int t, int h, int d) {
+    const size_t row = (size_t)t * A.h_q + h;
+    return RowPart{A.row_ml[2 * row], A.row_ml[2 * row + 1], *reinterpret_cast<const v4f*>(A.row_o + row * A.c.d + d)};
+}
+// 4 channels of a row whose parts are all in `sum`, but what kShared has left (`more`: there is such).
+template <Tokens P>
+__device__ __forceinline__ void finish(const AttnArgs& A, int t, int h, int d, Joined& sum, bool more, const RowPart& part) {
+    if constexpr (P == kShared) {
+        const size_t row = (size_t)t * A.h_q + h;
+        *reinterpret_cast<v4f*>(A.row_o + row * A.c.d + d) = sum.o;
+        if (d == 0) *reinterpret_cast<float2*>(A.row_ml + 2 * row) = make_float2(sum.m, sum.log2_sum());
+    } else {
+        if (P == kOwn && more) sum.more(part.m, part.lse, part.o);
+        store_out(A, t, h, d, outputs(sum.o, sum.log2_sum()));
+    }
+}
+
 constexpr int kSplitThreads = 256, kSplitWaves = kSplitThreads / kWave, kSplitRows = 16;
 // Tokens a wave takes at a time. Keys, values and sums of a 64-token tile are 3/4 D registers, which
 // leaves none at D = 256. Tiles of 32 at D = 128 are faster for some short sequences (48 windows of 1,028 tokens over 4 heads
@@ -386,7 +448,7 @@ constexpr int kSplitTok = D == 256 ? 32 : 64;
 // reach, 64 over 1 to 8,192, 16 heads over 2 of 256, 252 MB in 54 and join_kernel's 6. Short contexts are bound by the way to
 // the first tile (lengths, pages, codes: about 5 us with the launch), by whole tiles for each of four waves, and by the
 // second launch: 48 windows of 1,028 tokens over 4 heads of 128, 51 MB, take 21.0 us where reading takes 8.2.
-template <int D>
+template <int D, Tokens P>
 __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     constexpr int kC = D / 64, kM = D / 16, kPitch = D + 4, kTok = kSplitTok<D>, kS = kTok / 16;
     typedef typename std::conditional<kS == 4, uint4, uint2>::type Codes;     // 4 S values of a channel
@@ -402,7 +464,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     {
         const AttnArgs& Z = args_again();
         Share sh;
-        if (!share_of<kSplitRows, kTok>(Z, gridDim.x, blockIdx.x, lane, &sh)) {
+        if (!share_of<kSplitRows, kTok, P>(Z, gridDim.x, blockIdx.x, lane, &sh)) {
             if (tid == 0) Parts<kSplitRows, D>(Z.part, gridDim.x).cut[blockIdx.x].any = 0;
             return;
         }
@@ -415,6 +477,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     LaneSum sum;
     // What is left to do for the piece whose sums these are, in vector registers: the main loop needs the scalar ones.
     int o_e = 0, o_r0 = 0, o_rows = 0, o_s0 = 0, o_slot = 0;        // o_slot -1: the whole segment
+    [[maybe_unused]] int o_more = 0;                          // shared tokens come before it (kOwn)
     bool open = false;
     int pieces = 0;
     Cut cut{};
@@ -433,7 +496,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         // A tile's places in the cache: this lane's values, scores and scales are of its tokens `mine` on, its
         // keys of those from `keys` on (both within 16 tokens of a page). A lost page's memory is page 0's,
         // hidden below.
-        const int32_t* tab = Y.a.table + (size_t)b * Y.a.width;
+        const int32_t* tab = Seqs<P>::table(Y, b);
         const int kv = (int)min((long long)s.kv, (long long)Y.a.width << page_log), n_pages = Y.c.n_pages, h_kv = Y.c.h_kv;
         const int8_t *kb = Y.c.k + ((size_t)e << page_log) * D, *vb = Y.c.v + ((size_t)e << page_log) * D;
         const float *ksb = Y.c.k_scale + e, *vsb = Y.c.v_scale + e;
@@ -496,6 +559,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             for (int i = tid; i < kSplitRows * D / 4; i += kSplitThreads) {
                 const int row = i / (D / 4), d = i % (D / 4) * 4;
                 if (x_r0 + row >= x_rows) break;
+                const int token = (x_r0 + row) / Z.G, x_t = taken(o_s0) + token, x_h = taken(o_e) * Z.G + x_r0 + row - token * Z.G;
+                RowPart before{};
+                const bool more = P == kOwn && x_slot < 0 && taken(o_more);
+                if (more) before = row_part(Z, x_t, x_h, d);
                 Joined to;
 #pragma unroll
                 for (int k = 0; k < kSplitWaves; ++k) to.meet_m(lo_ml[(k * kSplitRows + row) * 2]);
@@ -506,8 +573,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
                     to.add(lo_ml[(k * kSplitRows + row) * 2], lo_ml[(k * kSplitRows + row) * 2 + 1],
                            *reinterpret_cast<const v4f*>(lo_o + (k * kSplitRows + row) * kPitch + d));
                 if (x_slot < 0) {
-                    const int token = (x_r0 + row) / Z.G;
-                    store_out(Z, taken(o_s0) + token, taken(o_e) * Z.G + x_r0 + row - token * Z.G, d, outputs(to.o, to.log2_sum()));
+                    finish<P>(Z, x_t, x_h, d, to, more, before);
                 } else {
                     *reinterpret_cast<v4f*>(parts.o + ((size_t)x_slot * kSplitRows + row) * D + d) = to.o;
                     if (d == 0) {
@@ -540,11 +606,11 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             lo_q[(2 * w) * kWave + lane] = raw[0];
             lo_q[(2 * w + 1) * kWave + lane] = raw[1];
         }
-        const int pos = r0 + n < rows ? s.first + (r0 + n) / Y.G : -1;
-        const int from = window > 0 ? pos - window + 1 : 0;   // the row sees from .. pos, and the sinks
+        const int pos = r0 + n >= rows ? -1 : P == kShared ? s.kv - 1 : s.first + (r0 + n) / Y.G;
+        const int from = P == kOwn ? s.from : P == kAll && window > 0 ? pos - window + 1 : 0;       // the row sees from .. pos, and the sinks
         // tiles that every row sees as a whole: those starting at full_lo .. full_hi
-        const int full_hi = s.first + r0 / Y.G - kTok + 1;
-        const int full_lo = window > 0 ? s.first + (min(r0 + kSplitRows, rows) - 1) / Y.G - window + 1 : 0;
+        const int full_hi = (P == kShared ? s.kv - 1 : s.first + r0 / Y.G) - kTok + 1;
+        const int full_lo = P == kOwn ? s.from : P == kAll && window > 0 ? s.first + (min(r0 + kSplitRows, rows) - 1) / Y.G - window + 1 : 0;
         lds_barrier();
 #pragma unroll
         for (int m = 0; m < kM; ++m) acc[m] = v4f{0, 0, 0, 0};
@@ -552,6 +618,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
 
         // Where its parts go, and whether it is cut at its end.
         o_e = parked(e), o_r0 = parked(r0), o_rows = parked(rows), o_s0 = parked(s.s0);
+        if constexpr (P == kOwn) o_more = parked(s.from > 0);
         o_slot = parked(t0 == 0 && t1 == s.nt ? -1 : 2 * (int)blockIdx.x + (pieces > 0));
         open = true;
         ++pieces;
@@ -559,7 +626,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             const int x = blockIdx.x, per = taken(w_per), before = v0 > start ? (v0 - start + per - 1) / per : 0;
             // the first part is its workgroup's only one so far where the segment began at or before the share
             cut = Cut{x - before, x + (s.nt + start - (t1 + start) + per - 1) / per, before ? 2 * (x - before) + (v0 < before * per) : o_slot,
-                      s.s0, e, r0, rows, 1};
+                      s.s0, e, r0, rows, P == kOwn && s.from > 0 ? 2 : 1};
         }
         const int n_left = parked(left - (s.nt + start - v0)), n_rb = parked(rb), n_b = parked(b), n_nrb = parked(s.nrb), n_start = parked(start);
 
@@ -648,7 +715,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             rb = 0;
             if (++e == Z.c.h_kv) {
                 e = 0;
-                do s = span_at<kSplitRows, kTok>(Z, ++b);     // left > 0: a sequence with rows follows
+                do s = span_at<kSplitRows, kTok, P>(Z, ++b);     // left > 0: a sequence with rows follows
                 while (s.nrb == 0);
             }
         }
@@ -660,9 +727,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
 // Where the outputs are fewer than the threads, several threads take every so many partial results of one and are
 // joined in LDS. The order of the sums is fixed.
 constexpr int kJoinThreads = 256;
-template <int D, class At>
+template <int D, Tokens P, class At>
 __device__ __forceinline__ void join_outputs(const AttnArgs& A, const float* po, const float* ml, int k0, int k1, At at_part, int from,
-                                             int to, int s0, int e, int r0) {
+                                             int to, int s0, int e, int r0, bool more) {
     __shared__ v4f lo_o[kJoinThreads];
     __shared__ float lo_m[kJoinThreads], lo_l[kJoinThreads];
     int wide = 1;                                             // outputs at a time
@@ -671,6 +738,9 @@ __device__ __forceinline__ void join_outputs(const AttnArgs& A, const float* po,
     for (int x0 = from; x0 < to; x0 += wide) {
         const int x = min(x0 + (int)(threadIdx.x & (wide - 1)), to - 1), row = x / (D / 4), d = x % (D / 4) * 4;
         Joined sum;
+        const int token = (r0 + row) / A.G, t = s0 + token, h = e * A.G + r0 + row - token * A.G;
+        RowPart before{};
+        if (P == kOwn && more && way == 0) before = row_part(A, t, h, d);
 #pragma unroll 4
         for (int k = k0 + way; k <= k1; k += ways) {
             const size_t at = at_part(k) + row;
@@ -685,16 +755,13 @@ __device__ __forceinline__ void join_outputs(const AttnArgs& A, const float* po,
             if (way < half) sum.more(lo_m[other], lo_l[other], lo_o[other]);
             __syncthreads();
         }
-        if (way == 0 && x0 + (int)threadIdx.x < to) {
-            const int token = (r0 + row) / A.G;
-            store_out(A, s0 + token, e * A.G + r0 + row - token * A.G, d, outputs(sum.o, sum.log2_sum()));
-        }
+        if (way == 0 && x0 + (int)threadIdx.x < to) finish<P>(A, t, h, d, sum, more, before);
     }
 }
 
 // Segments that several workgroups share. One that lies across n ends of shares has n workgroups here,
 // which take even parts of its outputs.
-template <int D>
+template <int D, Tokens P>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg) {
     const Parts<kSplitRows, D> parts(A.part, n_wg);
     const Cut c = parts.cut[blockIdx.x];
@@ -703,7 +770,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg
     const int all = min(kSplitRows, c.rows - c.r0) * (D / 4);
     const int from = (int)((long long)all * i / n), to = (int)((long long)all * (i + 1) / n);
     const auto at = [&](int k) { return (size_t)(k == c.first ? c.slot : 2 * k) * kSplitRows; };
-    join_outputs<D>(A, parts.o, parts.ml, c.first, c.last, at, from, to, c.row, c.e, c.r0);
+    join_outputs<D, P>(A, parts.o, parts.ml, c.first, c.last, at, from, to, c.row, c.e, c.r0, c.any == 2);
 }
 
 // Blocks of rows: prompts.
@@ -753,7 +820,7 @@ __device__ __forceinline__ void each(F f) {
 // behind 16,384, 128 blocks, took 356 us whole and take 170.
 struct BlockCut {
     int first, parts, step;                                   // partial results first, first + step ..
-    int s0, e, r0, rows, unused;                              // as in Cut
+    int s0, e, r0, rows, more;                                // as in Cut; more: of a sequence with shared tokens
 };
 template <int D>
 struct BlockParts {
@@ -780,9 +847,10 @@ __device__ __forceinline__ int wave_max_int(int v) {
     return lane_of(dpp_max<0x143, 0xC>(v), kWave - 1);
 }
 // The blocks of a sequence.
+template <Tokens P>
 __device__ __forceinline__ int blocks_of(const AttnArgs& A, int b) {
-    if (b >= A.a.n_seq) return 0;
-    const int rows = max(A.a.start(b + 1) - A.a.start(b), 0) * A.G;
+    if (b >= Seqs<P>::n(A)) return 0;
+    const int rows = Seqs<P>::rows(A, b, Seqs<P>::start(A, b), P == kShared ? Seqs<P>::kv(A, b) : 0) * A.G;
     return rows > A.small ? (rows + kBlockRows - 1) / kBlockRows : 0;
 }
 // The blocks of all sequences and heads, and in how many parts each is taken: lane p - 1 knows the time of p, in tiles,
@@ -793,19 +861,21 @@ struct Blocks {
 template <int D>
 constexpr float kPartCost = D == 256 ? 4.0f : 8.0f;           // tiles in the time of a part's start, its sums and their joining
 constexpr int kLeastPart = 4;         // tiles
-template <int D>
+template <int D, Tokens P>
 __device__ __forceinline__ Blocks all_blocks(const AttnArgs& A, int lane) {
     int sum = 0, kv = 0;
+    const int n_seq = Seqs<P>::n(A);
 #pragma unroll 4
-    for (int b0 = 0; b0 < A.a.n_seq; b0 += kWave) {
-        const int v = blocks_of(A, b0 + lane), held = A.a.kv_len[min(b0 + lane, A.a.n_seq - 1)];
+    for (int b0 = 0; b0 < n_seq; b0 += kWave) {
+        const int at = min(b0 + lane, n_seq - 1), v = blocks_of<P>(A, b0 + lane);
+        const int held = P == kAll ? A.a.kv_len[at] : Seqs<P>::kv(A, at) - Seqs<P>::from(A, at);
         sum += v;
         kv = max(kv, v > 0 ? held : 0);
     }
     Blocks out;
     out.n = lane_of(wave_scan_int(sum), kWave - 1) * A.c.h_kv;
     kv = wave_max_int(kv);
-    if (A.window > 0 && A.window < kv) kv = A.window + min(A.sinks, kv - A.window);
+    if (P == kAll && A.window > 0 && A.window < kv) kv = A.window + min(A.sinks, kv - A.window);
     const int p = lane + 1, rounds = (out.n * p + A.slots - 1) / A.slots;
     float cost = (float)rounds * ((float)kv / (float)(kBlockTok * p) + (p > 1 ? kPartCost<D> : 0.0f));
     if (p > 1 && (long long)out.n * p > A.items) cost = __builtin_inff();
@@ -814,7 +884,7 @@ __device__ __forceinline__ Blocks all_blocks(const AttnArgs& A, int lane) {
     return out;
 }
 
-template <int D, bool kCut>
+template <int D, bool kCut, Tokens P>
 __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(AttnArgs A) {
     constexpr int kC = D / 64, kM = D / 16;
     constexpr int kUnits = kBlockTok * D / 16, kPer = (kUnits + kBlockThreads - 1) / kBlockThreads;
@@ -829,14 +899,14 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     const int block = kCut ? (int)blockIdx.x : A.first + (int)blockIdx.x, e = block % A.c.h_kv;
     int b, rb, parts = 1, part = 0;
     if constexpr (kCut) {
-        const Blocks all = all_blocks<D>(A, lane);
+        const Blocks all = all_blocks<D, P>(A, lane);
         if ((int)blockIdx.x >= all.n * all.parts) return;
         const int i = blockIdx.x / A.c.h_kv;
         parts = all.parts;
         part = i % parts;
         rb = all.n / A.c.h_kv - 1 - i / parts;
         for (int b0 = 0;; b0 += kWave) {
-            const int v = blocks_of(A, b0 + lane), incl = wave_scan_int(v);
+            const int v = blocks_of<P>(A, b0 + lane), incl = wave_scan_int(v);
             const unsigned long long hit = __ballot(incl > rb);
             if (hit) {
                 const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
@@ -848,13 +918,14 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         }
     } else {
         const int j = A.blocks / A.c.h_kv - 1 - block / A.c.h_kv;
-        const auto key = [&](int b) { return (int)((long long)A.a.start(b) * A.G / kBlockRows) + b; };
-        b = wave_search(A.a.n_seq, j, lane, key);
+        const auto key = [&](int b) { return (int)((long long)Seqs<P>::start(A, b) * A.G / kBlockRows) + b; };
+        b = wave_search(Seqs<P>::n(A), j, lane, key);
         rb = j - key(b);
     }
-    const int s0 = A.a.start(b), q = A.a.start(b + 1) - s0, r0 = rb * kBlockRows, rows = max(q, 0) * A.G;
+    const int s0 = Seqs<P>::start(A, b), kv = Seqs<P>::kv(A, b), q = Seqs<P>::rows(A, b, s0, kv), r0 = rb * kBlockRows, rows = q * A.G;
     if (!kCut && (rows <= A.small || rb < 0 || r0 >= rows)) return;      // rb < 0: before the first sequence's rows
-    const int kv = max(A.a.kv_len[b], 0), first = kv - q;
+    const int first = kv - q, from = Seqs<P>::from(A, b);
+    const auto place = [&](int qi) { return P == kShared ? kv - 1 : first + qi; };       // of the sequence's new token qi
 
     // q of row n of the wave, channels 64 c + 16 g .. + 15
     const int w0 = r0 + 16 * w;
@@ -863,7 +934,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     float qc;
     {
         const int r = w0 + n, rc = min(r, rows - 1), qi = rc / A.G;
-        pos = r < rows ? first + qi : -1;
+        pos = r < rows ? place(qi) : -1;
         const uint16_t* qp = A.q + (long long)(s0 + qi) * A.q_stride + (size_t)(e * A.G + rc - qi * A.G) * D + 16 * g;
         u16x2 mb = {0, 0};
 #pragma unroll
@@ -882,22 +953,23 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     }
     // Of the wave's positions wave_first .. wave_last: tiles that start from full_lo to full_hi every row sees as a
     // whole, those below some_lo (the sinks aside) and above wave_last none does.
-    const int wave_first = first + min(w0, rows - 1) / A.G, wave_last = first + (min(w0 + 16, rows) - 1) / A.G;
-    const int full_hi = wave_first - kBlockTok + 1, full_lo = A.window > 0 ? wave_last - A.window + 1 : 0;
-    const int some_lo = A.window > 0 ? wave_first - A.window + 1 - kBlockTok + 1 : 0;
+    const bool window = P == kAll && A.window > 0;
+    const int wave_first = place(min(w0, rows - 1) / A.G), wave_last = place((min(w0 + 16, rows) - 1) / A.G);
+    const int full_hi = wave_first - kBlockTok + 1, full_lo = P == kOwn ? from : window ? wave_last - A.window + 1 : 0;
+    const int some_lo = window ? wave_first - A.window + 1 - kBlockTok + 1 : 0;
 
     // the block's tiles
-    const int block_first = first + r0 / A.G, block_last = first + (min(r0 + kBlockRows, rows) - 1) / A.G;
-    const int lo = A.window > 0 ? max(block_first - A.window + 1, 0) / kBlockTok : 0;
-    const int ns = A.window > 0 ? min(A.sinks / kBlockTok + (A.sinks % kBlockTok != 0), lo) : 0;
-    const int all = block_last < 0 ? 0 : ns + block_last / kBlockTok + 1 - lo;
+    const int block_first = place(r0 / A.G), block_last = place((min(r0 + kBlockRows, rows) - 1) / A.G);
+    const int lo = P == kOwn ? from / kBlockTok : window ? max(block_first - A.window + 1, 0) / kBlockTok : 0;
+    const int ns = window ? min(A.sinks / kBlockTok + (A.sinks % kBlockTok != 0), lo) : 0;
+    const int all = block_last < 0 ? 0 : max(ns + block_last / kBlockTok + 1 - lo, 0);
     int begin = 0, nt = all;                                  // this part's: tiles begin .. begin + nt - 1
     if constexpr (kCut) {
         if (parts > 1) {
             const int i = blockIdx.x / A.c.h_kv / parts;
             parts = min(parts, max(all / kLeastPart, 1));
             if (part == 0 && tid == 0)
-                BlockParts<D>(A.block_part, A.slots).cut[i * A.c.h_kv + e] = BlockCut{(int)blockIdx.x, parts, A.c.h_kv, s0, e, r0, rows, 0};
+                BlockParts<D>(A.block_part, A.slots).cut[i * A.c.h_kv + e] = BlockCut{(int)blockIdx.x, parts, A.c.h_kv, s0, e, r0, rows, from > 0};
             if (part >= parts) return;
             begin = all / parts * part + min(part, all % parts);
             nt = all / parts + (part < all % parts);
@@ -909,7 +981,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     // and in a page (or 64 tokens of it) channel by channel. The pieces of one wave's i are in one page.
     const int page_log = A.c.page_log, part_log = min(page_log, 6);
     constexpr int kDLog = D == 64 ? 6 : D == 128 ? 7 : 8;
-    const int32_t* tab = A.a.table + (size_t)b * A.a.width;
+    const int32_t* tab = Seqs<P>::table(A, b);
     const int kv_held = (int)min((long long)kv, (long long)A.a.width << page_log);
     // Lane g of 0 .. 3 holds the page of the tile's tokens 16 g .. + 15, loaded a tile ahead of its use.
     const auto pages = [&](int at) {
@@ -1026,8 +1098,8 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
             }
             if (at < full_lo || at > full_hi) {
                 asm volatile("");                             // a branch: most tiles are seen as a whole
-                const int j0 = at + 16 * g, from = A.window > 0 ? pos - A.window + 1 : 0;
-                const uint32_t seen = low_bits(pos - j0 + 1) & (low_bits(A.sinks - j0) | ~low_bits(from - j0));
+                const int j0 = at + 16 * g, least = P == kOwn ? from : window ? pos - A.window + 1 : 0;
+                const uint32_t seen = low_bits(pos - j0 + 1) & (low_bits(A.sinks - j0) | ~low_bits(least - j0));
 #pragma unroll
                 for (int y = 0; y < 16; ++y) p[y] = (seen >> y) & 1 ? p[y] : -__builtin_inff();
             }
@@ -1083,7 +1155,16 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         }
         return;
     }
-    if (r < rows) {
+    if (P != kAll && r < rows) {
+#pragma unroll
+        for (int m = 0; m < kM; ++m) {
+            RowPart before{};
+            if (P == kOwn && from > 0) before = row_part(A, s0 + qi, head, 16 * m + d0);
+            Joined sum;
+            sum.more(m_ref, lse, acc[m]);
+            finish<P>(A, s0 + qi, head, 16 * m + d0, sum, from > 0, before);
+        }
+    } else if (r < rows) {
         constexpr int kN = kM < 8 ? kM : 8;                   // pieces of 4 channels, their gates on the way together
 #pragma unroll
         for (int m0 = 0; m0 < kM; m0 += kN) {
@@ -1097,9 +1178,9 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
 }
 
 // Every block's outputs are shared out over as many workgroups as there are for each.
-template <int D>
+template <int D, Tokens P>
 __global__ void __launch_bounds__(kJoinThreads) block_join_kernel(AttnArgs A) {
-    const Blocks blocks = all_blocks<D>(A, threadIdx.x & (kWave - 1));
+    const Blocks blocks = all_blocks<D, P>(A, threadIdx.x & (kWave - 1));
     if (blocks.parts == 1) return;
     const int n = (int)gridDim.x / blocks.n, k = blockIdx.x % blocks.n, i = blockIdx.x / blocks.n;
     if (i >= n) return;
@@ -1108,8 +1189,8 @@ __global__ void __launch_bounds__(kJoinThreads) block_join_kernel(AttnArgs A) {
     if (c.parts == 1) return;
     const int all = min(kBlockRows, c.rows - c.r0) * (D / 4);
     const auto at = [&](int k) { return (size_t)(c.first + k * c.step) * kBlockRows; };
-    join_outputs<D>(A, parts.o, parts.ml, 0, c.parts - 1, at, (int)((long long)all * i / n), (int)((long long)all * (i + 1) / n),
-                    c.s0, c.e, c.r0);
+    join_outputs<D, P>(A, parts.o, parts.ml, 0, c.parts - 1, at, (int)((long long)all * i / n), (int)((long long)all * (i + 1) / n),
+                       c.s0, c.e, c.r0, c.more);
 }
 
 // Sequences of at most kSplitMost (token, head) rows a kv head are split_kernel's in any case, and so are all where the
@@ -1147,51 +1228,77 @@ template <int D>
 size_t attn_bytes(const Plan& p) { return split_bytes<D>(p) + (p.block ? BlockParts<D>::bytes(p.slots) : 0); }
 size_t attn_bytes(int d, const Plan& p) { return d == 64 ? attn_bytes<64>(p) : d == 128 ? attn_bytes<128>(p) : attn_bytes<256>(p); }
 
-template <int D, bool kCut>
+template <int D, bool kCut, Tokens P>
 hipError_t launch_blocks(AttnArgs& A, long long n, hipStream_t s) {
     static OncePerDevice once;
-    const hipError_t ready = allow_lds(once, &block_kernel<D, kCut>, BlockLds<D>::kBytes, s);
+    const hipError_t ready = allow_lds(once, &block_kernel<D, kCut, P>, BlockLds<D>::kBytes, s);
     if (ready != hipSuccess) return ready;
     A.blocks = (int)n;
     return launch_in_pieces(n, kBlockThreads, [&](long long first, unsigned count) {      // one, of blocks in parts
         A.first = (int)first;
-        hipLaunchKernelGGL((block_kernel<D, kCut>), dim3(count), dim3(kBlockThreads), BlockLds<D>::kBytes, s, A);
+        hipLaunchKernelGGL((block_kernel<D, kCut, P>), dim3(count), dim3(kBlockThreads), BlockLds<D>::kBytes, s, A);
     });
 }
 
-template <int D>
-hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
-    const int n_wg = p.n_wg;
+template <int D, Tokens P>
+hipError_t launch_tokens(AttnArgs& A, const Plan& p, hipStream_t s) {
+    const int n_wg = p.n_wg, n_seq = P == kShared ? A.n_groups : A.a.n_seq;
     // With at most max_q new tokens in each other one, a sequence of the batch has at least these. Where that is more than
     // kSplitMost rows all are block_kernel's (also those of a batch whose offsets end before T), and it is the only launch.
-    const long long shortest = A.a.T - (long long)(A.a.n_seq - 1) * p.max_q;
+    const long long shortest = A.a.T - (long long)(n_seq - 1) * p.max_q;
     const bool only = p.block && shortest * A.G > kSplitMost;
     A.small = only ? 0 : p.block ? kSplitMost : 0x7fffffff;
     // tiles: at most those of a whole table for each block of rows, and n_wg - 1 and a workgroup's share more in sums
-    const long long row_blocks = (long long)A.a.T * A.G / kSplitRows + A.a.n_seq;
+    const long long row_blocks = (long long)A.a.T * A.G / kSplitRows + n_seq;
     const long long tiles = ((long long)A.a.width << A.c.page_log) / kSplitTok<D> + 1;
     A.narrow = row_blocks < (1ll << 31) / tiles / A.c.h_kv / 2 - n_wg;
     if (p.block) {
         hipError_t e;
         if (p.cut) {
             // a sequence has at most one block that is not full, and more than kSplitMost rows
-            const long long most = only ? A.a.n_seq : std::min((long long)A.a.n_seq, (long long)A.a.T * A.G / kSplitMost);
+            const long long most = only ? n_seq : std::min((long long)n_seq, (long long)A.a.T * A.G / kSplitMost);
             const long long blocks = p.full + most * A.c.h_kv;
             A.slots = p.slots;
             A.items = 2 * p.slots;
             A.block_part = A.part + split_bytes<D>(p) / sizeof(float);
-            e = launch_blocks<D, true>(A, std::max(blocks, (long long)A.items), s);
-            if (e == hipSuccess) hipLaunchKernelGGL((block_join_kernel<D>), dim3((unsigned)(2 * n_wg)), dim3(kJoinThreads), 0, s, A);
+            e = launch_blocks<D, true, P>(A, std::max(blocks, (long long)A.items), s);
+            if (e == hipSuccess) hipLaunchKernelGGL((block_join_kernel<D, P>), dim3((unsigned)(2 * n_wg)), dim3(kJoinThreads), 0, s, A);
         } else {
-            e = launch_blocks<D, false>(A, p.full + (long long)A.a.n_seq * A.c.h_kv, s);
+            e = launch_blocks<D, false, P>(A, p.full + (long long)n_seq * A.c.h_kv, s);
         }
         if (e != hipSuccess) return e;
         if (only) return hipGetLastError();
     }
     const unsigned lds = kSplitWaves * kSplitRows * (D + 4 + 2 + 1) * sizeof(float) + D / 64 * 2 * kWave * sizeof(uint4);
-    hipLaunchKernelGGL((split_kernel<D>), dim3((unsigned)n_wg), dim3(kSplitThreads), lds, s, A);
-    if (n_wg > 1) hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)n_wg - 1), dim3(kJoinThreads), 0, s, A, n_wg);
+    hipLaunchKernelGGL((split_kernel<D, P>), dim3((unsigned)n_wg), dim3(kSplitThreads), lds, s, A);
+    if (n_wg > 1) hipLaunchKernelGGL((join_kernel<D, P>), dim3((unsigned)n_wg - 1), dim3(kJoinThreads), 0, s, A, n_wg);
     return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) { return launch_tokens<D, kAll>(A, p, s); }
+
+// Attention behind shared tokens. The workspace holds what either launch needs for itself, and the rows of kShared. Those of a
+// group are at most all of the batch's.
+struct SharedPlan {
+    Plan shared, own;
+    size_t scratch, rows, bytes;
+};
+SharedPlan shared_plan_of(int d, int h_kv, int G, int T, int max_q, hipStream_t s) {
+    SharedPlan p;
+    p.shared = plan_of(d, h_kv, G, T, T, s);
+    p.own = plan_of(d, h_kv, G, T, max_q, s);
+    p.scratch = (std::max(attn_bytes(d, p.shared), attn_bytes(d, p.own)) + 255) / 256 * 256;
+    p.rows = (size_t)T * h_kv * G;
+    p.bytes = p.scratch + p.rows * (d + 2) * sizeof(float);
+    return p;
+}
+template <int D>
+hipError_t launch_attn(AttnArgs& A, const SharedPlan& p, hipStream_t s) {
+    A.row_o = A.part + p.scratch / sizeof(float);
+    A.row_ml = A.row_o + p.rows * D;
+    const hipError_t e = launch_tokens<D, kShared>(A, p.shared, s);
+    return e != hipSuccess ? e : launch_tokens<D, kOwn>(A, p.own, s);
 }
 
 // The blocks of the batch are numbered in 31 bits.
@@ -1212,37 +1319,92 @@ size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, i
     return attn_bytes(c.d, plan_of(c.d, c.h_kv, h_q / c.h_kv, total_T, max_q, nullptr));
 }
 
+size_t ix_kv8_attn_shared_workspace_size(const ix_kv8* cache, int n_seq, int total_T, int max_q, int n_groups, int h_q) {
+    using namespace ixg;
+    Kv8 c;
+    if (!make_kv8(cache, &c) || !attn_shape_ok(c, n_seq, total_T, max_q, h_q) || n_groups < 0 || n_groups > 65535) return 0;
+    if (n_groups == 0) return ix_kv8_attn_workspace_size(cache, n_seq, total_T, max_q, h_q);
+    return shared_plan_of(c.d, c.h_kv, h_q / c.h_kv, total_T, max_q, nullptr).bytes;
+}
+
+}  // extern "C"
+
+namespace ixg {
+namespace {
+
+// What both calls check alike.
+bool make_attn(const ix_kv8* cache, int n_seq, int T, int max_q, const int32_t* cu, const int32_t* kv_len, const int32_t* table, int width,
+               int h_q, float scale, AttnArgs* A) {
+    if (!make_kv8(cache, &A->c) || !make_batch(n_seq, T, cu, kv_len, table, width, &A->a)) return false;
+    if (!attn_shape_ok(A->c, n_seq, T, max_q, h_q)) return false;
+    A->scale2 = scale * kLog2e;
+    A->h_q = h_q;
+    A->G = h_q / A->c.h_kv;
+    return true;
+}
+bool make_operands(const ix_rows* q, const ix_rows* gate, uint16_t* o, void* workspace, size_t bytes, size_t need, AttnArgs* A) {
+    const long long row = (long long)A->h_q * A->c.d;
+    if (!rows_ok(q, row) || (gate && !rows_ok(gate, row)) || !o || !ptr_aligned(o, 2)) return false;
+    if (!workspace || !ptr_aligned(workspace, 256) || bytes < need) return false;
+    A->q = q->p;
+    A->q_stride = q->stride;
+    if (gate) {
+        A->gate = gate->p;
+        A->gate_stride = gate->stride;
+    }
+    A->o = o;
+    A->part = static_cast<float*>(workspace);
+    return true;
+}
+template <class P>
+hipError_t launch(AttnArgs& A, const P& p, hipStream_t s) {
+    switch (A.c.d) {
+        case 64: return launch_attn<64>(A, p, s);
+        case 128: return launch_attn<128>(A, p, s);
+        default: return launch_attn<256>(A, p, s);
+    }
+}
+
+}  // namespace
+}  // namespace ixg
+
+extern "C" {
+
 hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens,
                        const int32_t* kv_len, const int32_t* table, int width, const ix_rows* q, int h_q, float scale,
                        int window, int sinks, const ix_rows* gate, uint16_t* o, void* workspace, size_t workspace_bytes,
                        hipStream_t s) {
     using namespace ixg;
     AttnArgs A{};
-    if (!make_kv8(cache, &A.c) || !make_batch(n_seq, total_T, cu_seqlens, kv_len, table, width, &A.a)) return hipErrorInvalidValue;
-    if (!attn_shape_ok(A.c, n_seq, total_T, max_q, h_q) || window < 0 || window > 1 << 30 || sinks < 0) return hipErrorInvalidValue;
+    if (!make_attn(cache, n_seq, total_T, max_q, cu_seqlens, kv_len, table, width, h_q, scale, &A)) return hipErrorInvalidValue;
+    if (window < 0 || window > 1 << 30 || sinks < 0) return hipErrorInvalidValue;
     if (total_T == 0) return hipSuccess;                      // of tensors without elements, whose addresses may be 0
-    if (!rows_ok(q, (long long)h_q * A.c.d) || (gate && !rows_ok(gate, (long long)h_q * A.c.d))) return hipErrorInvalidValue;
-    if (!o || !ptr_aligned(o, 2)) return hipErrorInvalidValue;
-    const Plan p = plan_of(A.c.d, A.c.h_kv, h_q / A.c.h_kv, total_T, max_q, s);
-    if (!workspace || !ptr_aligned(workspace, 256) || workspace_bytes < attn_bytes(A.c.d, p)) return hipErrorInvalidValue;
-    A.q = q->p;
-    A.q_stride = q->stride;
-    if (gate) {
-        A.gate = gate->p;
-        A.gate_stride = gate->stride;
-    }
-    A.o = o;
-    A.part = static_cast<float*>(workspace);
-    A.scale2 = scale * kLog2e;
-    A.h_q = h_q;
-    A.G = h_q / A.c.h_kv;
+    const Plan p = plan_of(A.c.d, A.c.h_kv, A.G, total_T, max_q, s);
+    if (!make_operands(q, gate, o, workspace, workspace_bytes, attn_bytes(A.c.d, p), &A)) return hipErrorInvalidValue;
     A.window = window;
     A.sinks = sinks;
-    switch (A.c.d) {
-        case 64: return launch_attn<64>(A, p, s);
-        case 128: return launch_attn<128>(A, p, s);
-        default: return launch_attn<256>(A, p, s);
-    }
+    return launch(A, p, s);
+}
+
+hipError_t ix_kv8_attn_shared(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens, const int32_t* kv_len,
+                              const int32_t* table, int width, int n_groups, const int32_t* groups, const int32_t* shared_len,
+                              const ix_rows* q, int h_q, float scale, const ix_rows* gate, uint16_t* o, void* workspace,
+                              size_t workspace_bytes, hipStream_t s) {
+    using namespace ixg;
+    if (n_groups == 0)
+        return ix_kv8_attn(cache, n_seq, total_T, max_q, cu_seqlens, kv_len, table, width, q, h_q, scale, 0, 0, gate, o, workspace,
+                           workspace_bytes, s);
+    AttnArgs A{};
+    if (!make_attn(cache, n_seq, total_T, max_q, cu_seqlens, kv_len, table, width, h_q, scale, &A)) return hipErrorInvalidValue;
+    if (n_groups < 0 || n_groups > 65535 || !groups || !shared_len || !ptr_aligned(groups, 4) || !ptr_aligned(shared_len, 4))
+        return hipErrorInvalidValue;
+    if (total_T == 0) return hipSuccess;
+    const SharedPlan p = shared_plan_of(A.c.d, A.c.h_kv, A.G, total_T, max_q, s);
+    if (!make_operands(q, gate, o, workspace, workspace_bytes, p.bytes, &A)) return hipErrorInvalidValue;
+    A.groups = groups;
+    A.shared = shared_len;
+    A.n_groups = n_groups;
+    return launch(A, p, s);
 }
 
 }  // extern "C"
