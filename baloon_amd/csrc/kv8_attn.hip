@@ -3,192 +3,16 @@
 //   o_r = sum_j p_rj v_j / sum_j p_rj,  p_rj = exp(scale q_r . k_j)  over the tokens j that row r sees
 //
 // with k_j = ks c_j and v_j = vs d_j, c and d the codes and ks, vs the scales of the token's page.
-#include <algorithm>
-#include <type_traits>
-
-#include "kv8.h"
+#include "kv8_attn.h"
 
 namespace ixg {
 namespace {
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-constexpr float kLog2e = 0x1.715476p+0f;
-// p is formed relative to a reference m that follows the running maximum only once that is kLag above it, and
-// 2^kLift times itself: between 2^-24 2^-kLift (fp16's smallest subnormal) and 2^(kLift + kLag), so that neither
-// a rescaling per tile nor a loss of small p comes of holding it in fp16.
-constexpr float kLag = 7.0f, kLift = 8.0f;
-
-struct AttnArgs {
-    Kv8 c;
-    Batch a;
-    const uint16_t *q, *gate;
-    long long q_stride, gate_stride;
-    uint16_t* o;
-    float* part;              // partial results, see Parts
-    float scale2;             // scale * log2(e)
-    int h_q, G, window, sinks;
-    int narrow;               // the batch has fewer than 2^31 tiles for split_kernel
-    int small;                // sequences of more (token, head) rows a kv head than this are block_kernel's
-    float* block_part;        // partial results of its blocks, see BlockParts
-    int slots, items;         // workgroups of it that the chip holds, and parts of blocks at most
-    int first, blocks;        // where a launch of it begins, and its workgroups in all launches
-    const int32_t *groups, *shared;      // sequences groups[g] .. groups[g + 1] - 1 have their first shared[g] tokens in common
-    int n_groups;
-    float *row_o, *row_ml;    // of kShared's rows: sums [T][h_q][d], and (m, lse) [T][h_q][2], as Joined takes them
-};
-
-// Which tokens a launch is about. kAll is attention as it is. Where the sequences of a group have their first tokens in common it
-// is two: kShared takes the rows of a group as those of one sequence, which see all of the shared tokens, and leaves a partial
-// result for each row; kOwn takes each sequence's tokens behind them, and adds that.
-enum Tokens { kAll, kShared, kOwn };
-// What stands for the batch: its sequences, or for kShared its groups.
-template <Tokens P>
-struct Seqs {
-    static __device__ __forceinline__ int n(const AttnArgs& A) { return P == kShared ? A.n_groups : A.a.n_seq; }
-    static __device__ __forceinline__ int first_of(const AttnArgs& A, int g) { return min(max(A.groups[g], 0), A.a.n_seq); }
-    static __device__ __forceinline__ int start(const AttnArgs& A, int b) { return A.a.start(P == kShared ? first_of(A, b) : b); }
-    static __device__ __forceinline__ int kv(const AttnArgs& A, int b) {
-        if constexpr (P == kShared) return (int)min((long long)max(A.shared[b], 0), (long long)A.a.width << A.c.page_log);
-        return max(A.a.kv_len[b], 0);
-    }
-    // New tokens; of a group that shares nothing none, kOwn does all for it.
-    static __device__ __forceinline__ int rows(const AttnArgs& A, int b, int s0, int kv) {
-        return P == kShared && kv == 0 ? 0 : max(start(A, b + 1) - s0, 0);
-    }
-    static __device__ __forceinline__ const int32_t* table(const AttnArgs& A, int b) {
-        return A.a.table + (size_t)(P == kShared ? first_of(A, b) : b) * A.a.width;
-    }
-    // The first token that kOwn takes.
-    static __device__ __forceinline__ int from(const AttnArgs& A, int b) {
-        if constexpr (P != kOwn) return 0;
-        int lo = 0, n = A.n_groups;                           // the last group that begins at b or before
-        while (n > 1) {
-            const int half = n / 2;
-            const bool right = A.groups[lo + half] <= b;
-            lo += right ? half : 0;
-            n = right ? n - half : half;
-        }
-        return b >= A.groups[lo] && b < A.groups[lo + 1] ? max(A.shared[lo], 0) : 0;
-    }
-};
-
-// The kernel's argument (its only one) read from memory again where it is used next: keeping all of it in
-// scalar registers over the main loop would spill them.
-__device__ __forceinline__ const AttnArgs& args_again() {
-    auto p = (const __attribute__((address_space(4))) AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(p));
-    return *(const AttnArgs*)p;
-}
-
-// A uniform value that waits in a vector register while the main loop needs the scalar ones.
-__device__ __forceinline__ int parked(int x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
-__device__ __forceinline__ int taken(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
-__device__ __forceinline__ float pair_max16(float v) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float pair_max32(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-// A page's value scale vs weighs its values, not its tokens, so the sum of p has a reference of its own. The values'
-// product takes p' = p vs = 2^(score + log2 vs) relative to the largest of those; the sum takes p = 2^score relative to 2^kFar
-// of a score among the lane's own tokens, so that it can grow by 2^kFar. A lane's tokens of a tile are of one page: p is p' times
-// one factor for all of them. Where that would be above 1 (the page's values next to nothing beside others) p' may be
-// gone from 32 bits, and p is worked out by itself; else what 32 bits lose of p' is under 2^(kFar - 126) of the sum.
-constexpr float kFar = 60.0f;
-// log2 of a page's scale. A page of zeros has none and only takes part in the sum: 2^kNoValue is so far under the least
-// scale, 2^-149, that what the product loses when such a page's p' is its largest is under any bf16 number.
-constexpr float kNoValue = -200.0f;
-__device__ __forceinline__ float log2_scale(float vs) { return vs == 0.0f ? kNoValue : log2f(vs); }
-
-// The sum of a lane's p: l 2^ref.
-struct LaneSum {
-    float l = 0.0f, ref = -__builtin_inff();
-    // What the sum of a tile's p' counts in l. The lane's tokens have p' = 2^(x[] - from) relative to 2^to, the largest of them 2^most
-    // (0 where none is seen); lv is log2 vs. 6 instructions and a power for most tiles.
-    template <int N>
-    __device__ __forceinline__ float factor(const float (&x)[N], float from, float most, float to, float lv) {
-        float a = ref - to + lv;                              // p' is p relative to 2^ref times 2^a
-        float f = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(-a), 0.0f, 1.0f);
-        // more than the least that is rare: a if that is >= 0, else next to everything
-        if (most > fminf(a, a * 0x1p100f)) {
-            asm volatile("");                                 // a branch: taken at a lane's first tokens, then hardly ever
-            if (most > a) {
-                const float was = a;
-                ref = most + kFar - lv + to;
-                a = ref - to + lv;
-                l *= __builtin_amdgcn_exp2f(was - a);
-            }
-            f = a < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-a);
-            if (a < 0.0f) {
-#pragma unroll
-                for (int y = 0; y < N; ++y) l += __builtin_amdgcn_exp2f(x[y] - from - a);
-            }
-        }
-        return f;
-    }
-    // log2 of the sum of a row's four lanes, less `to` (finite, near to ref or far below all): itself a score is as large as it likes,
-    // and a power of its rounding would be in the result.
-    __device__ __forceinline__ float log2_row(float to) const {
-        const float top = pair_max32(pair_max16(ref));
-        const float f = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - top);
-        return top - to + __builtin_amdgcn_logf(pair_sum32(pair_sum16(l * f)));
-    }
-};
-
-// The largest |x| among bf16 pairs as bits, on which NaN is above infinity.
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ u16x2 max_abs_bits(u16x2 m, const uint4& x) {
-    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
-    return m;
-}
-
-// 8 values of a row at any 2-byte address (the target reads and writes words unaligned).
-__device__ __forceinline__ uint4 load_row8(const uint16_t* p) {
-    uint4 x;
-    __builtin_memcpy(&x, p, sizeof(x));
-    return x;
-}
-
-// 16 bf16 values (a, b) times inv, at most 32639 of them, as 16-bit integers 256 hi + lo of two int8: hi in a, lo
-// in b. 1.5 2^23 added to a number leaves its nearest integer in the sum's low bits.
-__device__ __forceinline__ void split_q(uint4& a, uint4& b, float inv) {
-    constexpr float kMagic = 12582912.0f;
-    const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    uint32_t hi[4], lo[4], two[2];
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-        const uint32_t q0 = __float_as_uint(fmaf(__uint_as_float(u[x] << 16), inv, kMagic));
-        const uint32_t q1 = __float_as_uint(fmaf(__uint_as_float(u[x] & 0xffff0000u), inv, kMagic));
-        two[x & 1] = __builtin_amdgcn_perm(q1, q0, 0x05040100u);
-        if (x & 1) {
-            lo[x / 2] = __builtin_amdgcn_perm(two[1], two[0], 0x06040200u);
-#pragma unroll
-            for (int y = 0; y < 2; ++y) two[y] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, two[y]) + u16x2{128, 128});
-            hi[x / 2] = __builtin_amdgcn_perm(two[1], two[0], 0x07050301u);
-        }
-    }
-    a = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    b = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-}
-
 // What the rows of one sequence see together: `ns` tiles of sinks and those from `lo` on.
 struct Span {
     int s0, q, kv, first;     // rows s0 .. s0 + q - 1, at positions first ..
-    int ns, lo, nt, nrb;      // nt tiles in all (1 where nothing is seen: zeros are written), nrb blocks of rows
     int from;                 // the first token of all (kOwn)
+    int ns, lo, nt, nrb;      // nt tiles in all (1 where nothing is seen: zeros are written), nrb blocks of rows
     __device__ __forceinline__ int tile(int t) const { return t < ns ? t : lo + t - ns; }
 };
 template <int ROWS, int TOK, Tokens P>
@@ -199,7 +23,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& A, int s0, int q, int kv
     s.q = (long long)q * A.G <= A.small ? q : 0;
     s.kv = kv;
     s.first = s.kv - q;
-    s.lo = P == kOwn ? from / TOK : P == kAll && A.window > 0 ? max(s.first - A.window + 1, 0) / TOK : 0;
+    s.lo = P == kOwn ? from / TOK : A.window > 0 ? max(s.first - A.window + 1, 0) / TOK : 0;
     s.ns = P == kAll && A.window > 0 ? min(A.sinks / TOK + (A.sinks % TOK != 0), s.lo) : 0;
     const int held = (int)min((long long)kv, (long long)A.a.width << A.c.page_log);      // what the table has places for
     s.nt = max(s.ns + max(held / TOK + (held % TOK != 0) - s.lo, 0), 1);
@@ -208,35 +32,10 @@ __device__ __forceinline__ Span span_of(const AttnArgs& A, int s0, int q, int kv
 }
 template <int ROWS, int TOK, Tokens P>
 __device__ __forceinline__ Span span_at(const AttnArgs& A, int b) {
-    const int s0 = Seqs<P>::start(A, b), kv = Seqs<P>::kv(A, b);
-    return span_of<ROWS, TOK, P>(A, s0, Seqs<P>::rows(A, b, s0, kv), kv, Seqs<P>::from(A, b));
+    const int s0 = A.a.start(b);
+    return span_of<ROWS, TOK, P>(A, s0, max(A.a.start(b + 1) - s0, 0), max(A.a.kv_len[b], 0), P == kOwn ? A.seq[b].from : 0);
 }
 
-// Inclusive sum over lanes 0 .. l (the steps of wave_scan), and a lane's value in all, for 32 and 64 bits.
-template <int Ctrl, int RowMask>
-__device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, Ctrl, RowMask, 0xF, RowMask == 0xF);
-}
-template <int Ctrl, int RowMask>
-__device__ __forceinline__ long long dpp_add(long long v) {
-    const int lo = __builtin_amdgcn_update_dpp(0, (int)v, Ctrl, RowMask, 0xF, RowMask == 0xF);
-    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), Ctrl, RowMask, 0xF, RowMask == 0xF);
-    return v + (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
-}
-template <class Int>
-__device__ __forceinline__ Int wave_scan_int(Int v) {
-    v = dpp_add<0x111, 0xF>(v);
-    v = dpp_add<0x112, 0xF>(v);
-    v = dpp_add<0x114, 0xF>(v);
-    v = dpp_add<0x118, 0xF>(v);
-    v = dpp_add<0x142, 0xA>(v);
-    return dpp_add<0x143, 0xC>(v);
-}
-__device__ __forceinline__ int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
-__device__ __forceinline__ long long lane_of(long long v, int l) {
-    const unsigned lo = __builtin_amdgcn_readlane((int)v, l), hi = __builtin_amdgcn_readlane((int)(v >> 32), l);
-    return (long long)(((unsigned long long)hi << 32) | lo);
-}
 // a / b for a >= 0: in 64 bits (below 2^50) through the correctly rounded division in double.
 __device__ __forceinline__ int quotient(int a, int b) { return (int)((unsigned)a / (unsigned)b); }
 __device__ __forceinline__ long long quotient(long long a, int b) { return (long long)((double)a / (double)b); }
@@ -265,7 +64,7 @@ struct Share {
 };
 template <int ROWS, int TOK, Tokens P, class Int>
 __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int lane, Share* out) {
-    const int n = Seqs<P>::n(A), h_kv = A.c.h_kv;
+    const int n = A.a.n_seq, h_kv = A.c.h_kv;
     Span s{};
     const auto span = [&](int b0) {                          // of sequence b0 + lane; no rows behind the last
         s.nrb = 0;
@@ -320,7 +119,7 @@ __device__ __forceinline__ bool share_of(const AttnArgs& A, int n_wg, int w, int
 struct Cut {
     int first, last, slot;            // workgroups first .. last; slot of the first (2 w for the others)
     int row, e, r0, rows;             // its sequence's first row, kv head, first row of the block, rows of the sequence
-    int any;                          // 0: there is none; 2: of a sequence with shared tokens (kOwn)
+    int any;
 };
 template <int ROWS, int D>
 struct Parts {
@@ -331,101 +130,7 @@ struct Parts {
     static size_t bytes(int n_wg) { return (size_t)2 * n_wg * ROWS * (D + 2) * sizeof(float) + n_wg * sizeof(Cut); }
 };
 
-// The lowest n bits, of a n that may lie anywhere.
-__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
-
-// 4 codes to fp16: 0x6400 + (code + 128) is 1024 + code + 128, exactly.
-__device__ __forceinline__ void halves(uint32_t raw, f16x2* out) {
-    const uint32_t u = raw ^ 0x80808080u;
-    const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-    out[0] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
-    out[1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
-}
-__device__ __forceinline__ f16x8 halves8(uint32_t a, uint32_t b) {
-    f16x2 h[4];
-    halves(a, h);
-    halves(b, h + 2);
-    return f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
-}
-
-// sigmoid for a bf16 result: v_exp and v_rcp are within an ulp of 32 bits.
-__device__ __forceinline__ float sigmoid_16(float x) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -kLog2e));
-}
-
-__device__ __forceinline__ uint2 load_gate(const AttnArgs& A, int t, int h, int d) {
-    uint2 z = make_uint2(0, 0);
-    if (A.gate) __builtin_memcpy(&z, A.gate + (long long)t * A.gate_stride + (size_t)h * A.c.d + d, sizeof(z));
-    return z;
-}
-// 4 outputs of a row from its sum of p', o 2^m, and the logarithm of its sum of p, m + lse: o 2^-lse, of which the power alone can
-// leave the floats' range.
-__device__ __forceinline__ v4f outputs(v4f o, float lse) {
-    if (lse == -__builtin_inff()) return v4f{0, 0, 0, 0};
-    const float f = __builtin_amdgcn_exp2f(-0.5f * lse);
-    return o * f * f;
-}
-constexpr float kNone = -__FLT_MAX__;      // m of a part without a token: finite, so that lse, -inf, is 0 as a power, without a question
-// Partial results (m, lse, o) of a row put together.
-struct Joined {
-    float m = kNone, top = kNone, total = 0.0f;              // total 2^(m + top): the sum of p
-    v4f o = {0, 0, 0, 0};
-    // Several that are at hand: m of all, then top of all, then what they add.
-    __device__ __forceinline__ void meet_m(float pm) { m = fmaxf(m, pm); }
-    __device__ __forceinline__ void meet_sum(float pm, float lse) { top = fmaxf(top, pm - m + lse); }
-    __device__ __forceinline__ void add(float pm, float lse, const v4f& po) {
-        total += __builtin_amdgcn_exp2f(pm - m + lse - top);
-        o += po * __builtin_amdgcn_exp2f(pm - m);
-    }
-    // One more.
-    __device__ __forceinline__ void more(float pm, float lse, const v4f& po) {
-        const float now = fmaxf(m, pm), was = m - now + top;
-        o *= __builtin_amdgcn_exp2f(m - now);
-        m = now;
-        top = fmaxf(fmaxf(was, pm - m + lse), kNone);
-        total *= __builtin_amdgcn_exp2f(was - top);
-        add(pm, lse, po);
-    }
-    __device__ __forceinline__ float log2_sum() const { return top + __builtin_amdgcn_logf(total); }
-};
-// Writes 4 outputs of a row, gated by z.
-__device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d, v4f v, uint2 z) {
-    if (A.gate) {
-        v[0] *= sigmoid_16(__uint_as_float(z.x << 16));
-        v[1] *= sigmoid_16(__uint_as_float(z.x & 0xffff0000u));
-        v[2] *= sigmoid_16(__uint_as_float(z.y << 16));
-        v[3] *= sigmoid_16(__uint_as_float(z.y & 0xffff0000u));
-    }
-    const uint2 y = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-    __builtin_memcpy(A.o + ((size_t)t * A.h_q + h) * A.c.d + d, &y, sizeof(y));
-}
-__device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d, v4f v) {
-    store_out(A, t, h, d, v, load_gate(A, t, h, d));
-}
-
-// What kShared has left for 4 channels of a row.
-struct RowPart {
-    float m, lse;
-    v4f o;
-};
-__device__ __forceinline__ RowPart row_part(const AttnArgs& A, int t, int h, int d) {
-    const size_t row = (size_t)t * A.h_q + h;
-    return RowPart{A.row_ml[2 * row], A.row_ml[2 * row + 1], *reinterpret_cast<const v4f*>(A.row_o + row * A.c.d + d)};
-}
-// 4 channels of a row whose parts are all in `sum`, but what kShared has left (`more`: there is such).
-template <Tokens P>
-__device__ __forceinline__ void finish(const AttnArgs& A, int t, int h, int d, Joined& sum, bool more, const RowPart& part) {
-    if constexpr (P == kShared) {
-        const size_t row = (size_t)t * A.h_q + h;
-        *reinterpret_cast<v4f*>(A.row_o + row * A.c.d + d) = sum.o;
-        if (d == 0) *reinterpret_cast<float2*>(A.row_ml + 2 * row) = make_float2(sum.m, sum.log2_sum());
-    } else {
-        if (P == kOwn && more) sum.more(part.m, part.lse, part.o);
-        store_out(A, t, h, d, outputs(sum.o, sum.log2_sum()));
-    }
-}
-
-constexpr int kSplitThreads = 256, kSplitWaves = kSplitThreads / kWave, kSplitRows = 16;
+constexpr int kSplitThreads = 256, kSplitWaves = kSplitThreads / kWave;
 // Tokens a wave takes at a time. Keys, values and sums of a 64-token tile are 3/4 D registers, which
 // leaves none at D = 256. Tiles of 32 at D = 128 are faster for some short sequences (48 windows of 1,028 tokens over 4 heads
 // 18.6 us for 20.4) and slower for others (16 sequences of 1,000 over 8 heads 15.1 for 13.6), long ones take the same;
@@ -477,7 +182,6 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     LaneSum sum;
     // What is left to do for the piece whose sums these are, in vector registers: the main loop needs the scalar ones.
     int o_e = 0, o_r0 = 0, o_rows = 0, o_s0 = 0, o_slot = 0;        // o_slot -1: the whole segment
-    [[maybe_unused]] int o_more = 0;                          // shared tokens come before it (kOwn)
     bool open = false;
     int pieces = 0;
     Cut cut{};
@@ -496,7 +200,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
         // A tile's places in the cache: this lane's values, scores and scales are of its tokens `mine` on, its
         // keys of those from `keys` on (both within 16 tokens of a page). A lost page's memory is page 0's,
         // hidden below.
-        const int32_t* tab = Seqs<P>::table(Y, b);
+        const int32_t* tab = Y.a.table + (size_t)b * Y.a.width;
         const int kv = (int)min((long long)s.kv, (long long)Y.a.width << page_log), n_pages = Y.c.n_pages, h_kv = Y.c.h_kv;
         const int8_t *kb = Y.c.k + ((size_t)e << page_log) * D, *vb = Y.c.v + ((size_t)e << page_log) * D;
         const float *ksb = Y.c.k_scale + e, *vsb = Y.c.v_scale + e;
@@ -559,10 +263,6 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             for (int i = tid; i < kSplitRows * D / 4; i += kSplitThreads) {
                 const int row = i / (D / 4), d = i % (D / 4) * 4;
                 if (x_r0 + row >= x_rows) break;
-                const int token = (x_r0 + row) / Z.G, x_t = taken(o_s0) + token, x_h = taken(o_e) * Z.G + x_r0 + row - token * Z.G;
-                RowPart before{};
-                const bool more = P == kOwn && x_slot < 0 && taken(o_more);
-                if (more) before = row_part(Z, x_t, x_h, d);
                 Joined to;
 #pragma unroll
                 for (int k = 0; k < kSplitWaves; ++k) to.meet_m(lo_ml[(k * kSplitRows + row) * 2]);
@@ -573,7 +273,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
                     to.add(lo_ml[(k * kSplitRows + row) * 2], lo_ml[(k * kSplitRows + row) * 2 + 1],
                            *reinterpret_cast<const v4f*>(lo_o + (k * kSplitRows + row) * kPitch + d));
                 if (x_slot < 0) {
-                    finish<P>(Z, x_t, x_h, d, to, more, before);
+                    const int token = (x_r0 + row) / Z.G, t = taken(o_s0) + token, h = taken(o_e) * Z.G + x_r0 + row - token * Z.G;
+                    if constexpr (P == kOwn) store_row_part(Z, t, h, d, to.o, to.m, to.log2_sum());
+                    else store_out(Z, t, h, d, outputs(to.o, to.log2_sum()));
                 } else {
                     *reinterpret_cast<v4f*>(parts.o + ((size_t)x_slot * kSplitRows + row) * D + d) = to.o;
                     if (d == 0) {
@@ -606,11 +308,11 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             lo_q[(2 * w) * kWave + lane] = raw[0];
             lo_q[(2 * w + 1) * kWave + lane] = raw[1];
         }
-        const int pos = r0 + n >= rows ? -1 : P == kShared ? s.kv - 1 : s.first + (r0 + n) / Y.G;
-        const int from = P == kOwn ? s.from : P == kAll && window > 0 ? pos - window + 1 : 0;       // the row sees from .. pos, and the sinks
+        const int pos = r0 + n < rows ? s.first + (r0 + n) / Y.G : -1;
+        const int from = P == kOwn ? s.from : window > 0 ? pos - window + 1 : 0;     // the row sees from .. pos, and the sinks
         // tiles that every row sees as a whole: those starting at full_lo .. full_hi
-        const int full_hi = (P == kShared ? s.kv - 1 : s.first + r0 / Y.G) - kTok + 1;
-        const int full_lo = P == kOwn ? s.from : P == kAll && window > 0 ? s.first + (min(r0 + kSplitRows, rows) - 1) / Y.G - window + 1 : 0;
+        const int full_hi = s.first + r0 / Y.G - kTok + 1;
+        const int full_lo = P == kOwn ? s.from : window > 0 ? s.first + (min(r0 + kSplitRows, rows) - 1) / Y.G - window + 1 : 0;
         lds_barrier();
 #pragma unroll
         for (int m = 0; m < kM; ++m) acc[m] = v4f{0, 0, 0, 0};
@@ -618,7 +320,6 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
 
         // Where its parts go, and whether it is cut at its end.
         o_e = parked(e), o_r0 = parked(r0), o_rows = parked(rows), o_s0 = parked(s.s0);
-        if constexpr (P == kOwn) o_more = parked(s.from > 0);
         o_slot = parked(t0 == 0 && t1 == s.nt ? -1 : 2 * (int)blockIdx.x + (pieces > 0));
         open = true;
         ++pieces;
@@ -626,8 +327,11 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             const int x = blockIdx.x, per = taken(w_per), before = v0 > start ? (v0 - start + per - 1) / per : 0;
             // the first part is its workgroup's only one so far where the segment began at or before the share
             cut = Cut{x - before, x + (s.nt + start - (t1 + start) + per - 1) / per, before ? 2 * (x - before) + (v0 < before * per) : o_slot,
-                      s.s0, e, r0, rows, P == kOwn && s.from > 0 ? 2 : 1};
+                      s.s0, e, r0, rows, 1};
         }
+        if constexpr (P == kOwn)
+            if (t0 == 0 && tid == 0)                          // its first tile is here
+                Y.cuts[((size_t)s.s0 * Y.G + r0) * h_kv + e] = t1 == s.nt ? OwnCut{-1, 0, 0, 0} : OwnCut{cut.first, cut.last, cut.slot, 0};
         const int n_left = parked(left - (s.nt + start - v0)), n_rb = parked(rb), n_b = parked(b), n_nrb = parked(s.nrb), n_start = parked(start);
 
         for (; t < t1; t += kSplitWaves) {
@@ -729,7 +433,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
 constexpr int kJoinThreads = 256;
 template <int D, Tokens P, class At>
 __device__ __forceinline__ void join_outputs(const AttnArgs& A, const float* po, const float* ml, int k0, int k1, At at_part, int from,
-                                             int to, int s0, int e, int r0, bool more) {
+                                             int to, int s0, int e, int r0) {
     __shared__ v4f lo_o[kJoinThreads];
     __shared__ float lo_m[kJoinThreads], lo_l[kJoinThreads];
     int wide = 1;                                             // outputs at a time
@@ -738,9 +442,6 @@ __device__ __forceinline__ void join_outputs(const AttnArgs& A, const float* po,
     for (int x0 = from; x0 < to; x0 += wide) {
         const int x = min(x0 + (int)(threadIdx.x & (wide - 1)), to - 1), row = x / (D / 4), d = x % (D / 4) * 4;
         Joined sum;
-        const int token = (r0 + row) / A.G, t = s0 + token, h = e * A.G + r0 + row - token * A.G;
-        RowPart before{};
-        if (P == kOwn && more && way == 0) before = row_part(A, t, h, d);
 #pragma unroll 4
         for (int k = k0 + way; k <= k1; k += ways) {
             const size_t at = at_part(k) + row;
@@ -755,13 +456,17 @@ __device__ __forceinline__ void join_outputs(const AttnArgs& A, const float* po,
             if (way < half) sum.more(lo_m[other], lo_l[other], lo_o[other]);
             __syncthreads();
         }
-        if (way == 0 && x0 + (int)threadIdx.x < to) finish<P>(A, t, h, d, sum, more, before);
+        if (way == 0 && x0 + (int)threadIdx.x < to) {
+            const int token = (r0 + row) / A.G, t = s0 + token, h = e * A.G + r0 + row - token * A.G;
+            if constexpr (P == kOwn) store_row_part(A, t, h, d, sum.o, sum.m, sum.log2_sum());
+            else store_out(A, t, h, d, outputs(sum.o, sum.log2_sum()));
+        }
     }
 }
 
 // Segments that several workgroups share. One that lies across n ends of shares has n workgroups here,
 // which take even parts of its outputs.
-template <int D, Tokens P>
+template <int D>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg) {
     const Parts<kSplitRows, D> parts(A.part, n_wg);
     const Cut c = parts.cut[blockIdx.x];
@@ -770,7 +475,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg
     const int all = min(kSplitRows, c.rows - c.r0) * (D / 4);
     const int from = (int)((long long)all * i / n), to = (int)((long long)all * (i + 1) / n);
     const auto at = [&](int k) { return (size_t)(k == c.first ? c.slot : 2 * k) * kSplitRows; };
-    join_outputs<D, P>(A, parts.o, parts.ml, c.first, c.last, at, from, to, c.row, c.e, c.r0, c.any == 2);
+    join_outputs<D, kAll>(A, parts.o, parts.ml, c.first, c.last, at, from, to, c.row, c.e, c.r0);
 }
 
 // Blocks of rows: prompts.
@@ -820,7 +525,7 @@ __device__ __forceinline__ void each(F f) {
 // behind 16,384, 128 blocks, took 356 us whole and take 170.
 struct BlockCut {
     int first, parts, step;                                   // partial results first, first + step ..
-    int s0, e, r0, rows, more;                                // as in Cut; more: of a sequence with shared tokens
+    int s0, e, r0, rows, unused;                              // as in Cut
 };
 template <int D>
 struct BlockParts {
@@ -847,10 +552,9 @@ __device__ __forceinline__ int wave_max_int(int v) {
     return lane_of(dpp_max<0x143, 0xC>(v), kWave - 1);
 }
 // The blocks of a sequence.
-template <Tokens P>
 __device__ __forceinline__ int blocks_of(const AttnArgs& A, int b) {
-    if (b >= Seqs<P>::n(A)) return 0;
-    const int rows = Seqs<P>::rows(A, b, Seqs<P>::start(A, b), P == kShared ? Seqs<P>::kv(A, b) : 0) * A.G;
+    if (b >= A.a.n_seq) return 0;
+    const int rows = max(A.a.start(b + 1) - A.a.start(b), 0) * A.G;
     return rows > A.small ? (rows + kBlockRows - 1) / kBlockRows : 0;
 }
 // The blocks of all sequences and heads, and in how many parts each is taken: lane p - 1 knows the time of p, in tiles,
@@ -864,18 +568,17 @@ constexpr int kLeastPart = 4;         // tiles
 template <int D, Tokens P>
 __device__ __forceinline__ Blocks all_blocks(const AttnArgs& A, int lane) {
     int sum = 0, kv = 0;
-    const int n_seq = Seqs<P>::n(A);
 #pragma unroll 4
-    for (int b0 = 0; b0 < n_seq; b0 += kWave) {
-        const int at = min(b0 + lane, n_seq - 1), v = blocks_of<P>(A, b0 + lane);
-        const int held = P == kAll ? A.a.kv_len[at] : Seqs<P>::kv(A, at) - Seqs<P>::from(A, at);
+    for (int b0 = 0; b0 < A.a.n_seq; b0 += kWave) {
+        const int at = min(b0 + lane, A.a.n_seq - 1), v = blocks_of(A, b0 + lane);
+        const int held = P == kOwn ? max(A.a.kv_len[at], 0) - A.seq[at].from : A.a.kv_len[at];
         sum += v;
         kv = max(kv, v > 0 ? held : 0);
     }
     Blocks out;
     out.n = lane_of(wave_scan_int(sum), kWave - 1) * A.c.h_kv;
     kv = wave_max_int(kv);
-    if (P == kAll && A.window > 0 && A.window < kv) kv = A.window + min(A.sinks, kv - A.window);
+    if (A.window > 0 && A.window < kv) kv = A.window + min(A.sinks, kv - A.window);
     const int p = lane + 1, rounds = (out.n * p + A.slots - 1) / A.slots;
     float cost = (float)rounds * ((float)kv / (float)(kBlockTok * p) + (p > 1 ? kPartCost<D> : 0.0f));
     if (p > 1 && (long long)out.n * p > A.items) cost = __builtin_inff();
@@ -906,7 +609,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         part = i % parts;
         rb = all.n / A.c.h_kv - 1 - i / parts;
         for (int b0 = 0;; b0 += kWave) {
-            const int v = blocks_of<P>(A, b0 + lane), incl = wave_scan_int(v);
+            const int v = blocks_of(A, b0 + lane), incl = wave_scan_int(v);
             const unsigned long long hit = __ballot(incl > rb);
             if (hit) {
                 const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
@@ -918,14 +621,13 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         }
     } else {
         const int j = A.blocks / A.c.h_kv - 1 - block / A.c.h_kv;
-        const auto key = [&](int b) { return (int)((long long)Seqs<P>::start(A, b) * A.G / kBlockRows) + b; };
-        b = wave_search(Seqs<P>::n(A), j, lane, key);
+        const auto key = [&](int b) { return (int)((long long)A.a.start(b) * A.G / kBlockRows) + b; };
+        b = wave_search(A.a.n_seq, j, lane, key);
         rb = j - key(b);
     }
-    const int s0 = Seqs<P>::start(A, b), kv = Seqs<P>::kv(A, b), q = Seqs<P>::rows(A, b, s0, kv), r0 = rb * kBlockRows, rows = q * A.G;
+    const int s0 = A.a.start(b), q = A.a.start(b + 1) - s0, r0 = rb * kBlockRows, rows = max(q, 0) * A.G;
     if (!kCut && (rows <= A.small || rb < 0 || r0 >= rows)) return;      // rb < 0: before the first sequence's rows
-    const int first = kv - q, from = Seqs<P>::from(A, b);
-    const auto place = [&](int qi) { return P == kShared ? kv - 1 : first + qi; };       // of the sequence's new token qi
+    const int kv = max(A.a.kv_len[b], 0), first = kv - q, own = P == kOwn ? A.seq[b].from : 0;
 
     // q of row n of the wave, channels 64 c + 16 g .. + 15
     const int w0 = r0 + 16 * w;
@@ -934,7 +636,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     float qc;
     {
         const int r = w0 + n, rc = min(r, rows - 1), qi = rc / A.G;
-        pos = r < rows ? place(qi) : -1;
+        pos = r < rows ? first + qi : -1;
         const uint16_t* qp = A.q + (long long)(s0 + qi) * A.q_stride + (size_t)(e * A.G + rc - qi * A.G) * D + 16 * g;
         u16x2 mb = {0, 0};
 #pragma unroll
@@ -953,15 +655,14 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     }
     // Of the wave's positions wave_first .. wave_last: tiles that start from full_lo to full_hi every row sees as a
     // whole, those below some_lo (the sinks aside) and above wave_last none does.
-    const bool window = P == kAll && A.window > 0;
-    const int wave_first = place(min(w0, rows - 1) / A.G), wave_last = place((min(w0 + 16, rows) - 1) / A.G);
-    const int full_hi = wave_first - kBlockTok + 1, full_lo = P == kOwn ? from : window ? wave_last - A.window + 1 : 0;
-    const int some_lo = window ? wave_first - A.window + 1 - kBlockTok + 1 : 0;
+    const int wave_first = first + min(w0, rows - 1) / A.G, wave_last = first + (min(w0 + 16, rows) - 1) / A.G;
+    const int full_hi = wave_first - kBlockTok + 1, full_lo = P == kOwn ? own : A.window > 0 ? wave_last - A.window + 1 : 0;
+    const int some_lo = P == kAll && A.window > 0 ? wave_first - A.window + 1 - kBlockTok + 1 : 0;
 
     // the block's tiles
-    const int block_first = place(r0 / A.G), block_last = place((min(r0 + kBlockRows, rows) - 1) / A.G);
-    const int lo = P == kOwn ? from / kBlockTok : window ? max(block_first - A.window + 1, 0) / kBlockTok : 0;
-    const int ns = window ? min(A.sinks / kBlockTok + (A.sinks % kBlockTok != 0), lo) : 0;
+    const int block_first = first + r0 / A.G, block_last = first + (min(r0 + kBlockRows, rows) - 1) / A.G;
+    const int lo = P == kOwn ? own / kBlockTok : A.window > 0 ? max(block_first - A.window + 1, 0) / kBlockTok : 0;
+    const int ns = P == kAll && A.window > 0 ? min(A.sinks / kBlockTok + (A.sinks % kBlockTok != 0), lo) : 0;
     const int all = block_last < 0 ? 0 : max(ns + block_last / kBlockTok + 1 - lo, 0);
     int begin = 0, nt = all;                                  // this part's: tiles begin .. begin + nt - 1
     if constexpr (kCut) {
@@ -969,7 +670,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
             const int i = blockIdx.x / A.c.h_kv / parts;
             parts = min(parts, max(all / kLeastPart, 1));
             if (part == 0 && tid == 0)
-                BlockParts<D>(A.block_part, A.slots).cut[i * A.c.h_kv + e] = BlockCut{(int)blockIdx.x, parts, A.c.h_kv, s0, e, r0, rows, from > 0};
+                BlockParts<D>(A.block_part, A.slots).cut[i * A.c.h_kv + e] = BlockCut{(int)blockIdx.x, parts, A.c.h_kv, s0, e, r0, rows, 0};
             if (part >= parts) return;
             begin = all / parts * part + min(part, all % parts);
             nt = all / parts + (part < all % parts);
@@ -981,7 +682,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     // and in a page (or 64 tokens of it) channel by channel. The pieces of one wave's i are in one page.
     const int page_log = A.c.page_log, part_log = min(page_log, 6);
     constexpr int kDLog = D == 64 ? 6 : D == 128 ? 7 : 8;
-    const int32_t* tab = Seqs<P>::table(A, b);
+    const int32_t* tab = A.a.table + (size_t)b * A.a.width;
     const int kv_held = (int)min((long long)kv, (long long)A.a.width << page_log);
     // Lane g of 0 .. 3 holds the page of the tile's tokens 16 g .. + 15, loaded a tile ahead of its use.
     const auto pages = [&](int at) {
@@ -1098,8 +799,8 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
             }
             if (at < full_lo || at > full_hi) {
                 asm volatile("");                             // a branch: most tiles are seen as a whole
-                const int j0 = at + 16 * g, least = P == kOwn ? from : window ? pos - A.window + 1 : 0;
-                const uint32_t seen = low_bits(pos - j0 + 1) & (low_bits(A.sinks - j0) | ~low_bits(least - j0));
+                const int j0 = at + 16 * g, from = P == kOwn ? own : A.window > 0 ? pos - A.window + 1 : 0;
+                const uint32_t seen = low_bits(pos - j0 + 1) & (low_bits(A.sinks - j0) | ~low_bits(from - j0));
 #pragma unroll
                 for (int y = 0; y < 16; ++y) p[y] = (seen >> y) & 1 ? p[y] : -__builtin_inff();
             }
@@ -1155,15 +856,9 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         }
         return;
     }
-    if (P != kAll && r < rows) {
+    if (P == kOwn && r < rows) {
 #pragma unroll
-        for (int m = 0; m < kM; ++m) {
-            RowPart before{};
-            if (P == kOwn && from > 0) before = row_part(A, s0 + qi, head, 16 * m + d0);
-            Joined sum;
-            sum.more(m_ref, lse, acc[m]);
-            finish<P>(A, s0 + qi, head, 16 * m + d0, sum, from > 0, before);
-        }
+        for (int m = 0; m < kM; ++m) store_row_part(A, s0 + qi, head, 16 * m + d0, acc[m], m_ref, lse);
     } else if (r < rows) {
         constexpr int kN = kM < 8 ? kM : 8;                   // pieces of 4 channels, their gates on the way together
 #pragma unroll
@@ -1190,7 +885,7 @@ __global__ void __launch_bounds__(kJoinThreads) block_join_kernel(AttnArgs A) {
     const int all = min(kBlockRows, c.rows - c.r0) * (D / 4);
     const auto at = [&](int k) { return (size_t)(c.first + k * c.step) * kBlockRows; };
     join_outputs<D, P>(A, parts.o, parts.ml, 0, c.parts - 1, at, (int)((long long)all * i / n), (int)((long long)all * (i + 1) / n),
-                       c.s0, c.e, c.r0, c.more);
+                    c.s0, c.e, c.r0);
 }
 
 // Sequences of at most kSplitMost (token, head) rows a kv head are split_kernel's in any case, and so are all where the
@@ -1203,12 +898,6 @@ __global__ void __launch_bounds__(kJoinThreads) block_join_kernel(AttnArgs A) {
 constexpr int kSplitMost = 32;
 constexpr int least_blocks(int d) { return 4096 / d; }
 
-struct Plan {
-    bool block, cut;          // block_kernel for sequences of more than kSplitMost rows; in parts
-    int n_wg, slots;          // workgroups that the chip holds: of split_kernel two a CU, of block_kernel one or two
-    long long full;           // whole blocks that the batch's rows fill
-    int max_q;
-};
 Plan plan_of(int d, int h_kv, int G, int T, int max_q, hipStream_t s) {
     Plan p;
     const int n_cu = device_cu_count(s);
@@ -1226,7 +915,6 @@ size_t split_bytes(const Plan& p) { return (Parts<kSplitRows, D>::bytes(p.n_wg) 
 // Also where this batch's blocks stay whole: those of a smaller one, which the workspace has to do for as well, may not.
 template <int D>
 size_t attn_bytes(const Plan& p) { return split_bytes<D>(p) + (p.block ? BlockParts<D>::bytes(p.slots) : 0); }
-size_t attn_bytes(int d, const Plan& p) { return d == 64 ? attn_bytes<64>(p) : d == 128 ? attn_bytes<128>(p) : attn_bytes<256>(p); }
 
 template <int D, bool kCut, Tokens P>
 hipError_t launch_blocks(AttnArgs& A, long long n, hipStream_t s) {
@@ -1241,22 +929,22 @@ hipError_t launch_blocks(AttnArgs& A, long long n, hipStream_t s) {
 }
 
 template <int D, Tokens P>
-hipError_t launch_tokens(AttnArgs& A, const Plan& p, hipStream_t s) {
-    const int n_wg = p.n_wg, n_seq = P == kShared ? A.n_groups : A.a.n_seq;
+hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
+    const int n_wg = p.n_wg;
     // With at most max_q new tokens in each other one, a sequence of the batch has at least these. Where that is more than
     // kSplitMost rows all are block_kernel's (also those of a batch whose offsets end before T), and it is the only launch.
-    const long long shortest = A.a.T - (long long)(n_seq - 1) * p.max_q;
+    const long long shortest = A.a.T - (long long)(A.a.n_seq - 1) * p.max_q;
     const bool only = p.block && shortest * A.G > kSplitMost;
     A.small = only ? 0 : p.block ? kSplitMost : 0x7fffffff;
     // tiles: at most those of a whole table for each block of rows, and n_wg - 1 and a workgroup's share more in sums
-    const long long row_blocks = (long long)A.a.T * A.G / kSplitRows + n_seq;
+    const long long row_blocks = (long long)A.a.T * A.G / kSplitRows + A.a.n_seq;
     const long long tiles = ((long long)A.a.width << A.c.page_log) / kSplitTok<D> + 1;
     A.narrow = row_blocks < (1ll << 31) / tiles / A.c.h_kv / 2 - n_wg;
     if (p.block) {
         hipError_t e;
         if (p.cut) {
             // a sequence has at most one block that is not full, and more than kSplitMost rows
-            const long long most = only ? n_seq : std::min((long long)n_seq, (long long)A.a.T * A.G / kSplitMost);
+            const long long most = only ? A.a.n_seq : std::min((long long)A.a.n_seq, (long long)A.a.T * A.G / kSplitMost);
             const long long blocks = p.full + most * A.c.h_kv;
             A.slots = p.slots;
             A.items = 2 * p.slots;
@@ -1264,75 +952,37 @@ hipError_t launch_tokens(AttnArgs& A, const Plan& p, hipStream_t s) {
             e = launch_blocks<D, true, P>(A, std::max(blocks, (long long)A.items), s);
             if (e == hipSuccess) hipLaunchKernelGGL((block_join_kernel<D, P>), dim3((unsigned)(2 * n_wg)), dim3(kJoinThreads), 0, s, A);
         } else {
-            e = launch_blocks<D, false, P>(A, p.full + (long long)n_seq * A.c.h_kv, s);
+            e = launch_blocks<D, false, P>(A, p.full + (long long)A.a.n_seq * A.c.h_kv, s);
         }
         if (e != hipSuccess) return e;
         if (only) return hipGetLastError();
     }
     const unsigned lds = kSplitWaves * kSplitRows * (D + 4 + 2 + 1) * sizeof(float) + D / 64 * 2 * kWave * sizeof(uint4);
     hipLaunchKernelGGL((split_kernel<D, P>), dim3((unsigned)n_wg), dim3(kSplitThreads), lds, s, A);
-    if (n_wg > 1) hipLaunchKernelGGL((join_kernel<D, P>), dim3((unsigned)n_wg - 1), dim3(kJoinThreads), 0, s, A, n_wg);
+    if (P == kAll && n_wg > 1) hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)n_wg - 1), dim3(kJoinThreads), 0, s, A, n_wg);
     return hipGetLastError();
 }
 
-template <int D>
-hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) { return launch_tokens<D, kAll>(A, p, s); }
+template <Tokens P>
+hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
+    switch (A.c.d) {
+        case 64: return launch_attn<64, P>(A, p, s);
+        case 128: return launch_attn<128, P>(A, p, s);
+        default: return launch_attn<256, P>(A, p, s);
+    }
+}
 
-// Attention behind shared tokens. The workspace holds what either launch needs for itself, and the rows of kShared. Those of a
-// group are at most all of the batch's.
-struct SharedPlan {
-    Plan shared, own;
-    size_t scratch, rows, bytes;
-};
-SharedPlan shared_plan_of(int d, int h_kv, int G, int T, int max_q, hipStream_t s) {
-    SharedPlan p;
-    p.shared = plan_of(d, h_kv, G, T, T, s);
-    p.own = plan_of(d, h_kv, G, T, max_q, s);
-    p.scratch = (std::max(attn_bytes(d, p.shared), attn_bytes(d, p.own)) + 255) / 256 * 256;
-    p.rows = (size_t)T * h_kv * G;
-    p.bytes = p.scratch + p.rows * (d + 2) * sizeof(float);
-    return p;
-}
-template <int D>
-hipError_t launch_attn(AttnArgs& A, const SharedPlan& p, hipStream_t s) {
-    A.row_o = A.part + p.scratch / sizeof(float);
-    A.row_ml = A.row_o + p.rows * D;
-    const hipError_t e = launch_tokens<D, kShared>(A, p.shared, s);
-    return e != hipSuccess ? e : launch_tokens<D, kOwn>(A, p.own, s);
-}
+}  // namespace
+
+Plan attn_plan(int d, int h_kv, int G, int T, int max_q, hipStream_t s) { return plan_of(d, h_kv, G, T, max_q, s); }
+size_t attn_bytes(int d, const Plan& p) { return d == 64 ? attn_bytes<64>(p) : d == 128 ? attn_bytes<128>(p) : attn_bytes<256>(p); }
+hipError_t launch_own(AttnArgs& A, const Plan& p, hipStream_t s) { return launch_attn<kOwn>(A, p, s); }
 
 // The blocks of the batch are numbered in 31 bits.
 bool attn_shape_ok(const Kv8& c, int n_seq, int T, int max_q, int h_q) {
     return n_seq > 0 && n_seq <= 65535 && T >= 0 && max_q >= 0 && (T == 0 || max_q > 0) && h_q > 0 && h_q % c.h_kv == 0 &&
            h_q <= 65536 && (long long)T * h_q <= 1ll << 37;
 }
-
-}  // namespace
-}  // namespace ixg
-
-extern "C" {
-
-size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, int max_q, int h_q) {
-    using namespace ixg;
-    Kv8 c;
-    if (!make_kv8(cache, &c) || !attn_shape_ok(c, n_seq, total_T, max_q, h_q)) return 0;
-    return attn_bytes(c.d, plan_of(c.d, c.h_kv, h_q / c.h_kv, total_T, max_q, nullptr));
-}
-
-size_t ix_kv8_attn_shared_workspace_size(const ix_kv8* cache, int n_seq, int total_T, int max_q, int n_groups, int h_q) {
-    using namespace ixg;
-    Kv8 c;
-    if (!make_kv8(cache, &c) || !attn_shape_ok(c, n_seq, total_T, max_q, h_q) || n_groups < 0 || n_groups > 65535) return 0;
-    if (n_groups == 0) return ix_kv8_attn_workspace_size(cache, n_seq, total_T, max_q, h_q);
-    return shared_plan_of(c.d, c.h_kv, h_q / c.h_kv, total_T, max_q, nullptr).bytes;
-}
-
-}  // extern "C"
-
-namespace ixg {
-namespace {
-
-// What both calls check alike.
 bool make_attn(const ix_kv8* cache, int n_seq, int T, int max_q, const int32_t* cu, const int32_t* kv_len, const int32_t* table, int width,
                int h_q, float scale, AttnArgs* A) {
     if (!make_kv8(cache, &A->c) || !make_batch(n_seq, T, cu, kv_len, table, width, &A->a)) return false;
@@ -1356,19 +1006,17 @@ bool make_operands(const ix_rows* q, const ix_rows* gate, uint16_t* o, void* wor
     A->part = static_cast<float*>(workspace);
     return true;
 }
-template <class P>
-hipError_t launch(AttnArgs& A, const P& p, hipStream_t s) {
-    switch (A.c.d) {
-        case 64: return launch_attn<64>(A, p, s);
-        case 128: return launch_attn<128>(A, p, s);
-        default: return launch_attn<256>(A, p, s);
-    }
-}
 
-}  // namespace
 }  // namespace ixg
 
 extern "C" {
+
+size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, int max_q, int h_q) {
+    using namespace ixg;
+    Kv8 c;
+    if (!make_kv8(cache, &c) || !attn_shape_ok(c, n_seq, total_T, max_q, h_q)) return 0;
+    return attn_bytes(c.d, plan_of(c.d, c.h_kv, h_q / c.h_kv, total_T, max_q, nullptr));
+}
 
 hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens,
                        const int32_t* kv_len, const int32_t* table, int width, const ix_rows* q, int h_q, float scale,
@@ -1383,28 +1031,7 @@ hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, c
     if (!make_operands(q, gate, o, workspace, workspace_bytes, attn_bytes(A.c.d, p), &A)) return hipErrorInvalidValue;
     A.window = window;
     A.sinks = sinks;
-    return launch(A, p, s);
-}
-
-hipError_t ix_kv8_attn_shared(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens, const int32_t* kv_len,
-                              const int32_t* table, int width, int n_groups, const int32_t* groups, const int32_t* shared_len,
-                              const ix_rows* q, int h_q, float scale, const ix_rows* gate, uint16_t* o, void* workspace,
-                              size_t workspace_bytes, hipStream_t s) {
-    using namespace ixg;
-    if (n_groups == 0)
-        return ix_kv8_attn(cache, n_seq, total_T, max_q, cu_seqlens, kv_len, table, width, q, h_q, scale, 0, 0, gate, o, workspace,
-                           workspace_bytes, s);
-    AttnArgs A{};
-    if (!make_attn(cache, n_seq, total_T, max_q, cu_seqlens, kv_len, table, width, h_q, scale, &A)) return hipErrorInvalidValue;
-    if (n_groups < 0 || n_groups > 65535 || !groups || !shared_len || !ptr_aligned(groups, 4) || !ptr_aligned(shared_len, 4))
-        return hipErrorInvalidValue;
-    if (total_T == 0) return hipSuccess;
-    const SharedPlan p = shared_plan_of(A.c.d, A.c.h_kv, A.G, total_T, max_q, s);
-    if (!make_operands(q, gate, o, workspace, workspace_bytes, p.bytes, &A)) return hipErrorInvalidValue;
-    A.groups = groups;
-    A.shared = shared_len;
-    A.n_groups = n_groups;
-    return launch(A, p, s);
+    return launch_attn<kAll>(A, p, s);
 }
 
 }  // extern "C"

@@ -467,21 +467,19 @@ hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, c
                        int window, int sinks, const ix_rows* gate, uint16_t* o, void* workspace,
                        size_t workspace_bytes, hipStream_t s IX_GDN_DEFAULT_STREAM);
 
-/* Bytes of device workspace for ix_kv8_attn_shared: what ix_kv8_attn needs, and 4 (d + 2) for each (token, query head); 0 for
- * an invalid request. It does for every batch of the same cache and h_q with no more tokens in all and no larger max_q, of any
- * n_seq and n_groups. It needs no initialisation; calls that share it must be ordered. */
+/* Bytes of device workspace for ix_kv8_attn_shared (partial results of the rows, and of what workgroups share), or 0 for an
+ * invalid request. It does for every batch of the same cache and h_q with no more tokens in all, no larger max_q and no more
+ * groups, of any n_seq. It needs no initialisation; calls that share it must be ordered. */
 size_t ix_kv8_attn_shared_workspace_size(const ix_kv8* cache, int n_seq, int total_T, int max_q, int n_groups, int h_q);
 
 /* ix_kv8_attn (without window and sinks) of a batch whose sequences have their first tokens in common, which are read once for
  * all of a group's rows: samples of one prompt, requests behind one system prompt.
  *   groups      [n_groups+1] int32 device, non-decreasing: group g is sequences groups[g] .. groups[g+1] - 1
- *   shared_len  [n_groups] int32 device: their first shared_len[g] tokens (any number) are the same, and none of them is new:
- *               shared_len[g] <= kv_len - q for each of them. 0: none
- * The shared tokens are read from the pages of the group's first sequence, those behind them from each sequence's own; so the
- * table's entries for whole pages of shared tokens need to stand for the first sequence alone, and where the shared tokens end
- * inside a page each sequence has a page of its own for the others. Sequences of no group share nothing, and with n_groups 0
- * (groups and shared_len may be NULL) the call is ix_kv8_attn. Everything else as there; the lengths are read on the device
- * and may change between a graph's replays. */
+ *   shared_len  [n_groups] int32 device: their first shared_len[g] tokens (any number; 0: none) are the same, and none of them
+ *               is new: shared_len[g] <= kv_len - q for each of them
+ * Every sequence's table names its shared pages too, the same ones or copies: which of a group's tables a shared token is read
+ * through is not said. Sequences of no group share nothing, and with n_groups 0 (groups and shared_len may be NULL) the call
+ * is ix_kv8_attn. Everything else as there; the lengths are read on the device and may change between a graph's replays. */
 hipError_t ix_kv8_attn_shared(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens,
                               const int32_t* kv_len, const int32_t* table, int width, int n_groups, const int32_t* groups,
                               const int32_t* shared_len, const ix_rows* q, int h_q, float scale, const ix_rows* gate, uint16_t* o,

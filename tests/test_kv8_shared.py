@@ -64,13 +64,11 @@ class Shared(Problem):
         assert given == list(range(given[0], given[0] + len(given))) if given else True
         self.shared = [groups[i][0] for i in given]
         self.groups = [ends[i] for i in given] + [ends[given[-1] + 1]] if given else []
-        self.given = self.tables.copy()
         ref = self.p.ref
         for n, a, b in zip(self.shared, self.groups, self.groups[1:]):
             whole = n // page
             for i in range(a + 1, b):
                 self.tables[i, :whole] = self.tables[a, :whole]
-                self.given[i, :whole] = [-1, 1 << 30, 0][i % 3]            # not read
                 if n % page and self.tables[a, whole] >= 0:
                     for x in "kv":
                         ref.codes[x][self.tables[i, whole], :, :n % page] = ref.codes[x][self.tables[a, whole], :, :n % page]
@@ -82,7 +80,7 @@ class Shared(Problem):
         q = bf(self.q_bits) if q is None else q
         o = torch.full((max(self.T, 1), self.h * self.G, self.d), float("nan"), dtype=torch.bfloat16, device="cuda")
         a = (self.p.cache, len(self.q_len), self.T, max_q or max(max(self.q_len), 1), ints(cumulative(self.q_len)), ints(self.kv_len),
-             ints(self.given), self.given.shape[1])
+             ints(self.tables), self.tables.shape[1])
         n = bx.ix_kv8_attn_shared_workspace_size(self.p.cache, *a[1:4], len(self.shared), self.h * self.G)
         ws = torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")       # NaN, wherever it is read unwritten
         assert bx.ix_kv8_attn_shared(*a, len(self.shared), ints(self.groups) if self.groups else None, ints(self.shared) if self.groups else None, q,
@@ -173,11 +171,10 @@ def test_lost_pages():
         p = Shared([group(64, (1, 1), (1, 20), (2, 40))])
         for i in range(3):
             p.tables[i, lost] = -1
-        p.given[0, lost] = -1
         p.both()
     p = Shared([group(64, (1, 1), (1, 20), (2, 16))])
-    p.given[2, 4:] = p.tables[2, 4:] = p.p.ref.n_pages + 5
-    p.given[0, :4] = p.tables[:, :4] = -1
+    p.tables[2, 4:] = p.p.ref.n_pages + 5
+    p.tables[:, :4] = -1
     got = p.both()
     assert np.all(got[2:] == 0)                                 # of zeros, not of what the workspace held
 
@@ -201,9 +198,9 @@ def test_shared_tokens_that_are_new():
 @pytest.mark.parametrize("scales", [(1e-30, 1.0), (1.0, 1e-30), (1e30, 1e-6), (0.0, 1.0), (1.0, 0.0)])
 def test_scales_apart(scales):
     """Pages of shared and own tokens whose value scales lie far apart."""
-    p = Shared([group(48, (1, 1), (1, 32), (3, 40))], v_std=1.0)
+    p = Shared([group(128, (1, 1), (1, 32), (3, 40))], v_std=1.0)
     ref = p.p.ref
-    for x, at in zip(scales, (p.tables[0, :3], p.tables[:, 3:6])):
+    for x, at in zip(scales, (p.tables[0, :8], p.tables[:, 8:11])):
         at = at[at >= 0]
         ref.scale["v"][at] = np.float32(x) * ref.scale["v"][at] / np.float32(0.025)
     p.both()
@@ -224,8 +221,8 @@ def test_offsets_behind_the_first_row():
         n = bx.ix_kv8_attn_shared_workspace_size(p.p.cache, 3, T, max_q, 1, p.h * p.G)
         ws = torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")
         o.fill_(7.0)
-        assert bx.ix_kv8_attn_shared(p.p.cache, 3, T, max_q, ints(before + np.array(cumulative(p.q_len))), ints(p.kv_len), ints(p.given),
-                                     p.given.shape[1], 1, ints(p.groups), ints(p.shared), q, p.h * p.G, p.scale, None, o, ws, n) == 0
+        assert bx.ix_kv8_attn_shared(p.p.cache, 3, T, max_q, ints(before + np.array(cumulative(p.q_len))), ints(p.kv_len), ints(p.tables),
+                                     p.tables.shape[1], 1, ints(p.groups), ints(p.shared), q, p.h * p.G, p.scale, None, o, ws, n) == 0
         assert bool((o[:before] == 7).all()) and bool((o[before + p.T:] == 7).all())
         p.check(o[before:before + p.T].float().cpu().numpy())
 
@@ -239,7 +236,7 @@ def test_in_place_and_slices():
     wide[:, 3:] = bf(p.q_bits).view(p.T, -1)
     want = p.run()
     assert np.array_equal(p.run(q=wide[:, 3:]), want)
-    a = (p.p.cache, 3, p.T, 4, ints(cumulative(p.q_len)), ints(p.kv_len), ints(p.given), p.given.shape[1], 1, ints(p.groups), ints(p.shared))
+    a = (p.p.cache, 3, p.T, 4, ints(cumulative(p.q_len)), ints(p.kv_len), ints(p.tables), p.tables.shape[1], 1, ints(p.groups), ints(p.shared))
     n = bx.ix_kv8_attn_shared_workspace_size(p.p.cache, 3, p.T, 4, 1, p.h * p.G)
     ws = torch.empty(n, dtype=torch.uint8, device="cuda")
     q = bf(p.q_bits)
