@@ -42,8 +42,9 @@ struct AttnArgs {
     struct OwnCut* cuts;      // [T h_q / h_kv][h_kv] by a segment's first row
 };
 
-// Which tokens split_kernel and block_kernel take of a sequence: all, or those behind the shared ones, and leave partial results.
-enum Tokens { kAll, kOwn };
+// Which tokens a kernel takes: of a sequence all, or those behind the shared ones; or of a group those that its sequences share, all
+// of its rows together. The latter two leave partial results.
+enum Tokens { kAll, kOwn, kShared };
 struct SeqPlan {
     int from;                 // its first own token; 0: it shares none
     int block, s0, parts;     // its group's first block of rows, first row, and the parts in which each block is taken
@@ -195,6 +196,19 @@ __device__ __forceinline__ long long lane_of(long long v, int l) {
     return (long long)(((unsigned long long)hi << 32) | lo);
 }
 
+// The largest of all lanes' v.
+template <int Ctrl, int RowMask>
+__device__ __forceinline__ int dpp_max(int v) {
+    return max(v, __builtin_amdgcn_update_dpp(v, v, Ctrl, RowMask, 0xF, false));
+}
+__device__ __forceinline__ int wave_max_int(int v) {
+    v = dpp_max<0x111, 0xF>(v);
+    v = dpp_max<0x112, 0xF>(v);
+    v = dpp_max<0x114, 0xF>(v);
+    v = dpp_max<0x118, 0xF>(v);
+    v = dpp_max<0x142, 0xA>(v);
+    return lane_of(dpp_max<0x143, 0xC>(v), kWave - 1);
+}
 // The lowest n bits, of a n that may lie anywhere.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
@@ -273,6 +287,134 @@ __device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d
     store_out(A, t, h, d, v, load_gate(A, t, h, d));
 }
 
+constexpr int kGrain = 64;            // shared tokens are taken in whole 64s; what is left over is each sequence's own
+
+// A group's rows, and the tokens that are taken together.
+struct Group {
+    int s0, rows, kv;
+};
+__device__ __forceinline__ int group_first(const AttnArgs& A, int g) { return min(max(A.groups[g], 0), A.a.n_seq); }
+__device__ __forceinline__ Group group_at(const AttnArgs& A, int g) {
+    Group out{0, 0, 0};
+    if (g >= A.n_groups) return out;
+    const int first = group_first(A, g), last = group_first(A, g + 1), n = A.shared[g];
+    out.s0 = A.a.start(first);
+    const int tokens = A.a.start(last) - out.s0;
+    if (tokens > 0 && last - first > 1 && (long long)tokens * A.G <= 1 << 30) {
+        out.rows = tokens * A.G;
+        out.kv = (int)min((long long)max(n, 0), (long long)A.a.width << A.c.page_log) / kGrain * kGrain;
+    }
+    if (out.kv == 0) out.rows = 0;
+    return out;
+}
+
+// The blocks of kRows rows of all groups and heads are taken in parts of about as many tiles each, so that there are at most
+// a few items for each workgroup: group g has parts_of(kv) for each of its blocks, and item
+// ((blocks and parts of the groups before it) + block * parts + part) * h_kv + head.
+template <int kRows, int kTok>
+struct Cuts {
+    int chunk;                // tiles
+    static __device__ __forceinline__ int blocks(const Group& g) { return (g.rows + kRows - 1) / kRows; }
+    __device__ __forceinline__ int parts(const Group& g) const { return g.rows ? (g.kv / kTok + chunk - 1) / chunk : 0; }
+};
+// `least` tiles a part at least, `start` in the time of beginning one and joining it. The items are fewer than A.n_items. Up to 64
+// groups lane p - 1 knows the time of the longest group's tiles in p parts, beyond that the room for items is filled.
+template <int kRows, int kTok>
+__device__ __forceinline__ Cuts<kRows, kTok> cuts_of(const AttnArgs& A, int n_wg, int least, float start, int lane) {
+    typedef Cuts<kRows, kTok> C;
+    C out;
+    long long tiles = 0, blocks = 0;
+    int most = 0;
+    Group g{};
+    for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
+        g = group_at(A, g0 + lane);
+        tiles += (long long)C::blocks(g) * (g.kv / kTok);
+        blocks += C::blocks(g);
+        most = max(most, g.kv / kTok);
+    }
+    tiles = lane_of(wave_scan_int(tiles), kWave - 1) * A.c.h_kv;
+    blocks = lane_of(wave_scan_int(blocks), kWave - 1) * A.c.h_kv;
+    most = wave_max_int(most);
+    const int room = A.n_items - 1 - (int)blocks;             // parts beyond one a block
+    if (A.n_groups > kWave || room < n_wg / 8) {
+        out.chunk = room < n_wg / 8 ? max(most, 1) : (int)min(max((tiles + room - 1) / room, (long long)least), 0x7fffffffll);
+        return out;
+    }
+    const int chunk = max((most + lane) / (lane + 1), least), t = g.kv / kTok;
+    const float inv = 1.0f / (float)chunk;
+    int items = 0;                                            // at most 64 a block, of fewer than A.n_items
+    for (int x = 0; x < A.n_groups; ++x) {
+        const int tx = lane_of(t, x), full = (int)((float)tx * inv);      // or one less or more: at most 64
+        items += lane_of(C::blocks(g), x) * (full + (tx > full * chunk));
+    }
+    items *= A.c.h_kv;
+    const float cost = items < A.n_items ? (float)((items + n_wg - 1) / n_wg) * ((float)chunk + start) : __builtin_inff();
+    const int best = -wave_max_int(-__float_as_int(cost));    // numbers >= 0 are in the order of their bits
+    out.chunk = lane_of(chunk, __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(__float_as_int(cost) == best))));
+    return out;
+}
+
+// Partial results of the items: sums [item][kRows][D], then (m, lse) [item][kRows][2].
+template <int kRows, int D>
+struct ItemParts {
+    float *o, *ml;
+    __device__ __forceinline__ explicit ItemParts(const AttnArgs& A) : o(A.item_part), ml(A.item_part + (size_t)A.n_items * kRows * D) {}
+};
+
+// The item of a workgroup, found by every wave for itself.
+template <int kRows, int kTok>
+struct Item {
+    Group g;
+    int group, e, rb, t0, t1;             // its group, head, block of rows, and tiles t0 .. t1 - 1 (one at least)
+};
+template <int kRows, int kTok>
+__device__ __forceinline__ bool item_at(const AttnArgs& A, const Cuts<kRows, kTok>& cuts, int item, int lane, Item<kRows, kTok>* out) {
+    out->e = item % A.c.h_kv;
+    int left = item / A.c.h_kv;
+    for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
+        const Group x = group_at(A, g0 + lane);
+        const int p = cuts.parts(x), count = cuts.blocks(x) * p, incl = wave_scan_int(count);
+        const unsigned long long hit = __ballot(incl > left);
+        if (hit) {
+            const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
+            const int parts = lane_of(p, l), in = left - lane_of(incl - count, l), part = in % parts;
+            out->group = g0 + l;
+            out->g = Group{lane_of(x.s0, l), lane_of(x.rows, l), lane_of(x.kv, l)};
+            out->rb = in / parts;
+            const int all = out->g.kv / kTok;
+            out->t0 = (int)((long long)all * part / parts);
+            out->t1 = (int)((long long)all * (part + 1) / parts);
+            return true;
+        }
+        left -= lane_of(incl, kWave - 1);
+    }
+    return false;
+}
+
+// What the other launches ask of a sequence's group, by the launch's last workgroup, which has no item.
+template <int kRows, int kTok>
+__device__ __forceinline__ void write_plan(const AttnArgs& A, const Cuts<kRows, kTok>& cuts, int tid, int threads) {
+    const int lane = tid & (kWave - 1);
+    SeqPlan* plan = A.seq;
+    for (int b = tid; b < A.a.n_seq; b += threads) plan[b] = SeqPlan{0, 0, 0, 0};
+    __syncthreads();
+    if (tid >= kWave) return;
+    int base = 0;
+    for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
+        const Group g = group_at(A, g0 + lane);
+        const int items = cuts.blocks(g) * cuts.parts(g), incl = wave_scan_int(items);
+        const int first = g.rows ? group_first(A, g0 + lane) : 0, last = g.rows ? group_first(A, g0 + lane + 1) : 0;
+        unsigned long long todo = __ballot(g.rows > 0);
+        while (todo) {                                        // all lanes for one group's sequences
+            const int l = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const SeqPlan s{lane_of(g.kv, l), base + lane_of(incl - items, l), lane_of(g.s0, l), lane_of(cuts.parts(g), l)};
+            for (int b = lane_of(first, l) + lane; b < lane_of(last, l); b += kWave) plan[b] = s;
+        }
+        base += lane_of(incl, kWave - 1);
+    }
+}
+
 constexpr int kSplitRows = 16;        // (token, head) rows of a segment of split_kernel
 // The workgroups and ways of a batch (kv8_attn.hip).
 struct Plan {
@@ -283,8 +425,10 @@ struct Plan {
 };
 Plan attn_plan(int d, int h_kv, int G, int T, int max_q, hipStream_t s);
 size_t attn_bytes(int d, const Plan& p);
-// The partial results of all rows over the sequences' own tokens.
+// The partial results of all rows over the sequences' own tokens, and of the groups' rows over the shared ones in blocks.
 hipError_t launch_own(AttnArgs& A, const Plan& p, hipStream_t s);
+hipError_t launch_shared_blocks(AttnArgs& A, int n_wg, hipStream_t s);
+constexpr int kBlockRows = 128;       // rows of a block of block_kernel
 // What the calls check alike: the batch (a call without tokens needs no more), and its operands.
 bool make_attn(const ix_kv8* cache, int n_seq, int T, int max_q, const int32_t* cu, const int32_t* kv_len, const int32_t* table, int width,
                int h_q, float scale, AttnArgs* A);

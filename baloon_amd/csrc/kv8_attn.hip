@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg
 // instructions issued in 41% and LDS in 36%: the waves of a workgroup pass through products and exponentials together.
 // Half of them half a tile behind, with two barriers a tile, took 236 us, the next tile's scores between a tile's
 // exponentials and its second product 204 to 212.
-constexpr int kBlockThreads = 512, kBlockTok = 64, kBlockRows = 128;
+constexpr int kBlockThreads = 512, kBlockTok = 64;
 
 // LDS of block_kernel, two buffers of each: keys [64 tokens][D], values [D][64 tokens] fp16, and of each 16
 // tokens ks and log2 vs.
@@ -538,19 +538,6 @@ struct BlockParts {
         return (size_t)2 * slots * kBlockRows * (D + 2) * sizeof(float) + (size_t)slots * sizeof(BlockCut);
     }
 };
-// The largest of all lanes' v.
-template <int Ctrl, int RowMask>
-__device__ __forceinline__ int dpp_max(int v) {
-    return max(v, __builtin_amdgcn_update_dpp(v, v, Ctrl, RowMask, 0xF, false));
-}
-__device__ __forceinline__ int wave_max_int(int v) {
-    v = dpp_max<0x111, 0xF>(v);
-    v = dpp_max<0x112, 0xF>(v);
-    v = dpp_max<0x114, 0xF>(v);
-    v = dpp_max<0x118, 0xF>(v);
-    v = dpp_max<0x142, 0xA>(v);
-    return lane_of(dpp_max<0x143, 0xC>(v), kWave - 1);
-}
 // The blocks of a sequence.
 __device__ __forceinline__ int blocks_of(const AttnArgs& A, int b) {
     if (b >= A.a.n_seq) return 0;
@@ -599,9 +586,16 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
 
     // Block j of the grid, from the last: of the causal blocks the longest start first. Sequence b owns the
     // blocks from cu[b] G / 128 + b on; consecutive workgroups, which different XCDs take, are different heads.
-    const int block = kCut ? (int)blockIdx.x : A.first + (int)blockIdx.x, e = block % A.c.h_kv;
+    const int block = kCut ? (int)blockIdx.x : A.first + (int)blockIdx.x;
+    int e = block % A.c.h_kv;
     int b, rb, parts = 1, part = 0;
-    if constexpr (kCut) {
+    [[maybe_unused]] Item<kBlockRows, kBlockTok> it;
+    if constexpr (P == kShared) {
+        const auto cuts = cuts_of<kBlockRows, kBlockTok>(A, A.slots, kLeastPart, kPartCost<D>, lane);
+        if (block == A.n_items - 1) write_plan(A, cuts, tid, kBlockThreads);
+        if (!item_at(A, cuts, block, lane, &it)) return;
+        e = it.e, rb = it.rb, b = group_first(A, it.group);
+    } else if constexpr (kCut) {
         const Blocks all = all_blocks<D, P>(A, lane);
         if ((int)blockIdx.x >= all.n * all.parts) return;
         const int i = blockIdx.x / A.c.h_kv;
@@ -625,9 +619,11 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         b = wave_search(A.a.n_seq, j, lane, key);
         rb = j - key(b);
     }
-    const int s0 = A.a.start(b), q = A.a.start(b + 1) - s0, r0 = rb * kBlockRows, rows = max(q, 0) * A.G;
-    if (!kCut && (rows <= A.small || rb < 0 || r0 >= rows)) return;      // rb < 0: before the first sequence's rows
-    const int kv = max(A.a.kv_len[b], 0), first = kv - q, own = P == kOwn ? A.seq[b].from : 0;
+    const int s0 = P == kShared ? it.g.s0 : A.a.start(b), q = P == kShared ? 0 : A.a.start(b + 1) - s0, r0 = rb * kBlockRows;
+    const int rows = P == kShared ? it.g.rows : max(q, 0) * A.G;
+    if (P != kShared && !kCut && (rows <= A.small || rb < 0 || r0 >= rows)) return;      // rb < 0: before the first sequence's rows
+    const int kv = P == kShared ? it.g.kv : max(A.a.kv_len[b], 0), first = kv - q, own = P == kOwn ? A.seq[b].from : 0;
+    const auto place = [&](int qi) { return P == kShared ? kv - 1 : first + qi; };       // of new token qi
 
     // q of row n of the wave, channels 64 c + 16 g .. + 15
     const int w0 = r0 + 16 * w;
@@ -636,7 +632,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     float qc;
     {
         const int r = w0 + n, rc = min(r, rows - 1), qi = rc / A.G;
-        pos = r < rows ? first + qi : -1;
+        pos = r < rows ? place(qi) : -1;
         const uint16_t* qp = A.q + (long long)(s0 + qi) * A.q_stride + (size_t)(e * A.G + rc - qi * A.G) * D + 16 * g;
         u16x2 mb = {0, 0};
 #pragma unroll
@@ -655,17 +651,20 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     }
     // Of the wave's positions wave_first .. wave_last: tiles that start from full_lo to full_hi every row sees as a
     // whole, those below some_lo (the sinks aside) and above wave_last none does.
-    const int wave_first = first + min(w0, rows - 1) / A.G, wave_last = first + (min(w0 + 16, rows) - 1) / A.G;
+    const int wave_first = place(min(w0, rows - 1) / A.G), wave_last = place((min(w0 + 16, rows) - 1) / A.G);
     const int full_hi = wave_first - kBlockTok + 1, full_lo = P == kOwn ? own : A.window > 0 ? wave_last - A.window + 1 : 0;
     const int some_lo = P == kAll && A.window > 0 ? wave_first - A.window + 1 - kBlockTok + 1 : 0;
 
     // the block's tiles
-    const int block_first = first + r0 / A.G, block_last = first + (min(r0 + kBlockRows, rows) - 1) / A.G;
+    const int block_first = place(r0 / A.G), block_last = place((min(r0 + kBlockRows, rows) - 1) / A.G);
     const int lo = P == kOwn ? own / kBlockTok : A.window > 0 ? max(block_first - A.window + 1, 0) / kBlockTok : 0;
     const int ns = P == kAll && A.window > 0 ? min(A.sinks / kBlockTok + (A.sinks % kBlockTok != 0), lo) : 0;
     const int all = block_last < 0 ? 0 : max(ns + block_last / kBlockTok + 1 - lo, 0);
     int begin = 0, nt = all;                                  // this part's: tiles begin .. begin + nt - 1
-    if constexpr (kCut) {
+    if constexpr (P == kShared) {
+        begin = it.t0;
+        nt = it.t1 - it.t0;
+    } else if constexpr (kCut) {
         if (parts > 1) {
             const int i = blockIdx.x / A.c.h_kv / parts;
             parts = min(parts, max(all / kLeastPart, 1));
@@ -846,6 +845,16 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     int thread = tid;
     asm volatile("" : "+v"(thread));                          // the row is worked out again: it does not wait in registers
     const int r = w0 + (thread & 15), qi = r / A.G, head = e * A.G + r - qi * A.G, d0 = 4 * (thread >> 4 & 3);
+    if constexpr (P == kShared) {
+        const ItemParts<kBlockRows, D> to(A);
+        const size_t at = (size_t)block * kBlockRows + (r - r0);
+        if (r < rows) {
+            if (d0 == 0) *reinterpret_cast<float2*>(to.ml + 2 * at) = make_float2(m_ref, lse);
+#pragma unroll
+            for (int m = 0; m < kM; ++m) *reinterpret_cast<v4f*>(to.o + at * D + 16 * m + d0) = acc[m];
+        }
+        return;
+    }
     if (kCut && parts > 1) {
         const BlockParts<D> to(A.block_part, A.slots);
         const size_t at = (size_t)blockIdx.x * kBlockRows + (r - r0);
@@ -976,6 +985,14 @@ hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
 
 Plan attn_plan(int d, int h_kv, int G, int T, int max_q, hipStream_t s) { return plan_of(d, h_kv, G, T, max_q, s); }
 size_t attn_bytes(int d, const Plan& p) { return d == 64 ? attn_bytes<64>(p) : d == 128 ? attn_bytes<128>(p) : attn_bytes<256>(p); }
+hipError_t launch_shared_blocks(AttnArgs& A, int n_wg, hipStream_t s) {
+    A.slots = n_wg;
+    switch (A.c.d) {
+        case 64: return launch_blocks<64, false, kShared>(A, A.n_items, s);
+        case 128: return launch_blocks<128, false, kShared>(A, A.n_items, s);
+        default: return launch_blocks<256, false, kShared>(A, A.n_items, s);
+    }
+}
 hipError_t launch_own(AttnArgs& A, const Plan& p, hipStream_t s) { return launch_attn<kOwn>(A, p, s); }
 
 // The blocks of the batch are numbered in 31 bits.
