@@ -35,24 +35,22 @@ struct AttnArgs {
     // Of a batch with shared tokens (kv8_shared.hip):
     const int32_t *groups, *shared;   // sequences groups[g] .. groups[g + 1] - 1 have their first shared[g] tokens in common
     int n_groups;
-    struct SeqPlan* seq;      // [n_seq] written by shared_kernel
-    float* item_part;         // partial results of its items
-    int n_items;              // at most
-    float *row_o, *row_ml;    // partial results of rows, what their own tokens give: sums [T][h_q][d], (m, lse) [T][h_q][2] (see Joined)
-    struct OwnCut* cuts;      // [T h_q / h_kv][h_kv] by a segment's first row
+    struct SeqPlan* seq;      // [n_seq]
+    float *item_part, *shared_part;   // partial results of few_kernel's items and of block_kernel's over shared tokens
+    int n_items, n_shared;    // room for them
+    int few;                  // the groups' rows are few_kernel's
+    float *row_o, *row_ml;    // partial results of rows whose own tokens are block_kernel's: [T][h_q][d], (m, lse) [T][h_q][2]
 };
 
-// Which tokens a kernel takes: of a sequence all, or those behind the shared ones; or of a group those that its sequences share, all
-// of its rows together. The latter two leave partial results.
+// Which tokens block_kernel takes: of a sequence all, or those behind the shared ones; or of a group those that its sequences share,
+// all of its rows together. The latter two leave partial results.
 enum Tokens { kAll, kOwn, kShared };
+// What is where of a sequence: its first own token (0: it shares none), its first item over them and the parts of each of its
+// blocks of rows; its group's first item, first row and parts (0: none).
 struct SeqPlan {
-    int from;                 // its first own token; 0: it shares none
-    int block, s0, parts;     // its group's first block of rows, first row, and the parts in which each block is taken
-};
-// Where the parts of a segment of split_kernel are: in workgroups first .. last (slot of the first, 2 w for the others), or,
-// first < 0, in row_o as a whole.
-struct OwnCut {
-    int first, last, slot, unused;
+    int from, item, parts;
+    int shared_item, s0, shared_parts;
+    int unused[2];
 };
 
 // The kernel's argument (its only one) read from memory again where it is used next: keeping all of it in
@@ -308,112 +306,60 @@ __device__ __forceinline__ Group group_at(const AttnArgs& A, int g) {
     return out;
 }
 
-// The blocks of kRows rows of all groups and heads are taken in parts of about as many tiles each, so that there are at most
-// a few items for each workgroup: group g has parts_of(kv) for each of its blocks, and item
-// ((blocks and parts of the groups before it) + block * parts + part) * h_kv + head.
-template <int kRows, int kTok>
+// Many rows: the blocks of 128 rows of all groups and heads are taken in parts of about as many tiles each: group g has parts(g)
+// for each of its blocks, item ((blocks and parts of the groups before it) + block * parts + part) * h_kv + head.
+constexpr int kBlockRows = 128, kBlockTok = 64;
 struct Cuts {
     int chunk;                // tiles
-    static __device__ __forceinline__ int blocks(const Group& g) { return (g.rows + kRows - 1) / kRows; }
-    __device__ __forceinline__ int parts(const Group& g) const { return g.rows ? (g.kv / kTok + chunk - 1) / chunk : 0; }
+    static __device__ __forceinline__ int blocks(const Group& g) { return (g.rows + kBlockRows - 1) / kBlockRows; }
+    __device__ __forceinline__ int parts(const Group& g) const { return g.rows ? (g.kv / kBlockTok + chunk - 1) / chunk : 0; }
 };
-// `least` tiles a part at least, `start` in the time of beginning one and joining it. The items are fewer than A.n_items. Up to 64
-// groups lane p - 1 knows the time of the longest group's tiles in p parts, beyond that the room for items is filled.
-template <int kRows, int kTok>
-__device__ __forceinline__ Cuts<kRows, kTok> cuts_of(const AttnArgs& A, int n_wg, int least, float start, int lane) {
-    typedef Cuts<kRows, kTok> C;
-    C out;
+template <int D>
+constexpr float kPartCost = D == 256 ? 4.0f : 8.0f;           // tiles in the time of a part's start, its sums and their joining
+constexpr int kLeastPart = 4;         // tiles
+// The items are at most A.n_shared. Up to 64 groups lane p - 1 knows the time of the longest group's tiles in p parts, beyond
+// that the room for items is filled.
+template <int D>
+__device__ __forceinline__ Cuts cuts_of(const AttnArgs& A, int n_wg, int lane) {
+    Cuts out;
     long long tiles = 0, blocks = 0;
     int most = 0;
     Group g{};
     for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
         g = group_at(A, g0 + lane);
-        tiles += (long long)C::blocks(g) * (g.kv / kTok);
-        blocks += C::blocks(g);
-        most = max(most, g.kv / kTok);
+        tiles += (long long)Cuts::blocks(g) * (g.kv / kBlockTok);
+        blocks += Cuts::blocks(g);
+        most = max(most, g.kv / kBlockTok);
     }
     tiles = lane_of(wave_scan_int(tiles), kWave - 1) * A.c.h_kv;
     blocks = lane_of(wave_scan_int(blocks), kWave - 1) * A.c.h_kv;
     most = wave_max_int(most);
-    const int room = A.n_items - 1 - (int)blocks;             // parts beyond one a block
+    const int room = A.n_shared - (int)blocks;                // parts beyond one a block
     if (A.n_groups > kWave || room < n_wg / 8) {
-        out.chunk = room < n_wg / 8 ? max(most, 1) : (int)min(max((tiles + room - 1) / room, (long long)least), 0x7fffffffll);
+        out.chunk = room < n_wg / 8 ? max(most, 1) : (int)min(max((tiles + room - 1) / room, (long long)kLeastPart), 0x7fffffffll);
         return out;
     }
-    const int chunk = max((most + lane) / (lane + 1), least), t = g.kv / kTok;
+    const int chunk = max((most + lane) / (lane + 1), kLeastPart), t = g.kv / kBlockTok;
     const float inv = 1.0f / (float)chunk;
-    int items = 0;                                            // at most 64 a block, of fewer than A.n_items
+    int items = 0;                                            // at most 64 a block, of which there are at most A.n_shared
     for (int x = 0; x < A.n_groups; ++x) {
         const int tx = lane_of(t, x), full = (int)((float)tx * inv);      // or one less or more: at most 64
-        items += lane_of(C::blocks(g), x) * (full + (tx > full * chunk));
+        items += lane_of(Cuts::blocks(g), x) * (full + (tx > full * chunk));
     }
     items *= A.c.h_kv;
-    const float cost = items < A.n_items ? (float)((items + n_wg - 1) / n_wg) * ((float)chunk + start) : __builtin_inff();
+    const float cost = items <= A.n_shared ? (float)((items + n_wg - 1) / n_wg) * ((float)chunk + kPartCost<D>) : __builtin_inff();
     const int best = -wave_max_int(-__float_as_int(cost));    // numbers >= 0 are in the order of their bits
     out.chunk = lane_of(chunk, __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(__float_as_int(cost) == best))));
     return out;
 }
 
-// Partial results of the items: sums [item][kRows][D], then (m, lse) [item][kRows][2].
+// Partial results: sums [item][kRows][D], then (m, lse) [item][kRows][2].
 template <int kRows, int D>
 struct ItemParts {
     float *o, *ml;
-    __device__ __forceinline__ explicit ItemParts(const AttnArgs& A) : o(A.item_part), ml(A.item_part + (size_t)A.n_items * kRows * D) {}
+    __device__ __forceinline__ ItemParts(float* p, int n) : o(p), ml(p + (size_t)n * kRows * D) {}
+    static size_t bytes(long long n) { return (size_t)n * kRows * (D + 2) * sizeof(float); }
 };
-
-// The item of a workgroup, found by every wave for itself.
-template <int kRows, int kTok>
-struct Item {
-    Group g;
-    int group, e, rb, t0, t1;             // its group, head, block of rows, and tiles t0 .. t1 - 1 (one at least)
-};
-template <int kRows, int kTok>
-__device__ __forceinline__ bool item_at(const AttnArgs& A, const Cuts<kRows, kTok>& cuts, int item, int lane, Item<kRows, kTok>* out) {
-    out->e = item % A.c.h_kv;
-    int left = item / A.c.h_kv;
-    for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
-        const Group x = group_at(A, g0 + lane);
-        const int p = cuts.parts(x), count = cuts.blocks(x) * p, incl = wave_scan_int(count);
-        const unsigned long long hit = __ballot(incl > left);
-        if (hit) {
-            const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
-            const int parts = lane_of(p, l), in = left - lane_of(incl - count, l), part = in % parts;
-            out->group = g0 + l;
-            out->g = Group{lane_of(x.s0, l), lane_of(x.rows, l), lane_of(x.kv, l)};
-            out->rb = in / parts;
-            const int all = out->g.kv / kTok;
-            out->t0 = (int)((long long)all * part / parts);
-            out->t1 = (int)((long long)all * (part + 1) / parts);
-            return true;
-        }
-        left -= lane_of(incl, kWave - 1);
-    }
-    return false;
-}
-
-// What the other launches ask of a sequence's group, by the launch's last workgroup, which has no item.
-template <int kRows, int kTok>
-__device__ __forceinline__ void write_plan(const AttnArgs& A, const Cuts<kRows, kTok>& cuts, int tid, int threads) {
-    const int lane = tid & (kWave - 1);
-    SeqPlan* plan = A.seq;
-    for (int b = tid; b < A.a.n_seq; b += threads) plan[b] = SeqPlan{0, 0, 0, 0};
-    __syncthreads();
-    if (tid >= kWave) return;
-    int base = 0;
-    for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
-        const Group g = group_at(A, g0 + lane);
-        const int items = cuts.blocks(g) * cuts.parts(g), incl = wave_scan_int(items);
-        const int first = g.rows ? group_first(A, g0 + lane) : 0, last = g.rows ? group_first(A, g0 + lane + 1) : 0;
-        unsigned long long todo = __ballot(g.rows > 0);
-        while (todo) {                                        // all lanes for one group's sequences
-            const int l = __builtin_ctzll(todo);
-            todo &= todo - 1;
-            const SeqPlan s{lane_of(g.kv, l), base + lane_of(incl - items, l), lane_of(g.s0, l), lane_of(cuts.parts(g), l)};
-            for (int b = lane_of(first, l) + lane; b < lane_of(last, l); b += kWave) plan[b] = s;
-        }
-        base += lane_of(incl, kWave - 1);
-    }
-}
 
 constexpr int kSplitRows = 16;        // (token, head) rows of a segment of split_kernel
 // The workgroups and ways of a batch (kv8_attn.hip).
@@ -425,10 +371,11 @@ struct Plan {
 };
 Plan attn_plan(int d, int h_kv, int G, int T, int max_q, hipStream_t s);
 size_t attn_bytes(int d, const Plan& p);
-// The partial results of all rows over the sequences' own tokens, and of the groups' rows over the shared ones in blocks.
-hipError_t launch_own(AttnArgs& A, const Plan& p, hipStream_t s);
+// Sequences of more rows a kv head than this are block_kernel's.
+int attn_small(const AttnArgs& A, const Plan& p);
+// Their partial results over their own tokens, and those of all groups over the shared ones.
+hipError_t launch_own_blocks(AttnArgs& A, const Plan& p, hipStream_t s);
 hipError_t launch_shared_blocks(AttnArgs& A, int n_wg, hipStream_t s);
-constexpr int kBlockRows = 128;       // rows of a block of block_kernel
 // What the calls check alike: the batch (a call without tokens needs no more), and its operands.
 bool make_attn(const ix_kv8* cache, int n_seq, int T, int max_q, const int32_t* cu, const int32_t* kv_len, const int32_t* table, int width,
                int h_q, float scale, AttnArgs* A);

@@ -11,29 +11,27 @@ namespace {
 // What the rows of one sequence see together: `ns` tiles of sinks and those from `lo` on.
 struct Span {
     int s0, q, kv, first;     // rows s0 .. s0 + q - 1, at positions first ..
-    int from;                 // the first token of all (kOwn)
     int ns, lo, nt, nrb;      // nt tiles in all (1 where nothing is seen: zeros are written), nrb blocks of rows
     __device__ __forceinline__ int tile(int t) const { return t < ns ? t : lo + t - ns; }
 };
-template <int ROWS, int TOK, Tokens P>
-__device__ __forceinline__ Span span_of(const AttnArgs& A, int s0, int q, int kv, int from) {
+template <int ROWS, int TOK>
+__device__ __forceinline__ Span span_of(const AttnArgs& A, int s0, int q, int kv) {
     Span s;
-    s.from = from;
     s.s0 = s0;
     s.q = (long long)q * A.G <= A.small ? q : 0;
     s.kv = kv;
     s.first = s.kv - q;
-    s.lo = P == kOwn ? from / TOK : A.window > 0 ? max(s.first - A.window + 1, 0) / TOK : 0;
-    s.ns = P == kAll && A.window > 0 ? min(A.sinks / TOK + (A.sinks % TOK != 0), s.lo) : 0;
+    s.lo = A.window > 0 ? max(s.first - A.window + 1, 0) / TOK : 0;
+    s.ns = A.window > 0 ? min(A.sinks / TOK + (A.sinks % TOK != 0), s.lo) : 0;
     const int held = (int)min((long long)kv, (long long)A.a.width << A.c.page_log);      // what the table has places for
     s.nt = max(s.ns + max(held / TOK + (held % TOK != 0) - s.lo, 0), 1);
     s.nrb = (int)(((long long)s.q * A.G + ROWS - 1) / ROWS);
     return s;
 }
-template <int ROWS, int TOK, Tokens P>
+template <int ROWS, int TOK>
 __device__ __forceinline__ Span span_at(const AttnArgs& A, int b) {
     const int s0 = A.a.start(b);
-    return span_of<ROWS, TOK, P>(A, s0, max(A.a.start(b + 1) - s0, 0), max(A.a.kv_len[b], 0), P == kOwn ? A.seq[b].from : 0);
+    return span_of<ROWS, TOK>(A, s0, max(A.a.start(b + 1) - s0, 0), max(A.a.kv_len[b], 0));
 }
 
 // a / b for a >= 0: in 64 bits (below 2^50) through the correctly rounded division in double.
@@ -62,13 +60,13 @@ struct Share {
     int b, e, rb, v0;                 // where it begins: count v0 of a segment
     Span s;
 };
-template <int ROWS, int TOK, Tokens P, class Int>
+template <int ROWS, int TOK, class Int>
 __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int lane, Share* out) {
     const int n = A.a.n_seq, h_kv = A.c.h_kv;
     Span s{};
     const auto span = [&](int b0) {                          // of sequence b0 + lane; no rows behind the last
         s.nrb = 0;
-        if (b0 + lane < n) s = span_at<ROWS, TOK, P>(A, b0 + lane);
+        if (b0 + lane < n) s = span_at<ROWS, TOK>(A, b0 + lane);
     };
     Int tiles = 0, segments = 0;
 #pragma unroll 4
@@ -98,7 +96,7 @@ __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int
             const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
             const Int rel = cur - carry - lane_of((Int)(incl - v), l);
             out->b = b0 + l;
-            out->s = span_of<ROWS, TOK, P>(A, lane_of(s.s0, l), lane_of(s.q, l), lane_of(s.kv, l), P == kOwn ? lane_of(s.from, l) : 0);
+            out->s = span_of<ROWS, TOK>(A, lane_of(s.s0, l), lane_of(s.q, l), lane_of(s.kv, l));
             const int seg = __builtin_amdgcn_readfirstlane((int)quotient(rel, out->s.nt + start));
             out->v0 = __builtin_amdgcn_readfirstlane((int)(rel - (Int)seg * (out->s.nt + start)));
             out->e = quotient(seg, out->s.nrb);
@@ -108,9 +106,9 @@ __device__ __forceinline__ bool share_in(const AttnArgs& A, int n_wg, int w, int
         carry += lane_of(incl, kWave - 1);
     }
 }
-template <int ROWS, int TOK, Tokens P>
+template <int ROWS, int TOK>
 __device__ __forceinline__ bool share_of(const AttnArgs& A, int n_wg, int w, int lane, Share* out) {
-    return A.narrow ? share_in<ROWS, TOK, P, int>(A, n_wg, w, lane, out) : share_in<ROWS, TOK, P, long long>(A, n_wg, w, lane, out);
+    return A.narrow ? share_in<ROWS, TOK, int>(A, n_wg, w, lane, out) : share_in<ROWS, TOK, long long>(A, n_wg, w, lane, out);
 }
 
 // Partial results: workgroup w leaves that of the segment it starts in the middle of (or cuts at both
@@ -153,7 +151,7 @@ constexpr int kSplitTok = D == 256 ? 32 : 64;
 // reach, 64 over 1 to 8,192, 16 heads over 2 of 256, 252 MB in 54 and join_kernel's 6. Short contexts are bound by the way to
 // the first tile (lengths, pages, codes: about 5 us with the launch), by whole tiles for each of four waves, and by the
 // second launch: 48 windows of 1,028 tokens over 4 heads of 128, 51 MB, take 21.0 us where reading takes 8.2.
-template <int D, Tokens P>
+template <int D>
 __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     constexpr int kC = D / 64, kM = D / 16, kPitch = D + 4, kTok = kSplitTok<D>, kS = kTok / 16;
     typedef typename std::conditional<kS == 4, uint4, uint2>::type Codes;     // 4 S values of a channel
@@ -169,7 +167,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
     {
         const AttnArgs& Z = args_again();
         Share sh;
-        if (!share_of<kSplitRows, kTok, P>(Z, gridDim.x, blockIdx.x, lane, &sh)) {
+        if (!share_of<kSplitRows, kTok>(Z, gridDim.x, blockIdx.x, lane, &sh)) {
             if (tid == 0) Parts<kSplitRows, D>(Z.part, gridDim.x).cut[blockIdx.x].any = 0;
             return;
         }
@@ -273,9 +271,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
                     to.add(lo_ml[(k * kSplitRows + row) * 2], lo_ml[(k * kSplitRows + row) * 2 + 1],
                            *reinterpret_cast<const v4f*>(lo_o + (k * kSplitRows + row) * kPitch + d));
                 if (x_slot < 0) {
-                    const int token = (x_r0 + row) / Z.G, t = taken(o_s0) + token, h = taken(o_e) * Z.G + x_r0 + row - token * Z.G;
-                    if constexpr (P == kOwn) store_row_part(Z, t, h, d, to.o, to.m, to.log2_sum());
-                    else store_out(Z, t, h, d, outputs(to.o, to.log2_sum()));
+                    const int token = (x_r0 + row) / Z.G;
+                    store_out(Z, taken(o_s0) + token, taken(o_e) * Z.G + x_r0 + row - token * Z.G, d, outputs(to.o, to.log2_sum()));
                 } else {
                     *reinterpret_cast<v4f*>(parts.o + ((size_t)x_slot * kSplitRows + row) * D + d) = to.o;
                     if (d == 0) {
@@ -309,10 +306,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             lo_q[(2 * w + 1) * kWave + lane] = raw[1];
         }
         const int pos = r0 + n < rows ? s.first + (r0 + n) / Y.G : -1;
-        const int from = P == kOwn ? s.from : window > 0 ? pos - window + 1 : 0;     // the row sees from .. pos, and the sinks
+        const int from = window > 0 ? pos - window + 1 : 0;   // the row sees from .. pos, and the sinks
         // tiles that every row sees as a whole: those starting at full_lo .. full_hi
         const int full_hi = s.first + r0 / Y.G - kTok + 1;
-        const int full_lo = P == kOwn ? s.from : window > 0 ? s.first + (min(r0 + kSplitRows, rows) - 1) / Y.G - window + 1 : 0;
+        const int full_lo = window > 0 ? s.first + (min(r0 + kSplitRows, rows) - 1) / Y.G - window + 1 : 0;
         lds_barrier();
 #pragma unroll
         for (int m = 0; m < kM; ++m) acc[m] = v4f{0, 0, 0, 0};
@@ -329,9 +326,6 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             cut = Cut{x - before, x + (s.nt + start - (t1 + start) + per - 1) / per, before ? 2 * (x - before) + (v0 < before * per) : o_slot,
                       s.s0, e, r0, rows, 1};
         }
-        if constexpr (P == kOwn)
-            if (t0 == 0 && tid == 0)                          // its first tile is here
-                Y.cuts[((size_t)s.s0 * Y.G + r0) * h_kv + e] = t1 == s.nt ? OwnCut{-1, 0, 0, 0} : OwnCut{cut.first, cut.last, cut.slot, 0};
         const int n_left = parked(left - (s.nt + start - v0)), n_rb = parked(rb), n_b = parked(b), n_nrb = parked(s.nrb), n_start = parked(start);
 
         for (; t < t1; t += kSplitWaves) {
@@ -419,7 +413,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(AttnArgs A) {
             rb = 0;
             if (++e == Z.c.h_kv) {
                 e = 0;
-                do s = span_at<kSplitRows, kTok, P>(Z, ++b);     // left > 0: a sequence with rows follows
+                do s = span_at<kSplitRows, kTok>(Z, ++b);     // left > 0: a sequence with rows follows
                 while (s.nrb == 0);
             }
         }
@@ -493,7 +487,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnArgs A, int n_wg
 // instructions issued in 41% and LDS in 36%: the waves of a workgroup pass through products and exponentials together.
 // Half of them half a tile behind, with two barriers a tile, took 236 us, the next tile's scores between a tile's
 // exponentials and its second product 204 to 212.
-constexpr int kBlockThreads = 512, kBlockTok = 64;
+constexpr int kBlockThreads = 512;
 
 // LDS of block_kernel, two buffers of each: keys [64 tokens][D], values [D][64 tokens] fp16, and of each 16
 // tokens ks and log2 vs.
@@ -549,9 +543,6 @@ __device__ __forceinline__ int blocks_of(const AttnArgs& A, int b) {
 struct Blocks {
     int n, parts;
 };
-template <int D>
-constexpr float kPartCost = D == 256 ? 4.0f : 8.0f;           // tiles in the time of a part's start, its sums and their joining
-constexpr int kLeastPart = 4;         // tiles
 template <int D, Tokens P>
 __device__ __forceinline__ Blocks all_blocks(const AttnArgs& A, int lane) {
     int sum = 0, kv = 0;
@@ -574,6 +565,32 @@ __device__ __forceinline__ Blocks all_blocks(const AttnArgs& A, int lane) {
     return out;
 }
 
+// An item of kShared.
+struct Item {
+    Group g;
+    int group, rb, t0, t1;                // its group, block of rows, and tiles t0 .. t1 - 1 (one at least)
+};
+__device__ __forceinline__ bool item_at(const AttnArgs& A, const Cuts& cuts, int left, int lane, Item* out) {
+    for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
+        const Group x = group_at(A, g0 + lane);
+        const int p = cuts.parts(x), count = Cuts::blocks(x) * p, incl = wave_scan_int(count);
+        const unsigned long long hit = __ballot(incl > left);
+        if (hit) {
+            const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
+            const int parts = lane_of(p, l), in = left - lane_of(incl - count, l), part = in % parts;
+            out->group = g0 + l;
+            out->g = Group{lane_of(x.s0, l), lane_of(x.rows, l), lane_of(x.kv, l)};
+            out->rb = in / parts;
+            const int all = out->g.kv / kBlockTok;
+            out->t0 = (int)((long long)all * part / parts);
+            out->t1 = (int)((long long)all * (part + 1) / parts);
+            return true;
+        }
+        left -= lane_of(incl, kWave - 1);
+    }
+    return false;
+}
+
 template <int D, bool kCut, Tokens P>
 __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(AttnArgs A) {
     constexpr int kC = D / 64, kM = D / 16;
@@ -587,14 +604,12 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     // Block j of the grid, from the last: of the causal blocks the longest start first. Sequence b owns the
     // blocks from cu[b] G / 128 + b on; consecutive workgroups, which different XCDs take, are different heads.
     const int block = kCut ? (int)blockIdx.x : A.first + (int)blockIdx.x;
-    int e = block % A.c.h_kv;
+    const int e = block % A.c.h_kv;
     int b, rb, parts = 1, part = 0;
-    [[maybe_unused]] Item<kBlockRows, kBlockTok> it;
+    [[maybe_unused]] Item it;
     if constexpr (P == kShared) {
-        const auto cuts = cuts_of<kBlockRows, kBlockTok>(A, A.slots, kLeastPart, kPartCost<D>, lane);
-        if (block == A.n_items - 1) write_plan(A, cuts, tid, kBlockThreads);
-        if (!item_at(A, cuts, block, lane, &it)) return;
-        e = it.e, rb = it.rb, b = group_first(A, it.group);
+        if (!item_at(A, cuts_of<D>(A, A.slots, lane), block / A.c.h_kv, lane, &it)) return;
+        rb = it.rb, b = group_first(A, it.group);
     } else if constexpr (kCut) {
         const Blocks all = all_blocks<D, P>(A, lane);
         if ((int)blockIdx.x >= all.n * all.parts) return;
@@ -846,7 +861,7 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     asm volatile("" : "+v"(thread));                          // the row is worked out again: it does not wait in registers
     const int r = w0 + (thread & 15), qi = r / A.G, head = e * A.G + r - qi * A.G, d0 = 4 * (thread >> 4 & 3);
     if constexpr (P == kShared) {
-        const ItemParts<kBlockRows, D> to(A);
+        const ItemParts<kBlockRows, D> to(A.shared_part, A.n_shared);
         const size_t at = (size_t)block * kBlockRows + (r - r0);
         if (r < rows) {
             if (d0 == 0) *reinterpret_cast<float2*>(to.ml + 2 * at) = make_float2(m_ref, lse);
@@ -937,63 +952,63 @@ hipError_t launch_blocks(AttnArgs& A, long long n, hipStream_t s) {
     });
 }
 
+// With at most max_q new tokens in each other one, a sequence of the batch has at least these. Where that is more than
+// kSplitMost rows all are block_kernel's (also those of a batch whose offsets end before T), and it is the only launch.
+int small_of(const AttnArgs& A, const Plan& p) {
+    const long long shortest = A.a.T - (long long)(A.a.n_seq - 1) * p.max_q;
+    return p.block && shortest * A.G > kSplitMost ? 0 : p.block ? kSplitMost : 0x7fffffff;
+}
 template <int D, Tokens P>
+hipError_t launch_seq_blocks(AttnArgs& A, const Plan& p, hipStream_t s) {
+    if (!p.cut) return launch_blocks<D, false, P>(A, p.full + (long long)A.a.n_seq * A.c.h_kv, s);
+    // a sequence has at most one block that is not full, and more than kSplitMost rows
+    const long long most = A.small == 0 ? A.a.n_seq : std::min((long long)A.a.n_seq, (long long)A.a.T * A.G / kSplitMost);
+    const long long blocks = p.full + most * A.c.h_kv;
+    A.slots = p.slots;
+    A.items = 2 * p.slots;
+    A.block_part = A.part + split_bytes<D>(p) / sizeof(float);
+    const hipError_t e = launch_blocks<D, true, P>(A, std::max(blocks, (long long)A.items), s);
+    if (e == hipSuccess) hipLaunchKernelGGL((block_join_kernel<D, P>), dim3((unsigned)(2 * p.n_wg)), dim3(kJoinThreads), 0, s, A);
+    return e;
+}
+
+template <int D>
 hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
     const int n_wg = p.n_wg;
-    // With at most max_q new tokens in each other one, a sequence of the batch has at least these. Where that is more than
-    // kSplitMost rows all are block_kernel's (also those of a batch whose offsets end before T), and it is the only launch.
-    const long long shortest = A.a.T - (long long)(A.a.n_seq - 1) * p.max_q;
-    const bool only = p.block && shortest * A.G > kSplitMost;
-    A.small = only ? 0 : p.block ? kSplitMost : 0x7fffffff;
+    A.small = small_of(A, p);
     // tiles: at most those of a whole table for each block of rows, and n_wg - 1 and a workgroup's share more in sums
     const long long row_blocks = (long long)A.a.T * A.G / kSplitRows + A.a.n_seq;
     const long long tiles = ((long long)A.a.width << A.c.page_log) / kSplitTok<D> + 1;
     A.narrow = row_blocks < (1ll << 31) / tiles / A.c.h_kv / 2 - n_wg;
     if (p.block) {
-        hipError_t e;
-        if (p.cut) {
-            // a sequence has at most one block that is not full, and more than kSplitMost rows
-            const long long most = only ? A.a.n_seq : std::min((long long)A.a.n_seq, (long long)A.a.T * A.G / kSplitMost);
-            const long long blocks = p.full + most * A.c.h_kv;
-            A.slots = p.slots;
-            A.items = 2 * p.slots;
-            A.block_part = A.part + split_bytes<D>(p) / sizeof(float);
-            e = launch_blocks<D, true, P>(A, std::max(blocks, (long long)A.items), s);
-            if (e == hipSuccess) hipLaunchKernelGGL((block_join_kernel<D, P>), dim3((unsigned)(2 * n_wg)), dim3(kJoinThreads), 0, s, A);
-        } else {
-            e = launch_blocks<D, false, P>(A, p.full + (long long)A.a.n_seq * A.c.h_kv, s);
-        }
+        const hipError_t e = launch_seq_blocks<D, kAll>(A, p, s);
         if (e != hipSuccess) return e;
-        if (only) return hipGetLastError();
+        if (A.small == 0) return hipGetLastError();
     }
     const unsigned lds = kSplitWaves * kSplitRows * (D + 4 + 2 + 1) * sizeof(float) + D / 64 * 2 * kWave * sizeof(uint4);
-    hipLaunchKernelGGL((split_kernel<D, P>), dim3((unsigned)n_wg), dim3(kSplitThreads), lds, s, A);
-    if (P == kAll && n_wg > 1) hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)n_wg - 1), dim3(kJoinThreads), 0, s, A, n_wg);
+    hipLaunchKernelGGL((split_kernel<D>), dim3((unsigned)n_wg), dim3(kSplitThreads), lds, s, A);
+    if (n_wg > 1) hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)n_wg - 1), dim3(kJoinThreads), 0, s, A, n_wg);
     return hipGetLastError();
-}
-
-template <Tokens P>
-hipError_t launch_attn(AttnArgs& A, const Plan& p, hipStream_t s) {
-    switch (A.c.d) {
-        case 64: return launch_attn<64, P>(A, p, s);
-        case 128: return launch_attn<128, P>(A, p, s);
-        default: return launch_attn<256, P>(A, p, s);
-    }
 }
 
 }  // namespace
 
 Plan attn_plan(int d, int h_kv, int G, int T, int max_q, hipStream_t s) { return plan_of(d, h_kv, G, T, max_q, s); }
 size_t attn_bytes(int d, const Plan& p) { return d == 64 ? attn_bytes<64>(p) : d == 128 ? attn_bytes<128>(p) : attn_bytes<256>(p); }
+int attn_small(const AttnArgs& A, const Plan& p) { return small_of(A, p); }
+hipError_t launch_own_blocks(AttnArgs& A, const Plan& p, hipStream_t s) {
+    const hipError_t e = A.c.d == 64 ? launch_seq_blocks<64, kOwn>(A, p, s)
+                         : A.c.d == 128 ? launch_seq_blocks<128, kOwn>(A, p, s) : launch_seq_blocks<256, kOwn>(A, p, s);
+    return e == hipSuccess ? hipGetLastError() : e;
+}
 hipError_t launch_shared_blocks(AttnArgs& A, int n_wg, hipStream_t s) {
     A.slots = n_wg;
     switch (A.c.d) {
-        case 64: return launch_blocks<64, false, kShared>(A, A.n_items, s);
-        case 128: return launch_blocks<128, false, kShared>(A, A.n_items, s);
-        default: return launch_blocks<256, false, kShared>(A, A.n_items, s);
+        case 64: return launch_blocks<64, false, kShared>(A, A.n_shared, s);
+        case 128: return launch_blocks<128, false, kShared>(A, A.n_shared, s);
+        default: return launch_blocks<256, false, kShared>(A, A.n_shared, s);
     }
 }
-hipError_t launch_own(AttnArgs& A, const Plan& p, hipStream_t s) { return launch_attn<kOwn>(A, p, s); }
 
 // The blocks of the batch are numbered in 31 bits.
 bool attn_shape_ok(const Kv8& c, int n_seq, int T, int max_q, int h_q) {
@@ -1048,7 +1063,11 @@ hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, c
     if (!make_operands(q, gate, o, workspace, workspace_bytes, attn_bytes(A.c.d, p), &A)) return hipErrorInvalidValue;
     A.window = window;
     A.sinks = sinks;
-    return launch_attn<kAll>(A, p, s);
+    switch (A.c.d) {
+        case 64: return launch_attn<64>(A, p, s);
+        case 128: return launch_attn<128>(A, p, s);
+        default: return launch_attn<256>(A, p, s);
+    }
 }
 
 }  // extern "C"

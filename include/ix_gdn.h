@@ -468,8 +468,8 @@ hipError_t ix_kv8_attn(const ix_kv8* cache, int n_seq, int total_T, int max_q, c
                        size_t workspace_bytes, hipStream_t s IX_GDN_DEFAULT_STREAM);
 
 /* Bytes of device workspace for ix_kv8_attn_shared (partial results of the rows, and of what workgroups share), or 0 for an
- * invalid request. It does for every batch of the same cache and h_q with no more tokens in all, no larger max_q and no more
- * groups, of any n_seq. It needs no initialisation; calls that share it must be ordered. */
+ * invalid request. It does for every batch of the same cache and h_q with no more sequences, tokens in all and groups, and no
+ * larger max_q. It needs no initialisation; calls that share it must be ordered. */
 size_t ix_kv8_attn_shared_workspace_size(const ix_kv8* cache, int n_seq, int total_T, int max_q, int n_groups, int h_q);
 
 /* ix_kv8_attn (without window and sinks) of a batch whose sequences have their first tokens in common, which are read once for
