@@ -36,6 +36,7 @@ struct AttnArgs {
     const int32_t *groups, *shared;   // sequences groups[g] .. groups[g + 1] - 1 have their first shared[g] tokens in common
     int n_groups;
     struct SeqPlan* seq;      // [n_seq]
+    struct SharedItem* shared_items;  // of block_kernel, each for all heads
     float *item_part, *shared_part;   // partial results of few_kernel's items and of block_kernel's over shared tokens
     int n_items, n_shared;    // room for them
     int few;                  // the groups' rows are few_kernel's
@@ -47,6 +48,11 @@ struct AttnArgs {
 enum Tokens { kAll, kOwn, kShared };
 // What is where of a sequence: its first own token (0: it shares none), its first item over them and the parts of each of its
 // blocks of rows; its group's first item, first row and parts (0: none).
+struct SharedItem {
+    int s0, rows, r0, row;    // the group's first row of tokens and rows a head, the item's first, and the table's row (-1: there is no item)
+    int t0, t1;               // tiles t0 .. t1 - 1 (one at least)
+    int kv, unused;
+};
 struct SeqPlan {
     int from, item, parts;
     int shared_item, s0, shared_parts;
@@ -285,74 +291,11 @@ __device__ __forceinline__ void store_out(const AttnArgs& A, int t, int h, int d
     store_out(A, t, h, d, v, load_gate(A, t, h, d));
 }
 
-constexpr int kGrain = 64;            // shared tokens are taken in whole 64s; what is left over is each sequence's own
-
-// A group's rows, and the tokens that are taken together.
-struct Group {
-    int s0, rows, kv;
-};
-__device__ __forceinline__ int group_first(const AttnArgs& A, int g) { return min(max(A.groups[g], 0), A.a.n_seq); }
-__device__ __forceinline__ Group group_at(const AttnArgs& A, int g) {
-    Group out{0, 0, 0};
-    if (g >= A.n_groups) return out;
-    const int first = group_first(A, g), last = group_first(A, g + 1), n = A.shared[g];
-    out.s0 = A.a.start(first);
-    const int tokens = A.a.start(last) - out.s0;
-    if (tokens > 0 && last - first > 1 && (long long)tokens * A.G <= 1 << 30) {
-        out.rows = tokens * A.G;
-        out.kv = (int)min((long long)max(n, 0), (long long)A.a.width << A.c.page_log) / kGrain * kGrain;
-    }
-    if (out.kv == 0) out.rows = 0;
-    return out;
-}
-
-// Many rows: the blocks of 128 rows of all groups and heads are taken in parts of about as many tiles each: group g has parts(g)
-// for each of its blocks, item ((blocks and parts of the groups before it) + block * parts + part) * h_kv + head.
-constexpr int kBlockRows = 128, kBlockTok = 64;
-struct Cuts {
-    int chunk;                // tiles
-    static __device__ __forceinline__ int blocks(const Group& g) { return (g.rows + kBlockRows - 1) / kBlockRows; }
-    __device__ __forceinline__ int parts(const Group& g) const { return g.rows ? (g.kv / kBlockTok + chunk - 1) / chunk : 0; }
-};
+constexpr int kSplitRows = 16;        // (token, head) rows of a segment of split_kernel and of an item of few_kernel
+constexpr int kBlockRows = 128, kBlockTok = 64;               // rows of a block of block_kernel, tokens of its tiles
 template <int D>
 constexpr float kPartCost = D == 256 ? 4.0f : 8.0f;           // tiles in the time of a part's start, its sums and their joining
 constexpr int kLeastPart = 4;         // tiles
-// The items are at most A.n_shared. Up to 64 groups lane p - 1 knows the time of the longest group's tiles in p parts, beyond
-// that the room for items is filled.
-template <int D>
-__device__ __forceinline__ Cuts cuts_of(const AttnArgs& A, int n_wg, int lane) {
-    Cuts out;
-    long long tiles = 0, blocks = 0;
-    int most = 0;
-    Group g{};
-    for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
-        g = group_at(A, g0 + lane);
-        tiles += (long long)Cuts::blocks(g) * (g.kv / kBlockTok);
-        blocks += Cuts::blocks(g);
-        most = max(most, g.kv / kBlockTok);
-    }
-    tiles = lane_of(wave_scan_int(tiles), kWave - 1) * A.c.h_kv;
-    blocks = lane_of(wave_scan_int(blocks), kWave - 1) * A.c.h_kv;
-    most = wave_max_int(most);
-    const int room = A.n_shared - (int)blocks;                // parts beyond one a block
-    if (A.n_groups > kWave || room < n_wg / 8) {
-        out.chunk = room < n_wg / 8 ? max(most, 1) : (int)min(max((tiles + room - 1) / room, (long long)kLeastPart), 0x7fffffffll);
-        return out;
-    }
-    const int chunk = max((most + lane) / (lane + 1), kLeastPart), t = g.kv / kBlockTok;
-    const float inv = 1.0f / (float)chunk;
-    int items = 0;                                            // at most 64 a block, of which there are at most A.n_shared
-    for (int x = 0; x < A.n_groups; ++x) {
-        const int tx = lane_of(t, x), full = (int)((float)tx * inv);      // or one less or more: at most 64
-        items += lane_of(Cuts::blocks(g), x) * (full + (tx > full * chunk));
-    }
-    items *= A.c.h_kv;
-    const float cost = items <= A.n_shared ? (float)((items + n_wg - 1) / n_wg) * ((float)chunk + kPartCost<D>) : __builtin_inff();
-    const int best = -wave_max_int(-__float_as_int(cost));    // numbers >= 0 are in the order of their bits
-    out.chunk = lane_of(chunk, __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(__float_as_int(cost) == best))));
-    return out;
-}
-
 // Partial results: sums [item][kRows][D], then (m, lse) [item][kRows][2].
 template <int kRows, int D>
 struct ItemParts {
@@ -361,7 +304,6 @@ struct ItemParts {
     static size_t bytes(long long n) { return (size_t)n * kRows * (D + 2) * sizeof(float); }
 };
 
-constexpr int kSplitRows = 16;        // (token, head) rows of a segment of split_kernel
 // The workgroups and ways of a batch (kv8_attn.hip).
 struct Plan {
     bool block, cut;          // block_kernel for sequences of more than kSplitMost rows; in parts

@@ -565,32 +565,6 @@ __device__ __forceinline__ Blocks all_blocks(const AttnArgs& A, int lane) {
     return out;
 }
 
-// An item of kShared.
-struct Item {
-    Group g;
-    int group, rb, t0, t1;                // its group, block of rows, and tiles t0 .. t1 - 1 (one at least)
-};
-__device__ __forceinline__ bool item_at(const AttnArgs& A, const Cuts& cuts, int left, int lane, Item* out) {
-    for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
-        const Group x = group_at(A, g0 + lane);
-        const int p = cuts.parts(x), count = Cuts::blocks(x) * p, incl = wave_scan_int(count);
-        const unsigned long long hit = __ballot(incl > left);
-        if (hit) {
-            const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
-            const int parts = lane_of(p, l), in = left - lane_of(incl - count, l), part = in % parts;
-            out->group = g0 + l;
-            out->g = Group{lane_of(x.s0, l), lane_of(x.rows, l), lane_of(x.kv, l)};
-            out->rb = in / parts;
-            const int all = out->g.kv / kBlockTok;
-            out->t0 = (int)((long long)all * part / parts);
-            out->t1 = (int)((long long)all * (part + 1) / parts);
-            return true;
-        }
-        left -= lane_of(incl, kWave - 1);
-    }
-    return false;
-}
-
 template <int D, bool kCut, Tokens P>
 __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(AttnArgs A) {
     constexpr int kC = D / 64, kM = D / 16;
@@ -606,10 +580,11 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
     const int block = kCut ? (int)blockIdx.x : A.first + (int)blockIdx.x;
     const int e = block % A.c.h_kv;
     int b, rb, parts = 1, part = 0;
-    [[maybe_unused]] Item it;
+    [[maybe_unused]] SharedItem it;
     if constexpr (P == kShared) {
-        if (!item_at(A, cuts_of<D>(A, A.slots, lane), block / A.c.h_kv, lane, &it)) return;
-        rb = it.rb, b = group_first(A, it.group);
+        it = A.shared_items[block / A.c.h_kv];
+        if (it.row < 0) return;
+        rb = 0, b = it.row;
     } else if constexpr (kCut) {
         const Blocks all = all_blocks<D, P>(A, lane);
         if ((int)blockIdx.x >= all.n * all.parts) return;
@@ -634,10 +609,10 @@ __global__ void __launch_bounds__(kBlockThreads, D == 256 ? 2 : 4) block_kernel(
         b = wave_search(A.a.n_seq, j, lane, key);
         rb = j - key(b);
     }
-    const int s0 = P == kShared ? it.g.s0 : A.a.start(b), q = P == kShared ? 0 : A.a.start(b + 1) - s0, r0 = rb * kBlockRows;
-    const int rows = P == kShared ? it.g.rows : max(q, 0) * A.G;
+    const int s0 = P == kShared ? it.s0 : A.a.start(b), q = P == kShared ? 0 : A.a.start(b + 1) - s0;
+    const int r0 = P == kShared ? it.r0 : rb * kBlockRows, rows = P == kShared ? it.rows : max(q, 0) * A.G;
     if (P != kShared && !kCut && (rows <= A.small || rb < 0 || r0 >= rows)) return;      // rb < 0: before the first sequence's rows
-    const int kv = P == kShared ? it.g.kv : max(A.a.kv_len[b], 0), first = kv - q, own = P == kOwn ? A.seq[b].from : 0;
+    const int kv = P == kShared ? it.kv : max(A.a.kv_len[b], 0), first = kv - q, own = P == kOwn ? A.seq[b].from : 0;
     const auto place = [&](int qi) { return P == kShared ? kv - 1 : first + qi; };       // of new token qi
 
     // q of row n of the wave, channels 64 c + 16 g .. + 15
