@@ -139,16 +139,19 @@ __device__ __forceinline__ Turn turn_of(int i, int span_log) {
 // unrolled 8, 4 and 2 times a single token for 64 sequences took 7.9, 6.6 and 5.5 us of the kernel's time.
 //
 // With positions (Turned; ix_kv8_append_rope) the keys are normed, turned and rounded to bf16 where they lie in LDS, each wave
-// its own rows, so the codes are those of rows that ix_rope_rows has turned, bit for bit. The queries are the third part of
-// the grid, item by item (rope.h).
+// its own rows, so the codes are those of rows that ix_rope_rows has turned, bit for bit. Up to kFewTurned the queries are the
+// third part of the grid, item by item (rope.h). 16 sequences of 1 to 2,048 tokens, 2 heads of 256 of which 64 channels turn, and a
+// norm: 25 us of plain rows' 15, by the turn's registers (102: 2 workgroups a CU); a token for each of 64 sequences, queries of 16
+// heads with it: 5.5 us of 5.2.
 constexpr int kBatch = 4;
 struct Plain {
-    static constexpr bool any = false;
+    static constexpr bool any = false, queries = false;
 };
+template <bool kQueries>
 struct Turned {
-    static constexpr bool any = true;
+    static constexpr bool any = true, queries = kQueries;
     Rope k;
-    RopeRows q;                   // q.x NULL: no queries
+    RopeRows q;                   // of kQueries
     int table;                    // pairs of a wave's table
     long long wgs;                // of each part of the grid in all launches
 };
@@ -164,14 +167,15 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
     if constexpr (Pos::any) {
         const int w = __builtin_amdgcn_readfirstlane(tid / kWave);
         table = reinterpret_cast<float2*>(raw + c.page * c.d / 8) + w * turn.table;
-        if (blockIdx.z == 2) {
-            const long long wg = ((long long)first_slot + blockIdx.x) * c.h_kv + h, items = (long long)a.T * turn.q.groups;
-            for (long long i = wg * (kThreads / kWave) + w; i < items; i += turn.wgs * (kThreads / kWave)) {
-                const int t = (int)(i / turn.q.groups);
-                rope_item(turn.q, a, t, (int)(i - (long long)t * turn.q.groups), lane, table);
+        if constexpr (Pos::queries)
+            if (blockIdx.z == 2) {
+                const long long wg = ((long long)first_slot + blockIdx.x) * c.h_kv + h, items = (long long)a.T * turn.q.groups;
+                for (long long i = wg * (kThreads / kWave) + w; i < items; i += turn.wgs * (kThreads / kWave)) {
+                    const int t = (int)(i / turn.q.groups);
+                    rope_item(turn.q, a, t, (int)(i - (long long)t * turn.q.groups), lane, table);
+                }
+                return;
             }
-            return;
-        }
     }
     PageJob job;
     if (!page_job(a, c, first_slot + (int)blockIdx.x, lane, &job)) return;
@@ -365,21 +369,24 @@ hipError_t launch_append(const Kv8& c, const Batch& a, const ix_rows* k, const i
     static OncePerDevice once;
     size_t lds = c.page * c.d * sizeof(uint16_t);
     int most = 128 * 256 * sizeof(uint16_t);
-    unsigned parts = 2;
     const long long slots = page_slots(c, a);
     if constexpr (Pos::any) {
         lds += kThreads / kWave * turn.table * sizeof(float2);
         most += kThreads / kWave * kWave * 8 / 2 * sizeof(float2);                        // a pair for two of a wave's values
         turn.wgs = slots * c.h_kv;
-        if (turn.q.x) parts = 3;
     }
     const hipError_t ready = allow_lds(once, &append_kernel<kThreads, Pos>, most, s);
     if (ready != hipSuccess) return ready;
     return launch_in_pieces(slots, kThreads, [&](long long first, unsigned n) {
-        hipLaunchKernelGGL((append_kernel<kThreads, Pos>), dim3(n, (unsigned)c.h_kv, parts), dim3(kThreads), lds, s, c, a, k->p, k->stride,
+        hipLaunchKernelGGL((append_kernel<kThreads, Pos>), dim3(n, (unsigned)c.h_kv, Pos::queries ? 3 : 2), dim3(kThreads), lds, s, c, a, k->p, k->stride,
                            v->p, v->stride, (int)first, turn);
     });
 }
+
+// Queries of up to this many values are turned in the append's launch, more in one of their own: there a CU holds 16 waves for
+// them, here 12 or with 512 threads 8, but a launch is 4 us. us, of 16 heads of 256 for 1,024, 2,048, 8,192 and 32,768 tokens here 17,
+// 26, 62, 221, there 18, 25, 49, 171; of 32 of 128, pages of 32, 18, 24, 60, 257 and 23, 28, 62, 237 (a read of the cache in all).
+constexpr long long kFewTurned = 1 << 24;
 
 template <int kThreads>
 hipError_t launch_read(const Kv8& c, const Batch& a, uint16_t* k, uint16_t* v, hipStream_t s) {
@@ -412,7 +419,7 @@ hipError_t ix_kv8_append_rope(const ix_kv8* cache, int n_seq, int total_T, const
     using namespace ixg;
     Kv8 c;
     Batch a;
-    Turned turn{};
+    Turned<true> turn{};
     Rope rope;
     if (!make_kv8(cache, &c) || !make_batch(n_seq, total_T, cu_seqlens, kv_len, table, width, &a)) return hipErrorInvalidValue;
     if (!make_rope(rope_k, c.d, &turn.k)) return hipErrorInvalidValue;
@@ -420,9 +427,14 @@ hipError_t ix_kv8_append_rope(const ix_kv8* cache, int n_seq, int total_T, const
     if (total_T == 0) return hipSuccess;                      // of tensors without elements, whose addresses may be 0
     if (!rows_ok(k, (long long)c.h_kv * c.d) || !rows_ok(v, (long long)c.h_kv * c.d)) return hipErrorInvalidValue;
     if (q && !make_rope_rows(rope_q, q, h_q, c.d, q_out, &turn.q)) return hipErrorInvalidValue;
-    turn.table = std::max(turn.k.half << (6 - turn.k.per_log), q ? turn.q.r.half : 0);
-    const int few = a.T < (long long)c.page * a.n_seq ? 2 : 1;
-    return with_threads(c.page * c.d / 32 / few, [&](auto n) { return launch_append<n>(c, a, k, v, turn, s); });
+    const int few = a.T < (long long)c.page * a.n_seq ? 2 : 1, keys = turn.k.half << (6 - turn.k.per_log);
+    if (q && (long long)a.T * h_q * c.d <= kFewTurned) {
+        turn.table = std::max(keys, turn.q.r.half);
+        return with_threads(c.page * c.d / 32 / few, [&](auto n) { return launch_append<n>(c, a, k, v, turn, s); });
+    }
+    const hipError_t e = q ? launch_rope(turn.q, a, s) : hipSuccess;
+    if (e != hipSuccess) return e;
+    return with_threads(c.page * c.d / 32 / few, [&](auto n) { return launch_append<n>(c, a, k, v, Turned<false>{turn.k, {}, keys, 0}, s); });
 }
 
 hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_t* cu_seqlens, const int32_t* kv_len,

@@ -183,6 +183,9 @@ inline bool make_rope_rows(const ix_rope* rope, const ix_rows* x, int heads, int
     return true;
 }
 
+// rope.hip: the items of a batch as a launch of their own.
+hipError_t launch_rope(const RopeRows& A, const Batch& a, hipStream_t s);
+
 // `table`: this wave's own, of r.half pairs.
 __device__ __forceinline__ void rope_item(const RopeRows& A, const Batch& a, int t, int group, int lane, float2* table) {
     const Rope& r = A.r;

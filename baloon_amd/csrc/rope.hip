@@ -14,6 +14,14 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeRows A, Batch a,
 }
 
 }  // namespace
+
+hipError_t launch_rope(const RopeRows& A, const Batch& a, hipStream_t s) {
+    return launch_in_pieces((a.T + (long long)kRopeWaves - 1) / kRopeWaves, kRopeThreads, [&](long long first, unsigned n) {
+        hipLaunchKernelGGL(rope_kernel, dim3(n, (unsigned)A.groups), dim3(kRopeThreads), kRopeWaves * A.r.half * sizeof(float2), s, A, a,
+                           (int)first);
+    });
+}
+
 }  // namespace ixg
 
 extern "C" {
@@ -27,10 +35,7 @@ hipError_t ix_rope_rows(const ix_rope* rope, int n_seq, int total_T, const int32
     if (!make_rope(rope, d, &A.r) || heads <= 0 || heads > 65536) return hipErrorInvalidValue;
     if (total_T == 0) return hipSuccess;                      // of tensors without elements, whose addresses may be 0
     if (!make_rope_rows(rope, x, heads, d, y, &A)) return hipErrorInvalidValue;
-    return launch_in_pieces((a.T + (long long)kRopeWaves - 1) / kRopeWaves, kRopeThreads, [&](long long first, unsigned n) {
-        hipLaunchKernelGGL(rope_kernel, dim3(n, (unsigned)A.groups), dim3(kRopeThreads), kRopeWaves * A.r.half * sizeof(float2), s, A, a,
-                           (int)first);
-    });
+    return launch_rope(A, a, s);
 }
 
 }  // extern "C"

@@ -153,6 +153,15 @@ def test_many_groups():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n_groups", [2, 60, 300])
+def test_many_sequences(n_groups):
+    """More sequences and groups than are kept beside the kernel's rows, of more lengths than a wave has lanes."""
+    g = np.random.default_rng(n_groups)
+    each = 620 // n_groups
+    Shared([group(int(n), *[(int(m > 2), int(m)) for m in g.integers(1, 20, each)]) for n in g.integers(0, 200, n_groups)], h=1, G=2).both()
+
+
+@pytest.mark.gpu
 def test_as_without_groups():
     """Without groups the call is ix_kv8_attn; groups that share nothing, and groups of one sequence, are right."""
     lens = [(1, 300), (5, 90), (1, 1), (40, 700)]

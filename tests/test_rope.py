@@ -267,6 +267,16 @@ def test_append(page, h, d, G, rot, layout, norm, how):
 
 
 @pytest.mark.gpu
+def test_append_of_many_queries():
+    """More than 2^24 values of queries."""
+    p = Pair(72, 64, 1, 256, 12)
+    tables = tables_for(p.g, 72, [4140, 35], 64, 66)
+    (rk, _), (rq, _) = make(p.g, 256, 64), make(p.g, 256, 256, 1, False)
+    append_both(p, [4100, 5], [4100, 5], tables, 16, rk, rq)
+    append_both(p, [1, 30], [4101, 35], tables, 16, rk, rq)
+
+
+@pytest.mark.gpu
 def test_append_places():
     """Pages without a place, tokens before position 0, offsets behind the first row; no queries, and queries in place."""
     import torch
