@@ -39,24 +39,24 @@ struct AttnArgs {
     struct SharedItem* shared_items;  // of block_kernel, each for all heads
     float *item_part, *shared_part;   // partial results of few_kernel's items and of block_kernel's over shared tokens
     int n_items, n_shared;    // room for them
-    int few;                  // the groups' rows are few_kernel's
+    int many;                 // the groups' rows may be block_kernel's
     float *row_o, *row_ml;    // partial results of rows whose own tokens are block_kernel's: [T][h_q][d], (m, lse) [T][h_q][2]
 };
 
 // Which tokens block_kernel takes: of a sequence all, or those behind the shared ones; or of a group those that its sequences share,
 // all of its rows together. The latter two leave partial results.
 enum Tokens { kAll, kOwn, kShared };
-// What is where of a sequence: its first own token (0: it shares none), its first item over them and the parts of each of its
-// blocks of rows; its group's first item, first row and parts (0: none).
 struct SharedItem {
     int s0, rows, r0, row;    // the group's first row of tokens and rows a head, the item's first, and the table's row (-1: there is no item)
     int t0, t1;               // tiles t0 .. t1 - 1 (one at least)
     int kv, unused;
 };
+// What is where of a sequence: its first own token (0: it shares none), its first item over them and the parts of each of its
+// blocks of rows; its group's first item, first row and parts (0: none), and the rows of a block.
 struct SeqPlan {
     int from, item, parts;
-    int shared_item, s0, shared_parts;
-    int unused[2];
+    int shared_item, s0, shared_parts, shared_rows;
+    int unused;
 };
 
 // The kernel's argument (its only one) read from memory again where it is used next: keeping all of it in

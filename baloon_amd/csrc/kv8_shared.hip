@@ -109,16 +109,15 @@ __device__ __forceinline__ int first_own(const AttnArgs& A, const Groups& groups
     return b >= group_first(A, lo) && b < group_first(A, lo + 1) ? group_at(A, lo).kv : 0;
 }
 
-// What few_kernel takes: the groups, where they have few rows, and behind them the sequences of few rows.
+// What few_kernel takes: the groups, where block_kernel does not, and behind them the sequences of few rows.
 struct Unit {
     int s0, rows;             // rows s0 G .. of a kv head, in blocks of 16; 0: nothing to do
     int t0, nt;               // its tiles (one at least)
     int first, kv;            // position of row 0 (of a group far behind its tokens), and tokens
 };
 template <int D>
-__device__ __forceinline__ Unit unit_at(const AttnArgs& A, const Groups& groups, int u) {
+__device__ __forceinline__ Unit unit_at(const AttnArgs& A, const Groups& groups, int n_groups, int u) {
     constexpr int kTok = kTokOf<D>;
-    const int n_groups = A.few ? A.n_groups : 0;
     Unit out{};
     if (u < n_groups) {
         const Group g = group_at(A, u);
@@ -138,7 +137,7 @@ __device__ __forceinline__ int blocks_of(const Unit& u) { return (u.rows + kSpli
 // short: a workgroup's way to its first tile is longer than several of them (64 sequences of up to 1,000 own tokens behind 8,190
 // shared ones took split_kernel, whose shares are cut at one length, 16 us; drafts of 37 sequences of up to 500 took it 25).
 struct FewCuts {
-    int chunk, units;
+    int chunk, units, n_groups;           // groups among the units
     __device__ __forceinline__ int parts(const Unit& u) const { return (u.nt + chunk - 1) / chunk; }
 };
 // The items of `segments` blocks: at most this.
@@ -146,6 +145,13 @@ __host__ __device__ inline long long few_items(long long segments, int n_wg) {
     const long long rounds = segments / n_wg + 1;
     return (rounds * n_wg - segments < n_wg / 4 ? rounds + 1 : rounds) * n_wg;
 }
+// Groups of up to kFewRows rows a kv head in the mean are always few_kernel's, those of more where all of them have up to kFewTiles
+// tiles of 16 rows: block_kernel takes a tile in half the time, but has 14 us before its first and for its partial results, of
+// which 3 remain where it finds nothing to do. us there and here: 8 sequences of 16 heads over 2 of 256 behind 1,000 tokens (64 rows)
+// 30 and 16; 64 behind 1,024, 4,096 and 8,190 (2,000, 8,200 and 16,400 tiles) 41, 44, 50 and 29, 42, 56; 37 of 4 tokens, 32 over 8 of
+// 128, behind 2,049 and 4,096 (9,500 and 19,000) 42, 51 and 40, 58; 128 of 20 over 4 behind 2,048 and 4,096 (5,100 and 10,200) 54, 62
+// and 57, 65.
+constexpr int kFewRows = 64, kFewTiles = 10000;
 // The first units, worked out once and kept in LDS, and the sums of all waves.
 constexpr int kKept = 512;
 struct Kept {
@@ -153,13 +159,24 @@ struct Kept {
     long long tiles[kWaves], segments[kWaves];
 };
 template <int D>
+__device__ __forceinline__ int group_units(const AttnArgs& A, const Groups& groups, int lane) {
+    if (!A.many) return A.n_groups;
+    long long tiles = 0;
+    for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
+        const Group g = A.n_groups <= kWave ? groups.g : group_at(A, g0 + lane);
+        tiles += (long long)((g.rows + kSplitRows - 1) / kSplitRows) * (g.kv / kTokOf<D>);
+    }
+    return lane_of(wave_scan_int(tiles), kWave - 1) * A.c.h_kv <= kFewTiles ? A.n_groups : 0;
+}
+template <int D>
 __device__ __forceinline__ FewCuts few_cuts(const AttnArgs& A, const Groups& groups, Kept* kept, int n_wg, int tid) {
     FewCuts out;
-    out.units = (A.few ? A.n_groups : 0) + A.a.n_seq;
     const int lane = tid & (kWave - 1);
+    out.n_groups = group_units<D>(A, groups, lane);
+    out.units = out.n_groups + A.a.n_seq;
     long long tiles = 0, segments = 0;
     for (int u0 = tid - lane; u0 < out.units; u0 += kThreads) {
-        const Unit u = unit_at<D>(A, groups, u0 + lane);
+        const Unit u = unit_at<D>(A, groups, out.n_groups, u0 + lane);
         if (u0 + lane < kKept) {
             const int x[6] = {u.s0, u.rows, u.t0, u.nt, u.first, u.kv};
 #pragma unroll
@@ -189,10 +206,11 @@ __device__ __forceinline__ FewCuts few_cuts(const AttnArgs& A, const Groups& gro
     return out;
 }
 template <int D>
-__device__ __forceinline__ Unit kept_unit(const AttnArgs& A, const Kept* kept, int u, int units, int lane) {
-    if (units > kKept && (u | (kWave - 1)) >= kKept) return unit_at<D>(A, groups_in_lanes(A, lane), u);      // the same for the wave
+__device__ __forceinline__ Unit kept_unit(const AttnArgs& A, const Kept* kept, int u, const FewCuts& cuts, int lane) {
+    if (cuts.units > kKept && (u | (kWave - 1)) >= kKept)     // the same for the wave
+        return unit_at<D>(A, groups_in_lanes(A, lane), cuts.n_groups, u);
     Unit out{};
-    if (u < units)
+    if (u < cuts.units)
         out = Unit{kept->unit[0][u], kept->unit[1][u], kept->unit[2][u], kept->unit[3][u], kept->unit[4][u], kept->unit[5][u]};
     return out;
 }
@@ -203,17 +221,16 @@ struct Piece {
 };
 template <int D>
 __device__ __forceinline__ bool piece_at(const AttnArgs& A, const Kept* kept, const FewCuts& cuts, int item, int lane, Piece* out) {
-    const int n_groups = A.few ? A.n_groups : 0;
     int left = item / A.c.h_kv;
     for (int u0 = 0; u0 < cuts.units; u0 += kWave) {
-        const Unit u = kept_unit<D>(A, kept, u0 + lane, cuts.units, lane);
+        const Unit u = kept_unit<D>(A, kept, u0 + lane, cuts, lane);
         const int p = cuts.parts(u), count = blocks_of(u) * p, incl = wave_scan_int(count);
         const unsigned long long hit = __ballot(incl > left);
         if (hit) {
             const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
             const int parts = lane_of(p, l), in = left - lane_of(incl - count, l), rb = in / parts, part = in - rb * parts;
             const int t0 = lane_of(u.t0, l), nt = lane_of(u.nt, l);
-            const int row = u0 + l < n_groups ? group_first(A, u0 + l) : u0 + l - n_groups;
+            const int row = u0 + l < cuts.n_groups ? group_first(A, u0 + l) : u0 + l - cuts.n_groups;
             *out = Piece{row, item % A.c.h_kv, lane_of(u.s0, l), lane_of(u.rows, l), rb * kSplitRows, lane_of(u.first, l), lane_of(u.kv, l),
                          t0 + (int)((long long)nt * part / parts), t0 + (int)((long long)nt * (part + 1) / parts)};
             return true;
@@ -226,18 +243,19 @@ __device__ __forceinline__ bool piece_at(const AttnArgs& A, const Kept* kept, co
 // What block_kernel and gather_kernel ask of a sequence, by a workgroup that does nothing else.
 template <int D>
 __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& groups, const FewCuts& cuts, int tid) {
-    const int lane = tid & (kWave - 1), n_groups = A.few ? A.n_groups : 0;
+    const int lane = tid & (kWave - 1);
+    const bool few = cuts.n_groups == A.n_groups;
     for (int b = tid; b < A.a.n_seq; b += kThreads) A.seq[b] = SeqPlan{};
-    for (int i = tid; i <= A.n_shared / A.c.h_kv; i += kThreads) A.shared_items[i].row = -1;
+    for (int i = tid; A.many && i <= A.n_shared / A.c.h_kv; i += kThreads) A.shared_items[i].row = -1;
     __syncthreads();
     if (tid >= kWave) return;
-    const Cuts blocks = A.few ? Cuts{1} : cuts_of<D>(A, A.slots, lane);
+    const Cuts blocks = few ? Cuts{1} : cuts_of<D>(A, A.slots, lane);
     int base = 0;
     for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
         const Group g = group_at(A, g0 + lane);
         const int first = g.rows ? group_first(A, g0 + lane) : 0, last = g.rows ? group_first(A, g0 + lane + 1) : 0;
         const Unit u{g.s0, g.rows, 0, g.kv / kTokOf<D>, 0, 0};
-        const int parts = A.few ? cuts.parts(u) : blocks.parts(g), items = (A.few ? blocks_of(u) : Cuts::blocks(g)) * parts;
+        const int parts = few ? cuts.parts(u) : blocks.parts(g), items = (few ? blocks_of(u) : Cuts::blocks(g)) * parts;
         const int before = wave_scan_int(items) - items;
         unsigned long long todo = __ballot(g.rows > 0);
         while (todo) {                                        // all lanes for one group's sequences
@@ -248,8 +266,9 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
                 A.seq[b].shared_item = item;
                 A.seq[b].s0 = s0;
                 A.seq[b].shared_parts = n;
+                A.seq[b].shared_rows = few ? kSplitRows : kBlockRows;
             }
-            if (A.few) continue;
+            if (few) continue;
             const int rows = lane_of(g.rows, l), kv = lane_of(g.kv, l), all = kv / kBlockTok, row = lane_of(first, l);
             for (int i = lane; i < lane_of(items, l); i += kWave) {
                 const int rb = i / n, part = i - rb * n;
@@ -259,10 +278,10 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
         }
         base += lane_of(before + items, kWave - 1);
     }
-    base = A.few ? base : 0;
-    for (int u0 = n_groups; u0 < cuts.units; u0 += kWave) {
-        const Unit u = unit_at<D>(A, groups, u0 + lane);
-        const int parts = cuts.parts(u), items = blocks_of(u) * parts, before = wave_scan_int(items) - items, b = u0 - n_groups + lane;
+    base = few ? base : 0;
+    for (int u0 = cuts.n_groups; u0 < cuts.units; u0 += kWave) {
+        const Unit u = unit_at<D>(A, groups, cuts.n_groups, u0 + lane);
+        const int parts = cuts.parts(u), items = blocks_of(u) * parts, before = wave_scan_int(items) - items, b = u0 - cuts.n_groups + lane;
         if (b < A.a.n_seq) {
             A.seq[b].from = u.t0 * kTokOf<D>;
             A.seq[b].item = base + before;
@@ -285,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
     float* lo_ml = lds + kWaves * kSplitRows * kPitch;        // [waves][16][2]
     Kept* kept = reinterpret_cast<Kept*>(lds + kWaves * kSplitRows * (kPitch + 2));
     const int n_wg = gridDim.x - 1;
-    int chunk, units;                     // in vector registers: the main loop needs the scalar ones
+    int chunk, units, n_groups;           // in vector registers: the main loop needs the scalar ones
     {
         const AttnArgs& A = args_again();
         const Groups groups = groups_in_lanes(A, threadIdx.x & (kWave - 1));
@@ -294,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
             write_plan<D>(A, groups, cuts, threadIdx.x);
             return;
         }
-        chunk = parked(cuts.chunk), units = parked(cuts.units);
+        chunk = parked(cuts.chunk), units = parked(cuts.units), n_groups = parked(cuts.n_groups);
     }
     // The sums of an item, for rows n: of 2^(kLift - mref) p' v / vs, and of p; and what is left to do for it.
     v4f acc[kM];
@@ -311,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
         const AttnArgs& A = args_again();
         const int h_kv = A.c.h_kv, page_log = A.c.page_log, n_pages = A.c.n_pages;
         Piece it{};
-        const bool any = piece_at<D>(A, kept, FewCuts{taken(chunk), taken(units)}, item, lane, &it);
+        const bool any = piece_at<D>(A, kept, FewCuts{taken(chunk), taken(units), taken(n_groups)}, item, lane, &it);
         if (!any && !open) return;
         const int e = it.e, r0 = it.r0, kv = it.kv, t1 = it.t1;
         int t = it.t0 + w;
@@ -488,9 +507,9 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
 }
 
 // Puts each row's partial results together and writes it: a wave takes 64 outputs (in fours) of a token or, kWays, a workgroup's four
-// waves every fourth of their results each. kRows: the blocks of groups.
+// waves every fourth of their results each.
 constexpr int kOutputs = kWave;
-template <int D, int kRows, bool kWays>
+template <int D, bool kWays>
 __global__ void __launch_bounds__(kThreads) gather_kernel(AttnArgs A, int first) {
     __shared__ v4f lo_o[kThreads];
     __shared__ float2 lo_ml[kThreads];
@@ -526,9 +545,10 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(AttnArgs A, int first)
         sum.more(A.row_ml[2 * at], A.row_ml[2 * at + 1], *reinterpret_cast<const v4f*>(A.row_o + at * D + d));
     }
     if (plan.shared_parts > 0) {
-        const int r = (t - plan.s0) * A.G + in_token, block = r / kRows, in = r - block * kRows, from = kWays ? (way - own) & (kWaves - 1) : 0;
-        if constexpr (kRows == kSplitRows) add(few, block, kRows, plan.shared_item, plan.shared_parts, in, from);
-        else add(ItemParts<kRows, D>(A.shared_part, A.n_shared), block, kRows, plan.shared_item, plan.shared_parts, in, from);
+        const int r = (t - plan.s0) * A.G + in_token, n = plan.shared_rows, block = r / n, in = r - block * n;
+        const int from = kWays ? (way - own) & (kWaves - 1) : 0;
+        if (n == kSplitRows) add(few, block, kSplitRows, plan.shared_item, plan.shared_parts, in, from);
+        else add(ItemParts<kBlockRows, D>(A.shared_part, A.n_shared), block, kBlockRows, plan.shared_item, plan.shared_parts, in, from);
     }
     if constexpr (kWays) {
         lo_o[tid] = sum.o;
@@ -545,39 +565,32 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(AttnArgs A, int first)
 // any, partial results of the rows and of its items over the shared tokens.
 struct SharedPlan {
     Plan own;
-    bool few;                 // groups' rows are few_kernel's
+    bool many;                // groups' rows may be block_kernel's
     int n_wg;                 // workgroups of block_kernel that the chip holds
     long long n_items, n_shared;
     size_t seq, items, shared, shared_items, row_o, row_ml, bytes;
 };
-// Groups of up to this many rows a kv head in the mean are few_kernel's.
-constexpr int kFewRows = 32;
 SharedPlan shared_plan(int d, int h_kv, int G, int n_seq, int T, int max_q, int n_groups, hipStream_t s) {
     SharedPlan p;
     p.own = attn_plan(d, h_kv, G, T, max_q, s);
     const long long rows = (long long)T * G, nonempty = std::min(n_seq, T);
-    p.few = rows <= (long long)kFewRows * n_groups;
+    p.many = rows > (long long)kFewRows * n_groups;
     p.n_wg = d == 256 ? p.own.n_wg / 2 : p.own.n_wg;
-    // a sequence or group has at most one block that is not full
-    const auto segments = [&](bool few) { return (rows / kSplitRows + nonempty + (few ? rows / kSplitRows + n_groups : 0)) * h_kv; };
-    const auto blocks = [&] {
-        const long long n = (rows / kBlockRows + n_groups) * h_kv;
-        return n < p.n_wg / 2 ? p.n_wg : (n + p.n_wg - 1) / p.n_wg * p.n_wg + p.n_wg;
-    };
-    p.n_items = few_items(segments(p.few), p.own.n_wg - 1);
-    p.n_shared = p.few ? 0 : blocks();
+    // a sequence or group has at most one block that is not full; the groups may be few_kernel's
+    const long long segments = (2 * (rows / kSplitRows) + nonempty + n_groups) * h_kv, blocks = (rows / kBlockRows + n_groups) * h_kv;
+    p.n_items = few_items(segments, p.own.n_wg - 1);
+    p.n_shared = blocks < p.n_wg / 2 ? p.n_wg : (blocks + p.n_wg - 1) / p.n_wg * p.n_wg + p.n_wg;
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const auto item_bytes = [&](long long n, int block) { return up((size_t)n * block * (d + 2) * sizeof(float)); };
     p.seq = attn_bytes(d, p.own);
     p.items = p.seq + up(n_seq * sizeof(SeqPlan));
-    // room as for groups of many rows and of few: a smaller batch's may be either
-    p.shared = p.items + item_bytes(few_items(segments(true), p.own.n_wg - 1), kSplitRows);
-    p.shared_items = p.shared + item_bytes(blocks(), kBlockRows);
-    p.row_o = p.shared_items + up((blocks() / h_kv + 1) * sizeof(SharedItem));
+    p.shared = p.items + item_bytes(p.n_items, kSplitRows);
+    p.shared_items = p.shared + item_bytes(p.n_shared, kBlockRows);
+    p.row_o = p.shared_items + up((p.n_shared / h_kv + 1) * sizeof(SharedItem));
     p.row_ml = p.row_o + (p.own.block ? up((size_t)rows * h_kv * d * sizeof(float)) : 0);
     p.bytes = p.row_ml + (p.own.block ? up((size_t)rows * h_kv * 2 * sizeof(float)) : 0);
     // workgroups and items are numbered in 31 bits; a batch beyond that has more outputs than the GPU has memory
-    if (segments(true) > 1 << 28 || rows * h_kv * d / 256 > 1 << 30) p.bytes = 0;
+    if (segments > 1 << 28 || rows * h_kv * d / 256 > 1 << 30) p.bytes = 0;
     return p;
 }
 
@@ -592,7 +605,7 @@ hipError_t launch_shared(AttnArgs& A, const SharedPlan& p, hipStream_t s) {
     A.row_ml = reinterpret_cast<float*>(ws + p.row_ml);
     A.n_items = (int)p.n_items;
     A.n_shared = (int)p.n_shared;
-    A.few = p.few;
+    A.many = p.many;
     A.slots = p.n_wg;
     A.small = attn_small(A, p.own);
     constexpr unsigned lds = kWaves * kSplitRows * (D + 4 + 2) * sizeof(float) + sizeof(Kept);
@@ -601,22 +614,19 @@ hipError_t launch_shared(AttnArgs& A, const SharedPlan& p, hipStream_t s) {
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((few_kernel<D>), dim3((unsigned)p.own.n_wg), dim3(kThreads), lds, s, A);
     e = hipGetLastError();
-    if (e == hipSuccess && !p.few) e = launch_shared_blocks(A, p.n_wg, s);
+    if (e == hipSuccess && p.many) e = launch_shared_blocks(A, p.n_wg, s);
     if (e == hipSuccess && p.own.block) e = launch_own_blocks(A, p.own, s);
     if (e != hipSuccess) return e;
-    const auto gather = [&](auto rows, auto ways) {
+    const auto gather = [&](auto ways) {
         const long long waves = (long long)A.a.T * ((A.h_q * (D / 4) + kOutputs - 1) / kOutputs);
         return launch_in_pieces(ways ? waves : (waves + kWaves - 1) / kWaves, kThreads, [&](long long first, unsigned n) {
-            hipLaunchKernelGGL((gather_kernel<D, rows, ways>), dim3(n), dim3(kThreads), 0, s, A, (int)first);
+            hipLaunchKernelGGL((gather_kernel<D, ways>), dim3(n), dim3(kThreads), 0, s, A, (int)first);
         });
     };
     // Four waves for each output where the chip holds as many at once: 64 tokens of 16 heads of 256 9.1 us against 11.3 with one;
     // 148 drafted ones of 32 of 128 8.8 against 6.9.
     const bool ways = (long long)A.a.T * A.h_q * D <= (long long)p.own.n_wg * 1024;
-    const std::integral_constant<int, kSplitRows> few;
-    const std::integral_constant<int, kBlockRows> many;
-    if (p.few) return ways ? gather(few, std::true_type{}) : gather(few, std::false_type{});
-    return ways ? gather(many, std::true_type{}) : gather(many, std::false_type{});
+    return ways ? gather(std::true_type{}) : gather(std::false_type{});
 }
 
 }  // namespace
