@@ -9,7 +9,8 @@ construction (and for the prefill workspace, on first use of a given size), neve
 library calls.
 
 AttnLayer is the same for the softmax attention layers that stand between GDN layers: it owns a paged 8-bit
-cache of keys and values and the lengths of its sequences, and calls ``ix_kv8_append`` and ``ix_kv8_attn``.
+cache of keys and values and the lengths of its sequences, and calls ``ix_kv8_append`` and ``ix_kv8_attn``; with rotary
+positions ``ix_kv8_append_rope``, and for sequences that were forked from one prompt ``ix_kv8_attn_shared``.
 """
 from __future__ import annotations
 
@@ -17,7 +18,8 @@ import torch
 
 from . import (HIP_ERROR_INVALID_VALUE, Cfg, _rows, check, ix_gdn_decode, ix_gdn_decode_gated, ix_gdn_decode_workspace_size, ix_gdn_prefill,
                ix_gdn_prefill_gated, ix_gdn_prefill_gated_workspace_size, ix_gdn_prefill_workspace_size,
-               ix_kv8_append, ix_kv8_attn, ix_kv8_attn_workspace_size, kv8_cache, make_cfg, out_gate)
+               ix_kv8_append, ix_kv8_append_rope, ix_kv8_attn, ix_kv8_attn_shared, ix_kv8_attn_shared_workspace_size,
+               ix_kv8_attn_workspace_size, kv8_cache, make_cfg, out_gate)
 
 
 class GdnLayer:
@@ -84,14 +86,20 @@ class AttnLayer:
 
     All of a call is on one stream, the lengths and a new o among it: `stream` (a torch stream or an address), or torch's
     current one. The caller orders calls on different streams, and what else it does with the layer's tensors. The workspace
-    is allocated here for any batch (38 to 81 MiB), so a captured call's stays where it is."""
+    is allocated here for any batch (38 to 81 MiB), so a captured call's stays where it is.
+
+    rope (``baloon_amd.rope``) norms and turns queries by position before they attend, rope_k (rope itself if not given) keys
+    before they are stored. With max_forks, up to so many groups of slots may share a prompt (`fork`), which calls of up to 16
+    new tokens a slot in the mean then read once for all of them, where that is worth it (`worth`: codes of keys that need
+    not be read again)."""
 
     def __init__(self, n_slots: int, max_len: int, h_q=16, h_kv=2, d=256, page=64, n_pages=None, window=0, sinks=0,
-                 scale=None, device="cuda"):
+                 scale=None, device="cuda", rope=None, rope_k=None, max_forks=0, worth=200_000_000):
         self.n_slots, self.h_q, self.h_kv, self.d = n_slots, h_q, h_kv, d
         self.window, self.sinks, self.scale = window, sinks, d ** -0.5 if scale is None else scale
         self.device = torch.device(device)
         self.width = -(-max_len // page)
+        self._own_pages = n_pages is None
 
         def tensor(*shape, dtype):
             return torch.zeros(*shape, dtype=dtype, device=self.device)
@@ -109,6 +117,84 @@ class AttnLayer:
         most = min(2 ** 31 - 1, 2 ** 37 // max(h_q, 1))       # tokens of a call
         self._ws_bytes = ix_kv8_attn_workspace_size(self.cache, n_slots, most, most, h_q)
         self._ws = torch.empty(max(self._ws_bytes, 256), dtype=torch.uint8, device=self.device)
+        if rope is None and rope_k is not None:
+            raise ValueError("baloon_amd: rope_k goes with rope")
+        self.rope, self.rope_k = rope, rope if rope_k is None else rope_k
+        if max_forks < 0 or (max_forks and window):
+            raise ValueError("baloon_amd: forked sequences see all of their prompt: no window")
+        self.max_forks, self.worth, self._forks, self._n_groups, self._shared_pays = max_forks, worth, {}, 0, False
+        if max_forks:
+            most = 2 * max_forks                              # groups: the forks, and what lies between two
+            self._groups, self._shared = tensor(most + 1, dtype=torch.int32), tensor(most, dtype=torch.int32)
+            self._few = 16 * n_slots
+            n = max(ix_kv8_attn_shared_workspace_size(self.cache, n_slots, self._few, self._few, most, h_q), 256)
+            self._shared_ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+
+    def fork(self, slot, n, tokens, stream=None):
+        """Slots slot + 1 .. slot + n - 1 go on from the first `tokens` tokens of `slot`, which holds as many, and from nothing that
+        they held: its whole pages are theirs too, the page that the tokens end in is copied. Until `release`, none of the n may lose one of these
+        tokens (a shorter kv_len, then new tokens). Not to be captured; captured calls run with as many groups as there were,
+        so capture them again when a fork or a release has changed that (a fork released and made anew changes nothing)."""
+        others = range(slot + 1, slot + n)
+        if slot < 0 or n < 2 or slot + n > self.n_slots or not 0 < tokens <= self.width * self.cache.page:
+            raise ValueError("baloon_amd: a fork is of two slots or more, and of tokens that a slot can hold")
+        if len(self._forks) >= self.max_forks:
+            raise ValueError("baloon_amd: more than max_forks forks")
+        if any(slot < s + m and s < slot + n for s, (m, _) in self._forks.items()):
+            raise ValueError("baloon_amd: a slot of a fork already")
+        self._on(stream, self._fork, slot, others, tokens)
+
+    def _fork(self, slot, others, tokens):
+        whole, rest = divmod(tokens, self.cache.page)
+        if int(self.kv_len[slot]) < tokens:
+            raise ValueError("baloon_amd: the slot holds fewer tokens")
+        if rest:
+            source, *pages = self.table[slot:others.stop, whole].tolist()
+            if not all(0 <= p < self.cache.n_pages for p in (source, *pages)) or source in pages or len(set(pages)) < len(pages):
+                raise ValueError("baloon_amd: the page that the tokens end in has no place of its own in each slot")
+            for t in self.cache.tensors:
+                t[pages] = t[source].clone()
+        self._forks[slot] = (len(others) + 1, tokens)
+        self._regroup()
+        self.table[slot + 1:others.stop, :whole] = self.table[slot, :whole].clone()
+        self.kv_len[slot + 1:others.stop] = tokens
+
+    def release(self, slot, stream=None):
+        """Ends the fork of `slot`: the others of it are empty again, with pages of their own (where the caller keeps the
+        pages, without those that they shared)."""
+        if slot not in self._forks:
+            raise ValueError("baloon_amd: not a slot that others were forked from")
+        self._on(stream, self._release, slot)
+
+    def _release(self, slot):
+        n, tokens = self._forks.pop(slot)
+        whole = tokens // self.cache.page
+        rows = self.table[slot + 1:slot + n, :whole]
+        if self._own_pages:
+            first = torch.arange(slot + 1, slot + n, dtype=torch.int32, device=self.device)[:, None] * self.width
+            rows.copy_(first + torch.arange(whole, dtype=torch.int32, device=self.device))
+        else:
+            rows.fill_(-1)
+        self.kv_len[slot + 1:slot + n] = 0
+        self._regroup()
+
+    def _regroup(self):
+        """The groups of ix_kv8_attn_shared lie side by side: between two forks is one that shares nothing."""
+        ends, shared = [], []
+        for slot, (n, tokens) in sorted(self._forks.items()):
+            if ends and ends[-1] < slot:
+                ends.append(slot)
+                shared.append(0)
+            ends += [slot + n] if ends else [slot, slot + n]
+            shared.append(tokens)
+        self._n_groups = len(shared)
+        # Reading shared tokens once pays from about 2e8 codes of keys on that need not be read again. us with and without, 37
+        # sequences of 4 new tokens, 32 heads over 8 of 128, behind 4,096 tokens 52 and 44, behind 8,192 63 and 82; 64 of one,
+        # 16 over 2 of 256, behind 2,048, 4,096 and 8,190 33, 42, 50 and 30, 41, 62; 24 times 4 behind 300 to 6,000 57 and 101.
+        self._shared_pays = sum((n - 1) * tokens for n, tokens in self._forks.values()) * self.h_kv * self.d >= self.worth
+        if shared:
+            self._groups[:len(ends)] = torch.tensor(ends, dtype=torch.int32)
+            self._shared[:len(shared)] = torch.tensor(shared, dtype=torch.int32)
 
     def prefill(self, cu_seqlens, max_q, q, k, v, gate=None, o=None, stream=None):
         """Appends packed new tokens (cu_seqlens int32 [n_slots + 1] on the device, at most max_q of a sequence) and
@@ -118,23 +204,23 @@ class AttnLayer:
             raise ValueError("baloon_amd: cu_seqlens has an offset for each sequence and one more")
         if cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_cuda or not cu_seqlens.is_contiguous():
             raise ValueError("baloon_amd: cu_seqlens is int32, contiguous and on the GPU")
-        return self._on(stream, cu_seqlens, max_q, q, k, v, gate, o)
+        return self._on(stream, self._attend, cu_seqlens, max_q, q, k, v, gate, o)
 
     def decode(self, q, k, v, gate=None, o=None, stream=None):
         """The same for one token of every sequence."""
         if q.shape[0] != self.n_slots:
             raise ValueError("baloon_amd: one token for each sequence")
-        return self._on(stream, self._one_each, 1, q, k, v, gate, o)
+        return self._on(stream, self._attend, self._one_each, 1, q, k, v, gate, o)
 
-    def _on(self, stream, *args):
+    def _on(self, stream, call, *args):
         if stream is None:
-            return self._attend(*args)
+            return call(*args)
         if not isinstance(stream, torch.cuda.Stream):
             address = getattr(stream, "cuda_stream", getattr(stream, "value", stream)) or 0      # also a ctypes.c_void_p
             # torch takes an ExternalStream of address 0 for one that it is to choose
             stream = torch.cuda.ExternalStream(address, self.device) if address else torch.cuda.default_stream(self.device)
         with torch.cuda.stream(stream):
-            return self._attend(*args)
+            return call(*args)
 
     def _attend(self, cu_seqlens, max_q, q, k, v, gate, o):
         # What the calls below would refuse, or read and write beside the operands, is refused before anything is done.
@@ -154,9 +240,20 @@ class AttnLayer:
         where = (cu_seqlens, self.kv_len, self.table, self.width)
         self.kv_len += new
         try:
-            check("ix_kv8_append", ix_kv8_append(self.cache, self.n_slots, T, *where, k, v))
-            check("ix_kv8_attn", ix_kv8_attn(self.cache, self.n_slots, T, max_q, *where, q, self.h_q, self.scale, self.window,
-                                             self.sinks, gate, o, self._ws, self._ws.numel()))
+            if self.rope is None:
+                check("ix_kv8_append", ix_kv8_append(self.cache, self.n_slots, T, *where, k, v))
+            else:
+                turned = torch.empty(T, self.h_q, self.d, dtype=torch.bfloat16, device=self.device)      # not o: that may be the gate's
+                check("ix_kv8_append_rope", ix_kv8_append_rope(self.cache, self.n_slots, T, *where, k, v, self.rope_k, q, self.h_q,
+                                                               self.rope, turned))
+                q = turned
+            if self._shared_pays and T <= self._few:
+                check("ix_kv8_attn_shared", ix_kv8_attn_shared(self.cache, self.n_slots, T, min(max_q, T), *where, self._n_groups,
+                                                               self._groups, self._shared, q, self.h_q, self.scale, gate, o,
+                                                               self._shared_ws, self._shared_ws.numel()))
+            else:
+                check("ix_kv8_attn", ix_kv8_attn(self.cache, self.n_slots, T, max_q, *where, q, self.h_q, self.scale, self.window,
+                                                 self.sinks, gate, o, self._ws, self._ws.numel()))
         except BaseException:
             self.kv_len -= new                                # a call that raises leaves the lengths as they were
             raise

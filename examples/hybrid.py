@@ -3,7 +3,9 @@
 Between the layers the residual sum and the norm of the next one's input are one launch (ix_add_rms_norm). The attention
 layer keeps its keys and values in the 8-bit cache (AttnLayer) and its output is gated, the GDN layers their states
 (GdnLayer). Projections of prompts are torch products, those of single tokens ix_gdn_in_proj and ix_mmvq_q8_0, which
-reads the last norm's q8_1 output. Weights are random: run it with ``python -m examples.hybrid``.
+reads the last norm's q8_1 output. With rope_base the attention's queries and keys are normed and turned by position, and
+several continuations of a prompt may go on from one pass over it. Weights are random: run it with
+``python -m examples.hybrid``.
 """
 import torch
 import torch.nn.functional as F
@@ -12,7 +14,8 @@ import baloon_amd as bx
 
 
 class Hybrid:
-    def __init__(self, n_slots, max_len, hidden=1024, n_layers=4, h_q=8, h_kv=2, d=128, vocab=512, seed=0):
+    def __init__(self, n_slots, max_len, hidden=1024, n_layers=4, h_q=8, h_kv=2, d=128, vocab=512, seed=0, rope_base=None,
+                 **attention):
         self.n, self.hidden, self.h_q, self.h_kv, self.d, self.vocab = n_slots, hidden, h_q, h_kv, d, vocab
         self.cfg = c = bx.make_cfg(h_k=4, h_v=8)
         g = torch.Generator(device="cuda").manual_seed(seed)
@@ -20,13 +23,17 @@ class Hybrid:
         def weight(rows, cols):
             return (torch.randn(rows, cols, generator=g, device="cuda") * cols ** -0.5).bfloat16()
 
+        if rope_base:
+            freq = bx.rope_freq(d // 2, rope_base)[0].cuda()                             # half of the channels turn
+            q_norm, k_norm = (torch.randn(d, generator=g, device="cuda") * 0.1 for _ in "qk")
+            attention.update(rope=bx.rope(freq, norm=q_norm, norm_offset=1.0), rope_k=bx.rope(freq, norm=k_norm, norm_offset=1.0))
         self.embed = weight(vocab, hidden) * hidden ** 0.5
         self.layers = []
         for i in range(n_layers):
             norm = (torch.randn(hidden, generator=g, device="cuda") * 0.1)               # its weight is 1 + norm
             if i % 4 == 3:
                 w_in = weight((2 * h_q + 2 * h_kv) * d, hidden)                          # q | gate | k | v
-                self.layers.append((bx.AttnLayer(n_slots, max_len, h_q, h_kv, d), norm, w_in, weight(hidden, h_q * d)))
+                self.layers.append((bx.AttnLayer(n_slots, max_len, h_q, h_kv, d, **attention), norm, w_in, weight(hidden, h_q * d)))
             else:
                 layer = bx.GdnLayer(n_slots, c)
                 layer.conv_w.copy_(weight(c.channels, c.d_conv))
@@ -82,6 +89,16 @@ class Hybrid:
         return logits
 
 
+    def fork(self, slot, n, tokens):
+        """Slots slot .. slot + n - 1 go on from the `tokens` tokens that `slot` holds, all of them."""
+        for layer, *_ in self.layers:
+            if isinstance(layer, bx.AttnLayer):
+                layer.fork(slot, n, tokens)
+            else:
+                for t in (layer.state, layer.conv_state):
+                    t[slot + 1:slot + n] = t[slot].clone()
+
+
 def generate(prompts, steps, seed=0):
     """Greedy continuations of token lists, and the model."""
     lens = [len(p) for p in prompts]
@@ -95,7 +112,26 @@ def generate(prompts, steps, seed=0):
     return torch.stack(made, 1).tolist(), model
 
 
+def continuations(prompts, each, steps, seed=0):
+    """`each` continuations of every prompt from one pass over it, drawn by the last token's logits, and the model."""
+    lens, n = [len(p) for p in prompts], len(prompts) * each
+    model = Hybrid(n, max(lens) + steps, seed=seed, rope_base=1e4, max_forks=len(prompts))
+    cu = torch.tensor([0] + [x for m in lens for x in (m, *[0] * (each - 1))], dtype=torch.int32).cumsum(0, dtype=torch.int32).cuda()
+    logits = model.forward(torch.tensor(sum(prompts, []), device="cuda"), cu, max(lens))     # a slot without tokens: of those before it
+    for i, m in enumerate(lens):
+        if each > 1:
+            model.fork(i * each, each, m)
+    g, made = torch.Generator(device="cuda").manual_seed(seed), []
+    for _ in range(steps):
+        made.append(torch.multinomial(logits.softmax(1), 1, generator=g)[:, 0])
+        logits = model.forward(made[-1])
+    return torch.stack(made, 1).tolist(), model
+
+
 if __name__ == "__main__":
     tokens, _ = generate([[i % 512 for i in range(5, 305)], [1, 2, 3], list(range(64))], 16)
+    for t in tokens:
+        print(*t)
+    tokens, _ = continuations([[i % 512 for i in range(5, 305)], [1, 2, 3]], 3, 16)
     for t in tokens:
         print(*t)
