@@ -141,7 +141,7 @@ __device__ __forceinline__ Turn turn_of(int i, int span_log) {
 // With positions (Turned; ix_kv8_append_rope) the keys are normed, turned and rounded to bf16 where they lie in LDS, each wave
 // its own rows, so the codes are those of rows that ix_rope_rows has turned, bit for bit. Up to kFewTurned the queries are the
 // third part of the grid, item by item (rope.h). 16 sequences of 1 to 2,048 tokens, 2 heads of 256 of which 64 channels turn, and a
-// norm: 25 us of plain rows' 15, by the turn's registers (102: 2 workgroups a CU); a token for each of 64 sequences, queries of 16
+// norm: 23 us of plain rows' 15; a token for each of 64 sequences, queries of 16
 // heads with it: 5.5 us of 5.2.
 constexpr int kBatch = 4;
 struct Plain {
@@ -219,12 +219,12 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
                 uint4 x = make_uint4(0, 0, 0, 0), other = x;
                 if (i < chunks) {
                     x = held[i];
-                    other = L.load_other(r, reinterpret_cast<const uint16_t*>(held + (i >> per_log << per_log)),
+                    other = L.load_other(r, reinterpret_cast<const uint16_t*>(held + (i >> per_log << per_log)), x,
                                          [](const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); });
                 }
-                float C[8], S[8];
-                L.factors(r, table + (lane >> per_log) * r.half, C, S);
-                x = L.turned(r, x, other, C, S);
+                float F[8], S[8];
+                L.factors(r, table + (lane >> per_log) * r.half, F, S);
+                x = L.turned(r, x, other, F, S);
                 m = fmaxf(m, max_abs(x));
                 wave_lds_sync();
                 if (i < chunks) held[i] = x;
@@ -383,9 +383,9 @@ hipError_t launch_append(const Kv8& c, const Batch& a, const ix_rows* k, const i
     });
 }
 
-// Queries of up to this many values are turned in the append's launch, more in one of their own: there a CU holds 16 waves for
-// them, here 12 or with 512 threads 8, but a launch is 4 us. us, of 16 heads of 256 for 1,024, 2,048, 8,192 and 32,768 tokens here 17,
-// 26, 62, 221, there 18, 25, 49, 171; of 32 of 128, pages of 32, 18, 24, 60, 257 and 23, 28, 62, 237 (a read of the cache in all).
+// Queries of up to this many values are turned in the append's launch, more in one of their own: there a CU holds 20 waves for
+// them, here 16, but a launch is 4 us. us, of 16 heads of 256 for 1,024, 2,048, 8,192 and 32,768 tokens here 17, 23, 58, 202, there 18,
+// 22, 46, 159; of 32 of 128, pages of 32, 18, 22, 56, 236 and 22, 26, 59, 225 (a read of the cache in all).
 constexpr long long kFewTurned = 1 << 24;
 
 template <int kThreads>
