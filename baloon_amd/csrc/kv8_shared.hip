@@ -13,6 +13,7 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 template <int D>
 constexpr int kTokOf = D == 256 ? 32 : 64;
+constexpr int few_per_cu(int d) { return d == 256 ? 2 : d == 128 ? 3 : 4; }      // few_kernel's workgroups, by its registers
 
 constexpr int kGrain = 64;            // shared tokens are taken in whole 64s; what is left over is each sequence's own
 
@@ -157,6 +158,8 @@ constexpr int kKept = 512;
 struct Kept {
     int unit[6][kKept];
     long long tiles[kWaves], segments[kWaves];
+    FewCuts cuts;                         // and what the main loop has no registers for
+    int item, rows;
 };
 template <int D>
 __device__ __forceinline__ int group_units(const AttnArgs& A, const Groups& groups, int lane) {
@@ -294,7 +297,7 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
 // An item is 16 rows of a unit over a part of its tiles. A wave takes a tile of kTok tokens at a time by itself, all in registers,
 // with the next one's loads under way; products and the layout of P are those of split_kernel.
 template <int D>
-__global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
+__global__ void __launch_bounds__(kThreads, few_per_cu(D)) few_kernel(AttnArgs A_) {
     constexpr int kC = D / 64, kM = D / 16, kPitch = D + 4, kTok = kTokOf<D>, kS = kTok / 16;
     typedef typename std::conditional<kS == 4, uint4, uint2>::type Codes;     // 4 S values of a channel
     extern __shared__ float lds[];
@@ -304,7 +307,6 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
     float* lo_ml = lds + kWaves * kSplitRows * kPitch;        // [waves][16][2]
     Kept* kept = reinterpret_cast<Kept*>(lds + kWaves * kSplitRows * (kPitch + 2));
     const int n_wg = gridDim.x - 1;
-    int chunk, units, n_groups;           // in vector registers: the main loop needs the scalar ones
     {
         const AttnArgs& A = args_again();
         const Groups groups = groups_in_lanes(A, threadIdx.x & (kWave - 1));
@@ -313,14 +315,14 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
             write_plan<D>(A, groups, cuts, threadIdx.x);
             return;
         }
-        chunk = parked(cuts.chunk), units = parked(cuts.units), n_groups = parked(cuts.n_groups);
+        kept->cuts = cuts;                                    // by all waves the same
+        __syncthreads();
     }
     // The sums of an item, for rows n: of 2^(kLift - mref) p' v / vs, and of p; and what is left to do for it.
     v4f acc[kM];
     float mref;
     LaneSum sum;
     bool open = false;
-    int o_item = 0, o_rows = 0;
     for (int item = blockIdx.x;; item += n_wg) {
         // The next item's first loads are on their way while the last one's waves are joined.
         int tid = threadIdx.x;
@@ -330,16 +332,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
         const AttnArgs& A = args_again();
         const int h_kv = A.c.h_kv, page_log = A.c.page_log, n_pages = A.c.n_pages;
         Piece it{};
-        const bool any = piece_at<D>(A, kept, FewCuts{taken(chunk), taken(units), taken(n_groups)}, item, lane, &it);
+        const bool any = piece_at<D>(A, kept, FewCuts{taken(kept->cuts.chunk), taken(kept->cuts.units), taken(kept->cuts.n_groups)}, item, lane, &it);
         if (!any && !open) return;
         const int e = it.e, r0 = it.r0, kv = it.kv, t1 = it.t1;
         int t = it.t0 + w;
         const int32_t* tab = A.a.table + (size_t)it.table_row * A.a.width;
-        const int8_t *kb = A.c.k + ((size_t)e << page_log) * D, *vb = A.c.v + ((size_t)e << page_log) * D;
-        const float *ksb = A.c.k_scale + e, *vsb = A.c.v_scale + e;
-        int step = 16 << page_log;                            // of 16 channels
-        asm volatile("" : "+v"(ksb), "+v"(vsb), "+v"(kb), "+v"(vb), "+v"(step));           // not in scalar registers, which are few
-        const uint32_t page_bytes = (uint32_t)(h_kv << page_log) * D;
+        const int step = 16 << page_log;                      // of 16 channels
+        const uint32_t page_bytes = (uint32_t)(h_kv << page_log) * D, head = (uint32_t)(e << page_log) * D;      // both below 2^31
         // What is loaded of a tile behind the last is the last's again, and not used.
         const auto page_of = [&](int t, int off) {
             const int j = min(t, t1 - 1) * kTok + off, id = j < kv ? tab[j >> page_log] : -1;
@@ -349,17 +348,22 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
         uint4 kr[kS][kC];
         Codes vr[kM];
         const auto load_k = [&](int t, int page) {
-            const int8_t* p = kb + (size_t)max(page, 0) * page_bytes + (slot_of(t, keys) + (n & 3)) * D + 16 * g;
+            const int8_t* p = args_again().c.k + head + (size_t)max(page, 0) * page_bytes + (slot_of(t, keys) + (n & 3)) * D + 16 * g;
 #pragma unroll
             for (int i = 0; i < kS; ++i)
 #pragma unroll
                 for (int c = 0; c < kC; ++c) kr[i][c] = *reinterpret_cast<const uint4*>(p + 4 * i * D + 64 * c);
         };
         const auto values_at = [&](int t, int page) {
-            return vb + (size_t)max(page, 0) * page_bytes + (n << page_log) + slot_of(t, mine);
+            return args_again().c.v + head + (size_t)max(page, 0) * page_bytes + (n << page_log) + slot_of(t, mine);
         };
         int pv = -1, pk_next = -1, pv_next = -1;
         float ks = 0.0f, vs = 0.0f;
+        const auto load_scales = [&](int page) {
+            const size_t at = (size_t)max(page, 0) * h_kv + e;
+            ks = args_again().c.k_scale[at];
+            vs = args_again().c.v_scale[at];
+        };
         // q: wave c takes channels 64 c + 16 g .. + 15 of every row (row n its lanes'), as two int8 of 16 bits
         uint4 raw[2] = {};
         if (any) pv = page_of(t, mine), pk_next = page_of(t + kWaves, keys), pv_next = page_of(t + kWaves, mine);
@@ -374,13 +378,12 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
             const int8_t* p = values_at(t, pv);
 #pragma unroll
             for (int m = 0; m < kM; ++m, p += step) vr[m] = *reinterpret_cast<const Codes*>(p);
-            ks = ksb[(size_t)max(pv, 0) * h_kv];
-            vs = vsb[(size_t)max(pv, 0) * h_kv];
+            load_scales(pv);
         }
         if (open) {                                      // the four waves' parts of the last item together
             const ItemParts<kSplitRows, D> parts(args_again().item_part, args_again().n_items);
             const float m = mref == -__builtin_inff() ? kNone : mref - kLift, lse = sum.log2_row(m);
-            const int x_item = taken(o_item), x_rows = taken(o_rows);
+            const int x_item = taken(kept->item), x_rows = taken(kept->rows);
             lds_barrier();                                    // q has been read
             if (g == 0) {
                 lo_ml[(w * kSplitRows + n) * 2] = m;
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
         lds_barrier();
 
         mref = -__builtin_inff(), sum = LaneSum{};
-        o_item = parked(item), o_rows = parked(it.rows - r0);
+        kept->item = item, kept->rows = it.rows - r0;         // by all waves the same, behind the last item's
 #pragma unroll
         for (int m = 0; m < kM; ++m) acc[m] = v4f{0, 0, 0, 0};
         for (; t < t1; t += kWaves) {
@@ -452,8 +455,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(AttnArgs A_) {
             }
             __builtin_amdgcn_sched_barrier(0);
             load_k(t + kWaves, pk_next);
-            ks = ksb[(size_t)max(pv_next, 0) * h_kv];
-            vs = vsb[(size_t)max(pv_next, 0) * h_kv];
+            load_scales(pv_next);
             if (at > full || __ballot(lost)) {
                 asm volatile("");                             // a branch: most tiles are seen as a whole
                 const uint32_t seen = lost ? 0 : low_bits(pos - at - mine + 1);
@@ -566,7 +568,7 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(AttnArgs A, int first)
 struct SharedPlan {
     Plan own;
     bool many;                // groups' rows may be block_kernel's
-    int n_wg;                 // workgroups of block_kernel that the chip holds
+    int n_wg, few_wg;         // workgroups of block_kernel and of few_kernel that the chip holds
     long long n_items, n_shared;
     size_t seq, items, shared, shared_items, row_o, row_ml, bytes;
 };
@@ -578,7 +580,8 @@ SharedPlan shared_plan(int d, int h_kv, int G, int n_seq, int T, int max_q, int 
     p.n_wg = d == 256 ? p.own.n_wg / 2 : p.own.n_wg;
     // a sequence or group has at most one block that is not full; the groups may be few_kernel's
     const long long segments = (2 * (rows / kSplitRows) + nonempty + n_groups) * h_kv, blocks = (rows / kBlockRows + n_groups) * h_kv;
-    p.n_items = few_items(segments, p.own.n_wg - 1);
+    p.few_wg = p.own.n_wg / 2 * few_per_cu(d);
+    p.n_items = few_items(segments, p.few_wg - 1);
     p.n_shared = blocks < p.n_wg / 2 ? p.n_wg : (blocks + p.n_wg - 1) / p.n_wg * p.n_wg + p.n_wg;
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const auto item_bytes = [&](long long n, int block) { return up((size_t)n * block * (d + 2) * sizeof(float)); };
@@ -612,7 +615,7 @@ hipError_t launch_shared(AttnArgs& A, const SharedPlan& p, hipStream_t s) {
     static OncePerDevice once;
     hipError_t e = allow_lds(once, &few_kernel<D>, lds, s);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((few_kernel<D>), dim3((unsigned)p.own.n_wg), dim3(kThreads), lds, s, A);
+    hipLaunchKernelGGL((few_kernel<D>), dim3((unsigned)p.few_wg), dim3(kThreads), lds, s, A);
     e = hipGetLastError();
     if (e == hipSuccess && p.many) e = launch_shared_blocks(A, p.n_wg, s);
     if (e == hipSuccess && p.own.block) e = launch_own_blocks(A, p.own, s);
