@@ -384,8 +384,8 @@ hipError_t launch_append(const Kv8& c, const Batch& a, const ix_rows* k, const i
 }
 
 // Queries of up to this many values are turned in the append's launch, more in one of their own: there a CU holds 20 waves for
-// them, here 16, but a launch is 4 us. us, of 16 heads of 256 for 1,024, 2,048, 8,192 and 32,768 tokens here 17, 23, 58, 202, there 18,
-// 22, 46, 159; of 32 of 128, pages of 32, 18, 22, 56, 236 and 22, 26, 59, 225 (a read of the cache in all).
+// them, here 16, but a launch is 4 us. us, of 16 heads of 256 for 1,024, 2,048, 8,192 and 32,768 tokens here 17, 23, 48, 184, there 17,
+// 23, 47, 159; of 32 of 128, pages of 32, 18, 22, 56, 240 and 22, 27, 58, 226 (a read of the cache in all).
 constexpr long long kFewTurned = 1 << 24;
 
 template <int kThreads>
