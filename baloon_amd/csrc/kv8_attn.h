@@ -34,7 +34,7 @@ struct AttnArgs {
     int first, blocks;        // where a launch of it begins, and its workgroups in all launches
     // Of a batch with shared tokens (kv8_shared.hip):
     const int32_t *groups, *shared;   // sequences groups[g] .. groups[g + 1] - 1 have their first shared[g] tokens in common
-    int n_groups;
+    int n_groups, max_q;
     struct SeqPlan* seq;      // [n_seq]
     struct SharedItem* shared_items;  // of block_kernel, each for all heads
     float *item_part, *shared_part;   // partial results of few_kernel's items and of block_kernel's over shared tokens

@@ -160,6 +160,7 @@ struct Kept {
     long long tiles[kWaves], segments[kWaves];
     FewCuts cuts;                         // and what the main loop has no registers for
     int item, rows;
+    int2 found[kWaves];                   // where a wave found its last item: the 64 units, and the items before them (for one head)
 };
 template <int D>
 __device__ __forceinline__ int group_units(const AttnArgs& A, const Groups& groups, int lane) {
@@ -223,13 +224,15 @@ struct Piece {
     int table_row, e, s0, rows, r0, first, kv, t0, t1;
 };
 template <int D>
-__device__ __forceinline__ bool piece_at(const AttnArgs& A, const Kept* kept, const FewCuts& cuts, int item, int lane, Piece* out) {
-    int left = item / A.c.h_kv;
-    for (int u0 = 0; u0 < cuts.units; u0 += kWave) {
+__device__ __forceinline__ bool piece_at(const AttnArgs& A, Kept* kept, const FewCuts& cuts, int item, int w, int lane, Piece* out) {
+    const int2 from = kept->found[w];                         // a workgroup's items ascend
+    int left = item / A.c.h_kv - taken(from.y);
+    for (int u0 = taken(from.x); u0 < cuts.units; u0 += kWave) {
         const Unit u = kept_unit<D>(A, kept, u0 + lane, cuts, lane);
         const int p = cuts.parts(u), count = blocks_of(u) * p, incl = wave_scan_int(count);
         const unsigned long long hit = __ballot(incl > left);
         if (hit) {
+            if (lane == 0) kept->found[w] = make_int2(u0, item / A.c.h_kv - left);
             const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
             const int parts = lane_of(p, l), in = left - lane_of(incl - count, l), rb = in / parts, part = in - rb * parts;
             const int t0 = lane_of(u.t0, l), nt = lane_of(u.nt, l);
@@ -316,6 +319,7 @@ __global__ void __launch_bounds__(kThreads, few_per_cu(D)) few_kernel(AttnArgs A
             return;
         }
         kept->cuts = cuts;                                    // by all waves the same
+        if (threadIdx.x < kWaves) kept->found[threadIdx.x] = make_int2(0, 0);
         __syncthreads();
     }
     // The sums of an item, for rows n: of 2^(kLift - mref) p' v / vs, and of p; and what is left to do for it.
@@ -332,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, few_per_cu(D)) few_kernel(AttnArgs A
         const AttnArgs& A = args_again();
         const int h_kv = A.c.h_kv, page_log = A.c.page_log, n_pages = A.c.n_pages;
         Piece it{};
-        const bool any = piece_at<D>(A, kept, FewCuts{taken(kept->cuts.chunk), taken(kept->cuts.units), taken(kept->cuts.n_groups)}, item, lane, &it);
+        const bool any = piece_at<D>(A, kept, FewCuts{taken(kept->cuts.chunk), taken(kept->cuts.units), taken(kept->cuts.n_groups)}, item, w, lane, &it);
         if (!any && !open) return;
         const int e = it.e, r0 = it.r0, kv = it.kv, t1 = it.t1;
         int t = it.t0 + w;
@@ -522,7 +526,7 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(AttnArgs A, int first)
     const int t = __builtin_amdgcn_readfirstlane((int)(all / per)), out = (int)(all - (long long)t * per) * kOutputs + lane;
     const int b = wave_search(A.a.n_seq, t, lane, [&](int i) { return A.a.start(i); });
     const int s0 = A.a.start(b), end = A.a.start(b + 1);
-    if (t < s0 || t >= end) return;                           // of no sequence
+    if (t < s0 || t >= end || end - s0 > A.max_q) return;     // of no sequence, or of one that has no partial results
     const bool any = out < A.h_q * (D / 4);
     const int h = any ? out / (D / 4) : 0, d = out % (D / 4) * 4, e = h / A.G, in_token = h - e * A.G, rows = (end - s0) * A.G;
     const SeqPlan plan = A.seq[b];
@@ -609,6 +613,7 @@ hipError_t launch_shared(AttnArgs& A, const SharedPlan& p, hipStream_t s) {
     A.n_items = (int)p.n_items;
     A.n_shared = (int)p.n_shared;
     A.many = p.many;
+    A.max_q = p.own.max_q;
     A.slots = p.n_wg;
     A.small = attn_small(A, p.own);
     constexpr unsigned lds = kWaves * kSplitRows * (D + 4 + 2) * sizeof(float) + sizeof(Kept);

@@ -162,6 +162,25 @@ def test_many_sequences(n_groups):
 
 
 @pytest.mark.gpu
+def test_thousands_of_sequences():
+    """2,500 of one token each in 3 groups, 5,000 without new tokens among them."""
+    g = np.random.default_rng(8)
+    lens = [(int(i % 3 == 0), int(n)) for i, n in enumerate(g.integers(1, 5, 7500))]
+    Shared([group(64, *lens[:3000]), group(0, *lens[3000:3100]), group(100, *lens[3100:])], h=1, G=1).both()
+
+
+@pytest.mark.gpu
+def test_sequences_longer_than_said():
+    """Rows of sequences with more new tokens than max_q says are not written, those of the others are right."""
+    for new, G in ((3, 2), (200, 8)):
+        p = Shared([group(130, (1, 1), (new, new + 9), (2, 2))], h=2, G=G, seed=new)
+        got = p.run(max_q=new - 1)
+        assert np.isnan(got[1:1 + new]).all()
+        got[1:1 + new] = p.run()[1:1 + new]
+        p.check(got)
+
+
+@pytest.mark.gpu
 def test_as_without_groups():
     """Without groups the call is ix_kv8_attn; groups that share nothing, and groups of one sequence, are right."""
     lens = [(1, 300), (5, 90), (1, 1), (40, 700)]
