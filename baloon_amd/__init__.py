@@ -552,7 +552,7 @@ def ix_rope_rows(rope: Rope, n_seq, total_T, cu_seqlens, kv_len, x, heads, d, y,
 
 def ix_kv8_append_rope(cache: Kv8, n_seq, total_T, cu_seqlens, kv_len, table, width, k, v, rope_k, q=None, h_q=0, rope_q=None,
                        q_out=None, s=None) -> int:
-    """ix_kv8_append with keys that are normed and turned on the way, and in the same launch the queries: q_out
+    """ix_kv8_append with keys that are normed and turned on the way, and beside them the queries: q_out
     [total_T][h_q][d] bf16 is what ix_rope_rows makes of q with rope_q. q is a bf16 tensor of rows [h_q][d] of any stride."""
     if cache is not None:
         _check_norm(rope_k, cache.d)

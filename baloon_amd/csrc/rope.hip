@@ -1,4 +1,9 @@
 // rope.hip -- rows of heads normed and turned by position (ix_rope_rows; the formulas are rope.h's).
+//
+// Every value is read and written once, so HBM bounds it: a wave takes one token's 4 rows of 512 channels, 8 of 256, 16 of 128,
+// its loads under way while it works out the token's cosines and sines, which stand in LDS for all of them. 4,096 tokens of 32 heads
+// of 128, all channels turned: 67 MB in 13.6 us, 4.9 TB/s of a copy's 5.45; with a norm, 16 heads of 256 of which 64 channels turn,
+// 15,059 tokens: 247 MB in 53 us, 4.7 TB/s. A single token: 3.9 us, the call's launch.
 #include "rope.h"
 
 namespace ixg {

@@ -91,7 +91,7 @@ class AttnLayer:
     rope (``baloon_amd.rope``) norms and turns queries by position before they attend, rope_k (rope itself if not given) keys
     before they are stored. With max_forks, up to so many groups of slots may share a prompt (`fork`), which calls of up to 16
     new tokens a slot in the mean then read once for all of them, where that is worth it (`worth`: codes of keys that need
-    not be read again)."""
+    not be read again), with a workspace of their own (57, 202 and 420 MiB for 4, 64 and 256 slots of 2 heads of 256)."""
 
     def __init__(self, n_slots: int, max_len: int, h_q=16, h_kv=2, d=256, page=64, n_pages=None, window=0, sinks=0,
                  scale=None, device="cuda", rope=None, rope_k=None, max_forks=0, worth=200_000_000):
