@@ -276,7 +276,8 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
             }
             if (few) continue;
             const int rows = lane_of(g.rows, l), kv = lane_of(g.kv, l), all = kv / kBlockTok, row = lane_of(first, l);
-            for (int i = lane; i < lane_of(items, l); i += kWave) {
+            const int last_item = item < 0 ? 0 : min(lane_of(items, l), A.n_shared / A.c.h_kv - item);     // all, unless groups overlap
+            for (int i = lane; i < last_item; i += kWave) {
                 const int rb = i / n, part = i - rb * n;
                 A.shared_items[item + i] = SharedItem{s0, rows, rb * kBlockRows, row, (int)((long long)all * part / n),
                                                       (int)((long long)all * (part + 1) / n), kv, 0};
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, few_per_cu(D)) few_kernel(AttnArgs A
         const AttnArgs& A = args_again();
         const int h_kv = A.c.h_kv, page_log = A.c.page_log, n_pages = A.c.n_pages;
         Piece it{};
-        const bool any = piece_at<D>(A, kept, FewCuts{taken(kept->cuts.chunk), taken(kept->cuts.units), taken(kept->cuts.n_groups)}, item, w, lane, &it);
+        const bool any = item < A.n_items && piece_at<D>(A, kept, FewCuts{taken(kept->cuts.chunk), taken(kept->cuts.units), taken(kept->cuts.n_groups)}, item, w, lane, &it);
         if (!any && !open) return;
         const int e = it.e, r0 = it.r0, kv = it.kv, t1 = it.t1;
         int t = it.t0 + w;
@@ -538,8 +539,9 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(AttnArgs A, int first)
     if (!kWays || w == 0) z = load_gate(A, t, h, d);
     Joined sum;
     const int way = kWays ? w : 0, step = kWays ? kWaves : 1;
-    const auto add = [&](const auto& parts, int block, int rows_of, int first_item, int n, int in, int from) {
-        size_t at = ((size_t)(first_item + block * n + from) * h_kv + e) * rows_of + in;
+    const auto add = [&](const auto& parts, int room, int rows_of, int first, int n, int in, int from) {
+        if (first < 0 || first > room / h_kv - n) return;     // only where sequences or groups overlap, which is not allowed
+        size_t at = ((size_t)(first + from) * h_kv + e) * rows_of + in;
 #pragma unroll 8
         for (int k = from; k < n; k += step, at += (size_t)step * h_kv * rows_of)
             sum.more(parts.ml[2 * at], parts.ml[2 * at + 1], *reinterpret_cast<const v4f*>(parts.o + at * D + d));
@@ -549,7 +551,7 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(AttnArgs A, int first)
     if (rows <= A.small) {
         const int r = (t - s0) * A.G + in_token, rb = r / kSplitRows;
         own = plan.parts;
-        add(few, rb, kSplitRows, plan.item, own, r - rb * kSplitRows, way);
+        add(few, A.n_items, kSplitRows, plan.item + rb * own, own, r - rb * kSplitRows, way);
     } else if (way == 0) {
         const size_t at = (size_t)t * A.h_q + h;
         sum.more(A.row_ml[2 * at], A.row_ml[2 * at + 1], *reinterpret_cast<const v4f*>(A.row_o + at * D + d));
@@ -557,8 +559,9 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(AttnArgs A, int first)
     if (plan.shared_parts > 0) {
         const int r = (t - plan.s0) * A.G + in_token, n = plan.shared_rows, block = r / n, in = r - block * n;
         const int from = kWays ? (way - own) & (kWaves - 1) : 0;
-        if (n == kSplitRows) add(few, block, kSplitRows, plan.shared_item, plan.shared_parts, in, from);
-        else add(ItemParts<kBlockRows, D>(A.shared_part, A.n_shared), block, kBlockRows, plan.shared_item, plan.shared_parts, in, from);
+        const int first = plan.shared_item + block * plan.shared_parts;
+        if (n == kSplitRows) add(few, A.n_items, kSplitRows, first, plan.shared_parts, in, from);
+        else add(ItemParts<kBlockRows, D>(A.shared_part, A.n_shared), A.n_shared, kBlockRows, first, plan.shared_parts, in, from);
     }
     if constexpr (kWays) {
         lo_o[tid] = sum.o;

@@ -218,6 +218,10 @@ def test_shared_tokens_that_are_new():
     for groups in ([0, 1 << 30], [-7, 2], [2, 0]):
         p.shared, p.groups = [64], groups
         p.run()
+    p = Shared([group(64, *[(1, 20)] * 40)], G=16)
+    for n in (3, 700):                                          # groups that overlap, over and over
+        p.shared, p.groups = [64] * n, ([0, 40] * n)[:n + 1]
+        p.run()
 
 
 @pytest.mark.gpu
