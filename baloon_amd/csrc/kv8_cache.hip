@@ -205,16 +205,13 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
             const Rope& r = turn.k;
             RopeLane L;
             L.begin(r, lane);
-            const int rows_log = 6 - per_log, n = r.half << rows_log;
+            const int row = lane >> per_log, per = 1 << per_log;             // a row's pairs are those of the lanes that hold it
             wave_lds_sync();
 #pragma unroll 1
             for (int i0 = tid - lane; i0 < chunks; i0 += kThreads) {                      // the wave's own chunks, whole rows of them
-                const int i = i0 + lane, first = job.pos + job.held + (i0 >> per_log);
+                const int i = i0 + lane, pos = job.pos + job.held + (i0 >> per_log) + row;
 #pragma unroll 1
-                for (int j = lane; j < n; j += kWave) {
-                    const int row = (int)((unsigned)j / (unsigned)r.half);
-                    table[j] = cos_sin(r, first + row, r.freq[j - row * r.half]);
-                }
+                for (int j = lane & (per - 1); j < r.half; j += per) table[row * r.half + j] = cos_sin(r, pos, r.freq[j]);
                 wave_lds_sync();
                 uint4 x = make_uint4(0, 0, 0, 0), other = x;
                 if (i < chunks) {
@@ -223,7 +220,7 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
                                          [](const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); });
                 }
                 float F[8], S[8];
-                L.factors(r, table + (lane >> per_log) * r.half, F, S);
+                L.factors(r, table + row * r.half, F, S);
                 x = L.turned(r, x, other, F, S);
                 m = fmaxf(m, max_abs(x));
                 wave_lds_sync();
