@@ -173,6 +173,35 @@ def test_captured():
         assert layer.kv_len.tolist() == [8] + [tokens + 8] * 5
 
 
+@pytest.mark.parametrize("as_address", [False, True])
+def test_a_stream_that_is_behind(as_address):
+    """A prompt, a fork, tokens and a release, all on a stream that is busy when the first is made."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(6)
+    rq, rk = ropes(g, 64)
+    layer, other = (bx.AttnLayer(3, 400, 4, 2, 64, 16, rope=rq, rope_k=rk, max_forks=1, worth=0) for _ in "ab")
+    prompt, steps = drawn(g, 301, 4, 2, 64), [drawn(g, 3, 4, 2, 64) for _ in range(4)]
+    side, busy = torch.cuda.Stream(), torch.randn(4096, 4096, device="cuda")
+    cu = ints([0, 301, 301, 301])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy = busy @ busy * 1e-3
+    s = side.cuda_stream if as_address else side
+    got = [layer.prefill(cu, 301, *prompt, stream=s)]
+    behind = not side.query()
+    layer.fork(0, 3, 301, stream=s)
+    got += [layer.decode(*x, stream=s) for x in steps]
+    layer.release(0, stream=s)
+    side.synchronize()
+    assert behind
+    want = [other.prefill(cu, 301, *prompt)]
+    other.fork(0, 3, 301)
+    want += [other.decode(*x) for x in steps]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert layer.kv_len.tolist() == [305, 0, 0]
+
+
 def test_refusals():
     import torch
     g = torch.Generator(device="cuda").manual_seed(1)
