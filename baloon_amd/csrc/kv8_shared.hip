@@ -141,9 +141,9 @@ struct FewCuts {
     int chunk, units, n_groups;           // groups among the units
     __device__ __forceinline__ int parts(const Unit& u) const { return (u.nt + chunk - 1) / chunk; }
 };
-// The items of `segments` blocks: at most this.
-__host__ __device__ inline long long few_items(long long segments, int n_wg) {
-    const long long rounds = segments / n_wg + 1;
+// The items of `segments` blocks (below 2^29): at most this.
+__host__ __device__ inline int few_items(int segments, int n_wg) {
+    const int rounds = (int)((unsigned)segments / (unsigned)n_wg) + 1;
     return (rounds * n_wg - segments < n_wg / 4 ? rounds + 1 : rounds) * n_wg;
 }
 // Groups of up to kFewRows rows a kv head in the mean are always few_kernel's, those of more where all of them have up to kFewTiles
@@ -157,7 +157,8 @@ constexpr int kFewRows = 64, kFewTiles = 10000;
 constexpr int kKept = 512;
 struct Kept {
     int unit[6][kKept];
-    long long tiles[kWaves], segments[kWaves];
+    float tiles[kWaves];
+    int segments[kWaves];
     FewCuts cuts;                         // and what the main loop has no registers for
     int item, rows;
     int2 found[kWaves];                   // where a wave found its last item: the 64 units, and the items before them (for one head)
@@ -178,7 +179,8 @@ __device__ __forceinline__ FewCuts few_cuts(const AttnArgs& A, const Groups& gro
     const int lane = tid & (kWave - 1);
     out.n_groups = group_units<D>(A, groups, lane);
     out.units = out.n_groups + A.a.n_seq;
-    long long tiles = 0, segments = 0;
+    float tiles = 0.0f;
+    int segments = 0;
     for (int u0 = tid - lane; u0 < out.units; u0 += kThreads) {
         const Unit u = unit_at<D>(A, groups, out.n_groups, u0 + lane);
         if (u0 + lane < kKept) {
@@ -186,27 +188,26 @@ __device__ __forceinline__ FewCuts few_cuts(const AttnArgs& A, const Groups& gro
 #pragma unroll
             for (int i = 0; i < 6; ++i) kept->unit[i][u0 + lane] = x[i];
         }
-        tiles += (long long)blocks_of(u) * u.nt;
+        tiles += (float)blocks_of(u) * (float)u.nt;
         segments += blocks_of(u);
     }
-    tiles = lane_of(wave_scan_int(tiles), kWave - 1);
-    segments = lane_of(wave_scan_int(segments), kWave - 1);
-    if (lane == 0) {
+    tiles = wave_sum(tiles);
+    segments = wave_scan_int(segments);
+    if (lane == kWave - 1) {
         kept->tiles[tid / kWave] = tiles;
         kept->segments[tid / kWave] = segments;
     }
     __syncthreads();
-    tiles = segments = 0;
+    tiles = 0.0f, segments = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         tiles += kept->tiles[w];
         segments += kept->segments[w];
     }
-    tiles *= A.c.h_kv;
+    // chunk * room >= tiles: at most `room` items more than blocks. The sums' roundings are under 2^-16 of them.
     segments *= A.c.h_kv;
-    const long long room = few_items(segments, n_wg) - segments;
-    out.chunk = (int)min(max((tiles + room - 1) / room, (long long)kWaves), 0x7fffffffll);
-    out.chunk = __builtin_amdgcn_readfirstlane(out.chunk);
+    const float room = (float)(few_items(segments, n_wg) - segments), chunk = tiles * (float)A.c.h_kv * (1.0f + 0x1p-14f) / room;
+    out.chunk = __builtin_amdgcn_readfirstlane(max((int)fminf(ceilf(chunk), 0x1p30f), kWaves));
     return out;
 }
 template <int D>
@@ -235,10 +236,10 @@ __device__ __forceinline__ bool piece_at(const AttnArgs& A, Kept* kept, const Fe
             if (lane == 0) kept->found[w] = make_int2(u0, item / A.c.h_kv - left);
             const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
             const int parts = lane_of(p, l), in = left - lane_of(incl - count, l), rb = in / parts, part = in - rb * parts;
-            const int t0 = lane_of(u.t0, l), nt = lane_of(u.nt, l);
+            const int t0 = lane_of(u.t0, l), nt = lane_of(u.nt, l), each = nt / parts, more = nt - each * parts;
             const int row = u0 + l < cuts.n_groups ? group_first(A, u0 + l) : u0 + l - cuts.n_groups;
             *out = Piece{row, item % A.c.h_kv, lane_of(u.s0, l), lane_of(u.rows, l), rb * kSplitRows, lane_of(u.first, l), lane_of(u.kv, l),
-                         t0 + (int)((long long)nt * part / parts), t0 + (int)((long long)nt * (part + 1) / parts)};
+                         t0 + part * each + min(part, more), t0 + (part + 1) * each + min(part + 1, more)};
             return true;
         }
         left -= lane_of(incl, kWave - 1);
@@ -528,7 +529,8 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(AttnArgs A, int first)
     const int per = (A.h_q * (D / 4) + kOutputs - 1) / kOutputs;         // waves of a token
     const long long all = ((long long)first + blockIdx.x) * (kWays ? 1 : kWaves) + (kWays ? 0 : w);
     if (all >= (long long)A.a.T * per) return;                // all threads with kWays, which alone have a barrier
-    const int t = __builtin_amdgcn_readfirstlane((int)(all / per)), out = (int)(all - (long long)t * per) * kOutputs + lane;
+    const int t = __builtin_amdgcn_readfirstlane(all >> 32 == 0 ? (int)((unsigned)all / (unsigned)per) : (int)(all / per));
+    const int out = (int)(all - (long long)t * per) * kOutputs + lane;
     const int b = wave_search(A.a.n_seq, t, lane, [&](int i) { return A.a.start(i); });
     const int s0 = A.a.start(b), end = A.a.start(b + 1);
     if (t < s0 || t >= end || end - s0 > A.max_q) return;     // of no sequence, or of one that has no partial results
@@ -592,7 +594,7 @@ SharedPlan shared_plan(int d, int h_kv, int G, int n_seq, int T, int max_q, int 
     // a sequence or group has at most one block that is not full; the groups may be few_kernel's
     const long long segments = (2 * (rows / kSplitRows) + nonempty + n_groups) * h_kv, blocks = (rows / kBlockRows + n_groups) * h_kv;
     p.few_wg = p.own.n_wg / 2 * few_per_cu(d);
-    p.n_items = few_items(segments, p.few_wg - 1);
+    p.n_items = segments > 1 << 28 ? 0 : few_items((int)segments, p.few_wg - 1);
     p.n_shared = blocks < p.n_wg / 2 ? p.n_wg : (blocks + p.n_wg - 1) / p.n_wg * p.n_wg + p.n_wg;
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const auto item_bytes = [&](long long n, int block) { return up((size_t)n * block * (d + 2) * sizeof(float)); };
