@@ -247,15 +247,11 @@ __device__ __forceinline__ bool piece_at(const AttnArgs& A, Kept* kept, const Fe
     return false;
 }
 
-// What block_kernel and gather_kernel ask of a sequence, by a workgroup that does nothing else.
+// What block_kernel and gather_kernel ask of a sequence, by a wave that does nothing else. A field is written once: the sequences that
+// share something are those whose own tokens begin behind the first.
 template <int D>
-__device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& groups, const FewCuts& cuts, int tid) {
-    const int lane = tid & (kWave - 1);
+__device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& groups, const FewCuts& cuts, int lane) {
     const bool few = cuts.n_groups == A.n_groups;
-    for (int b = tid; b < A.a.n_seq; b += kThreads) A.seq[b] = SeqPlan{};
-    for (int i = tid; A.many && i <= A.n_shared / A.c.h_kv; i += kThreads) A.shared_items[i].row = -1;
-    __syncthreads();
-    if (tid >= kWave) return;
     const Cuts blocks = few ? Cuts{1} : cuts_of<D>(A, A.slots, lane);
     int base = 0;
     for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
@@ -276,16 +272,18 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
                 A.seq[b].shared_rows = few ? kSplitRows : kBlockRows;
             }
             if (few) continue;
-            const int rows = lane_of(g.rows, l), kv = lane_of(g.kv, l), all = kv / kBlockTok, row = lane_of(first, l);
+            const int rows = lane_of(g.rows, l), kv = lane_of(g.kv, l), row = lane_of(first, l);
+            const int each = kv / kBlockTok / n, more = kv / kBlockTok - each * n;         // tiles of a part, and parts of one more
             const int last_item = item < 0 ? 0 : min(lane_of(items, l), A.n_shared / A.c.h_kv - item);     // all, unless groups overlap
             for (int i = lane; i < last_item; i += kWave) {
                 const int rb = i / n, part = i - rb * n;
-                A.shared_items[item + i] = SharedItem{s0, rows, rb * kBlockRows, row, (int)((long long)all * part / n),
-                                                      (int)((long long)all * (part + 1) / n), kv, 0};
+                A.shared_items[item + i] = SharedItem{s0, rows, rb * kBlockRows, row, part * each + min(part, more),
+                                                      (part + 1) * each + min(part + 1, more), kv, 0};
             }
         }
         base += lane_of(before + items, kWave - 1);
     }
+    for (int i = (few ? 0 : max(base, 0)) + lane; A.many && i <= A.n_shared / A.c.h_kv; i += kWave) A.shared_items[i].row = -1;
     base = few ? base : 0;
     for (int u0 = cuts.n_groups; u0 < cuts.units; u0 += kWave) {
         const Unit u = unit_at<D>(A, groups, cuts.n_groups, u0 + lane);
@@ -294,6 +292,7 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
             A.seq[b].from = u.t0 * kTokOf<D>;
             A.seq[b].item = base + before;
             A.seq[b].parts = parts;
+            if (u.t0 == 0) A.seq[b].shared_parts = 0;
         }
         base += lane_of(before + items, kWave - 1);
     }
@@ -320,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, few_per_cu(D)) few_kernel(AttnArgs A
         const Groups groups = groups_in_lanes(A, threadIdx.x & (kWave - 1));
         const FewCuts cuts = few_cuts<D>(A, groups, kept, n_wg, threadIdx.x);
         if ((int)blockIdx.x == n_wg) {
-            write_plan<D>(A, groups, cuts, threadIdx.x);
+            if (threadIdx.x < kWave) write_plan<D>(A, groups, cuts, threadIdx.x);
             return;
         }
         kept->cuts = cuts;                                    // by all waves the same
