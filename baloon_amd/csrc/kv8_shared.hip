@@ -36,6 +36,20 @@ __device__ __forceinline__ Group group_at(const AttnArgs& A, int g) {
     return out;
 }
 
+// The groups in the lanes of a wave, if there are up to 64.
+struct Groups {
+    Group g;
+    int first, last;
+};
+__device__ __forceinline__ Groups groups_in_lanes(const AttnArgs& A, int lane) {
+    Groups out{};
+    if (A.n_groups > kWave || lane >= A.n_groups) return out;
+    out.g = group_at(A, lane);
+    out.first = group_first(A, lane);
+    out.last = group_first(A, lane + 1);
+    return out;
+}
+
 // Many rows: the blocks of 128 rows of all groups and heads are taken in parts of about as many tiles each: group g has parts(g)
 // for each of its blocks, item ((blocks and parts of the groups before it) + block * parts + part) * h_kv + head.
 struct Cuts {
@@ -46,13 +60,13 @@ struct Cuts {
 // The items are at most A.n_shared. Up to 64 groups lane p - 1 knows the time of the longest group's tiles in p parts, beyond
 // that the room for items is filled.
 template <int D>
-__device__ __forceinline__ Cuts cuts_of(const AttnArgs& A, int n_wg, int lane) {
+__device__ __forceinline__ Cuts cuts_of(const AttnArgs& A, const Groups& groups, int n_wg, int lane) {
     Cuts out;
     long long tiles = 0, blocks = 0;
     int most = 0;
     Group g{};
     for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
-        g = group_at(A, g0 + lane);
+        g = A.n_groups <= kWave ? groups.g : group_at(A, g0 + lane);
         tiles += (long long)Cuts::blocks(g) * (g.kv / kBlockTok);
         blocks += Cuts::blocks(g);
         most = max(most, g.kv / kBlockTok);
@@ -79,19 +93,6 @@ __device__ __forceinline__ Cuts cuts_of(const AttnArgs& A, int n_wg, int lane) {
     return out;
 }
 
-// The groups in the lanes of a wave, if there are up to 64.
-struct Groups {
-    Group g;
-    int first, last;
-};
-__device__ __forceinline__ Groups groups_in_lanes(const AttnArgs& A, int lane) {
-    Groups out{};
-    if (A.n_groups > kWave || lane >= A.n_groups) return out;
-    out.g = group_at(A, lane);
-    out.first = group_first(A, lane);
-    out.last = group_first(A, lane + 1);
-    return out;
-}
 // The first own token of sequence b, a lane's own.
 __device__ __forceinline__ int first_own(const AttnArgs& A, const Groups& groups, int b) {
     int from = 0;
@@ -121,7 +122,7 @@ __device__ __forceinline__ Unit unit_at(const AttnArgs& A, const Groups& groups,
     constexpr int kTok = kTokOf<D>;
     Unit out{};
     if (u < n_groups) {
-        const Group g = group_at(A, u);
+        const Group g = A.n_groups <= kWave ? groups.g : group_at(A, u);       // the lane's own: these units are the first 64
         out = Unit{g.s0, g.rows, 0, g.kv / kTok, 1 << 30, g.kv};
     } else if (u - n_groups < A.a.n_seq) {
         const int b = u - n_groups, s0 = A.a.start(b), q = max(A.a.start(b + 1) - s0, 0), kv = max(A.a.kv_len[b], 0);
@@ -252,10 +253,10 @@ __device__ __forceinline__ bool piece_at(const AttnArgs& A, Kept* kept, const Fe
 template <int D>
 __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& groups, const FewCuts& cuts, int lane) {
     const bool few = cuts.n_groups == A.n_groups;
-    const Cuts blocks = few ? Cuts{1} : cuts_of<D>(A, A.slots, lane);
+    const Cuts blocks = few ? Cuts{1} : cuts_of<D>(A, groups, A.slots, lane);
     int base = 0;
     for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
-        const Group g = group_at(A, g0 + lane);
+        const Group g = A.n_groups <= kWave ? groups.g : group_at(A, g0 + lane);
         const int first = g.rows ? group_first(A, g0 + lane) : 0, last = g.rows ? group_first(A, g0 + lane + 1) : 0;
         const Unit u{g.s0, g.rows, 0, g.kv / kTokOf<D>, 0, 0};
         const int parts = few ? cuts.parts(u) : blocks.parts(g), items = (few ? blocks_of(u) : Cuts::blocks(g)) * parts;
@@ -302,7 +303,7 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
 // with the next one's loads under way; products and the layout of P are those of split_kernel. Every workgroup works out the cuts by
 // itself (2.5 us, where a kernel ahead of this one costs a launch); the way to an item's first tile is a chain of three reads, which
 // lies under the last item's join. Long own parts are bound by HBM: 96 sequences in groups of 4, 32 heads over 8 of 128, 225 MB
-// with the page tables in 48 us, 4.7 TB/s; shorter ones by that chain (64 of up to 1,000 own tokens 17.5 us, 11 for none).
+// with the page tables in 48 us, 4.7 TB/s; shorter ones by that chain (64 of up to 1,000 own tokens 17 us, 10 where there is next to nothing to do).
 template <int D>
 __global__ void __launch_bounds__(kThreads, few_per_cu(D)) few_kernel(AttnArgs A_) {
     constexpr int kC = D / 64, kM = D / 16, kPitch = D + 4, kTok = kTokOf<D>, kS = kTok / 16;
@@ -315,6 +316,10 @@ __global__ void __launch_bounds__(kThreads, few_per_cu(D)) few_kernel(AttnArgs A
     Kept* kept = reinterpret_cast<Kept*>(lds + kWaves * kSplitRows * (kPitch + 2));
     const int n_wg = gridDim.x - 1;
     {
+        // The argument's cache lines, asked for at once: else each is waited for where it is first used.
+        const int* line = reinterpret_cast<const int*>(&args_again());
+        static_assert(sizeof(AttnArgs) > 256 && sizeof(AttnArgs) <= 320);
+        asm volatile("" ::"s"(line[0]), "s"(line[16]), "s"(line[32]), "s"(line[48]), "s"(line[64]));
         const AttnArgs& A = args_again();
         const Groups groups = groups_in_lanes(A, threadIdx.x & (kWave - 1));
         const FewCuts cuts = few_cuts<D>(A, groups, kept, n_wg, threadIdx.x);
