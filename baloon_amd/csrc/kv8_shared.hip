@@ -20,26 +20,42 @@ constexpr int kGrain = 64;            // shared tokens are taken in whole 64s; w
 // A group's rows, and the tokens that are taken together.
 struct Group {
     int s0, rows, kv;
+    int alone;                // blocks of 16 rows of its sequences each for itself, about
 };
 __device__ __forceinline__ int group_first(const AttnArgs& A, int g) { return min(max(A.groups[g], 0), A.a.n_seq); }
 __device__ __forceinline__ Group group_at(const AttnArgs& A, int g) {
-    Group out{0, 0, 0};
+    Group out{};
     if (g >= A.n_groups) return out;
     const int first = group_first(A, g), last = group_first(A, g + 1), n = A.shared[g];
     out.s0 = A.a.start(first);
     const int tokens = A.a.start(last) - out.s0;
     if (tokens > 0 && last - first > 1 && (long long)tokens * A.G <= 1 << 30) {
         out.rows = tokens * A.G;
+        out.alone = (last - first) * (((unsigned)out.rows / (unsigned)(last - first) + kSplitRows - 1) / kSplitRows);
         out.kv = (int)min((long long)max(n, 0), (long long)A.a.width << A.c.page_log) / kGrain * kGrain;
     }
     if (out.kv == 0) out.rows = 0;
     return out;
 }
 
+// Whether few_kernel takes a group's tokens together: where that is fewer tiles, with 8 more for each block more that it begins.
+// Together and not, us: 37 sequences of 16 rows behind 2,049 tokens 38 and 35, 102 behind 208 56 and 48, 89 of 24 behind 75 28 and 22.
+template <int D>
+__device__ __forceinline__ bool few_shares(const Group& g) {
+    const float tiles = (float)(g.kv / kTokOf<D>);
+    return (float)g.alone * tiles > (float)((g.rows + kSplitRows - 1) / kSplitRows) * (tiles + 8.0f);
+}
+// few: those that are not worth it share nothing.
+template <int D>
+__device__ __forceinline__ Group settled(Group g, bool few) {
+    if (few && !few_shares<D>(g)) g.rows = g.kv = 0;
+    return g;
+}
 // The groups in the lanes of a wave, if there are up to 64.
 struct Groups {
     Group g;
     int first, last;
+    bool few;
 };
 __device__ __forceinline__ Groups groups_in_lanes(const AttnArgs& A, int lane) {
     Groups out{};
@@ -94,6 +110,7 @@ __device__ __forceinline__ Cuts cuts_of(const AttnArgs& A, const Groups& groups,
 }
 
 // The first own token of sequence b, a lane's own.
+template <int D>
 __device__ __forceinline__ int first_own(const AttnArgs& A, const Groups& groups, int b) {
     int from = 0;
     if (A.n_groups <= kWave) {
@@ -108,7 +125,7 @@ __device__ __forceinline__ int first_own(const AttnArgs& A, const Groups& groups
         lo += right ? half : 0;
         n = right ? n - half : half;
     }
-    return b >= group_first(A, lo) && b < group_first(A, lo + 1) ? group_at(A, lo).kv : 0;
+    return b >= group_first(A, lo) && b < group_first(A, lo + 1) ? settled<D>(group_at(A, lo), groups.few).kv : 0;
 }
 
 // What few_kernel takes: the groups, where block_kernel does not, and behind them the sequences of few rows.
@@ -122,12 +139,12 @@ __device__ __forceinline__ Unit unit_at(const AttnArgs& A, const Groups& groups,
     constexpr int kTok = kTokOf<D>;
     Unit out{};
     if (u < n_groups) {
-        const Group g = A.n_groups <= kWave ? groups.g : group_at(A, u);       // the lane's own: these units are the first 64
+        const Group g = A.n_groups <= kWave ? groups.g : settled<D>(group_at(A, u), groups.few);       // the lane's own: these units are the first 64
         out = Unit{g.s0, g.rows, 0, g.kv / kTok, 1 << 30, g.kv};
     } else if (u - n_groups < A.a.n_seq) {
         const int b = u - n_groups, s0 = A.a.start(b), q = max(A.a.start(b + 1) - s0, 0), kv = max(A.a.kv_len[b], 0);
         const int held = (int)min((long long)kv, (long long)A.a.width << A.c.page_log);
-        const int t0 = first_own(A, groups, b) / kTok;
+        const int t0 = first_own<D>(A, groups, b) / kTok;
         out = Unit{s0, (long long)q * A.G <= A.small ? q * A.G : 0, t0, max(held / kTok + (held % kTok != 0) - t0, 1), kv - q, held};
     }
     return out;
@@ -150,9 +167,8 @@ __host__ __device__ inline int few_items(int segments, int n_wg) {
 // Groups of up to kFewRows rows a kv head in the mean are always few_kernel's, those of more where all of them have up to kFewTiles
 // tiles of 16 rows: block_kernel takes a tile in half the time, but has 14 us before its first and for its partial results, of
 // which 3 remain where it finds nothing to do. us there and here: 8 sequences of 16 heads over 2 of 256 behind 1,000 tokens (64 rows)
-// 30 and 16; 64 behind 1,024, 4,096 and 8,190 (2,000, 8,200 and 16,400 tiles) 41, 44, 50 and 29, 42, 56; 37 of 4 tokens, 32 over 8 of
-// 128, behind 2,049 and 4,096 (9,500 and 19,000) 42, 51 and 40, 58; 128 of 20 over 4 behind 2,048 and 4,096 (5,100 and 10,200) 54, 62
-// and 57, 65.
+// 30 and 16, 16 of them 32 and 18; 64 behind 1,024, 4,096 and 8,190 (2,000, 8,200 and 16,400 tiles) 40, 44, 49 and 28, 41, 56; 128 of 20
+// over 4 of 128 behind 1,024, 2,048 and 4,096 (2,600, 5,100 and 10,200) 53, 54, 62 and 42, 45, 61.
 constexpr int kFewRows = 64, kFewTiles = 10000;
 // The first units, worked out once and kept in LDS, and the sums of all waves.
 constexpr int kKept = 512;
@@ -164,21 +180,27 @@ struct Kept {
     int item, rows;
     int2 found[kWaves];                   // where a wave found its last item: the 64 units, and the items before them (for one head)
 };
+// Whether the groups are few_kernel's, which settles what they share. Tiles that it would not share count less: they are no items of
+// their own. us as blocks of 128 and so: 37 sequences of 16 rows, 8 heads of 128, behind 2,049 and 4,096 tokens (9,500 and 19,000
+// tiles) 41, 48 and 36, 53; 64 of 16 and of 32 rows, 2 heads of 256, behind 2,048 (8,200 and 16,400) 49, 56 and 42, 75.
 template <int D>
-__device__ __forceinline__ int group_units(const AttnArgs& A, const Groups& groups, int lane) {
-    if (!A.many) return A.n_groups;
-    long long tiles = 0;
+__device__ __forceinline__ bool few_take(const AttnArgs& A, const Groups& groups, int lane) {
+    if (!A.many) return true;
+    float tiles = 0.0f;
     for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
         const Group g = A.n_groups <= kWave ? groups.g : group_at(A, g0 + lane);
-        tiles += (long long)((g.rows + kSplitRows - 1) / kSplitRows) * (g.kv / kTokOf<D>);
+        const float blocks = few_shares<D>(g) ? (float)((g.rows + kSplitRows - 1) / kSplitRows) : (D == 256 ? 0.8f : 0.6f) * (float)g.alone;
+        tiles += blocks * (float)(g.kv / kTokOf<D>);
     }
-    return lane_of(wave_scan_int(tiles), kWave - 1) * A.c.h_kv <= kFewTiles ? A.n_groups : 0;
+    return __builtin_amdgcn_readfirstlane((int)(wave_sum(tiles) * (float)A.c.h_kv <= (float)kFewTiles));
 }
 template <int D>
-__device__ __forceinline__ FewCuts few_cuts(const AttnArgs& A, const Groups& groups, Kept* kept, int n_wg, int tid) {
+__device__ __forceinline__ FewCuts few_cuts(const AttnArgs& A, Groups& groups, Kept* kept, int n_wg, int tid) {
     FewCuts out;
     const int lane = tid & (kWave - 1);
-    out.n_groups = group_units<D>(A, groups, lane);
+    groups.few = few_take<D>(A, groups, lane);
+    groups.g = settled<D>(groups.g, groups.few);
+    out.n_groups = groups.few ? A.n_groups : 0;
     out.units = out.n_groups + A.a.n_seq;
     float tiles = 0.0f;
     int segments = 0;
@@ -213,8 +235,12 @@ __device__ __forceinline__ FewCuts few_cuts(const AttnArgs& A, const Groups& gro
 }
 template <int D>
 __device__ __forceinline__ Unit kept_unit(const AttnArgs& A, const Kept* kept, int u, const FewCuts& cuts, int lane) {
-    if (cuts.units > kKept && (u | (kWave - 1)) >= kKept)     // the same for the wave
-        return unit_at<D>(A, groups_in_lanes(A, lane), cuts.n_groups, u);
+    if (cuts.units > kKept && (u | (kWave - 1)) >= kKept) {   // the same for the wave
+        Groups groups = groups_in_lanes(A, lane);
+        groups.few = cuts.n_groups > 0;
+        groups.g = settled<D>(groups.g, groups.few);
+        return unit_at<D>(A, groups, cuts.n_groups, u);
+    }
     Unit out{};
     if (u < cuts.units)
         out = Unit{kept->unit[0][u], kept->unit[1][u], kept->unit[2][u], kept->unit[3][u], kept->unit[4][u], kept->unit[5][u]};
@@ -256,7 +282,7 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
     const Cuts blocks = few ? Cuts{1} : cuts_of<D>(A, groups, A.slots, lane);
     int base = 0;
     for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
-        const Group g = A.n_groups <= kWave ? groups.g : group_at(A, g0 + lane);
+        const Group g = A.n_groups <= kWave ? groups.g : settled<D>(group_at(A, g0 + lane), groups.few);
         const int first = g.rows ? group_first(A, g0 + lane) : 0, last = g.rows ? group_first(A, g0 + lane + 1) : 0;
         const Unit u{g.s0, g.rows, 0, g.kv / kTokOf<D>, 0, 0};
         const int parts = few ? cuts.parts(u) : blocks.parts(g), items = (few ? blocks_of(u) : Cuts::blocks(g)) * parts;
@@ -321,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, few_per_cu(D)) few_kernel(AttnArgs A
         static_assert(sizeof(AttnArgs) > 256 && sizeof(AttnArgs) <= 320);
         asm volatile("" ::"s"(line[0]), "s"(line[16]), "s"(line[32]), "s"(line[48]), "s"(line[64]));
         const AttnArgs& A = args_again();
-        const Groups groups = groups_in_lanes(A, threadIdx.x & (kWave - 1));
+        Groups groups = groups_in_lanes(A, threadIdx.x & (kWave - 1));
         const FewCuts cuts = few_cuts<D>(A, groups, kept, n_wg, threadIdx.x);
         if ((int)blockIdx.x == n_wg) {
             if (threadIdx.x < kWave) write_plan<D>(A, groups, cuts, threadIdx.x);

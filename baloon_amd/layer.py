@@ -189,8 +189,8 @@ class AttnLayer:
             shared.append(tokens)
         self._n_groups = len(shared)
         # Reading shared tokens once pays from about 2e8 codes of keys on that need not be read again. us with and without, 37
-        # sequences of 4 new tokens, 32 heads over 8 of 128, behind 4,096 tokens 52 and 44, behind 8,192 63 and 82; 64 of one,
-        # 16 over 2 of 256, behind 2,048, 4,096 and 8,190 33, 42, 50 and 30, 41, 62; 24 times 4 behind 300 to 6,000 57 and 101.
+        # sequences of 4 new tokens, 32 heads over 8 of 128, behind 4,096 tokens 48 and 44, behind 8,192 59 and 83; 64 of one,
+        # 16 over 2 of 256, behind 2,048, 4,096 and 8,190 32, 42, 49 and 30, 41, 62; 24 times 4 behind 300 to 6,000 55 and 101.
         self._shared_pays = sum((n - 1) * tokens for n, tokens in self._forks.values()) * self.h_kv * self.d >= self.worth
         if shared:
             self._groups[:len(ends)] = torch.tensor(ends, dtype=torch.int32)
