@@ -162,6 +162,21 @@ def test_many_sequences(n_groups):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n_groups,each", [(100, 6), (20, 30), (70, 3)])
+def test_groups_that_save_something_and_groups_that_do_not(n_groups, each):
+    """Shared tokens from none to 12 tiles of them, in up to and over 64 groups, of up to and over 512 units."""
+    g = np.random.default_rng(each)
+    Shared([group(int(n), *[(1, int(m)) for m in g.integers(1, 30, each)]) for n in g.integers(0, 800, n_groups)], h=1, G=2).both()
+
+
+@pytest.mark.gpu
+def test_many_groups_of_many_rows():
+    """Over 64 groups by blocks of 128 rows, whose parts are then cut by the room for them."""
+    g = np.random.default_rng(3)
+    Shared([group(int(n), (1, 9), (1, 1), (1, 30)) for n in g.integers(2500, 3500, 66)], page=128, h=1, d=64, G=48).both()
+
+
+@pytest.mark.gpu
 def test_thousands_of_sequences():
     """2,500 of one token each in 3 groups, 5,000 without new tokens among them."""
     g = np.random.default_rng(8)
