@@ -6,6 +6,7 @@
 // together. few_kernel takes 16 rows a workgroup: each sequence's own tokens, and the shared ones of groups of few rows, all of
 // these in one launch; block_kernel (kv8_attn.hip) takes 128: the shared tokens of groups of many rows, and prompts.
 #include "kv8_attn.h"
+#include "shared_list.h"
 
 namespace ixg {
 namespace {
@@ -301,8 +302,8 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
             if (few) continue;
             const int rows = lane_of(g.rows, l), kv = lane_of(g.kv, l), row = lane_of(first, l);
             const int each = kv / kBlockTok / n, more = kv / kBlockTok - each * n;         // tiles of a part, and parts of one more
-            const int last_item = item < 0 ? 0 : min(lane_of(items, l), A.n_shared / A.c.h_kv - item);     // all, unless groups overlap
-            for (int i = lane; i < last_item; i += kWave) {
+            const int listed = items_listed(item, lane_of(items, l), A.n_shared / A.c.h_kv);
+            for (int i = lane; i < listed; i += kWave) {
                 const int rb = i / n, part = i - rb * n;
                 A.shared_items[item + i] = SharedItem{s0, rows, rb * kBlockRows, row, part * each + min(part, more),
                                                       (part + 1) * each + min(part + 1, more), kv, 0};
@@ -310,7 +311,8 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
         }
         base += lane_of(before + items, kWave - 1);
     }
-    for (int i = (few ? 0 : max(base, 0)) + lane; A.many && i <= A.n_shared / A.c.h_kv; i += kWave) A.shared_items[i].row = -1;
+    for (int i = (few ? 0 : list_end(base, A.n_shared / A.c.h_kv)) + lane; A.many && i <= A.n_shared / A.c.h_kv; i += kWave)
+        A.shared_items[i].row = -1;
     base = few ? base : 0;
     for (int u0 = cuts.n_groups; u0 < cuts.units; u0 += kWave) {
         const Unit u = unit_at<D>(A, groups, cuts.n_groups, u0 + lane);
