@@ -16,7 +16,8 @@ template <int D>
 constexpr int kTokOf = D == 256 ? 32 : 64;
 constexpr int few_per_cu(int d) { return d == 256 ? 2 : d == 128 ? 3 : 4; }      // few_kernel's workgroups, by its registers
 
-constexpr int kGrain = 64;            // shared tokens are taken in whole 64s; what is left over is each sequence's own
+constexpr int kGrain = 64;            // shared tokens are taken in whole 64s; what is left over is each sequence's own,
+constexpr int kFarthest = 1 << 30;    // and so are those from here on: where rows of a group are taken to stand, with room for as many of them
 
 // A group's rows, and the tokens that are taken together.
 struct Group {
@@ -30,10 +31,10 @@ __device__ __forceinline__ Group group_at(const AttnArgs& A, int g) {
     const int first = group_first(A, g), last = group_first(A, g + 1), n = A.shared[g];
     out.s0 = A.a.start(first);
     const int tokens = A.a.start(last) - out.s0;
-    if (tokens > 0 && last - first > 1 && (long long)tokens * A.G <= 1 << 30) {
+    if (tokens > 0 && last - first > 1 && (long long)tokens * A.G <= kFarthest) {
         out.rows = tokens * A.G;
         out.alone = (last - first) * (((unsigned)out.rows / (unsigned)(last - first) + kSplitRows - 1) / kSplitRows);
-        out.kv = (int)min((long long)max(n, 0), (long long)A.a.width << A.c.page_log) / kGrain * kGrain;
+        out.kv = (int)min((long long)min(max(n, 0), kFarthest), (long long)A.a.width << A.c.page_log) / kGrain * kGrain;
     }
     if (out.kv == 0) out.rows = 0;
     return out;
@@ -141,7 +142,7 @@ __device__ __forceinline__ Unit unit_at(const AttnArgs& A, const Groups& groups,
     Unit out{};
     if (u < n_groups) {
         const Group g = A.n_groups <= kWave ? groups.g : settled<D>(group_at(A, u), groups.few);       // the lane's own: these units are the first 64
-        out = Unit{g.s0, g.rows, 0, g.kv / kTok, 1 << 30, g.kv};
+        out = Unit{g.s0, g.rows, 0, g.kv / kTok, kFarthest, g.kv};
     } else if (u - n_groups < A.a.n_seq) {
         const int b = u - n_groups, s0 = A.a.start(b), q = max(A.a.start(b + 1) - s0, 0), kv = max(A.a.kv_len[b], 0);
         const int held = (int)min((long long)kv, (long long)A.a.width << A.c.page_log);
