@@ -133,8 +133,8 @@ class AttnLayer:
     def fork(self, slot, n, tokens, stream=None):
         """Slots slot + 1 .. slot + n - 1 go on from the first `tokens` tokens of `slot`, which holds as many, and from nothing that
         they held: its whole pages are theirs too, the page that the tokens end in is copied. Until `release`, none of the n may lose one of these
-        tokens (a shorter kv_len, then new tokens). Not to be captured; captured calls run with as many groups as there were,
-        so capture them again when a fork or a release has changed that (a fork released and made anew changes nothing)."""
+        tokens (a shorter kv_len, then new tokens). Not to be captured; calls that were captured before stay right, but take together
+        only what they knew of: with more forks, or where sharing has come to pay, capture them again."""
         others = range(slot + 1, slot + n)
         if slot < 0 or n < 2 or slot + n > self.n_slots or not 0 < tokens <= self.width * self.cache.page:
             raise ValueError("baloon_amd: a fork is of two slots or more, and of tokens that a slot can hold")
@@ -192,9 +192,10 @@ class AttnLayer:
         # sequences of 4 new tokens, 32 heads over 8 of 128, behind 4,096 tokens 48 and 44, behind 8,192 59 and 83; 64 of one,
         # 16 over 2 of 256, behind 2,048, 4,096 and 8,190 32, 42, 49 and 30, 41, 62; 24 times 4 behind 300 to 6,000 55 and 101.
         self._shared_pays = sum((n - 1) * tokens for n, tokens in self._forks.values()) * self.h_kv * self.d >= self.worth
-        if shared:
-            self._groups[:len(ends)] = torch.tensor(ends, dtype=torch.int32)
-            self._shared[:len(shared)] = torch.tensor(shared, dtype=torch.int32)
+        # A captured call has the groups that there were then: what is more than there are now is empty and shares nothing.
+        ends += [ends[-1] if ends else 0] * (len(self._groups) - len(ends))
+        self._groups.copy_(torch.tensor(ends, dtype=torch.int32))
+        self._shared.copy_(torch.tensor(shared + [0] * (len(self._shared) - len(shared)), dtype=torch.int32))
 
     def prefill(self, cu_seqlens, max_q, q, k, v, gate=None, o=None, stream=None):
         """Appends packed new tokens (cu_seqlens int32 [n_slots + 1] on the device, at most max_q of a sequence) and
