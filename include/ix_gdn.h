@@ -417,7 +417,8 @@ size_t ix_kv8_attn_workspace_size(const ix_kv8* cache, int n_seq, int total_T, i
  * the first `rot` channels is turned by its angle, the token's position times freq[i],
  *   y_a = amplitude * (f_a cos - f_b sin),  y_b = amplitude * (f_b cos + f_a sin)
  * and the channels behind them are f. Pair i is (i, i + rot / 2) in IX_ROPE_HALVES, (2 i, 2 i + 1) in IX_ROPE_PAIRS. However
- * positions are scaled for long contexts is in freq and amplitude; angles are exact to 2^-22 at any position. */
+ * positions are scaled for long contexts is in freq and amplitude. An angle (in radians, before whole turns are taken off) is
+ * off by at most 2^-23 and 2^-51 of itself: by 2^-22 up to 2^28, by under 2^-20 + 2^-23 at any position if freq is at most 1. */
 enum { IX_ROPE_HALVES = 0, IX_ROPE_PAIRS = 1 };
 typedef struct ix_rope {
     int rot;                  /* even, 0 (none) .. d */
