@@ -171,6 +171,12 @@ __host__ __device__ inline int few_items(int segments, int n_wg) {
 // which 3 remain where it finds nothing to do. us there and here: 8 sequences of 16 heads over 2 of 256 behind 1,000 tokens (64 rows)
 // 30 and 16, 16 of them 32 and 18; 64 behind 1,024, 4,096 and 8,190 (2,000, 8,200 and 16,400 tiles) 40, 44, 49 and 28, 41, 56; 128 of 20
 // over 4 of 128 behind 1,024, 2,048 and 4,096 (2,600, 5,100 and 10,200) 53, 54, 62 and 42, 45, 61.
+//
+// The mean says little where one group has most of the rows (of a captured call's groups many can be empty). So the device chooses
+// also where one group of all rows over a whole table would have over twice kFewTiles: 2 us where block_kernel then has nothing
+// to do (24 groups of 4 sequences over a table that wide 56 and 58). One group beside 63 empty ones with few_kernel alone and with
+// the choice, us: 64 sequences of 16 heads over 2 of 256 behind 8,192 and 16,384 tokens (18,400 and 34,800 such tiles) 56, 92 and (48), 59;
+// 128 behind 4,096 and 16,384 (20,500, 69,600) 88, 280 and 61, 86; 200 of 32 over 8 of 128 behind 16,384 (105,600) 199 and 122.
 constexpr int kFewRows = 64, kFewTiles = 10000;
 // The first units, worked out once and kept in LDS, and the sums of all waves.
 constexpr int kKept = 512;
@@ -182,19 +188,22 @@ struct Kept {
     int item, rows;
     int2 found[kWaves];                   // where a wave found its last item: the 64 units, and the items before them (for one head)
 };
-// Whether the groups are few_kernel's, which settles what they share. Tiles that it would not share count less: they are no items of
+// Whether the groups are few_kernel's, which settles what they share: where it has few tiles, or no more than as blocks of 128, which take
+// the time of kFewRows however few of them are rows. Of few tiles those that it would not share count less: they are no items of
 // their own. us as blocks of 128 and so: 37 sequences of 16 rows, 8 heads of 128, behind 2,049 and 4,096 tokens (9,500 and 19,000
 // tiles) 41, 48 and 36, 53; 64 of 16 and of 32 rows, 2 heads of 256, behind 2,048 (8,200 and 16,400) 49, 56 and 42, 75.
 template <int D>
 __device__ __forceinline__ bool few_take(const AttnArgs& A, const Groups& groups, int lane) {
     if (!A.many) return true;
-    float tiles = 0.0f;
+    float tiles = 0.0f, more = 0.0f;                          // more: than as blocks of 128
     for (int g0 = 0; g0 < A.n_groups; g0 += kWave) {
         const Group g = A.n_groups <= kWave ? groups.g : group_at(A, g0 + lane);
-        const float blocks = few_shares<D>(g) ? (float)((g.rows + kSplitRows - 1) / kSplitRows) : (D == 256 ? 0.8f : 0.6f) * (float)g.alone;
-        tiles += blocks * (float)(g.kv / kTokOf<D>);
+        const bool shares = few_shares<D>(g);
+        const int blocks = shares ? (g.rows + kSplitRows - 1) / kSplitRows : g.alone, t = g.kv / kTokOf<D>;
+        tiles += (shares ? 1.0f : D == 256 ? 0.8f : 0.6f) * (float)blocks * (float)t;
+        more += (float)(blocks - (g.rows + kBlockRows - 1) / kBlockRows * (kFewRows / kSplitRows)) * (float)t;
     }
-    return __builtin_amdgcn_readfirstlane((int)(wave_sum(tiles) * (float)A.c.h_kv <= (float)kFewTiles));
+    return __builtin_amdgcn_readfirstlane((int)(wave_sum(tiles) * (float)A.c.h_kv <= (float)kFewTiles || wave_sum(more) <= 0.0f));
 }
 template <int D>
 __device__ __forceinline__ FewCuts few_cuts(const AttnArgs& A, Groups& groups, Kept* kept, int n_wg, int tid) {
@@ -618,11 +627,12 @@ struct SharedPlan {
     long long n_items, n_shared;
     size_t seq, items, shared, shared_items, row_o, row_ml, bytes;
 };
-SharedPlan shared_plan(int d, int h_kv, int G, int n_seq, int T, int max_q, int n_groups, hipStream_t s) {
+SharedPlan shared_plan(int d, int h_kv, int G, int n_seq, int T, int max_q, int n_groups, long long table_tokens, hipStream_t s) {
     SharedPlan p;
     p.own = attn_plan(d, h_kv, G, T, max_q, s);
     const long long rows = (long long)T * G, nonempty = std::min(n_seq, T);
-    p.many = rows > (long long)kFewRows * n_groups;
+    const double tiles = (double)((rows + kSplitRows - 1) / kSplitRows) * (double)(table_tokens / (d == 256 ? kTokOf<256> : kTokOf<128>)) * h_kv;
+    p.many = rows > (long long)kFewRows * n_groups || (rows > kFewRows && tiles > 2.0 * kFewTiles);
     p.n_wg = d == 256 ? p.own.n_wg / 2 : p.own.n_wg;
     // a sequence or group has at most one block that is not full; the groups may be few_kernel's
     const long long segments = (2 * (rows / kSplitRows) + nonempty + n_groups) * h_kv, blocks = (rows / kBlockRows + n_groups) * h_kv;
@@ -689,7 +699,7 @@ size_t ix_kv8_attn_shared_workspace_size(const ix_kv8* cache, int n_seq, int tot
     Kv8 c;
     if (!make_kv8(cache, &c) || !attn_shape_ok(c, n_seq, total_T, max_q, h_q) || n_groups < 0 || n_groups > 65535) return 0;
     if (n_groups == 0) return ix_kv8_attn_workspace_size(cache, n_seq, total_T, max_q, h_q);
-    return shared_plan(c.d, c.h_kv, h_q / c.h_kv, n_seq, total_T, max_q, n_groups, nullptr).bytes;
+    return shared_plan(c.d, c.h_kv, h_q / c.h_kv, n_seq, total_T, max_q, n_groups, 0, nullptr).bytes;      // whatever the tables
 }
 
 hipError_t ix_kv8_attn_shared(const ix_kv8* cache, int n_seq, int total_T, int max_q, const int32_t* cu_seqlens, const int32_t* kv_len,
@@ -705,7 +715,7 @@ hipError_t ix_kv8_attn_shared(const ix_kv8* cache, int n_seq, int total_T, int m
     if (n_groups < 0 || n_groups > 65535 || !groups || !shared_len || !ptr_aligned(groups, 4) || !ptr_aligned(shared_len, 4))
         return hipErrorInvalidValue;
     if (total_T == 0) return hipSuccess;                      // of tensors without elements, whose addresses may be 0
-    const SharedPlan p = shared_plan(A.c.d, A.c.h_kv, A.G, n_seq, total_T, max_q, n_groups, s);
+    const SharedPlan p = shared_plan(A.c.d, A.c.h_kv, A.G, n_seq, total_T, max_q, n_groups, (long long)width << A.c.page_log, s);
     if (!p.bytes || !make_operands(q, gate, o, workspace, workspace_bytes, p.bytes, &A)) return hipErrorInvalidValue;
     A.groups = groups;
     A.shared = shared_len;
