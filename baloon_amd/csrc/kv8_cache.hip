@@ -139,7 +139,7 @@ __device__ __forceinline__ Turn turn_of(int i, int span_log) {
 // unrolled 8, 4 and 2 times a single token for 64 sequences took 7.9, 6.6 and 5.5 us of the kernel's time.
 //
 // With positions (Turned; ix_kv8_append_rope) the keys are normed, turned and rounded to bf16 where they lie in LDS, each wave
-// its own rows, so the codes are those of rows that ix_rope_rows has turned, bit for bit. Up to kFewTurned the queries are the
+// its own rows, so the codes are those of rows that ix_rope_rows has turned, bit for bit. Few queries (kFewTurned, kTurnedPerWave) are the
 // third part of the grid, item by item (rope.h). 16 sequences of 1 to 2,048 tokens, 2 heads of 256 of which 64 channels turn, and a
 // norm: 23 us of plain rows' 15; a token for each of 64 sequences, queries of 16
 // heads with it: 5.5 us of 5.2.
@@ -353,12 +353,15 @@ long long page_slots(const Kv8& c, const Batch& a) { return (a.T >> c.page_log) 
 // 9.2, 8.1, 9.7; 256 single tokens 16.7, 14.2, 14.2, 14.8, and on 2 heads of 256, pages of 64, 9.9, 8.7, 8.6, 9.7. A read of
 // the first takes 17.9, 17.7, 17.9, 17.6, of 64 pages of 16 tokens on 2 heads of 256 3.3, 3.5, 3.6, 3.6, of 1 x 4,096 4.5,
 // 4.6, 5.2, 5.2.
+constexpr int threads_for(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
 template <class F>
 hipError_t with_threads(int n, F launch) {
-    if (n <= 64) return launch(std::integral_constant<int, 64>{});
-    if (n <= 128) return launch(std::integral_constant<int, 128>{});
-    if (n <= 256) return launch(std::integral_constant<int, 256>{});
-    return launch(std::integral_constant<int, 512>{});
+    switch (threads_for(n)) {
+        case 64: return launch(std::integral_constant<int, 64>{});
+        case 128: return launch(std::integral_constant<int, 128>{});
+        case 256: return launch(std::integral_constant<int, 256>{});
+        default: return launch(std::integral_constant<int, 512>{});
+    }
 }
 
 template <int kThreads, class Pos>
@@ -384,6 +387,11 @@ hipError_t launch_append(const Kv8& c, const Batch& a, const ix_rows* k, const i
 // them, here 16, but a launch is 4 us. us, of 16 heads of 256 for 1,024, 2,048, 8,192 and 32,768 tokens here 17, 23, 48, 184, there 17,
 // 23, 47, 159; of 32 of 128, pages of 32, 18, 22, 56, 240 and 22, 27, 58, 226 (a read of the cache in all).
 constexpr long long kFewTurned = 1 << 24;
+// And where the append's part of the grid for them, as large as that for keys, has fewer than so many items a wave: each is a chain of
+// its own, and a launch of their own has a wave for each. us here and there, one sequence: 1,000 tokens of 32 heads over 8 of 128,
+// pages of 32 (3.8 a wave), 13 and 15; 120 of 16 over 2 of 256, pages of 64 (5.0), 15 and 12, 1,000 (7.4) 24 and 14; 1,024 of 16 over 1 of
+// 256, pages of 128 (26), 68 and 18, of 64 over 1 of 64 (51) 125 and 15; of 16 over 4 of 64, pages of 64, 120 (5.0) 12 and 13.
+constexpr int kTurnedPerWave = 4;
 
 template <int kThreads>
 hipError_t launch_read(const Kv8& c, const Batch& a, uint16_t* k, uint16_t* v, hipStream_t s) {
@@ -424,14 +432,15 @@ hipError_t ix_kv8_append_rope(const ix_kv8* cache, int n_seq, int total_T, const
     if (total_T == 0) return hipSuccess;                      // of tensors without elements, whose addresses may be 0
     if (!rows_ok(k, (long long)c.h_kv * c.d) || !rows_ok(v, (long long)c.h_kv * c.d)) return hipErrorInvalidValue;
     if (q && !make_rope_rows(rope_q, q, h_q, c.d, q_out, &turn.q)) return hipErrorInvalidValue;
-    const int few = a.T < (long long)c.page * a.n_seq ? 2 : 1, keys = turn.k.half << (6 - turn.k.per_log);
-    if (q && (long long)a.T * h_q * c.d <= kFewTurned) {
+    const int few = a.T < (long long)c.page * a.n_seq ? 2 : 1, keys = turn.k.half << (6 - turn.k.per_log), threads = c.page * c.d / 32 / few;
+    const long long waves = page_slots(c, a) * c.h_kv * (threads_for(threads) / kWave);
+    if (q && (long long)a.T * h_q * c.d <= kFewTurned && (long long)a.T * turn.q.groups < kTurnedPerWave * waves) {
         turn.table = std::max(keys, turn.q.r.half);
-        return with_threads(c.page * c.d / 32 / few, [&](auto n) { return launch_append<n>(c, a, k, v, turn, s); });
+        return with_threads(threads, [&](auto n) { return launch_append<n>(c, a, k, v, turn, s); });
     }
     const hipError_t e = q ? launch_rope(turn.q, a, s) : hipSuccess;
     if (e != hipSuccess) return e;
-    return with_threads(c.page * c.d / 32 / few, [&](auto n) { return launch_append<n>(c, a, k, v, Turned<false>{turn.k, {}, keys, 0}, s); });
+    return with_threads(threads, [&](auto n) { return launch_append<n>(c, a, k, v, Turned<false>{turn.k, {}, keys, 0}, s); });
 }
 
 hipError_t ix_kv8_read(const ix_kv8* cache, int n_seq, int total_T, const int32_t* cu_seqlens, const int32_t* kv_len,

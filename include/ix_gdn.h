@@ -435,8 +435,8 @@ typedef struct ix_rope {
 hipError_t ix_rope_rows(const ix_rope* rope, int n_seq, int total_T, const int32_t* cu_seqlens, const int32_t* kv_len,
                         const ix_rows* x, int heads, int d, uint16_t* y, hipStream_t s IX_GDN_DEFAULT_STREAM);
 
-/* ix_kv8_append with keys that are turned on the way, and the batch's queries turned beside them (in one launch up to 2^24
- * values of queries). The codes and scales are those of ix_kv8_append on the rows that ix_rope_rows would make of k (bf16), bit for bit; q_out
+/* ix_kv8_append with keys that are turned on the way, and the batch's queries turned beside them (in one launch where
+ * they are few: up to 2^24 values of them, and a few heads' rows for each page of new tokens). The codes and scales are those of ix_kv8_append on the rows that ix_rope_rows would make of k (bf16), bit for bit; q_out
  * [total_T][h_q][d] is what it makes of q (rows of [h_q][d]) with rope_q. q may be NULL: then h_q, rope_q and q_out have no
  * meaning. q_out may be the memory of q where that is packed, but not of k or v. */
 hipError_t ix_kv8_append_rope(const ix_kv8* cache, int n_seq, int total_T, const int32_t* cu_seqlens, const int32_t* kv_len,
