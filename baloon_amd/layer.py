@@ -86,7 +86,8 @@ class AttnLayer:
 
     All of a call is on one stream, the lengths and a new o among it: `stream` (a torch stream or an address), or torch's
     current one. The caller orders calls on different streams, and what else it does with the layer's tensors. The workspace
-    is allocated here for any batch (38 to 81 MiB), so a captured call's stays where it is.
+    is allocated here for any batch (38 to 81 MiB), so a captured call's stays where it is. Layers whose calls are ordered, as those
+    of a stack are, need one between them: `beside`, another layer, whose workspaces this one takes where they are large enough.
 
     rope (``baloon_amd.rope``) norms and turns queries by position before they attend, rope_k (rope itself if not given) keys
     before they are stored. With max_forks, up to so many groups of slots may share a prompt (`fork`), which calls of up to 16
@@ -94,7 +95,7 @@ class AttnLayer:
     not be read again), with a workspace of their own (57, 202 and 420 MiB for 4, 64 and 256 slots of 2 heads of 256)."""
 
     def __init__(self, n_slots: int, max_len: int, h_q=16, h_kv=2, d=256, page=64, n_pages=None, window=0, sinks=0,
-                 scale=None, device="cuda", rope=None, rope_k=None, max_forks=0, worth=200_000_000):
+                 scale=None, device="cuda", rope=None, rope_k=None, max_forks=0, worth=200_000_000, beside=None):
         self.n_slots, self.h_q, self.h_kv, self.d = n_slots, h_q, h_kv, d
         self.window, self.sinks, self.scale = window, sinks, d ** -0.5 if scale is None else scale
         self.device = torch.device(device)
@@ -116,7 +117,15 @@ class AttnLayer:
         self._one_each = torch.arange(n_slots + 1, dtype=torch.int32, device=self.device)
         most = min(2 ** 31 - 1, 2 ** 37 // max(h_q, 1))       # tokens of a call
         self._ws_bytes = ix_kv8_attn_workspace_size(self.cache, n_slots, most, most, h_q)
-        self._ws = torch.empty(max(self._ws_bytes, 256), dtype=torch.uint8, device=self.device)
+        if beside is not None and not isinstance(beside, AttnLayer):
+            raise ValueError("baloon_amd: beside is another AttnLayer")
+
+        def workspace(n, theirs):
+            if theirs is not None and theirs.numel() >= n and theirs.device == self.kv_len.device:
+                return theirs
+            return torch.empty(max(n, 256), dtype=torch.uint8, device=self.device)
+
+        self._ws = workspace(self._ws_bytes, getattr(beside, "_ws", None))
         if rope is None and rope_k is not None:
             raise ValueError("baloon_amd: rope_k goes with rope")
         self.rope, self.rope_k = rope, rope if rope_k is None else rope_k
@@ -127,8 +136,8 @@ class AttnLayer:
             most = 2 * max_forks                              # groups: the forks, and what lies between two
             self._groups, self._shared = tensor(most + 1, dtype=torch.int32), tensor(most, dtype=torch.int32)
             self._few = 16 * n_slots
-            n = max(ix_kv8_attn_shared_workspace_size(self.cache, n_slots, self._few, self._few, most, h_q), 256)
-            self._shared_ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+            n = ix_kv8_attn_shared_workspace_size(self.cache, n_slots, self._few, self._few, most, h_q)
+            self._shared_ws = workspace(n, getattr(beside, "_shared_ws", None))
 
     def fork(self, slot, n, tokens, stream=None):
         """Slots slot + 1 .. slot + n - 1 go on from the first `tokens` tokens of `slot`, which holds as many, and from nothing that

@@ -28,12 +28,13 @@ class Hybrid:
             q_norm, k_norm = (torch.randn(d, generator=g, device="cuda") * 0.1 for _ in "qk")
             attention.update(rope=bx.rope(freq, norm=q_norm, norm_offset=1.0), rope_k=bx.rope(freq, norm=k_norm, norm_offset=1.0))
         self.embed = weight(vocab, hidden) * hidden ** 0.5
-        self.layers = []
+        self.layers, last = [], None
         for i in range(n_layers):
             norm = (torch.randn(hidden, generator=g, device="cuda") * 0.1)               # its weight is 1 + norm
             if i % 4 == 3:
                 w_in = weight((2 * h_q + 2 * h_kv) * d, hidden)                          # q | gate | k | v
-                self.layers.append((bx.AttnLayer(n_slots, max_len, h_q, h_kv, d, **attention), norm, w_in, weight(hidden, h_q * d)))
+                last = bx.AttnLayer(n_slots, max_len, h_q, h_kv, d, beside=last, **attention)       # the stack's layers run one after the other
+                self.layers.append((last, norm, w_in, weight(hidden, h_q * d)))
             else:
                 layer = bx.GdnLayer(n_slots, c)
                 layer.conv_w.copy_(weight(c.channels, c.d_conv))
