@@ -113,10 +113,11 @@ def generate(prompts, steps, seed=0):
     return torch.stack(made, 1).tolist(), model
 
 
-def continuations(prompts, each, steps, seed=0):
-    """`each` continuations of every prompt from one pass over it, drawn by the last token's logits, and the model."""
+def continuations(prompts, each, steps, seed=0, **attention):
+    """`each` continuations of every prompt from one pass over it, drawn by the last token's logits, and the model (whose attention
+    layers take what else is given)."""
     lens, n = [len(p) for p in prompts], len(prompts) * each
-    model = Hybrid(n, max(lens) + steps, seed=seed, rope_base=1e4, max_forks=len(prompts))
+    model = Hybrid(n, max(lens) + steps, seed=seed, rope_base=1e4, max_forks=len(prompts), **attention)
     cu = torch.tensor([0] + [x for m in lens for x in (m, *[0] * (each - 1))], dtype=torch.int32).cumsum(0, dtype=torch.int32).cuda()
     logits = model.forward(torch.tensor(sum(prompts, []), device="cuda"), cu, max(lens))     # a slot without tokens: of those before it
     for i, m in enumerate(lens):
