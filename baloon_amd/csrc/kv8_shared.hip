@@ -166,8 +166,8 @@ __host__ __device__ inline int few_items(int segments, int n_wg) {
     const int rounds = (int)((unsigned)segments / (unsigned)n_wg) + 1;
     return (rounds * n_wg - segments < n_wg / 4 ? rounds + 1 : rounds) * n_wg;
 }
-// Groups of up to kFewRows rows a kv head in the mean are always few_kernel's, those of more where all of them have up to kFewTiles
-// tiles of 16 rows: block_kernel takes a tile in half the time, but has 14 us before its first and for its partial results, of
+// Where groups have up to kFewRows rows a kv head in the mean, they are few_kernel's without a question (but see below), else where
+// all of them have up to kFewTiles tiles of 16 rows: block_kernel takes a tile in half the time, but has 14 us before its first and for its partial results, of
 // which 3 remain where it finds nothing to do. us there and here: 8 sequences of 16 heads over 2 of 256 behind 1,000 tokens (64 rows)
 // 30 and 16, 16 of them 32 and 18; 64 behind 1,024, 4,096 and 8,190 (2,000, 8,200 and 16,400 tiles) 40, 44, 49 and 28, 41, 56; 128 of 20
 // over 4 of 128 behind 1,024, 2,048 and 4,096 (2,600, 5,100 and 10,200) 53, 54, 62 and 42, 45, 61.
@@ -175,8 +175,9 @@ __host__ __device__ inline int few_items(int segments, int n_wg) {
 // The mean says little where one group has most of the rows (of a captured call's groups many can be empty). So the device chooses
 // also where one group of all rows over a whole table would have over twice kFewTiles: 2 us where block_kernel then has nothing
 // to do (24 groups of 4 sequences over a table that wide 56 and 58). One group beside 63 empty ones with few_kernel alone and with
-// the choice, us: 64 sequences of 16 heads over 2 of 256 behind 8,192 and 16,384 tokens (18,400 and 34,800 such tiles) 56, 92 and (48), 59;
-// 128 behind 4,096 and 16,384 (20,500, 69,600) 88, 280 and 61, 86; 200 of 32 over 8 of 128 behind 16,384 (105,600) 199 and 122.
+// the choice, us: 64 sequences of 16 heads over 2 of 256 behind 16,384 tokens (34,800 such tiles) 92 and 59, behind 8,192 (18,400, where there
+// is none) 56, 48 as the only group; 128 behind 4,096 and 16,384 (20,500, 69,600) 88, 280 and 61, 86; 200 of 32 over 8 of 128
+// behind 16,384 (105,600) 199 and 122.
 constexpr int kFewRows = 64, kFewTiles = 10000;
 // The first units, worked out once and kept in LDS, and the sums of all waves.
 constexpr int kKept = 512;
@@ -340,8 +341,8 @@ __device__ __forceinline__ void write_plan(const AttnArgs& A, const Groups& grou
 // An item is 16 rows of a unit over a part of its tiles. A wave takes a tile of kTok tokens at a time by itself, all in registers,
 // with the next one's loads under way; products and the layout of P are those of split_kernel. Every workgroup works out the cuts by
 // itself (2.5 us, where a kernel ahead of this one costs a launch); the way to an item's first tile is a chain of three reads, which
-// lies under the last item's join. Long own parts are bound by HBM: 96 sequences in groups of 4, 32 heads over 8 of 128, 225 MB
-// with the page tables in 48 us, 4.7 TB/s; shorter ones by that chain (64 of up to 1,000 own tokens 17 us, 10 where there is next to nothing to do).
+// lies under the last item's join. Long own parts are bound by HBM: 96 sequences in groups of 4, 32 heads over 8 of 128, 226 MB
+// with the page tables in 49 us, 4.6 TB/s; shorter ones by that chain (64 of up to 1,000 own tokens 17 us, 10 where there is next to nothing to do).
 template <int D>
 __global__ void __launch_bounds__(kThreads, few_per_cu(D)) few_kernel(AttnArgs A_) {
     constexpr int kC = D / 64, kM = D / 16, kPitch = D + 4, kTok = kTokOf<D>, kS = kTok / 16;
