@@ -47,6 +47,13 @@ inline bool rows_ok(const ix_rows* r, long long least) {
     return r && r->p && ptr_aligned(r->p, 2) && r->stride >= least;
 }
 
+// 8 values of a row, bf16, at any 2-byte address (the target reads and writes words unaligned).
+__device__ __forceinline__ uint4 load_row8(const uint16_t* p) {
+    uint4 x;
+    __builtin_memcpy(&x, p, sizeof(x));
+    return x;
+}
+
 // The last b in [0, n) with key(b) <= j, or 0 where there is none, for a key that does not fall: each step the wave's
 // lanes try 64 places (one load's latency for 64 sequences, two for 4,096). The same in every lane.
 template <class Key>

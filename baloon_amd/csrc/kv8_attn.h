@@ -145,13 +145,6 @@ __device__ __forceinline__ u16x2 max_abs_bits(u16x2 m, const uint4& x) {
     return m;
 }
 
-// 8 values of a row at any 2-byte address (the target reads and writes words unaligned).
-__device__ __forceinline__ uint4 load_row8(const uint16_t* p) {
-    uint4 x;
-    __builtin_memcpy(&x, p, sizeof(x));
-    return x;
-}
-
 // 16 bf16 values (a, b) times inv, at most 32639 of them, as 16-bit integers 256 hi + lo of two int8: hi in a, lo
 // in b. 1.5 2^23 added to a number leaves its nearest integer in the sum's low bits.
 __device__ __forceinline__ void split_q(uint4& a, uint4& b, float inv) {

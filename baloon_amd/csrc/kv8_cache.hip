@@ -117,13 +117,6 @@ __device__ __forceinline__ uint32_t older(uint32_t was, uint32_t now, float r, i
     return first(recode4(was, r), keep) | (now & ~first_mask(keep));
 }
 
-// 8 values of a row, bf16, at any 2-byte address (the target reads words unaligned).
-__device__ __forceinline__ uint4 load8(const uint16_t* p) {
-    uint4 x;
-    __builtin_memcpy(&x, p, sizeof(x));
-    return x;
-}
-
 // A page's values pass through LDS slot by slot. A lane takes 4 channels of 16 slots, which it turns 4 x 4 bytes at
 // a time; consecutive lanes take the 16s of the same channels, which lie side by side in the page.
 struct Turn {
@@ -185,7 +178,7 @@ append_kernel(Kv8 c, Batch a, const uint16_t* __restrict__ kr, long long k_strid
     const size_t ph = (size_t)job.id * c.h_kv + h;
     float* scale = (is_v ? c.v_scale : c.k_scale) + ph;
     int8_t* codes = (is_v ? c.v : c.k) + ph * c.page * c.d;
-    const auto load = [&](int i) { return load8(rows + (i >> per_log) * stride + ((i & ((1 << per_log) - 1)) << 3)); };
+    const auto load = [&](int i) { return load_row8(rows + (i >> per_log) * stride + ((i & ((1 << per_log) - 1)) << 3)); };
 
     const float old = job.held > 0 ? *scale : 0.0f;
     float m = 0.0f;

@@ -40,12 +40,6 @@ __device__ __forceinline__ float2 cos_sin(const Rope& r, int pos, float freq) {
     return make_float2(c * r.amplitude, s * r.amplitude);
 }
 
-// 8 values of a row at any 2-byte address (the target reads and writes words unaligned).
-__device__ __forceinline__ uint4 rope_load8(const uint16_t* p) {
-    uint4 x;
-    __builtin_memcpy(&x, p, sizeof(x));
-    return x;
-}
 __device__ __forceinline__ void widen8(const uint4& x, float (&f)[8]) {
     const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -208,8 +202,8 @@ __device__ __forceinline__ void rope_item(const RopeRows& A, const Batch& a, int
         const int h = heads0 + (i << (6 - r.per_log));
         const uint16_t* row = A.x + (long long)t * A.stride + (size_t)h * r.d;
         const bool any = h < A.heads && L.c < r.d;
-        own[i] = any ? rope_load8(row + L.c) : make_uint4(0, 0, 0, 0);
-        other[i] = any ? L.load_other(r, row, own[i], rope_load8) : make_uint4(0, 0, 0, 0);
+        own[i] = any ? load_row8(row + L.c) : make_uint4(0, 0, 0, 0);
+        other[i] = any ? L.load_other(r, row, own[i], load_row8) : make_uint4(0, 0, 0, 0);
     }
     const int pos = a.kv_len[b] - (end - t);
 #pragma unroll 1
