@@ -635,8 +635,10 @@ SharedPlan shared_plan(int d, int h_kv, int G, int n_seq, int T, int max_q, int 
     const double tiles = (double)((rows + kSplitRows - 1) / kSplitRows) * (double)(table_tokens / (d == 256 ? kTokOf<256> : kTokOf<128>)) * h_kv;
     p.many = rows > (long long)kFewRows * n_groups || (rows > kFewRows && tiles > 2.0 * kFewTiles);
     p.n_wg = d == 256 ? p.own.n_wg / 2 : p.own.n_wg;
-    // a sequence or group has at most one block that is not full; the groups may be few_kernel's
-    const long long segments = (2 * (rows / kSplitRows) + nonempty + n_groups) * h_kv, blocks = (rows / kBlockRows + n_groups) * h_kv;
+    // a sequence or group has at most one block that is not full; a group with rows to share has two sequences or more, and a token;
+    // the groups may be few_kernel's
+    const long long with_rows = std::min({n_groups, n_seq / 2, T});
+    const long long segments = (2 * (rows / kSplitRows) + nonempty + with_rows) * h_kv, blocks = (rows / kBlockRows + with_rows) * h_kv;
     p.few_wg = p.own.n_wg / 2 * few_per_cu(d);
     p.n_items = segments > 1 << 28 ? 0 : few_items((int)segments, p.few_wg - 1);
     p.n_shared = blocks < p.n_wg / 2 ? p.n_wg : (blocks + p.n_wg - 1) / p.n_wg * p.n_wg + p.n_wg;
