@@ -161,8 +161,8 @@ struct RopeLane {
 };
 
 // Token rows of heads that are turned into packed ones: a wave's item is one token's kRopeSteps 2^(6 - per_log) heads.
-// With 2, 4 and 8 steps the kernel takes, over four inputs in turn (us): 4,096 tokens of 32 heads of 128 16.1, 16.8 and 14.0 (HBM alone
-// over one input: 13.5 with 4), 15,800 of 16 of 256 60.5, 53.5 and 53.2, 2,541 of these far on 11.1, 10.8 and 11.6, a single one 3.2, 3.8
+// With 2, 4 and 8 steps the kernel takes, over four inputs in turn (us): 4,096 tokens of 32 heads of 128 16.1, 16.8 and 14.0,
+// 15,800 of 16 of 256 60.5, 53.5 and 53.2, 2,541 of these far on 11.1, 10.8 and 11.6, a single one 3.2, 3.8
 // and 4.9, 256 of 32 of 128 3.6, 4.2 and 5.5. The append's grid holds 3 waves a SIMD with 8, 5 with 4 (it spills scalar registers with 8).
 constexpr int kRopeSteps = 4;
 struct RopeRows {

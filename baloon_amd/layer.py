@@ -142,8 +142,8 @@ class AttnLayer:
     def fork(self, slot, n, tokens, stream=None):
         """Slots slot + 1 .. slot + n - 1 go on from the first `tokens` tokens of `slot`, which holds as many, and from nothing that
         they held: its whole pages are theirs too, the page that the tokens end in is copied. Until `release`, none of the n may lose one of these
-        tokens (a shorter kv_len, then new tokens). Not to be captured; calls that were captured before stay right, but take together
-        only what they knew of: with more forks, or where sharing has come to pay, capture them again."""
+        tokens (a shorter kv_len, then new tokens). Not to be captured; calls that were captured before stay right, but take
+        no more groups together than there were: with more forks, or where sharing has come to pay, capture them again."""
         others = range(slot + 1, slot + n)
         if slot < 0 or n < 2 or slot + n > self.n_slots or not 0 < tokens <= self.width * self.cache.page:
             raise ValueError("baloon_amd: a fork is of two slots or more, and of tokens that a slot can hold")
